@@ -20,6 +20,7 @@
  *   nls_dual_predict        decision_function / predict_std (dual)       _neo_ls_svm.py:666-671, 470-477
  *   nls_factor_create       cho_solve(self.L_, .) state of predict_std   _neo_ls_svm.py:464-469 (the factor kept on the device)
  *   nls_primal_fit_grid     the gamma x sigma grid (extension): the fit above once per sigma, one call
+ *   nls_quantize_rows, nls_int8_*, nls_orthogonalize   (no counterpart: matrix operators of few bits, extension)
  *   nls_comm_*, nls_group_* (no counterpart: the reference is single-process; SURVEY.md 8(b) "multi-GPU is internal to the ctx", 8(e))
  *
  * Conventions
@@ -35,7 +36,7 @@
  *     which (hipPointerGetAttributes).  Device-resident inputs are used in place, host inputs are
  *     staged with one H2D copy.  Small parameter arrays (shift, scale, B, gammas, beta, L, alpha) and
  *     all outputs are host pointers.  Nothing is retained after a call returns.
- *   - Calls are blocking; one host thread per context.  Several contexts of one process may run fits on the same GPU at the same time (each
+ *   - Calls are blocking (the matrix operators of few bits, at the end, are not: their section says how); one host thread per context.  Several contexts of one process may run fits on the same GPU at the same time (each
  *     owns its streams, handles and workspace): tests/test_gpu_two_contexts.py holds two contexts with fits in flight to the bits of the same fits
  *     run alone.  (Round 3's failures in this mode were rocsolver_zpotrf, which is not safe on two handles at once in this ROCm build -
  *     profiles/r04_two_contexts.md; the fit path no longer calls it.  NLS_POTRF=rocsolver, a diagnostic knob, brings it back: single context only.)
@@ -433,6 +434,52 @@ int nls_dual_fit(nls_ctx* ctx, const nls_dual_fit_args* args);
 /* yhat = k(Xq, Xt) alpha + sum(alpha); sigma = sqrt(1 - sum K o cho_solve(L, K^T)^T). */
 int nls_dual_predict(nls_ctx* ctx, const double* Xq, int64_t m, const double* Xt, int64_t n, int r,
                      const double* alpha, const double* L, double* yhat, double* sigma);
+
+/* ---- matrix operators of few bits ----------------------------------------------------------------------------------------------------
+ * (no counterpart: the reference computes in 64 bits only.)  Next to the 64-bit matrix calls above: the 8-bit form of rows, products of 8-bit rows,
+ * and orthogonalisation by Newton-Schulz products, for float32, float16 and bfloat16 matrices.
+ * Unlike the calls above these take DEVICE pointers only and do not block: the work is put on `stream` (a hipStream_t of the context's device; NULL is
+ * HIP's default stream, nls_ctx_stream gives the context's own) and the arrays must stay valid until it has run.  Nothing is allocated, waited for or
+ * kept: scratch memory is the caller's `workspace` (256-byte aligned, at least what the _workspace function says; two calls that may run at the same
+ * time - other streams, graphs that are replayed side by side - need two).  Calls can be captured into a graph.  The caller's current device is left
+ * as it was.  Results do not depend on timing: the same call gives the same bits.  Sizes of zero rows, columns or matrices are fine (nothing is
+ * written); sums over nothing (k = 0) are refused. */
+#define NLS_TYPE_F32 0
+#define NLS_TYPE_F16 1
+#define NLS_TYPE_BF16 2
+int nls_ctx_stream(nls_ctx* ctx, void** stream);
+/* scale[i] = max_k |x[i, k]| / 127,  q[i, k] = 127 x[i, k] / max_k |x[i, k]| to the nearest integer, ties to even, as in exact arithmetic.
+ * A row of zeros: scale 0, q 0.  A row that holds a NaN or an infinity: scale NaN or infinity, q 0 (products of the row are NaN then).
+ * x: element (i, k) at i * row_stride + k * col_stride (elements; any strides).  q: rows ldq bytes apart, ldq and q multiples of 16, ldq >= k rounded
+ * up to 16; bytes k .. ldq - 1 of every row are written as zeros.  scale: rows floats. */
+int nls_quantize_rows(nls_ctx* ctx, const void* x, int type, int64_t rows, int64_t k, int64_t row_stride, int64_t col_stride, int8_t* q, int64_t ldq,
+                      float* scale, void* stream);
+/* y[i, j] = a_scale[i] * b_scale[j] * sum_k a[i, k] b[j, k] (+ bias[j]);  a: m rows lda bytes apart, b: n rows ldb bytes apart (channels x k),
+ * y: m x n without gaps, of `type`.  The sum is exact (32-bit integers, hence k <= NLS_INT8_MAX_K), the rest is float32, rounded once to `type`.
+ * bias: n elements, float32 or of `type` (bias_type), or NULL.  Rows that start at multiples of 16 bytes are read in place; k need not be a multiple of
+ * 16 if the flag says that the bytes up to the next one may be read in every row, the last included (what they hold does not matter).  Other rows are
+ * copied to the workspace first. */
+#define NLS_INT8_MAX_K 131071
+#define NLS_INT8_A_PADDED 1
+#define NLS_INT8_B_PADDED 2
+int nls_int8_matmul_workspace(int64_t m, int64_t n, int64_t k, size_t* bytes);
+int nls_int8_matmul(nls_ctx* ctx, const int8_t* a, int64_t lda, const float* a_scale, const int8_t* b, int64_t ldb, const float* b_scale,
+                    const void* bias, int bias_type, int64_t m, int64_t n, int64_t k, void* y, int type, int flags, void* workspace,
+                    size_t workspace_bytes, void* stream);
+/* The two calls above in one: x (m x k, `type`, any strides) is quantised row by row and multiplied; y is of `type` too. */
+int nls_int8_linear_workspace(int64_t m, int64_t n, int64_t k, size_t* bytes);
+int nls_int8_linear(nls_ctx* ctx, const void* x, int type, int64_t row_stride, int64_t col_stride, const int8_t* b, int64_t ldb, const float* b_scale,
+                    const void* bias, int bias_type, int64_t m, int64_t n, int64_t k, void* y, int flags, void* workspace, size_t workspace_bytes,
+                    void* stream);
+/* X = G / (|G|_F + eps), then for every step t: X <- a_t X + (b_t A + c_t A A) X with A = X X^T (of the shorter side; a matrix with m > n is worked on
+ * transposed).  coefficients: steps x 3 (a, b, c), host.  G: `batch` matrices m x n of `type`, element (l, i, j) at l batch_stride + i row_stride +
+ * j col_stride; out: batch x m x n without gaps, of `type`, not overlapping G.  Each matrix has its own norm; one that holds a NaN or an infinity
+ * comes out as NaN, one of zeros as zeros.  Products and sums carry 22 bits or more; for 16-bit results the early steps carry 11 (error of the result
+ * against 64 bits below its own rounding).  The coefficients may not let a singular value of X pass 1e6. */
+int nls_orthogonalize_workspace(int64_t batch, int64_t m, int64_t n, size_t* bytes);
+int nls_orthogonalize(nls_ctx* ctx, const void* g, int type, int64_t batch, int64_t m, int64_t n, int64_t batch_stride, int64_t row_stride,
+                      int64_t col_stride, const double* coefficients, int steps, double eps, void* out, void* workspace, size_t workspace_bytes,
+                      void* stream);
 
 #ifdef __cplusplus
 }

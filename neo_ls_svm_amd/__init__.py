@@ -28,6 +28,8 @@ from .hotpath import (  # noqa: F401
     twostage_stage,
 )
 
+from .lowbit import NEWTON_SCHULZ, int8_linear, int8_matmul, orthogonalize, quantize_rows  # noqa: F401
+
 from .estimator import (  # noqa: E402,F401
     AffineFeatureMap,
     AffineNormalizer,
@@ -72,4 +74,9 @@ __all__ = [
     "stedc",
     "cholesky",
     "twostage_stage",
+    "NEWTON_SCHULZ",
+    "quantize_rows",
+    "int8_matmul",
+    "int8_linear",
+    "orthogonalize",
 ]

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import threading
 from pathlib import Path
 
 import numpy as np
@@ -221,6 +222,25 @@ SIGNATURES = {
         C.c_int,
         [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p],
     ),
+    "nls_ctx_stream": (C.c_int, [C.c_void_p, C.POINTER(C.c_void_p)]),
+    "nls_quantize_rows": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int] + [C.c_int64] * 4 + [C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]),
+    "nls_int8_matmul_workspace": (C.c_int, [C.c_int64] * 3 + [C.POINTER(C.c_size_t)]),
+    "nls_int8_matmul": (
+        C.c_int,
+        [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int]
+        + [C.c_int64] * 3 + [C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p],
+    ),
+    "nls_int8_linear_workspace": (C.c_int, [C.c_int64] * 3 + [C.POINTER(C.c_size_t)]),
+    "nls_int8_linear": (
+        C.c_int,
+        [C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int]
+        + [C.c_int64] * 3 + [C.c_void_p, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p],
+    ),
+    "nls_orthogonalize_workspace": (C.c_int, [C.c_int64] * 3 + [C.POINTER(C.c_size_t)]),
+    "nls_orthogonalize": (
+        C.c_int,
+        [C.c_void_p, C.c_void_p, C.c_int] + [C.c_int64] * 6 + [C.c_void_p, C.c_int, C.c_double, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p],
+    ),
 }
 
 _lib = None
@@ -267,12 +287,13 @@ def raise_for(code: int, message: str):
 
 
 class DeviceArray:
-    """A float64 array resident in HBM, owned by a Context (plain pointer + shape, no torch)."""
+    """A dense array resident in HBM, owned by a Context (plain pointer + shape, no torch): float64, as the hot path takes it, unless said otherwise."""
 
-    def __init__(self, ctx: "Context", shape):
+    def __init__(self, ctx: "Context", shape, dtype=np.float64):
         self.ctx = ctx
         self.shape = tuple(int(x) for x in np.atleast_1d(shape))
-        self.nbytes = int(np.prod(self.shape)) * 8
+        self.dtype = np.dtype(dtype)
+        self.nbytes = int(np.prod(self.shape)) * self.dtype.itemsize
         p = C.c_void_p()
         ctx._check(ctx.lib.nls_device_malloc(ctx.handle, max(self.nbytes, 8), C.byref(p)))
         self.ptr = p.value
@@ -280,16 +301,16 @@ class DeviceArray:
     # Lets an array library (cupy, ...) wrap the buffer without a copy.
     @property
     def __cuda_array_interface__(self):
-        return {"shape": self.shape, "typestr": "<f8", "data": (self.ptr, False), "version": 2, "strides": None}
+        return {"shape": self.shape, "typestr": self.dtype.str, "data": (self.ptr, False), "version": 2, "strides": None}
 
     def copy_from_host(self, a: np.ndarray) -> "DeviceArray":
-        a = np.ascontiguousarray(a, dtype=np.float64)
+        a = np.ascontiguousarray(a, dtype=self.dtype)
         assert a.nbytes == self.nbytes
         self.ctx._check(self.ctx.lib.nls_memcpy_h2d(self.ctx.handle, self.ptr, a.ctypes.data, a.nbytes))
         return self
 
     def to_host(self) -> np.ndarray:
-        out = np.empty(self.shape, dtype=np.float64)
+        out = np.empty(self.shape, dtype=self.dtype)
         self.ctx._check(self.ctx.lib.nls_memcpy_d2h(self.ctx.handle, out.ctypes.data, self.ptr, out.nbytes))
         return out
 
@@ -379,6 +400,7 @@ class Context:
             h = C.c_void_p(_borrowed)
         self.handle = h
         self.device = int(device)
+        self.lock = threading.Lock()  # held by the calls that do not block (lowbit.py) from launch to error message
         self.comm_world = 1  # world size of the native communicator this context has joined (1: none, or one rank)
         self._hook = None  # keep the ctypes callback alive
 
@@ -500,12 +522,12 @@ class Context:
         self._check(self.lib.nls_device_info(self.handle, name, 256, C.byref(cus), C.byref(hbm)))
         return {"name": name.value.decode(), "compute_units": cus.value, "hbm_bytes": hbm.value}
 
-    def to_device(self, a: np.ndarray) -> DeviceArray:
-        a = np.ascontiguousarray(a, dtype=np.float64)
-        return DeviceArray(self, a.shape).copy_from_host(a)
+    def to_device(self, a: np.ndarray, dtype=np.float64) -> DeviceArray:
+        a = np.ascontiguousarray(a, dtype=dtype)
+        return DeviceArray(self, a.shape, dtype).copy_from_host(a)
 
-    def empty(self, shape) -> DeviceArray:
-        return DeviceArray(self, shape)
+    def empty(self, shape, dtype=np.float64) -> DeviceArray:
+        return DeviceArray(self, shape, dtype)
 
     # ---- one upload per fit ------------------------------------------------------------------------
     def hold(self, a: np.ndarray):

@@ -611,7 +611,7 @@ static int ensure_copy_stream(nls_ctx* ctx, int nblk) {
   }
   return NLS_OK;
 }
-__global__ void k_conj_block(double2* A, long ld, long r0, long c0, long rows, long cols) {
+static __global__ void k_conj_block(double2* A, long ld, long r0, long c0, long rows, long cols) {
   const long idx = blockIdx.x * (long)blockDim.x + threadIdx.x;
   if (idx >= rows * cols) return;
   double2* p = A + (r0 + idx % rows) + (c0 + idx / rows) * ld;
@@ -637,7 +637,7 @@ static int download_block_columns(nls_ctx* ctx, void* host, void* dev, int n, lo
   return NLS_OK;
 }
 // infos[b] (relative to block b, 0 = fine) -> out = the first failure as a global 1-based index
-__global__ void k_merge_block_info(const int* infos, int nblk, int nbk, int* out) {
+static __global__ void k_merge_block_info(const int* infos, int nblk, int nbk, int* out) {
   if (threadIdx.x != 0 || blockIdx.x != 0) return;
   int r = 0;
   for (int b = 0; b < nblk && r == 0; ++b)

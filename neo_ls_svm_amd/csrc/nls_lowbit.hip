@@ -1,0 +1,354 @@
+// Matrix operators of few bits behind the C ABI: nls_quantize_rows, nls_int8_matmul, nls_int8_linear, nls_orthogonalize (include/neolssvm_hip.h).
+// A translation unit of its own: the kernels here are 8- and 16-bit matrix code with a float epilogue and take other compiler options than the
+// 64-bit engines (Makefile).  All arrays are the caller's device memory, the workspace included, and every launch goes to the caller's stream: nothing
+// is allocated, waited for or kept, so calls on different streams do not meet and any of them can be captured into a graph.
+#include "nls_host.h"
+
+#include "nls_int8.h"
+#include "nls_ortho.h"
+
+using namespace lb;
+
+namespace {
+
+// The context's device for the length of a call; the caller's current device comes back afterwards.
+struct DeviceGuard {
+  int before = -1;
+  hipError_t err = hipSuccess;
+  explicit DeviceGuard(int device) {
+    err = hipGetDevice(&before);
+    if (err == hipSuccess && before != device)
+      err = hipSetDevice(device);
+    else
+      before = -1;
+  }
+  ~DeviceGuard() {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+};
+
+#define LAUNCHED(ctx, what)                                                                             \
+  do {                                                                                                  \
+    const hipError_t e__ = hipGetLastError();                                                           \
+    if (e__ != hipSuccess) return fail(ctx, NLS_ERR_HIP, "%s: launch failed: %s", what, hipGetErrorString(e__)); \
+  } while (0)
+
+// Dynamic LDS beyond 64 KB has to be asked for once per kernel and device; asking again costs a table lookup.
+template <class F>
+int ask_lds(nls_ctx* ctx, F f, int bytes) {
+  if (bytes > 65536) HIPCHK(ctx, hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  return NLS_OK;
+}
+
+int type_size(int t) { return t == NLS_TYPE_F32 ? 4 : (t == NLS_TYPE_F16 || t == NLS_TYPE_BF16) ? 2 : 0; }
+
+// ---- quantise ----
+template <class T>
+int quantize(nls_ctx* ctx, const T* x, long rows, long k, long rs, long cs, signed char* q, long ldq, float* scale, hipStream_t st) {
+  const bool vec = cs == 1 && rs % 4 == 0 && (uintptr_t)x % (4 * sizeof(T)) == 0;
+  const bool narrow = k <= 512;
+  const dim3 grid((unsigned)(narrow ? (rows + 3) / 4 : rows));
+  if (vec)
+    narrow ? (void)(k_quantize_rows<T, 64, true><<<grid, 256, 0, st>>>(x, rows, k, rs, cs, q, ldq, scale))
+           : (void)(k_quantize_rows<T, 256, true><<<grid, 256, 0, st>>>(x, rows, k, rs, cs, q, ldq, scale));
+  else
+    narrow ? (void)(k_quantize_rows<T, 64, false><<<grid, 256, 0, st>>>(x, rows, k, rs, cs, q, ldq, scale))
+           : (void)(k_quantize_rows<T, 256, false><<<grid, 256, 0, st>>>(x, rows, k, rs, cs, q, ldq, scale));
+  LAUNCHED(ctx, "quantize_rows");
+  return NLS_OK;
+}
+int quantize_any(nls_ctx* ctx, const void* x, int type, long rows, long k, long rs, long cs, signed char* q, long ldq, float* scale, hipStream_t st) {
+  switch (type) {
+    case NLS_TYPE_F32: return quantize(ctx, (const float*)x, rows, k, rs, cs, q, ldq, scale, st);
+    case NLS_TYPE_F16: return quantize(ctx, (const _Float16*)x, rows, k, rs, cs, q, ldq, scale, st);
+    default: return quantize(ctx, (const __bf16*)x, rows, k, rs, cs, q, ldq, scale, st);
+  }
+}
+
+// ---- 8-bit product ----
+template <class T, int BI, int BJ, int WI, int WJ>
+int int8_tile(nls_ctx* ctx, const Int8Args& g, hipStream_t st) {
+  using TL = Tile<MODE_I8, BI, BJ, WI, WJ>;
+  const int ti = (g.n + BI - 1) / BI, tj = (g.m + BJ - 1) / BJ;
+  NLSCHK(ask_lds(ctx, k_int8_tile<T, BI, BJ, WI, WJ>, TL::LDS));
+  k_int8_tile<T, BI, BJ, WI, WJ><<<dim3((unsigned)((long)ti * tj)), TL::THREADS, TL::LDS, st>>>(g, ti, tj, 8);
+  LAUNCHED(ctx, "int8_matmul");
+  return NLS_OK;
+}
+template <class T>
+int int8_product(nls_ctx* ctx, const Int8Args& g, hipStream_t st) {
+  const long big = (long)((g.n + 127) / 128) * ((g.m + 127) / 128);
+  if (big >= ctx->cus) return int8_tile<T, 128, 128, 2, 2>(ctx, g, st);
+  return int8_tile<T, 64, 64, 2, 2>(ctx, g, st);
+}
+int int8_product_any(nls_ctx* ctx, const Int8Args& g, int type, hipStream_t st) {
+  switch (type) {
+    case NLS_TYPE_F32: return int8_product<float>(ctx, g, st);
+    case NLS_TYPE_F16: return int8_product<_Float16>(ctx, g, st);
+    default: return int8_product<__bf16>(ctx, g, st);
+  }
+}
+
+long up16(long k) { return (k + 15) / 16 * 16; }
+size_t up256(size_t b) { return (b + 255) / 256 * 256; }
+
+bool aligned_rows(const void* p, long ld, long k, int flags, int flag) {
+  return (uintptr_t)p % 16 == 0 && ld % 16 == 0 && ld >= up16(k) && (k % 16 == 0 || (flags & flag));
+}
+
+int check_int8(nls_ctx* ctx, const char* what, int64_t m, int64_t n, int64_t k, int type, int bias_type, const void* bias) {
+  if (m < 0 || n < 0) return fail(ctx, NLS_ERR_ARG, "%s: negative size", what);
+  if (k < 1 || k > NLS_INT8_MAX_K) return fail(ctx, NLS_ERR_ARG, "%s: k = %lld; 1 .. %d products are summed in 32 bits without overflow", what, (long long)k, NLS_INT8_MAX_K);
+  if (m > INT32_MAX - 256 || n > INT32_MAX - 256) return fail(ctx, NLS_ERR_ARG, "%s: more than 2^31 rows", what);
+  if (type_size(type) == 0) return fail(ctx, NLS_ERR_ARG, "%s: unknown element type %d", what, type);
+  if (bias && bias_type != NLS_TYPE_F32 && bias_type != type) return fail(ctx, NLS_ERR_ARG, "%s: the bias must be float32 or of the result's type", what);
+  return NLS_OK;
+}
+
+// a and b as the kernels take them: laid out again in the workspace where the caller's rows do not start at multiples of 16 bytes.
+int aligned_operand(nls_ctx* ctx, const int8_t* p, long rows, long k, long ld, bool ok, char** ws, char* end, Operand* out, hipStream_t st) {
+  if (ok) {
+    *out = Operand{(const char*)p, (unsigned)ld, (int)rows};
+    return NLS_OK;
+  }
+  const long ldy = up16(k);
+  const size_t need = up256((size_t)rows * ldy);
+  if ((size_t)(end - *ws) < need) return fail(ctx, NLS_ERR_ARG, "int8_matmul: workspace too small (nls_int8_matmul_workspace)");
+  const long work = rows * (ldy / 4);
+  k_align_rows<<<dim3((unsigned)std::min<long>((work + 255) / 256, 65536)), 256, 0, st>>>((const signed char*)p, rows, k, ld, (signed char*)*ws, ldy);
+  LAUNCHED(ctx, "int8_matmul (alignment)");
+  *out = Operand{*ws, (unsigned)ldy, (int)rows};
+  *ws += need;
+  return NLS_OK;
+}
+
+// ---- Newton-Schulz ----
+struct NsPlan {
+  long p, q;
+  size_t x, xt, a, parts, scales, batch_bytes, total;
+};
+NsPlan ns_plan(long m, long n, long batch) {
+  NsPlan w;
+  w.p = std::min(m, n);
+  w.q = std::max(m, n);
+  w.x = (size_t)w.p * pair_ld(w.q);
+  w.xt = (size_t)w.q * pair_ld(w.p);
+  w.a = (size_t)w.p * pair_ld(w.p);
+  w.batch_bytes = w.x + 2 * w.xt + 2 * w.a;
+  w.parts = up256((size_t)batch * NS_PARTS * sizeof(double));
+  w.scales = up256((size_t)batch * sizeof(NsScales));
+  w.total = w.parts + w.scales + (size_t)batch * w.batch_bytes;
+  return w;
+}
+
+template <int KIND, class T, int MODE, int B, int W>
+int ns_product_tile(nls_ctx* ctx, NsArgs g, long batch, hipStream_t st) {
+  using TL = Tile<MODE, B, B, W, W>;
+  constexpr int LDS = TL::LDS > TL::WAVES * 32 * 33 * 4 ? TL::LDS : TL::WAVES * 32 * 33 * 4;
+  g.ti = (g.I + B - 1) / B;
+  g.tj = (g.J + B - 1) / B;
+  g.strip = 8;
+  constexpr bool SYM = KIND == NS_GRAM || KIND == NS_POLY;
+  const long tiles = SYM ? (long)g.ti * (g.ti + 1) / 2 : (long)g.ti * g.tj;
+  NLSCHK(ask_lds(ctx, k_ns_product<KIND, T, MODE, B, B, W, W>, LDS));
+  k_ns_product<KIND, T, MODE, B, B, W, W><<<dim3((unsigned)tiles, 1, (unsigned)batch), TL::THREADS, LDS, st>>>(g);
+  LAUNCHED(ctx, "orthogonalize");
+  return NLS_OK;
+}
+template <int KIND, class T>
+int ns_product(nls_ctx* ctx, const NsArgs& g, bool pairs, long batch, hipStream_t st) {
+  const long big = (long)((g.I + 127) / 128) * ((g.J + 127) / 128) * batch;
+  if (big >= ctx->cus) return pairs ? ns_product_tile<KIND, T, MODE_F16PAIR, 128, 2>(ctx, g, batch, st) : ns_product_tile<KIND, T, MODE_F16, 128, 2>(ctx, g, batch, st);
+  return pairs ? ns_product_tile<KIND, T, MODE_F16PAIR, 64, 2>(ctx, g, batch, st) : ns_product_tile<KIND, T, MODE_F16, 64, 2>(ctx, g, batch, st);
+}
+
+template <class T>
+int orthogonalize(nls_ctx* ctx, const NsMatrix& w, const NsPlan& plan, bool tall, long batch, const NsCoef& cf, int steps, double eps, T* out, char* ws, hipStream_t st) {
+  double* parts = (double*)ws;
+  NsScales* scales = (NsScales*)(ws + plan.parts);
+  char* base = ws + plan.parts + plan.scales;
+  char *X = base, *XT = X + plan.x, *XU = XT + plan.xt, *A = XU + plan.xt, *B = A + plan.a;
+  const int count = (int)std::min<long>(NS_PARTS, (std::max(w.p, w.q) + 3) / 4);
+  k_ns_norm<T><<<dim3(count, (unsigned)batch), 256, 0, st>>>(w, parts);
+  k_ns_scales<<<dim3((unsigned)batch), 64, 0, st>>>(parts, count, eps, cf, steps, scales);
+  k_ns_pack<T><<<dim3((unsigned)((w.q + 63) / 64), (unsigned)((w.p + 63) / 64), (unsigned)batch), 256, 0, st>>>(w, scales, X, XT, plan.batch_bytes);
+  LAUNCHED(ctx, "orthogonalize");
+  // The first steps may work on the hi halves alone where the result has few bits: what a rounding to 11 bits does to an early iterate is carried
+  // along as a slightly different matrix would be, and the steps after it pull its singular values to the same curve.
+  const int exact = sizeof(T) == 4 ? steps : std::is_same<T, __bf16>::value ? 2 : 3;
+  NsArgs g{};
+  g.scales = scales;
+  g.batch_bytes = plan.batch_bytes;
+  const int p = (int)w.p, q = (int)w.q;
+  for (int t = 0; t < steps; ++t) {
+    const bool pairs = t >= steps - exact;
+    g.t = t;
+    g.a = (float)cf.a[t];
+    g.b = (float)cf.b[t];
+    g.c = (float)cf.c[t];
+    g.P = g.Q = X;
+    g.D = A;
+    g.I = g.J = p;
+    g.K = q;
+    NLSCHK((ns_product<NS_GRAM, float>(ctx, g, pairs, batch, st)));
+    g.P = g.Q = g.E = A;
+    g.D = B;
+    g.K = p;
+    NLSCHK((ns_product<NS_POLY, float>(ctx, g, pairs, batch, st)));
+    g.P = XT;
+    g.Q = B;
+    g.E = X;
+    g.I = q;
+    if (t + 1 < steps) {
+      g.D = X;
+      g.DT = XU;
+      NLSCHK((ns_product<NS_STEP, float>(ctx, g, pairs, batch, st)));
+      std::swap(XT, XU);
+    } else {
+      g.out = out;
+      g.out_stride = (size_t)p * q;
+      g.transposed = tall;
+      NLSCHK((ns_product<NS_LAST, T>(ctx, g, pairs, batch, st)));
+    }
+  }
+  return NLS_OK;
+}
+
+}  // namespace
+
+extern "C" int nls_ctx_stream(nls_ctx* ctx, void** stream) {
+  if (!ctx || !stream) return NLS_ERR_ARG;
+  *stream = ctx->stream;
+  return NLS_OK;
+}
+
+extern "C" int nls_quantize_rows(nls_ctx* ctx, const void* x, int type, int64_t rows, int64_t k, int64_t row_stride, int64_t col_stride, int8_t* q,
+                                 int64_t ldq, float* scale, void* stream) {
+  if (!ctx) return NLS_ERR_ARG;
+  if (type_size(type) == 0) return fail(ctx, NLS_ERR_ARG, "quantize_rows: unknown element type %d", type);
+  if (rows < 0 || k < 1) return fail(ctx, NLS_ERR_ARG, "quantize_rows: %lld rows of %lld elements", (long long)rows, (long long)k);
+  if (rows > INT32_MAX) return fail(ctx, NLS_ERR_ARG, "quantize_rows: more than 2^31 rows");
+  if (ldq < up16(k) || ldq % 16 != 0 || (uintptr_t)q % 16 != 0) return fail(ctx, NLS_ERR_ARG, "quantize_rows: rows of q must start at multiples of 16 bytes and hold k rounded up to them");
+  if (rows == 0) return NLS_OK;
+  if (!x || !q || !scale) return fail(ctx, NLS_ERR_ARG, "quantize_rows: null pointer");
+  DeviceGuard dev(ctx->device);
+  HIPCHK(ctx, dev.err);
+  return quantize_any(ctx, x, type, rows, k, row_stride, col_stride, (signed char*)q, ldq, scale, (hipStream_t)stream);
+}
+
+extern "C" int nls_int8_matmul_workspace(int64_t m, int64_t n, int64_t k, size_t* bytes) {
+  if (!bytes || m < 0 || n < 0 || k < 1) return NLS_ERR_ARG;
+  *bytes = up256((size_t)m * up16(k)) + up256((size_t)n * up16(k)) + 256;
+  return NLS_OK;
+}
+
+extern "C" int nls_int8_matmul(nls_ctx* ctx, const int8_t* a, int64_t lda, const float* a_scale, const int8_t* b, int64_t ldb, const float* b_scale,
+                               const void* bias, int bias_type, int64_t m, int64_t n, int64_t k, void* y, int type, int flags, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  if (!ctx) return NLS_ERR_ARG;
+  NLSCHK(check_int8(ctx, "int8_matmul", m, n, k, type, bias_type, bias));
+  if (lda < k || ldb < k || lda > UINT32_MAX / 512 || ldb > UINT32_MAX / 512) return fail(ctx, NLS_ERR_ARG, "int8_matmul: row strides %lld, %lld", (long long)lda, (long long)ldb);
+  if (m == 0 || n == 0) return NLS_OK;
+  if (!a || !a_scale || !b || !b_scale || !y) return fail(ctx, NLS_ERR_ARG, "int8_matmul: null pointer");
+  DeviceGuard dev(ctx->device);
+  HIPCHK(ctx, dev.err);
+  hipStream_t st = (hipStream_t)stream;
+  char* ws = (char*)workspace;
+  char* end = ws + workspace_bytes;
+  if ((uintptr_t)ws % 256) return fail(ctx, NLS_ERR_ARG, "int8_matmul: the workspace must be aligned to 256 bytes");
+  Int8Args g{};
+  NLSCHK(aligned_operand(ctx, a, m, k, lda, aligned_rows(a, lda, k, flags, NLS_INT8_A_PADDED), &ws, end, &g.a, st));
+  NLSCHK(aligned_operand(ctx, b, n, k, ldb, aligned_rows(b, ldb, k, flags, NLS_INT8_B_PADDED), &ws, end, &g.b, st));
+  g.a_scale = a_scale;
+  g.b_scale = b_scale;
+  g.bias = bias;
+  g.bias_type = bias_type;
+  g.m = (int)m;
+  g.n = (int)n;
+  g.k = (int)k;
+  g.y = y;
+  return int8_product_any(ctx, g, type, st);
+}
+
+extern "C" int nls_int8_linear_workspace(int64_t m, int64_t n, int64_t k, size_t* bytes) {
+  if (!bytes || m < 0 || n < 0 || k < 1) return NLS_ERR_ARG;
+  *bytes = up256((size_t)m * up16(k)) + up256((size_t)m * 4) + up256((size_t)n * up16(k)) + 256;
+  return NLS_OK;
+}
+
+extern "C" int nls_int8_linear(nls_ctx* ctx, const void* x, int type, int64_t row_stride, int64_t col_stride, const int8_t* b, int64_t ldb,
+                               const float* b_scale, const void* bias, int bias_type, int64_t m, int64_t n, int64_t k, void* y, int flags,
+                               void* workspace, size_t workspace_bytes, void* stream) {
+  if (!ctx) return NLS_ERR_ARG;
+  NLSCHK(check_int8(ctx, "int8_linear", m, n, k, type, bias_type, bias));
+  if (ldb < k || ldb > UINT32_MAX / 512) return fail(ctx, NLS_ERR_ARG, "int8_linear: row stride %lld", (long long)ldb);
+  if (m == 0 || n == 0) return NLS_OK;
+  if (!x || !b || !b_scale || !y || !workspace) return fail(ctx, NLS_ERR_ARG, "int8_linear: null pointer");
+  DeviceGuard dev(ctx->device);
+  HIPCHK(ctx, dev.err);
+  hipStream_t st = (hipStream_t)stream;
+  const long ldq = up16(k);
+  const size_t rows = up256((size_t)m * ldq), scales = up256((size_t)m * 4);
+  char* ws = (char*)workspace;
+  char* end = ws + workspace_bytes;
+  if (workspace_bytes < rows + scales) return fail(ctx, NLS_ERR_ARG, "int8_linear: workspace too small (nls_int8_linear_workspace)");
+  if ((uintptr_t)ws % 256) return fail(ctx, NLS_ERR_ARG, "int8_linear: the workspace must be aligned to 256 bytes");
+  signed char* q = (signed char*)ws;
+  float* scale = (float*)(ws + rows);
+  ws += rows + scales;
+  Int8Args g{};
+  NLSCHK(aligned_operand(ctx, b, n, k, ldb, aligned_rows(b, ldb, k, flags, NLS_INT8_B_PADDED), &ws, end, &g.b, st));
+  NLSCHK(quantize_any(ctx, x, type, m, k, row_stride, col_stride, q, ldq, scale, st));
+  g.a = Operand{(const char*)q, (unsigned)ldq, (int)m};
+  g.a_scale = scale;
+  g.b_scale = b_scale;
+  g.bias = bias;
+  g.bias_type = bias_type;
+  g.m = (int)m;
+  g.n = (int)n;
+  g.k = (int)k;
+  g.y = y;
+  return int8_product_any(ctx, g, type, st);
+}
+
+extern "C" int nls_orthogonalize_workspace(int64_t batch, int64_t m, int64_t n, size_t* bytes) {
+  if (!bytes || batch < 0 || m < 0 || n < 0) return NLS_ERR_ARG;
+  *bytes = ns_plan(m, n, batch).total;
+  return NLS_OK;
+}
+
+extern "C" int nls_orthogonalize(nls_ctx* ctx, const void* g, int type, int64_t batch, int64_t m, int64_t n, int64_t batch_stride, int64_t row_stride,
+                                 int64_t col_stride, const double* coefficients, int steps, double eps, void* out, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
+  if (!ctx) return NLS_ERR_ARG;
+  if (type_size(type) == 0) return fail(ctx, NLS_ERR_ARG, "orthogonalize: unknown element type %d", type);
+  if (batch < 0 || m < 0 || n < 0) return fail(ctx, NLS_ERR_ARG, "orthogonalize: negative size");
+  if (steps < 1 || steps > NS_MAX_STEPS) return fail(ctx, NLS_ERR_ARG, "orthogonalize: %d steps; 1 .. %d", steps, NS_MAX_STEPS);
+  if (!(eps >= 0.0) || !(eps < 1e30)) return fail(ctx, NLS_ERR_ARG, "orthogonalize: eps must be a number >= 0");
+  if (!coefficients) return fail(ctx, NLS_ERR_ARG, "orthogonalize: null pointer");
+  NsCoef cf{};
+  double u = 1.0;
+  for (int t = 0; t < steps; ++t) {
+    cf.a[t] = coefficients[3 * t];
+    cf.b[t] = coefficients[3 * t + 1];
+    cf.c[t] = coefficients[3 * t + 2];
+    u = ns_peak_x(cf.a[t], cf.b[t], cf.c[t], u) * (1.0 + 1e-3);
+    if (!(u < 1e6)) return fail(ctx, NLS_ERR_ARG, "orthogonalize: the coefficients let singular values grow past 1e6 in step %d", t + 1);
+  }
+  if (m > (1 << 20) || n > (1 << 20) || batch > 65535) return fail(ctx, NLS_ERR_ARG, "orthogonalize: at most 2^20 rows and columns and 65535 matrices");
+  if (batch == 0 || m == 0 || n == 0) return NLS_OK;
+  if (!g || !out || !workspace) return fail(ctx, NLS_ERR_ARG, "orthogonalize: null pointer");
+  const NsPlan plan = ns_plan(m, n, batch);
+  if (workspace_bytes < plan.total) return fail(ctx, NLS_ERR_ARG, "orthogonalize: workspace of %zu bytes, %zu needed", workspace_bytes, plan.total);
+  if ((uintptr_t)workspace % 256) return fail(ctx, NLS_ERR_ARG, "orthogonalize: the workspace must be aligned to 256 bytes");
+  DeviceGuard dev(ctx->device);
+  HIPCHK(ctx, dev.err);
+  const bool tall = m > n;
+  NsMatrix w{g, plan.p, plan.q, tall ? col_stride : row_stride, tall ? row_stride : col_stride, batch_stride};
+  hipStream_t st = (hipStream_t)stream;
+  switch (type) {
+    case NLS_TYPE_F32: return orthogonalize(ctx, w, plan, tall, batch, cf, steps, eps, (float*)out, (char*)workspace, st);
+    case NLS_TYPE_F16: return orthogonalize(ctx, w, plan, tall, batch, cf, steps, eps, (_Float16*)out, (char*)workspace, st);
+    default: return orthogonalize(ctx, w, plan, tall, batch, cf, steps, eps, (__bf16*)out, (char*)workspace, st);
+  }
+}

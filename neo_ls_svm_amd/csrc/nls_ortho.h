@@ -1,0 +1,296 @@
+// Newton-Schulz orthogonalisation: X = G / (|G|_F + eps), then `steps` times X <- a X + (b A + c A A) X with A = X X^T (G taken p x q, p <= q).
+//
+// Three products a step, all of the form sum_k P[i][k] Q[j][k] (nls_tile.h): A = X X^T and B = b A + c A A^T are symmetric - the tiles on and below
+// the diagonal are computed and written twice - and B X reads the transposed copy of X that the step before wrote beside X.
+//
+// Every matrix between the products is held as a pair of fp16, hi + lo: 22 significant bits, scaled by a power of two that follows from a bound on
+// the singular values (polynomial extrema, from the norm on), so that entries stay below 2^15 and neither half leaves fp16's range.  A product of
+// pairs is hi hi + lo hi + hi lo (the dropped lo lo is below 2^-22 of a term), three matrix instructions at 16 x the rate of the fp32 one.
+#pragma once
+#include "nls_tile.h"
+
+namespace lb {
+
+constexpr int NS_MAX_STEPS = 64;
+constexpr int NS_PARTS = 256;  // partial sums of squares a matrix
+
+struct NsScales {  // one per matrix
+  double inv;      // 1 / (|G|_F + eps); NaN when the norm is not finite: the whole result is then NaN
+  int ex[NS_MAX_STEPS + 1], ea[NS_MAX_STEPS], eb[NS_MAX_STEPS];  // X_t, A_t, B_t are held times 2^ex, 2^ea, 2^eb
+};
+struct NsCoef {
+  double a[NS_MAX_STEPS], b[NS_MAX_STEPS], c[NS_MAX_STEPS];
+};
+
+// A matrix of fp16 pairs: granules of 32 elements, 64 bytes hi then 64 bytes lo; rows padded with zeros to 64 elements.
+__host__ __device__ inline size_t pair_ld(long k) { return (size_t)((k + 63) / 64 * 64) * 4; }
+__device__ __forceinline__ size_t pair_at(size_t row, size_t k, size_t ld) { return row * ld + (k >> 5) * 128 + (k & 31) * 2; }
+
+struct NsMatrix {
+  const void* g;
+  long p, q;                       // p <= q
+  long row_stride, col_stride, batch_stride;  // in elements
+};
+
+template <class T>
+__global__ __launch_bounds__(256) void k_ns_norm(NsMatrix w, double* parts) {
+  const T* g = (const T*)w.g + blockIdx.y * w.batch_stride;
+  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
+  double s = 0.0;
+  // lanes along the direction whose neighbours are neighbours in memory
+  const bool along_q = w.col_stride <= w.row_stride;
+  const long outer = along_q ? w.p : w.q, inner = along_q ? w.q : w.p;
+  const long os = along_q ? w.row_stride : w.col_stride, is = along_q ? w.col_stride : w.row_stride;
+  for (long o = (long)blockIdx.x * 4 + y; o < outer; o += (long)gridDim.x * 4)
+    for (long i = x; i < inner; i += 64) {
+      const double v = (double)to_f32(g[o * os + i * is]);
+      s += v * v;
+    }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+  __shared__ double part[4];
+  if (x == 0) part[y] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) parts[(size_t)blockIdx.y * NS_PARTS + blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+__host__ __device__ inline double ns_peak_x(double a, double b, double c, double u) {  // max |a s + b s^3 + c s^5| on [0, u]
+  auto f = [&](double s) { return fabs(s * (a + s * s * (b + c * s * s))); };
+  double top = f(u);
+  const double d = 9.0 * b * b - 20.0 * a * c;
+  if (c != 0.0 && d >= 0.0) {
+    for (int k = -1; k <= 1; k += 2) {
+      const double z = (-3.0 * b + k * sqrt(d)) / (10.0 * c);
+      if (z > 0.0 && z < u * u) top = fmax(top, f(sqrt(z)));
+    }
+  } else if (c == 0.0 && b != 0.0) {
+    const double z = -a / (3.0 * b);
+    if (z > 0.0 && z < u * u) top = fmax(top, f(sqrt(z)));
+  }
+  return top;
+}
+__host__ __device__ inline double ns_peak_b(double b, double c, double u) {  // max |b z + c z^2| on [0, u^2]
+  auto f = [&](double z) { return fabs(z * (b + c * z)); };
+  double top = f(u * u);
+  if (c != 0.0) {
+    const double z = -b / (2.0 * c);
+    if (z > 0.0 && z < u * u) top = fmax(top, f(z));
+  }
+  return top;
+}
+// 15 - e with |v| < 2^e: what is bounded by v is held below 2^15 (fp16 ends at 65504: a factor of two for the roundings)
+__device__ __forceinline__ int ns_exponent(double v) {
+  if (!(v > 0.0) || !(v < 1e300)) return 0;
+  int e;
+  (void)frexp(v, &e);
+  return 15 - e;
+}
+
+__global__ __launch_bounds__(64) void k_ns_scales(const double* parts, int count, double eps, NsCoef cf, int steps, NsScales* out) {
+  double s = 0.0;
+  for (int i = threadIdx.x; i < count; i += 64) s += parts[(size_t)blockIdx.x * NS_PARTS + i];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+  if (threadIdx.x != 0) return;
+  NsScales& z = out[blockIdx.x];
+  const double norm = sqrt(s);
+  const bool fine = norm < 1e300;
+  z.inv = fine ? (norm + eps > 0.0 ? 1.0 / (norm + eps) : 0.0) : __longlong_as_double(0x7ff8000000000000ll);
+  double u = fine ? norm * z.inv * (1.0 + 1e-3) : 1.0;  // |X_0| <= |X_0|_F
+  for (int t = 0; t < steps; ++t) {
+    z.ex[t] = ns_exponent(u);
+    z.ea[t] = ns_exponent(u * u);
+    z.eb[t] = ns_exponent(ns_peak_b(cf.b[t], cf.c[t], u));
+    u = ns_peak_x(cf.a[t], cf.b[t], cf.c[t], u) * (1.0 + 1e-3);
+  }
+  z.ex[steps] = ns_exponent(u);
+}
+
+__device__ __forceinline__ void split(float v, _Float16* hi, _Float16* lo) {
+  *hi = (_Float16)v;
+  *lo = (_Float16)(v - (float)*hi);
+}
+
+// G -> X_0 (p rows) and its transpose (q rows), zero-padded.  One 64 x 64 tile a workgroup.
+template <class T>
+__global__ __launch_bounds__(256) void k_ns_pack(NsMatrix w, const NsScales* scales, char* x, char* xt, size_t batch_bytes) {
+  __shared__ float tile[64][65];
+  const T* g = (const T*)w.g + blockIdx.z * w.batch_stride;
+  x += blockIdx.z * batch_bytes;
+  xt += blockIdx.z * batch_bytes;
+  const NsScales& z = scales[blockIdx.z];
+  const double f = ldexp(z.inv, z.ex[0]);
+  const long p0 = (long)blockIdx.y * 64, q0 = (long)blockIdx.x * 64;
+  const bool along_q = w.col_stride <= w.row_stride;
+  const int l = threadIdx.x & 63, r = threadIdx.x >> 6;
+  for (int o = r; o < 64; o += 4) {
+    const int pi = along_q ? o : l, qi = along_q ? l : o;
+    float v = 0.0f;
+    if (p0 + pi < w.p && q0 + qi < w.q) v = (float)((double)to_f32(g[(p0 + pi) * w.row_stride + (q0 + qi) * w.col_stride]) * f);
+    tile[pi][qi] = v;
+  }
+  __syncthreads();
+  const size_t ldx = pair_ld(w.q), ldt = pair_ld(w.p);
+  const int row = threadIdx.x >> 2, part = (threadIdx.x & 3) * 16;
+  for (int turn = 0; turn < 2; ++turn) {
+    char* base = turn ? xt + pair_at(q0 + row, p0 + part, ldt) : x + pair_at(p0 + row, q0 + part, ldx);
+    if (turn ? q0 + row >= w.q : p0 + row >= w.p) continue;
+    f16x8 hi[2], lo[2];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      _Float16 h, o;
+      split(turn ? tile[part + e][row] : tile[row][part + e], &h, &o);
+      hi[e >> 3][e & 7] = h;
+      lo[e >> 3][e & 7] = o;
+    }
+    *(f16x8*)base = hi[0];
+    *(f16x8*)(base + 16) = hi[1];
+    *(f16x8*)(base + 64) = lo[0];
+    *(f16x8*)(base + 80) = lo[1];
+  }
+}
+
+enum NsKind { NS_GRAM, NS_POLY, NS_STEP, NS_LAST };
+
+struct NsArgs {
+  const char *P, *Q;      // operands of the product (pairs)
+  const char* E;          // the matrix the epilogue adds, natural orientation (POLY: A, STEP / LAST: X)
+  char *D, *DT;           // result and its transpose (pairs); symmetric products write both halves of D
+  void* out;              // LAST: the caller's matrix
+  const NsScales* scales;
+  size_t batch_bytes;     // from a matrix of the batch to the next, workspace
+  size_t out_stride;      // elements, out
+  int I, J, K;
+  int ti, tj, strip;
+  int t;                  // step
+  float a, b, c;
+  int transposed;         // LAST: out is stored q x p
+};
+
+// One 32 x 32 block, value(i, j) in the accumulator's places, to row-major pairs with rows i (the transposed orientation), through the wave's own LDS.
+__device__ __forceinline__ void block_turn(const f32x16& v, float* scratch, float* line) {
+  const int l = (int)(threadIdx.x & 63);
+#pragma unroll
+  for (int r = 0; r < 16; ++r) scratch[(8 * (r >> 2) + 4 * (l >> 5) + (r & 3)) * 33 + (l & 31)] = v[r];
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int e = 0; e < 16; ++e) line[e] = scratch[(l >> 1) * 33 + (l & 1) * 16 + e];
+  __builtin_amdgcn_wave_barrier();
+}
+
+template <int KIND, class T, int MODE, int BI, int BJ, int WI, int WJ>
+__global__ __launch_bounds__(64 * WI * WJ) void k_ns_product(NsArgs g) {
+  using TL = Tile<MODE, BI, BJ, WI, WJ>;
+  extern __shared__ char lds[];
+  constexpr bool SYM = KIND == NS_GRAM || KIND == NS_POLY;
+  int bi, bj;
+  if (SYM) {  // tiles bj <= bi, row by row
+    const int t = die_order(blockIdx.x, g.ti * (g.ti + 1) / 2);
+    bi = (int)((sqrtf(8.0f * t + 1.0f) - 1.0f) * 0.5f);
+    while ((bi + 1) * (bi + 2) / 2 <= t) ++bi;
+    while (bi * (bi + 1) / 2 > t) --bi;
+    bj = t - bi * (bi + 1) / 2;
+  } else {
+    strip_order(die_order(blockIdx.x, g.ti * g.tj), g.ti, g.tj, g.strip, &bi, &bj);
+  }
+  const int i0 = bi * BI, j0 = bj * BJ;
+  const size_t off = blockIdx.z * g.batch_bytes;
+  const size_t ldk = pair_ld(g.K), ldi = pair_ld(g.I), ldj = pair_ld(g.J);
+  TL t;
+  const int per = MODE == MODE_F16 ? 64 : 32;
+  t.run(Operand{g.P + off, (unsigned)ldk, g.I}, i0, Operand{g.Q + off, (unsigned)ldk, g.J}, j0, 0, (g.K + per - 1) / per, 128, lds);
+  const NsScales& z = g.scales[blockIdx.z];
+  const int ex = z.ex[g.t], ea = z.ea[g.t], eb = z.eb[g.t], en = z.ex[g.t + 1];
+  const char* E = g.E + off;
+  char* D = g.D + off;
+  char* DT = g.DT + off;
+  T* out = (T*)g.out + blockIdx.z * g.out_stride;
+  __syncthreads();  // the tile's LDS becomes the waves' scratch
+  float* scratch = (float*)lds + TL::wave() * (32 * 33);
+  const int l = TL::lane();
+#pragma unroll
+  for (int b = 0; b < TL::MJ; ++b) {
+    const int j = j0 + TL::col_of(b);
+#pragma unroll
+    for (int a = 0; a < TL::MI; ++a) {
+      f32x16 v = t.acc[a][b];
+      const int ib = i0 + TL::row_of(a);  // + 8 (r / 4) + r % 4
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int i = ib + 2 * r;
+        float e[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (KIND != NS_GRAM && j < g.J && i < g.I) {  // (rows of E are padded: whole groups of four)
+          const char* at = E + pair_at(j, i, ldi);
+          const f16x4 h = *(const f16x4*)at, o = *(const f16x4*)(at + 64);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) e[k] = (float)h[k] + (float)o[k];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float w = v[r + k];
+          if (KIND == NS_GRAM) w = ldexpf(w, ea - 2 * ex);
+          if (KIND == NS_POLY) w = ldexpf(g.b * e[k], eb - ea) + ldexpf(g.c * w, eb - 2 * ea);
+          if (KIND == NS_STEP) w = ldexpf(g.a * e[k], en - ex) + ldexpf(w, en - eb - ex);
+          if (KIND == NS_LAST) w = ldexpf(g.a * e[k] + ldexpf(w, -eb), -ex);
+          v[r + k] = (i + k < g.I && j < g.J) ? w : 0.0f;
+        }
+        if (KIND != NS_LAST) {
+          if (j < g.J && (size_t)i * 4 < ldi) {
+            f16x4 h, o;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              _Float16 hk, ok;
+              split(v[r + k], &hk, &ok);
+              h[k] = hk;
+              o[k] = ok;
+            }
+            char* at = D + pair_at(j, i, ldi);
+            *(f16x4*)at = h;
+            *(f16x4*)(at + 64) = o;
+          }
+        } else if (!g.transposed && j < g.J) {
+          if (g.I % 4 == 0 && i < g.I) {
+            typename Vec4<T>::type y;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) y[k] = (T)v[r + k];
+            *(typename Vec4<T>::type*)(out + (size_t)j * g.I + i) = y;
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (i + k < g.I) out[(size_t)j * g.I + i + k] = (T)v[r + k];
+          }
+        }
+      }
+      const bool turn = KIND == NS_LAST ? g.transposed != 0 : SYM ? bi != bj : true;
+      if (turn) {
+        float line[16];
+        block_turn(v, scratch, line);
+        const int i = i0 + (TL::wave() / WJ * TL::MI + a) * 32 + (l >> 1);
+        const int jb = j0 + (TL::wave() % WJ * TL::MJ + b) * 32 + (l & 1) * 16;
+        if (KIND == NS_LAST) {
+          if (i < g.I) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+              if (jb + k < g.J) out[(size_t)i * g.J + jb + k] = (T)line[k];
+          }
+        } else if (i < g.I && (size_t)jb * 4 < ldj) {
+          f16x8 hi[2], lo[2];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            _Float16 h, o;
+            split(line[k], &h, &o);
+            hi[k >> 3][k & 7] = h;
+            lo[k >> 3][k & 7] = o;
+          }
+          char* at = (SYM ? D : DT) + pair_at(i, jb, ldj);
+          *(f16x8*)at = hi[0];
+          *(f16x8*)(at + 16) = hi[1];
+          *(f16x8*)(at + 64) = lo[0];
+          *(f16x8*)(at + 80) = lo[1];
+        }
+      }
+    }
+  }
+}
+
+}  // namespace lb

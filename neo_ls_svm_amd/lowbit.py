@@ -1,0 +1,400 @@
+"""Matrix operators of few bits: 8-bit rows and their products, and orthogonalisation by Newton-Schulz products.
+
+They stand next to the 64-bit matrix calls of ``hotpath`` (``gram``, ``rotate``, ``eigh``, ``cholesky``) and take float32, float16 and bfloat16
+matrices.  (The reference computes in 64 bits throughout: it has no counterpart.)  Three kinds of arrays go in, and the same kind comes out:
+
+* tensors of a tensor library that the caller has imported (torch on the GPU): the call is put on the tensor's device's current stream and does not
+  wait; it can be captured into a graph.  Nothing is imported here for it.  The operators are not differentiated: a tensor that asks for gradients is
+  refused while gradients are recorded.
+* ``DeviceArray``: the context's own stream; the call returns when the result is there.
+* NumPy arrays: copied to the GPU and back.
+
+Wrong shapes, types and devices raise ``ValueError`` before anything is launched.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+import math
+import sys
+
+import numpy as np
+
+from ._lib import Context, DeviceArray, default_context
+
+__all__ = ["NEWTON_SCHULZ", "quantize_rows", "int8_matmul", "int8_linear", "orthogonalize"]
+
+#: (a, b, c) of X <- a X + (b A + c A A) X: odd polynomial of degree five that takes singular values in (0, 1] to about 0.7 .. 1.2 in five steps
+#: (slope 3.44 at zero).  A step with (1.5, -0.5, 0) or (1.875, -1.25, 0.375) afterwards takes them on towards 1.
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
+
+MAX_K = 131071  # NLS_INT8_MAX_K
+_A_PADDED, _B_PADDED = 1, 2
+_TYPES = {"float32": 0, "float16": 1, "bfloat16": 2}
+_NAMES = tuple(_TYPES)
+
+
+def _name(dtype) -> str:
+    """The plain name of a dtype given as text, as NumPy's or as a tensor library's."""
+    text = str(dtype)
+    if text.startswith("torch."):
+        return text[6:]
+    try:
+        return np.dtype(dtype).name
+    except TypeError:
+        return text
+
+
+def _float_type(dtype, what) -> int:
+    code = _TYPES.get(_name(dtype))
+    if code is None:
+        raise ValueError(f"{what} is {_name(dtype)}; the operators of few bits take {', '.join(_NAMES)}")
+    return code
+
+
+def _up16(k: int) -> int:
+    return -(-k // 16) * 16
+
+
+class _Tensors:
+    """Tensors of an imported tensor library, on their device's current stream."""
+
+    def __init__(self, lib, first, ctx):
+        self.lib, self.ctx = lib, ctx
+        if not first.is_cuda:
+            raise ValueError("tensors must be on the GPU (host data: NumPy arrays)")
+        self.device = first.device
+        if ctx is not None and ctx.device != self.device.index:
+            raise ValueError(f"tensors are on GPU {self.device.index}, the context on GPU {ctx.device}")
+
+    def begin(self):
+        index = self.device.index
+        if self.ctx is None:
+            with self.lib.cuda.device(index):  # (the first use of a device creates its context, which makes that device the current one)
+                self.ctx = default_context(index)
+        self.stream = self.lib.cuda.current_stream(self.device).cuda_stream
+        return self.ctx.lib
+
+    def take(self, x, what):
+        if not isinstance(x, self.lib.Tensor):
+            raise ValueError(f"{what} must be a tensor like the other arguments, not {type(x).__name__}")
+        if x.device != self.device:
+            raise ValueError(f"{what} is on {x.device}, the other arguments on {self.device}")
+        if x.layout is not self.lib.strided:
+            raise ValueError(f"{what} must be a dense tensor")
+        if x.requires_grad and self.lib.is_grad_enabled():
+            raise ValueError(f"{what} asks for gradients, which this operator does not give: detach it, or call under no_grad")
+        return x.resolve_neg() if x.is_neg() else x
+
+    @staticmethod
+    def name(x):
+        return str(x.dtype)[6:]
+
+    @staticmethod
+    def ptr(x):
+        return x.data_ptr()
+
+    @staticmethod
+    def strides(x):
+        return x.stride()
+
+    @staticmethod
+    def dense(x):
+        return x.contiguous()
+
+    @staticmethod
+    def room(x):
+        """Bytes of the tensor's memory from its first element on."""
+        return x.untyped_storage().nbytes() - x.storage_offset() * x.element_size()
+
+    def empty(self, shape, name):
+        return self.lib.empty(shape, dtype=getattr(self.lib, name), device=self.device)
+
+    def rows(self, rows, k, ld, lead):
+        held = self.lib.empty((rows, ld), dtype=self.lib.int8, device=self.device)
+        return held, held.view(*lead, ld)[..., :k]
+
+    def scratch(self, nbytes):
+        return self.lib.empty(nbytes, dtype=self.lib.uint8, device=self.device)
+
+    def done(self, result):
+        return result
+
+
+class _Arrays:
+    """NumPy arrays and DeviceArrays, on the context's own stream; results come back as what went in."""
+
+    def __init__(self, first, ctx):
+        self.host = isinstance(first, np.ndarray)
+        self.ctx = first.ctx if ctx is None and not self.host else ctx
+        self._keep = []  # device copies and scratch live until the stream has been waited for
+
+    def begin(self):
+        if self.ctx is None:
+            self.ctx = default_context()
+        stream = C.c_void_p()
+        self.ctx._check(self.ctx.lib.nls_ctx_stream(self.ctx.handle, C.byref(stream)))
+        self.stream = stream.value
+        return self.ctx.lib
+
+    def take(self, x, what):
+        if self.host != isinstance(x, np.ndarray) or not isinstance(x, (np.ndarray, DeviceArray)):
+            raise ValueError(f"{what} must be an array like the other arguments, not {type(x).__name__}")
+        if not self.host and x.ctx.device != self.ctx.device:
+            raise ValueError(f"{what} is on GPU {x.ctx.device}, the context on GPU {self.ctx.device}")
+        return x
+
+    @staticmethod
+    def name(x):
+        return x.dtype.name
+
+    def ptr(self, x):
+        if isinstance(x, DeviceArray):
+            return x.ptr
+        d = self.ctx.to_device(x, dtype=x.dtype)
+        self._keep.append(d)
+        return d.ptr
+
+    @staticmethod
+    def strides(x):  # (what ptr() uploads has no gaps)
+        out, step = [], 1
+        for s in reversed(x.shape):
+            out.append(step)
+            step *= s
+        return tuple(reversed(out))
+
+    @staticmethod
+    def dense(x):
+        return x
+
+    @staticmethod
+    def room(x):
+        return x.nbytes
+
+    def empty(self, shape, name):
+        return DeviceArray(self.ctx, shape, dtype=name)
+
+    def rows(self, rows, k, ld, lead):
+        held = DeviceArray(self.ctx, (rows, ld), dtype="int8")
+        return held, _Rows(held, k, lead)
+
+    def scratch(self, nbytes):
+        d = DeviceArray(self.ctx, (nbytes,), dtype="int8")
+        self._keep.append(d)
+        return d
+
+    def done(self, result):
+        self.ctx.synchronize()
+        for d in self._keep:
+            d.free()
+        many = isinstance(result, tuple)
+        out = []
+        for r in result if many else (result,):
+            if isinstance(r, _Rows):
+                r = r.host() if self.host else r.device(self.ctx)
+            elif self.host:
+                d, r = r, r.to_host()
+                d.free()
+            out.append(r)
+        return tuple(out) if many else out[0]
+
+
+class _Rows:
+    """8-bit rows as the kernel writes them (padded to 16 bytes), on their way to the caller's shape."""
+
+    def __init__(self, held, k, lead):
+        self.held, self.k, self.shape = held, k, (*lead, k)
+
+    def host(self):
+        a = self.held.to_host()[:, : self.k].reshape(self.shape)
+        self.held.free()
+        return np.ascontiguousarray(a)
+
+    def device(self, ctx):
+        if self.held.shape[1] == self.k:
+            self.held.shape = self.shape
+            return self.held
+        return ctx.to_device(self.host(), dtype="int8")
+
+
+def _space(first, ctx):
+    lib = sys.modules.get("torch")
+    if lib is not None and isinstance(first, lib.Tensor):
+        return _Tensors(lib, first, ctx)
+    if isinstance(first, (np.ndarray, DeviceArray)):
+        return _Arrays(first, ctx)
+    raise ValueError(f"expected a tensor on the GPU, a DeviceArray or a NumPy array, not {type(first).__name__}")
+
+
+def _call(ctx: Context, fn, *args):
+    with ctx.lock:  # the message of a failure belongs to the call that failed
+        ctx._check(fn(ctx.handle, *args))
+
+
+def _float_rows(sp, x, what):
+    """(x as a matrix, leading shape, rows, k, row stride, column stride, type)"""
+    x = sp.take(x, what)
+    shape = tuple(x.shape)
+    if len(shape) < 1:
+        raise ValueError(f"{what} must have at least one axis")
+    kind = _float_type(sp.name(x), what)
+    k, lead = shape[-1], shape[:-1]
+    if k < 1:
+        raise ValueError(f"{what} has rows of no elements")
+    rows = int(np.prod(lead)) if lead else 1
+    if len(shape) != 2:
+        if isinstance(x, DeviceArray):
+            rs, cs = k, 1
+        else:
+            x = x.reshape(rows, k)
+            rs, cs = sp.strides(x)
+    else:
+        rs, cs = sp.strides(x)
+    return x, lead, rows, k, rs, cs, kind
+
+
+def _int8_rows(sp, x, what, scale, scale_what):
+    """(matrix, its scales, leading shape, rows, k, row stride, whether each row may be read up to a multiple of 16 bytes)"""
+    x, scale = sp.take(x, what), sp.take(scale, scale_what)
+    shape = tuple(x.shape)
+    if len(shape) < 1 or sp.name(x) != "int8":
+        raise ValueError(f"{what} must be a matrix of int8")
+    k, lead = shape[-1], shape[:-1]
+    if not 1 <= k <= MAX_K:
+        raise ValueError(f"{what} has rows of {k} elements; 1 to {MAX_K} products are summed in 32 bits without overflow")
+    if tuple(scale.shape) != lead or sp.name(scale) != "float32":
+        raise ValueError(f"{scale_what} must be float32 of shape {lead}, not {sp.name(scale)} of shape {tuple(scale.shape)}")
+    rows = int(np.prod(lead)) if lead else 1
+    if not isinstance(x, DeviceArray) and len(shape) != 2:
+        x = x.reshape(rows, k)
+    st = (k, 1) if isinstance(x, DeviceArray) else sp.strides(x)
+    if (k > 1 and st[1] != 1) or (rows > 1 and st[0] < k):  # columns apart, or rows that share memory
+        x = sp.dense(x)
+        st = sp.strides(x)
+    ld = max(st[0], k) if rows > 1 else max(_up16(k), k) if sp.room(x) >= _up16(k) else k
+    padded = ld >= _up16(k) and sp.room(x) >= (rows - 1) * ld + _up16(k)
+    return x, sp.dense(scale), lead, rows, k, ld, padded
+
+
+def _bias(sp, bias, n, kind):
+    if bias is None:
+        return None, 0
+    bias = sp.take(bias, "bias")
+    code = _float_type(sp.name(bias), "bias")
+    if tuple(bias.shape) != (n,) or code not in (0, kind):
+        raise ValueError(f"bias must have shape ({n},) and be float32 or of the result's type, not {sp.name(bias)} of shape {tuple(bias.shape)}")
+    return sp.dense(bias), code
+
+
+def quantize_rows(x, ctx: Context | None = None):
+    """(q, scale): the rows of ``x`` (its last axis) as 8-bit integers with one scale a row, ``x ~ scale[..., None] * q``.
+
+    ``scale = max|x| / 127`` and ``q = 127 x / max|x|`` to the nearest integer, ties to even, decided as in exact arithmetic.  A row of zeros has
+    scale 0; a row with a NaN or an infinity has that for its scale and zeros in ``q``.  The rows of a ``q`` on the GPU start at multiples of 16
+    bytes (its last axis is dense, its rows may have gaps): that is how ``int8_matmul`` and ``int8_linear`` read them without a copy."""
+    sp = _space(x, ctx)
+    x, lead, rows, k, rs, cs, kind = _float_rows(sp, x, "x")
+    lib = sp.begin()
+    ld = _up16(k)
+    held, q = sp.rows(rows, k, ld, lead)
+    scale = sp.empty(lead, "float32")
+    if rows:
+        _call(sp.ctx, lib.nls_quantize_rows, sp.ptr(x), kind, rows, k, rs, cs, sp.ptr(held), ld, sp.ptr(scale), sp.stream)
+    return sp.done((q, scale))
+
+
+def int8_matmul(a, a_scale, b, b_scale, bias=None, dtype="float32", ctx: Context | None = None):
+    """``y[..., j] = a_scale[...] * b_scale[j] * sum_k a[..., k] b[j, k] (+ bias[j])`` of ``dtype``.
+
+    ``a`` (..., k) and ``b`` (n, k) int8, ``a_scale`` (...) and ``b_scale`` (n) float32, ``bias`` (n) float32 or of ``dtype``.  The sum is exact
+    (k <= 131071), the rest is float32, rounded once.  Rows that do not start at multiples of 16 bytes are copied first; ``quantize_rows`` lays them
+    out so that they do."""
+    sp = _space(a, ctx)
+    kind = _float_type(dtype, "dtype")
+    if kind == 2 and isinstance(sp, _Arrays):
+        raise ValueError("dtype: NumPy arrays and DeviceArrays have no bfloat16")
+    a, a_scale, lead, m, k, lda, apad = _int8_rows(sp, a, "a", a_scale, "a_scale")
+    b, b_scale, blead, n, kb, ldb, bpad = _int8_rows(sp, b, "b", b_scale, "b_scale")
+    if len(blead) != 1 or kb != k:
+        raise ValueError(f"b must be a matrix with rows of {k} elements, not of shape {(*blead, kb)}")
+    bias, bias_kind = _bias(sp, bias, n, kind)
+    lib = sp.begin()
+    y = sp.empty((*lead, n), _NAMES[kind])
+    if m and n:
+        need = C.c_size_t()
+        lib.nls_int8_matmul_workspace(m, n, k, C.byref(need))
+        ws = sp.scratch(need.value)
+        _call(
+            sp.ctx, lib.nls_int8_matmul, sp.ptr(a), lda, sp.ptr(a_scale), sp.ptr(b), ldb, sp.ptr(b_scale), None if bias is None else sp.ptr(bias),
+            bias_kind, m, n, k, sp.ptr(y), kind, (_A_PADDED if apad else 0) | (_B_PADDED if bpad else 0), sp.ptr(ws), need.value, sp.stream,
+        )  # fmt: skip
+    return sp.done(y)
+
+
+def int8_linear(x, b, b_scale, bias=None, ctx: Context | None = None):
+    """``int8_matmul(*quantize_rows(x), b, b_scale, bias, dtype=x.dtype)`` in one call: ``x`` (..., k) in 16 or 32 bits against rows held in 8."""
+    sp = _space(x, ctx)
+    x, lead, m, k, rs, cs, kind = _float_rows(sp, x, "x")
+    b, b_scale, blead, n, kb, ldb, bpad = _int8_rows(sp, b, "b", b_scale, "b_scale")
+    if len(blead) != 1 or kb != k:
+        raise ValueError(f"b must be a matrix with rows of {k} elements, not of shape {(*blead, kb)}")
+    bias, bias_kind = _bias(sp, bias, n, kind)
+    lib = sp.begin()
+    y = sp.empty((*lead, n), _NAMES[kind])
+    if m and n:
+        need = C.c_size_t()
+        lib.nls_int8_linear_workspace(m, n, k, C.byref(need))
+        ws = sp.scratch(need.value)
+        _call(
+            sp.ctx, lib.nls_int8_linear, sp.ptr(x), kind, rs, cs, sp.ptr(b), ldb, sp.ptr(b_scale), None if bias is None else sp.ptr(bias), bias_kind,
+            m, n, k, sp.ptr(y), _B_PADDED if bpad else 0, sp.ptr(ws), need.value, sp.stream,
+        )  # fmt: skip
+    return sp.done(y)
+
+
+def orthogonalize(g, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: float = 1e-7, ctx: Context | None = None):
+    """Newton-Schulz orthogonalisation of a matrix, or of every matrix of a batch (the last two axes), in the type it comes in.
+
+    ``X = G / (|G|_F + eps)``, then ``steps`` times ``X <- a X + (b A + c A A) X`` with ``A = X X^T`` taken on the shorter side.  ``coefficients``: one
+    (a, b, c) for all steps or one for each.  Every singular value s of X goes through the polynomials a s + b s^3 + c s^5 while the singular vectors
+    stay: with coefficients that lead to 1 the result is the orthogonal factor of the polar decomposition (what a QR of a Gaussian matrix gives
+    ``orf_frequencies`` up to rotation of the draw), with the default ones the near-orthogonal update of a training step.
+
+    Products and sums carry 22 bits or more; for a 16-bit ``g`` the early steps carry 11, which stays below the rounding of the result."""
+    sp = _space(g, ctx)
+    g = sp.take(g, "g")
+    shape = tuple(g.shape)
+    if len(shape) < 2:
+        raise ValueError("g must be a matrix or a batch of matrices")
+    kind = _float_type(sp.name(g), "g")
+    if isinstance(steps, bool) or int(steps) != steps or not 1 <= steps <= 64:
+        raise ValueError("steps must be a whole number from 1 to 64")
+    steps = int(steps)
+    try:
+        rows = [tuple(float(v) for v in row) for row in coefficients] if hasattr(coefficients[0], "__len__") else [tuple(float(v) for v in coefficients)] * steps
+    except (TypeError, ValueError, IndexError):
+        rows = []
+    if len(rows) != steps or any(len(row) != 3 or not all(math.isfinite(v) for v in row) for row in rows):
+        raise ValueError(f"coefficients must be three finite numbers, or three for each of the {steps} steps")
+    eps = float(eps)
+    if not 0.0 <= eps < 1e30:
+        raise ValueError("eps must be a number >= 0")
+    table = (C.c_double * (3 * steps))(*(v for row in rows for v in row))
+    m, n = shape[-2:]
+    batch = int(np.prod(shape[:-2])) if len(shape) > 2 else 1
+    if isinstance(g, DeviceArray):
+        st = (m * n, n, 1)
+    else:
+        if len(shape) != 3:
+            g = g.reshape(batch, m, n)
+        st = sp.strides(g)
+    lib = sp.begin()
+    out = sp.empty(shape, _NAMES[kind])
+    need = C.c_size_t()
+    lib.nls_orthogonalize_workspace(batch, m, n, C.byref(need))
+    ws = sp.scratch(need.value) if batch and m and n else None
+    _call(
+        sp.ctx, lib.nls_orthogonalize, sp.ptr(g) if ws is not None else None, kind, batch, m, n, *st, table, steps, eps, sp.ptr(out),
+        None if ws is None else sp.ptr(ws), need.value if ws is not None else 0, sp.stream,
+    )  # fmt: skip
+    return sp.done(out)

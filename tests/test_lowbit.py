@@ -1,0 +1,81 @@
+"""CPU checks of the few-bit matrix operators: refusals before anything reaches a GPU, and the arithmetic the kernels rely on."""
+
+from __future__ import annotations
+
+from fractions import Fraction
+
+import numpy as np
+import pytest
+
+import neo_ls_svm_amd as nls
+
+X = np.ones((3, 32), dtype=np.float32)
+Q = np.ones((3, 32), dtype=np.int8)
+S = np.ones(3, dtype=np.float32)
+
+
+@pytest.mark.parametrize(
+    "call",
+    [
+        lambda: nls.quantize_rows(X.astype(np.float64)),
+        lambda: nls.quantize_rows(X.astype(np.int32)),
+        lambda: nls.quantize_rows(np.float32(1.0)),
+        lambda: nls.quantize_rows([[1.0, 2.0]]),
+        lambda: nls.quantize_rows(np.empty((3, 0), dtype=np.float32)),
+        lambda: nls.int8_matmul(X, S, Q, S),
+        lambda: nls.int8_matmul(Q, S, Q.astype(np.uint8), S),
+        lambda: nls.int8_matmul(Q, S, Q[:, :16], S),
+        lambda: nls.int8_matmul(Q, S[:2], Q, S),
+        lambda: nls.int8_matmul(Q, S, Q, S[:2]),
+        lambda: nls.int8_matmul(Q, S.astype(np.float64), Q, S),
+        lambda: nls.int8_matmul(Q, S, Q[None], S[None]),
+        lambda: nls.int8_matmul(Q, S, Q, S, bias=S[:2]),
+        lambda: nls.int8_matmul(Q, S, Q, S, bias=S.astype(np.float16)),
+        lambda: nls.int8_matmul(Q, S, Q, S, dtype="float64"),
+        lambda: nls.int8_matmul(Q, S, Q, S, dtype="bfloat16"),
+        lambda: nls.int8_matmul(Q, S, Q, S, dtype="nonsense"),
+        lambda: nls.int8_matmul(np.ones((1, 131072), np.int8), S[:1], np.ones((1, 131072), np.int8), S[:1]),
+        lambda: nls.int8_matmul(np.ones((1, 0), np.int8), S[:1], np.ones((1, 0), np.int8), S[:1]),
+        lambda: nls.int8_linear(X, Q[:, :16], S),
+        lambda: nls.int8_linear(X.astype(np.float64), Q, S),
+        lambda: nls.int8_linear(X, Q, S, bias=X),
+        lambda: nls.orthogonalize(X.astype(np.float64)),
+        lambda: nls.orthogonalize(X[0]),
+        lambda: nls.orthogonalize(X, steps=0),
+        lambda: nls.orthogonalize(X, steps=65),
+        lambda: nls.orthogonalize(X, steps=2.5),
+        lambda: nls.orthogonalize(X, steps=3, coefficients=[(1.5, -0.5, 0.0)] * 2),
+        lambda: nls.orthogonalize(X, coefficients=(1.5, -0.5)),
+        lambda: nls.orthogonalize(X, coefficients=(float("nan"), 0.0, 0.0)),
+        lambda: nls.orthogonalize(X, eps=-1.0),
+        lambda: nls.orthogonalize(X, eps=float("nan")),
+    ],
+)
+def test_refused_before_any_gpu_is_asked_for(call):
+    with pytest.raises(ValueError):
+        call()
+
+
+def test_host_tensors_and_mixed_arguments_are_refused():
+    torch = pytest.importorskip("torch")
+    with pytest.raises(ValueError, match="GPU"):
+        nls.quantize_rows(torch.ones(3, 32))
+    with pytest.raises(ValueError, match="like the other"):
+        nls.int8_matmul(Q, S, torch.ones(3, 32, dtype=torch.int8), S)
+
+
+def test_sixty_four_bits_decide_a_quotient_next_to_a_half():
+    """127 x / top of two float32 numbers: the 64-bit quotient rounds to the integer the exact one rounds to (the kernel's slow path), and the
+    32-bit product x * fl(127 / top) is never further from it than the kernel's window of 2e-5 around a half (its fast path)."""
+    rng = np.random.default_rng(0)
+    top = rng.uniform(1.0, 2.0, 4000).astype(np.float32)
+    j = rng.integers(-127, 127, 4000)
+    x = ((2 * j + 1).astype(np.float64) * top.astype(np.float64) / 254.0).astype(np.float32)  # as near to a half as float32 gets
+    x = np.concatenate([x, np.nextafter(x, np.float32(9)), np.float32([63.5, 0.5, 1.5, -2.5])])
+    top = np.concatenate([top, top, np.float32([127.0] * 4)])
+    wide = np.rint(x.astype(np.float64) * 127.0 / top.astype(np.float64))
+    fast = x * (np.float32(127.0) / top)
+    for xi, ti, wi, fi in zip(x, top, wide, fast):
+        r = Fraction(float(xi)) * 127 / Fraction(float(ti))
+        assert round(r) == int(wi)  # (Fraction rounds ties to even)
+        assert abs(Fraction(float(fi)) - r) < Fraction(2, 100000)
