@@ -440,7 +440,8 @@ int nls_dual_predict(nls_ctx* ctx, const double* Xq, int64_t m, const double* Xt
  * and orthogonalisation by Newton-Schulz products, for float32, float16 and bfloat16 matrices.
  * Unlike the calls above these take DEVICE pointers only and do not block: the work is put on `stream` (a hipStream_t of the context's device; NULL is
  * HIP's default stream, nls_ctx_stream gives the context's own) and the arrays must stay valid until it has run.  Nothing is allocated, waited for or
- * kept: scratch memory is the caller's `workspace` (256-byte aligned, at least what the _workspace function says; two calls that may run at the same
+ * kept: scratch memory is the caller's `workspace` (256-byte aligned, at least what the _workspace function says for the same
+ * arguments, which may be nothing; two calls that may run at the same
  * time - other streams, graphs that are replayed side by side - need two).  Calls can be captured into a graph.  The caller's current device is left
  * as it was.  Results do not depend on timing: the same call gives the same bits.  Sizes of zero rows, columns or matrices are fine (nothing is
  * written); sums over nothing (k = 0) are refused. */
@@ -462,12 +463,12 @@ int nls_quantize_rows(nls_ctx* ctx, const void* x, int type, int64_t rows, int64
 #define NLS_INT8_MAX_K 131071
 #define NLS_INT8_A_PADDED 1
 #define NLS_INT8_B_PADDED 2
-int nls_int8_matmul_workspace(int64_t m, int64_t n, int64_t k, size_t* bytes);
+int nls_int8_matmul_workspace(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, int64_t m, int64_t n, int64_t k, int flags, size_t* bytes);
 int nls_int8_matmul(nls_ctx* ctx, const int8_t* a, int64_t lda, const float* a_scale, const int8_t* b, int64_t ldb, const float* b_scale,
                     const void* bias, int bias_type, int64_t m, int64_t n, int64_t k, void* y, int type, int flags, void* workspace,
                     size_t workspace_bytes, void* stream);
 /* The two calls above in one: x (m x k, `type`, any strides) is quantised row by row and multiplied; y is of `type` too. */
-int nls_int8_linear_workspace(int64_t m, int64_t n, int64_t k, size_t* bytes);
+int nls_int8_linear_workspace(const int8_t* b, int64_t ldb, int64_t m, int64_t n, int64_t k, int flags, size_t* bytes);
 int nls_int8_linear(nls_ctx* ctx, const void* x, int type, int64_t row_stride, int64_t col_stride, const int8_t* b, int64_t ldb, const float* b_scale,
                     const void* bias, int bias_type, int64_t m, int64_t n, int64_t k, void* y, int flags, void* workspace, size_t workspace_bytes,
                     void* stream);

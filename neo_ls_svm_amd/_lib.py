@@ -224,13 +224,16 @@ SIGNATURES = {
     ),
     "nls_ctx_stream": (C.c_int, [C.c_void_p, C.POINTER(C.c_void_p)]),
     "nls_quantize_rows": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int] + [C.c_int64] * 4 + [C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]),
-    "nls_int8_matmul_workspace": (C.c_int, [C.c_int64] * 3 + [C.POINTER(C.c_size_t)]),
+    "nls_int8_matmul_workspace": (
+        C.c_int,
+        [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64] + [C.c_int64] * 3 + [C.c_int, C.POINTER(C.c_size_t)],
+    ),
     "nls_int8_matmul": (
         C.c_int,
         [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int]
         + [C.c_int64] * 3 + [C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p],
     ),
-    "nls_int8_linear_workspace": (C.c_int, [C.c_int64] * 3 + [C.POINTER(C.c_size_t)]),
+    "nls_int8_linear_workspace": (C.c_int, [C.c_void_p, C.c_int64] + [C.c_int64] * 3 + [C.c_int, C.POINTER(C.c_size_t)]),
     "nls_int8_linear": (
         C.c_int,
         [C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int]

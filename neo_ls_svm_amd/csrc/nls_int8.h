@@ -42,23 +42,61 @@ __device__ __forceinline__ unsigned wave_max(unsigned v) {
   return v;
 }
 
-// A group of G threads takes a row; four neighbouring elements a thread and turn.  VEC: the row starts are aligned to four elements.
-template <class T, int G, bool VEC>
+// Elements a thread takes at once: 16 bytes where the rows are dense and their starts aligned to that, else four elements one by one.
+template <class T, bool VEC>
+struct Few {
+  static constexpr int N = VEC ? 16 / (int)sizeof(T) : 4;
+  typedef T type __attribute__((ext_vector_type(N)));
+};
+template <class T, bool VEC>
+__device__ __forceinline__ typename Few<T, VEC>::type few_at(const T* x, long c, long k, long col_stride) {
+  constexpr int N = Few<T, VEC>::N;
+  typename Few<T, VEC>::type v = {};
+  if (VEC && c + N <= k) {
+    v = *(const typename Few<T, VEC>::type*)(x + c);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (c + e < k) v[e] = x[(c + e) * col_stride];
+  }
+  return v;
+}
+template <int N, class V>
+__device__ __forceinline__ void quantise_store(const V& v, const RowScale& s, signed char* at) {
+  unsigned w[N / 4];
+#pragma unroll
+  for (int e = 0; e < N; e += 4) w[e / 4] = pack4(quantise(to_f32(v[e]), s), quantise(to_f32(v[e + 1]), s), quantise(to_f32(v[e + 2]), s), quantise(to_f32(v[e + 3]), s));
+  if constexpr (N == 8)
+    *(i32x2*)at = i32x2{(int)w[0], (int)w[1]};
+  else
+    *(unsigned*)at = w[0];
+}
+
+// A group of G threads takes a row.  HELD > 0: the row fits into HELD pieces a thread, is read once and stays in registers between the maximum and
+// the rounding; HELD = 0: longer rows are read twice (the second time mostly from L2).  Bound by memory: 8192 x 8192 bfloat16 (134 MB in, 67 MB out).
+template <class T, int G, bool VEC, int HELD>
 __global__ __launch_bounds__(256) void k_quantize_rows(const T* x, long rows, long k, long row_stride, long col_stride, signed char* q, long ldq,
                                                        float* scale) {
-  using V = typename Vec4<T>::type;
+  using F = Few<T, VEC>;
+  constexpr int N = F::N;
   const int g = threadIdx.x % G;
   const long row = (long)blockIdx.x * (256 / G) + threadIdx.x / G;
   const bool live = row < rows;
   const T* xr = x + (live ? row : rows - 1) * row_stride;
   unsigned top = 0;
-  for (long c = 4 * g; c < k; c += 4 * G) {
-    if (VEC && c + 4 <= k) {
-      const V v = *(const V*)(xr + c);
+  typename F::type held[HELD ? HELD : 1];
+  if constexpr (HELD > 0) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) top = max(top, magnitude(to_f32(v[e])));
-    } else {
-      for (int e = 0; e < 4 && c + e < k; ++e) top = max(top, magnitude(to_f32(xr[(c + e) * col_stride])));
+    for (int h = 0; h < HELD; ++h) held[h] = few_at<T, VEC>(xr, (long)N * (g + G * h), k, col_stride);
+#pragma unroll
+    for (int h = 0; h < HELD; ++h)
+#pragma unroll
+      for (int e = 0; e < N; ++e) top = max(top, magnitude(to_f32(held[h][e])));
+  } else {
+    for (long c = N * g; c < k; c += N * G) {
+      const typename F::type v = few_at<T, VEC>(xr, c, k, col_stride);
+#pragma unroll
+      for (int e = 0; e < N; ++e) top = max(top, magnitude(to_f32(v[e])));
     }
   }
   top = wave_max(top);
@@ -71,11 +109,16 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const T* x, long rows, lo
   if (!live) return;
   const RowScale s = row_scale(top);
   if (g == 0) scale[row] = s.top / 127.0f;
-  signed char* qr = q + row * ldq;
-  for (long c = 4 * g; c < ldq; c += 4 * G) {  // the row's padding is written as zeros
-    int v[4];
-    for (int e = 0; e < 4; ++e) v[e] = c + e < k ? quantise(to_f32(xr[(c + e) * col_stride]), s) : 0;
-    *(unsigned*)(qr + c) = pack4(v[0], v[1], v[2], v[3]);
+  signed char* qr = q + row * ldq;  // the row's padding is written as zeros (ldq is a multiple of N)
+  if constexpr (HELD > 0) {
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+      const long c = (long)N * (g + G * h);
+      if (c < ldq) quantise_store<N>(held[h], s, qr + c);
+    }
+    for (long c = (long)N * (g + G * HELD); c < ldq; c += N * G) quantise_store<N>(typename F::type{}, s, qr + c);
+  } else {
+    for (long c = N * g; c < ldq; c += N * G) quantise_store<N>(few_at<T, VEC>(xr, c, k, col_stride), s, qr + c);
   }
 }
 
@@ -142,6 +185,171 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_int8_tile(Int8Args g, int ti, 
             if (n + e < g.n) y[(size_t)m * g.n + n + e] = (T)scaled(t.acc[a][b][r + e], as, g.b_scale[n + e], bias_at<T>(g, n + e));
         }
       }
+  }
+}
+
+// ---- few rows ------------------------------------------------------------------------------------------------------------------------------
+// Up to 64 rows of a against all of b: bound by reading b once.  A workgroup takes 16 NG rows of b; its eight waves deal the K range out among
+// themselves in pairs of 64 bytes (a wave reads 128 bytes of 16 rows: whole lines) straight into the fragments of the 16 x 16 x 64 instruction,
+// U loads under way before the first is used, and add their sums up in LDS - integers, so the order does not matter.  No second launch, no scratch memory.
+// a comes from L2 for every workgroup: MG fragments for NG of b.
+// FUSED: a is not there yet - the workgroup quantises the rows of x into LDS itself while the first reads of b are under way (rows, k as the caller
+// allows them: see the host code).
+constexpr int FEW_U = 8;
+
+struct FewX {  // FUSED: the rows to quantise
+  const void* x;
+  long row_stride, col_stride;
+  int vec;
+};
+
+template <class TX>
+__device__ __forceinline__ void few_quantise(const Int8Args& g, const FewX& f, signed char* rows, long ld, float* scales, unsigned* parts) {
+  // all 512 threads share a row: piece of eight elements number threadIdx.x, + 512, ...
+  const int w = threadIdx.x >> 6;
+  for (int m = 0; m < g.m; ++m) {
+    const TX* x = (const TX*)f.x + m * f.row_stride;
+    unsigned top = 0;
+    for (int c = 8 * threadIdx.x; c < g.k; c += 8 * 512) {
+      typedef TX V __attribute__((ext_vector_type(8)));
+      V v = {};
+      if (f.vec && c + 8 <= g.k) {
+        v = *(const V*)(x + c);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c + e < g.k) v[e] = x[(c + e) * f.col_stride];
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = max(top, magnitude(to_f32(v[e])));
+    }
+    top = wave_max(top);
+    if ((threadIdx.x & 63) == 0) parts[m * 8 + w] = top;
+  }
+  __syncthreads();
+  for (int m = 0; m < g.m; ++m) {
+    unsigned top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, parts[m * 8 + i]);
+    const RowScale s = row_scale(top);
+    if (threadIdx.x == 0) scales[m] = s.top / 127.0f;
+    const TX* x = (const TX*)f.x + m * f.row_stride;
+    for (int c = 8 * threadIdx.x; c < ld - 16; c += 8 * 512) {
+      typedef TX V __attribute__((ext_vector_type(8)));
+      V v = {};
+      if (f.vec && c + 8 <= g.k) {
+        v = *(const V*)(x + c);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c + e < g.k) v[e] = x[(c + e) * f.col_stride];
+      }
+      quantise_store<8>(v, s, rows + m * ld + c);
+    }
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ i32x4 keep_bytes(i32x4 v, int n) {  // the first n of 16 bytes, the others zero
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const int b = n - 4 * w;
+    v[w] = b >= 4 ? v[w] : b <= 0 ? 0 : (v[w] & ((1 << (8 * b)) - 1));
+  }
+  return v;
+}
+
+template <class T, int MG, int NG, bool FUSED>
+__global__ __launch_bounds__(512) void k_int8_few(Int8Args g, FewX f) {
+  extern __shared__ char lds[];
+  const int l = (int)(threadIdx.x & 63), w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int row = l & 15, quarter = l >> 4;
+  const int n0 = blockIdx.x * 16 * NG;
+  const int blocks = (g.k + 63) / 64;
+  const char* pb[NG];
+#pragma unroll
+  for (int j = 0; j < NG; ++j) pb[j] = g.b.base + (size_t)min(n0 + 16 * j + row, g.n - 1) * g.b.ld + quarter * 16;
+  // FUSED: rows of the LDS copy are 64 bytes of every block and 16 more apart (the 16 rows of a fragment then start in different banks)
+  const long ldf = (long)blocks * 64 + 16;
+  signed char* rows = (signed char*)lds;
+  float* scales = (float*)(lds + (FUSED ? g.m * ldf : 0));
+  unsigned* parts = (unsigned*)(scales + 16);
+  const char* pa[MG];
+#pragma unroll
+  for (int i = 0; i < MG; ++i) {
+    const int m = min(16 * i + row, g.m - 1);
+    pa[i] = FUSED ? (const char*)rows + m * ldf + quarter * 16 : g.a.base + (size_t)m * g.a.ld + quarter * 16;
+  }
+  i32x4 acc[MG][NG];
+#pragma unroll
+  for (int i = 0; i < MG; ++i)
+#pragma unroll
+    for (int j = 0; j < NG; ++j) acc[i][j] = i32x4{};
+
+  // block u of round s: the wave's pairs are s * U / 2 + u / 2, dealt out over the waves
+  const int rounds = (blocks + 8 * FEW_U - 1) / (8 * FEW_U);
+  const int up = (g.k + 15) / 16 * 16;
+  auto block_of = [&](int s, int u) { return ((s * (FEW_U / 2) + u / 2) * 8 + w) * 2 + (u & 1); };
+  auto load_b = [&](int s, i32x4 (&v)[FEW_U][NG]) {
+#pragma unroll
+    for (int u = 0; u < FEW_U; ++u) {
+      const int b = block_of(s, u);
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        if (b * 64 + 64 <= g.k) {
+          v[u][j] = *(const i32x4*)(pb[j] + (size_t)b * 64);
+        } else {
+          v[u][j] = i32x4{};
+          const int c = b * 64 + quarter * 16;
+          if (c < up) v[u][j] = keep_bytes(*(const i32x4*)(pb[j] + (size_t)b * 64), g.k - c);
+        }
+      }
+    }
+  };
+  auto multiply = [&](int s, i32x4 (&v)[FEW_U][NG]) {
+#pragma unroll
+    for (int u = 0; u < FEW_U; ++u) {
+      const int b = block_of(s, u);
+      if (b < blocks) {
+        const bool there = FUSED || b * 64 + quarter * 16 < up;
+        i32x4 a[MG];
+#pragma unroll
+        for (int i = 0; i < MG; ++i) a[i] = *(const i32x4*)(pa[i] + (there ? (size_t)b * 64 : 0));  // (what stands in for a missing chunk meets zeros)
+#pragma unroll
+        for (int i = 0; i < MG; ++i)
+#pragma unroll
+          for (int j = 0; j < NG; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(v[u][j], a[i], acc[i][j], 0, 0, 0);
+      }
+    }
+  };
+  i32x4 v[FEW_U][NG];
+  load_b(0, v);
+  if constexpr (FUSED) few_quantise<T>(g, f, rows, ldf, scales, parts);
+  for (int s = 0;;) {
+    multiply(s, v);
+    if (++s == rounds) break;
+    load_b(s, v);
+  }
+
+  __syncthreads();  // (FUSED: the rows are read no more)
+  i32x4* red = (i32x4*)(lds + (FUSED ? (g.m * ldf + 64 + 512 + 255) / 256 * 256 : 0));
+#pragma unroll
+  for (int i = 0; i < MG; ++i)
+#pragma unroll
+    for (int j = 0; j < NG; ++j) red[(w * MG * NG + i * NG + j) * 64 + l] = acc[i][j];
+  __syncthreads();
+  T* y = (T*)g.y;
+  for (int t = threadIdx.x; t < MG * NG * 64; t += 512) {
+    i32x4 sum = red[t];
+#pragma unroll
+    for (int o = 1; o < 8; ++o) sum += red[o * MG * NG * 64 + t];
+    const int lane = t & 63, j = (t >> 6) % NG, i = (t >> 6) / NG;
+    const int m = 16 * i + (lane & 15), n = n0 + 16 * j + 4 * (lane >> 4);
+    if (m >= g.m) continue;
+    const float as = FUSED ? scales[m] : g.a_scale[m];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < g.n) y[(size_t)m * g.n + n + e] = (T)scaled(sum[e], as, g.b_scale[n + e], bias_at<T>(g, n + e));
   }
 }
 

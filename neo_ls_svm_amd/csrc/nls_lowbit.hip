@@ -43,19 +43,32 @@ int ask_lds(nls_ctx* ctx, F f, int bytes) {
 int type_size(int t) { return t == NLS_TYPE_F32 ? 4 : (t == NLS_TYPE_F16 || t == NLS_TYPE_BF16) ? 2 : 0; }
 
 // ---- quantise ----
-template <class T>
+// Short rows: a wave each; others: a workgroup.  The number of pieces a thread holds follows from the length; rows past 8 pieces are read twice.
+template <class T, bool VEC>
 int quantize(nls_ctx* ctx, const T* x, long rows, long k, long rs, long cs, signed char* q, long ldq, float* scale, hipStream_t st) {
-  const bool vec = cs == 1 && rs % 4 == 0 && (uintptr_t)x % (4 * sizeof(T)) == 0;
-  const bool narrow = k <= 512;
-  const dim3 grid((unsigned)(narrow ? (rows + 3) / 4 : rows));
-  if (vec)
-    narrow ? (void)(k_quantize_rows<T, 64, true><<<grid, 256, 0, st>>>(x, rows, k, rs, cs, q, ldq, scale))
-           : (void)(k_quantize_rows<T, 256, true><<<grid, 256, 0, st>>>(x, rows, k, rs, cs, q, ldq, scale));
+  constexpr long N = Few<T, VEC>::N;
+  const dim3 waves((unsigned)((rows + 3) / 4)), groups((unsigned)rows);
+#define QUANTIZE(G, HELD, GRID) k_quantize_rows<T, G, VEC, HELD><<<GRID, 256, 0, st>>>(x, rows, k, rs, cs, q, ldq, scale)
+  if (k <= 64 * N)
+    QUANTIZE(64, 1, waves);
+  else if (k <= 128 * N)
+    QUANTIZE(64, 2, waves);
+  else if (k <= 512 * N)
+    QUANTIZE(256, 2, groups);
+  else if (k <= 1024 * N)
+    QUANTIZE(256, 4, groups);
+  else if (k <= 2048 * N)
+    QUANTIZE(256, 8, groups);
   else
-    narrow ? (void)(k_quantize_rows<T, 64, false><<<grid, 256, 0, st>>>(x, rows, k, rs, cs, q, ldq, scale))
-           : (void)(k_quantize_rows<T, 256, false><<<grid, 256, 0, st>>>(x, rows, k, rs, cs, q, ldq, scale));
+    QUANTIZE(256, 0, groups);
+#undef QUANTIZE
   LAUNCHED(ctx, "quantize_rows");
   return NLS_OK;
+}
+template <class T>
+int quantize(nls_ctx* ctx, const T* x, long rows, long k, long rs, long cs, signed char* q, long ldq, float* scale, hipStream_t st) {
+  const bool vec = cs == 1 && (uintptr_t)x % 16 == 0 && (rows == 1 || rs * sizeof(T) % 16 == 0);
+  return vec ? quantize<T, true>(ctx, x, rows, k, rs, cs, q, ldq, scale, st) : quantize<T, false>(ctx, x, rows, k, rs, cs, q, ldq, scale, st);
 }
 int quantize_any(nls_ctx* ctx, const void* x, int type, long rows, long k, long rs, long cs, signed char* q, long ldq, float* scale, hipStream_t st) {
   switch (type) {
@@ -75,11 +88,35 @@ int int8_tile(nls_ctx* ctx, const Int8Args& g, hipStream_t st) {
   LAUNCHED(ctx, "int8_matmul");
   return NLS_OK;
 }
+template <class T, int MG, int NG, bool FUSED>
+int int8_few(nls_ctx* ctx, const Int8Args& g, const FewX& f, hipStream_t st) {
+  const size_t rows = FUSED ? ((size_t)g.m * ((g.k + 63) / 64 * 64 + 16) + 64 + 512 + 255) / 256 * 256 : 0;
+  const size_t lds = rows + (size_t)8 * MG * NG * 1024;
+  k_int8_few<T, MG, NG, FUSED><<<dim3((unsigned)((g.n + 16 * NG - 1) / (16 * NG))), 512, lds, st>>>(g, f);
+  LAUNCHED(ctx, "int8_matmul");
+  return NLS_OK;
+}
+// Two row groups of b a workgroup halve what is read of a; taken where that leaves a workgroup for every compute unit.
+template <class T, int MG>
+int int8_few(nls_ctx* ctx, const Int8Args& g, hipStream_t st) {
+  if (MG > 1 && (g.n + 31) / 32 >= ctx->cus) return int8_few<T, MG, 2, false>(ctx, g, FewX{}, st);
+  return int8_few<T, MG, 1, false>(ctx, g, FewX{}, st);
+}
 template <class T>
 int int8_product(nls_ctx* ctx, const Int8Args& g, hipStream_t st) {
+  if (g.m <= 16) return int8_few<T, 1>(ctx, g, st);
+  if (g.m <= 32) return int8_few<T, 2>(ctx, g, st);
+  if (g.m <= 48) return int8_few<T, 3>(ctx, g, st);
+  if (g.m <= 64) return int8_few<T, 4>(ctx, g, st);
   const long big = (long)((g.n + 127) / 128) * ((g.m + 127) / 128);
   if (big >= ctx->cus) return int8_tile<T, 128, 128, 2, 2>(ctx, g, st);
   return int8_tile<T, 64, 64, 2, 2>(ctx, g, st);
+}
+// Whether int8_linear quantises inside the product: every workgroup does all the rows of x over again, which has to stay small beside its share of b.
+bool int8_fused(long m, long k) { return m <= 4 && m * k <= 32768; }
+template <class T>
+int int8_fused_product(nls_ctx* ctx, const Int8Args& g, const FewX& f, hipStream_t st) {
+  return int8_few<T, 1, 1, true>(ctx, g, f, st);
 }
 int int8_product_any(nls_ctx* ctx, const Int8Args& g, int type, hipStream_t st) {
   switch (type) {
@@ -106,19 +143,17 @@ int check_int8(nls_ctx* ctx, const char* what, int64_t m, int64_t n, int64_t k, 
 }
 
 // a and b as the kernels take them: laid out again in the workspace where the caller's rows do not start at multiples of 16 bytes.
-int aligned_operand(nls_ctx* ctx, const int8_t* p, long rows, long k, long ld, bool ok, char** ws, char* end, Operand* out, hipStream_t st) {
-  if (ok) {
+int operand(nls_ctx* ctx, const int8_t* p, long rows, long k, long ld, bool ready, char** ws, Operand* out, hipStream_t st) {
+  if (ready) {
     *out = Operand{(const char*)p, (unsigned)ld, (int)rows};
     return NLS_OK;
   }
   const long ldy = up16(k);
-  const size_t need = up256((size_t)rows * ldy);
-  if ((size_t)(end - *ws) < need) return fail(ctx, NLS_ERR_ARG, "int8_matmul: workspace too small (nls_int8_matmul_workspace)");
   const long work = rows * (ldy / 4);
   k_align_rows<<<dim3((unsigned)std::min<long>((work + 255) / 256, 65536)), 256, 0, st>>>((const signed char*)p, rows, k, ld, (signed char*)*ws, ldy);
   LAUNCHED(ctx, "int8_matmul (alignment)");
   *out = Operand{*ws, (unsigned)ldy, (int)rows};
-  *ws += need;
+  *ws += up256((size_t)rows * ldy);
   return NLS_OK;
 }
 
@@ -236,9 +271,11 @@ extern "C" int nls_quantize_rows(nls_ctx* ctx, const void* x, int type, int64_t 
   return quantize_any(ctx, x, type, rows, k, row_stride, col_stride, (signed char*)q, ldq, scale, (hipStream_t)stream);
 }
 
-extern "C" int nls_int8_matmul_workspace(int64_t m, int64_t n, int64_t k, size_t* bytes) {
+extern "C" int nls_int8_matmul_workspace(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, int64_t m, int64_t n, int64_t k, int flags,
+                                         size_t* bytes) {
   if (!bytes || m < 0 || n < 0 || k < 1) return NLS_ERR_ARG;
-  *bytes = up256((size_t)m * up16(k)) + up256((size_t)n * up16(k)) + 256;
+  *bytes = (aligned_rows(a, lda, k, flags, NLS_INT8_A_PADDED) ? 0 : up256((size_t)m * up16(k))) +
+           (aligned_rows(b, ldb, k, flags, NLS_INT8_B_PADDED) ? 0 : up256((size_t)n * up16(k)));
   return NLS_OK;
 }
 
@@ -250,15 +287,17 @@ extern "C" int nls_int8_matmul(nls_ctx* ctx, const int8_t* a, int64_t lda, const
   if (lda < k || ldb < k || lda > UINT32_MAX / 512 || ldb > UINT32_MAX / 512) return fail(ctx, NLS_ERR_ARG, "int8_matmul: row strides %lld, %lld", (long long)lda, (long long)ldb);
   if (m == 0 || n == 0) return NLS_OK;
   if (!a || !a_scale || !b || !b_scale || !y) return fail(ctx, NLS_ERR_ARG, "int8_matmul: null pointer");
+  size_t need = 0;
+  (void)nls_int8_matmul_workspace(a, lda, b, ldb, m, n, k, flags, &need);
+  if (workspace_bytes < need) return fail(ctx, NLS_ERR_ARG, "int8_matmul: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  if ((uintptr_t)workspace % 256) return fail(ctx, NLS_ERR_ARG, "int8_matmul: the workspace must be aligned to 256 bytes");
   DeviceGuard dev(ctx->device);
   HIPCHK(ctx, dev.err);
   hipStream_t st = (hipStream_t)stream;
   char* ws = (char*)workspace;
-  char* end = ws + workspace_bytes;
-  if ((uintptr_t)ws % 256) return fail(ctx, NLS_ERR_ARG, "int8_matmul: the workspace must be aligned to 256 bytes");
   Int8Args g{};
-  NLSCHK(aligned_operand(ctx, a, m, k, lda, aligned_rows(a, lda, k, flags, NLS_INT8_A_PADDED), &ws, end, &g.a, st));
-  NLSCHK(aligned_operand(ctx, b, n, k, ldb, aligned_rows(b, ldb, k, flags, NLS_INT8_B_PADDED), &ws, end, &g.b, st));
+  NLSCHK(operand(ctx, a, m, k, lda, aligned_rows(a, lda, k, flags, NLS_INT8_A_PADDED), &ws, &g.a, st));
+  NLSCHK(operand(ctx, b, n, k, ldb, aligned_rows(b, ldb, k, flags, NLS_INT8_B_PADDED), &ws, &g.b, st));
   g.a_scale = a_scale;
   g.b_scale = b_scale;
   g.bias = bias;
@@ -270,9 +309,10 @@ extern "C" int nls_int8_matmul(nls_ctx* ctx, const int8_t* a, int64_t lda, const
   return int8_product_any(ctx, g, type, st);
 }
 
-extern "C" int nls_int8_linear_workspace(int64_t m, int64_t n, int64_t k, size_t* bytes) {
+extern "C" int nls_int8_linear_workspace(const int8_t* b, int64_t ldb, int64_t m, int64_t n, int64_t k, int flags, size_t* bytes) {
   if (!bytes || m < 0 || n < 0 || k < 1) return NLS_ERR_ARG;
-  *bytes = up256((size_t)m * up16(k)) + up256((size_t)m * 4) + up256((size_t)n * up16(k)) + 256;
+  *bytes = (int8_fused(m, k) ? 0 : up256((size_t)m * up16(k)) + up256((size_t)m * 4)) +
+           (aligned_rows(b, ldb, k, flags, NLS_INT8_B_PADDED) ? 0 : up256((size_t)n * up16(k)));
   return NLS_OK;
 }
 
@@ -283,24 +323,16 @@ extern "C" int nls_int8_linear(nls_ctx* ctx, const void* x, int type, int64_t ro
   NLSCHK(check_int8(ctx, "int8_linear", m, n, k, type, bias_type, bias));
   if (ldb < k || ldb > UINT32_MAX / 512) return fail(ctx, NLS_ERR_ARG, "int8_linear: row stride %lld", (long long)ldb);
   if (m == 0 || n == 0) return NLS_OK;
-  if (!x || !b || !b_scale || !y || !workspace) return fail(ctx, NLS_ERR_ARG, "int8_linear: null pointer");
+  if (!x || !b || !b_scale || !y) return fail(ctx, NLS_ERR_ARG, "int8_linear: null pointer");
+  size_t need = 0;
+  (void)nls_int8_linear_workspace(b, ldb, m, n, k, flags, &need);
+  if (workspace_bytes < need) return fail(ctx, NLS_ERR_ARG, "int8_linear: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  if ((uintptr_t)workspace % 256) return fail(ctx, NLS_ERR_ARG, "int8_linear: the workspace must be aligned to 256 bytes");
   DeviceGuard dev(ctx->device);
   HIPCHK(ctx, dev.err);
   hipStream_t st = (hipStream_t)stream;
-  const long ldq = up16(k);
-  const size_t rows = up256((size_t)m * ldq), scales = up256((size_t)m * 4);
   char* ws = (char*)workspace;
-  char* end = ws + workspace_bytes;
-  if (workspace_bytes < rows + scales) return fail(ctx, NLS_ERR_ARG, "int8_linear: workspace too small (nls_int8_linear_workspace)");
-  if ((uintptr_t)ws % 256) return fail(ctx, NLS_ERR_ARG, "int8_linear: the workspace must be aligned to 256 bytes");
-  signed char* q = (signed char*)ws;
-  float* scale = (float*)(ws + rows);
-  ws += rows + scales;
   Int8Args g{};
-  NLSCHK(aligned_operand(ctx, b, n, k, ldb, aligned_rows(b, ldb, k, flags, NLS_INT8_B_PADDED), &ws, end, &g.b, st));
-  NLSCHK(quantize_any(ctx, x, type, m, k, row_stride, col_stride, q, ldq, scale, st));
-  g.a = Operand{(const char*)q, (unsigned)ldq, (int)m};
-  g.a_scale = scale;
   g.b_scale = b_scale;
   g.bias = bias;
   g.bias_type = bias_type;
@@ -308,6 +340,22 @@ extern "C" int nls_int8_linear(nls_ctx* ctx, const void* x, int type, int64_t ro
   g.n = (int)n;
   g.k = (int)k;
   g.y = y;
+  NLSCHK(operand(ctx, b, n, k, ldb, aligned_rows(b, ldb, k, flags, NLS_INT8_B_PADDED), &ws, &g.b, st));
+  if (int8_fused(m, k)) {
+    const int size = type_size(type);
+    const FewX f{x, row_stride, col_stride, col_stride == 1 && (uintptr_t)x % (8 * size) == 0 && (m == 1 || row_stride % 8 == 0)};
+    switch (type) {
+      case NLS_TYPE_F32: return int8_fused_product<float>(ctx, g, f, st);
+      case NLS_TYPE_F16: return int8_fused_product<_Float16>(ctx, g, f, st);
+      default: return int8_fused_product<__bf16>(ctx, g, f, st);
+    }
+  }
+  const long ldq = up16(k);
+  signed char* q = (signed char*)ws;
+  float* scale = (float*)(ws + up256((size_t)m * ldq));
+  NLSCHK(quantize_any(ctx, x, type, m, k, row_stride, col_stride, q, ldq, scale, st));
+  g.a = Operand{(const char*)q, (unsigned)ldq, (int)m};
+  g.a_scale = scale;
   return int8_product_any(ctx, g, type, st);
 }
 

@@ -20,7 +20,7 @@ import sys
 
 import numpy as np
 
-from ._lib import Context, DeviceArray, default_context
+from ._lib import Context, DeviceArray, _default_ctx, default_context
 
 __all__ = ["NEWTON_SCHULZ", "quantize_rows", "int8_matmul", "int8_linear", "orthogonalize"]
 
@@ -30,65 +30,56 @@ NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
 
 MAX_K = 131071  # NLS_INT8_MAX_K
 _A_PADDED, _B_PADDED = 1, 2
-_TYPES = {"float32": 0, "float16": 1, "bfloat16": 2}
-_NAMES = tuple(_TYPES)
+_NAMES = ("float32", "float16", "bfloat16")  # the position is the type's number in the C ABI
 
 
-def _name(dtype) -> str:
-    """The plain name of a dtype given as text, as NumPy's or as a tensor library's."""
+def _kind_of(dtype, what) -> int:
+    """The number of a float type given as text, as NumPy's or as a tensor library's."""
     text = str(dtype)
     if text.startswith("torch."):
-        return text[6:]
-    try:
-        return np.dtype(dtype).name
-    except TypeError:
-        return text
-
-
-def _float_type(dtype, what) -> int:
-    code = _TYPES.get(_name(dtype))
-    if code is None:
-        raise ValueError(f"{what} is {_name(dtype)}; the operators of few bits take {', '.join(_NAMES)}")
-    return code
+        text = text[6:]
+    elif text not in _NAMES:
+        try:
+            text = np.dtype(dtype).name
+        except TypeError:
+            pass
+    if text not in _NAMES:
+        raise ValueError(f"{what} is {text}; the operators of few bits take {', '.join(_NAMES)}")
+    return _NAMES.index(text)
 
 
 def _up16(k: int) -> int:
-    return -(-k // 16) * 16
+    return (k + 15) & -16
 
 
 class _Tensors:
-    """Tensors of an imported tensor library, on their device's current stream."""
+    """Tensors of an imported tensor library on one device, worked on in that device's current stream."""
 
-    def __init__(self, lib, first, ctx):
-        self.lib, self.ctx = lib, ctx
-        if not first.is_cuda:
-            raise ValueError("tensors must be on the GPU (host data: NumPy arrays)")
-        self.device = first.device
-        if ctx is not None and ctx.device != self.device.index:
-            raise ValueError(f"tensors are on GPU {self.device.index}, the context on GPU {ctx.device}")
+    host = False
+
+    def __init__(self, lib, index, ctx):
+        self.lib, self.index, self.ctx = lib, index, ctx
+        self.device = lib.device("cuda", index)
+        self.kinds = {getattr(lib, name): i for i, name in enumerate(_NAMES)}
+        self.types = tuple(getattr(lib, name) for name in _NAMES)
+        self.int8, self.float32, self.uint8, self.strided, self.Tensor = lib.int8, lib.float32, lib.uint8, lib.strided, lib.Tensor
+        self._raw_stream = getattr(lib._C, "_cuda_getCurrentRawStream", None)
 
     def begin(self):
-        index = self.device.index
-        if self.ctx is None:
-            with self.lib.cuda.device(index):  # (the first use of a device creates its context, which makes that device the current one)
-                self.ctx = default_context(index)
-        self.stream = self.lib.cuda.current_stream(self.device).cuda_stream
-        return self.ctx.lib
+        if self._raw_stream is not None:
+            return self._raw_stream(self.index)
+        return self.lib.cuda.current_stream(self.device).cuda_stream
 
     def take(self, x, what):
-        if not isinstance(x, self.lib.Tensor):
+        if not isinstance(x, self.Tensor):
             raise ValueError(f"{what} must be a tensor like the other arguments, not {type(x).__name__}")
-        if x.device != self.device:
+        if x.get_device() != self.index:
             raise ValueError(f"{what} is on {x.device}, the other arguments on {self.device}")
-        if x.layout is not self.lib.strided:
+        if x.layout is not self.strided:
             raise ValueError(f"{what} must be a dense tensor")
         if x.requires_grad and self.lib.is_grad_enabled():
             raise ValueError(f"{what} asks for gradients, which this operator does not give: detach it, or call under no_grad")
         return x.resolve_neg() if x.is_neg() else x
-
-    @staticmethod
-    def name(x):
-        return str(x.dtype)[6:]
 
     @staticmethod
     def ptr(x):
@@ -107,22 +98,27 @@ class _Tensors:
         """Bytes of the tensor's memory from its first element on."""
         return x.untyped_storage().nbytes() - x.storage_offset() * x.element_size()
 
-    def empty(self, shape, name):
-        return self.lib.empty(shape, dtype=getattr(self.lib, name), device=self.device)
+    def empty(self, shape, dtype):
+        return self.lib.empty(shape, dtype=dtype, device=self.device)
 
     def rows(self, rows, k, ld, lead):
-        held = self.lib.empty((rows, ld), dtype=self.lib.int8, device=self.device)
-        return held, held.view(*lead, ld)[..., :k]
+        held = self.lib.empty((*lead, ld), dtype=self.int8, device=self.device)
+        return held, held if ld == k else held[..., :k]
 
     def scratch(self, nbytes):
-        return self.lib.empty(nbytes, dtype=self.lib.uint8, device=self.device)
+        return self.lib.empty(nbytes, dtype=self.uint8, device=self.device)
 
-    def done(self, result):
+    @staticmethod
+    def done(result):
         return result
 
 
 class _Arrays:
     """NumPy arrays and DeviceArrays, on the context's own stream; results come back as what went in."""
+
+    kinds = {np.dtype("float32"): 0, np.dtype("float16"): 1}
+    types = (np.dtype("float32"), np.dtype("float16"))
+    int8, float32 = np.dtype("int8"), np.dtype("float32")
 
     def __init__(self, first, ctx):
         self.host = isinstance(first, np.ndarray)
@@ -134,8 +130,7 @@ class _Arrays:
             self.ctx = default_context()
         stream = C.c_void_p()
         self.ctx._check(self.ctx.lib.nls_ctx_stream(self.ctx.handle, C.byref(stream)))
-        self.stream = stream.value
-        return self.ctx.lib
+        return stream.value
 
     def take(self, x, what):
         if self.host != isinstance(x, np.ndarray) or not isinstance(x, (np.ndarray, DeviceArray)):
@@ -143,10 +138,6 @@ class _Arrays:
         if not self.host and x.ctx.device != self.ctx.device:
             raise ValueError(f"{what} is on GPU {x.ctx.device}, the context on GPU {self.ctx.device}")
         return x
-
-    @staticmethod
-    def name(x):
-        return x.dtype.name
 
     def ptr(self, x):
         if isinstance(x, DeviceArray):
@@ -171,8 +162,8 @@ class _Arrays:
     def room(x):
         return x.nbytes
 
-    def empty(self, shape, name):
-        return DeviceArray(self.ctx, shape, dtype=name)
+    def empty(self, shape, dtype):
+        return DeviceArray(self.ctx, shape, dtype=dtype)
 
     def rows(self, rows, k, ld, lead):
         held = DeviceArray(self.ctx, (rows, ld), dtype="int8")
@@ -217,10 +208,24 @@ class _Rows:
         return ctx.to_device(self.host(), dtype="int8")
 
 
+_on_device: dict[int, _Tensors] = {}  # a device's default context and what the tensor library calls its types
+
+
 def _space(first, ctx):
     lib = sys.modules.get("torch")
     if lib is not None and isinstance(first, lib.Tensor):
-        return _Tensors(lib, first, ctx)
+        index = first.get_device()
+        if index < 0 or not first.is_cuda:
+            raise ValueError("tensors must be on the GPU (host data: NumPy arrays)")
+        if ctx is not None:
+            if ctx.device != index:
+                raise ValueError(f"tensors are on GPU {index}, the context on GPU {ctx.device}")
+            return _Tensors(lib, index, ctx)
+        sp = _on_device.get(index)
+        if sp is None or sp.ctx is not _default_ctx.get(index):
+            with lib.cuda.device(index):  # (the first use of a device creates its context, which makes that device the current one)
+                sp = _on_device[index] = _Tensors(lib, index, default_context(index))
+        return sp
     if isinstance(first, (np.ndarray, DeviceArray)):
         return _Arrays(first, ctx)
     raise ValueError(f"expected a tensor on the GPU, a DeviceArray or a NumPy array, not {type(first).__name__}")
@@ -228,61 +233,75 @@ def _space(first, ctx):
 
 def _call(ctx: Context, fn, *args):
     with ctx.lock:  # the message of a failure belongs to the call that failed
-        ctx._check(fn(ctx.handle, *args))
+        rc = fn(ctx.handle, *args)
+        if rc:
+            ctx._check(rc)
+
+
+def _kind(sp, x, what) -> int:
+    kind = sp.kinds.get(x.dtype)
+    return _kind_of(x.dtype, what) if kind is None else kind  # (which refuses it)
 
 
 def _float_rows(sp, x, what):
     """(x as a matrix, leading shape, rows, k, row stride, column stride, type)"""
     x = sp.take(x, what)
     shape = tuple(x.shape)
+    kind = _kind(sp, x, what)
     if len(shape) < 1:
         raise ValueError(f"{what} must have at least one axis")
-    kind = _float_type(sp.name(x), what)
     k, lead = shape[-1], shape[:-1]
     if k < 1:
         raise ValueError(f"{what} has rows of no elements")
-    rows = int(np.prod(lead)) if lead else 1
-    if len(shape) != 2:
-        if isinstance(x, DeviceArray):
-            rs, cs = k, 1
-        else:
-            x = x.reshape(rows, k)
-            rs, cs = sp.strides(x)
+    rows = math.prod(lead)
+    if len(shape) == 2:
+        rs, cs = sp.strides(x)
+    elif isinstance(x, DeviceArray):
+        rs, cs = k, 1
     else:
+        x = x.reshape(rows, k)
         rs, cs = sp.strides(x)
     return x, lead, rows, k, rs, cs, kind
 
 
 def _int8_rows(sp, x, what, scale, scale_what):
-    """(matrix, its scales, leading shape, rows, k, row stride, whether each row may be read up to a multiple of 16 bytes)"""
+    """(matrix, its scales, leading shape, rows, k, row stride, whether the rows can be read where they are)
+
+    They can when each starts at a multiple of 16 bytes and the bytes up to the next multiple behind its end exist."""
     x, scale = sp.take(x, what), sp.take(scale, scale_what)
     shape = tuple(x.shape)
-    if len(shape) < 1 or sp.name(x) != "int8":
+    if len(shape) < 1 or x.dtype != sp.int8:
         raise ValueError(f"{what} must be a matrix of int8")
     k, lead = shape[-1], shape[:-1]
     if not 1 <= k <= MAX_K:
         raise ValueError(f"{what} has rows of {k} elements; 1 to {MAX_K} products are summed in 32 bits without overflow")
-    if tuple(scale.shape) != lead or sp.name(scale) != "float32":
-        raise ValueError(f"{scale_what} must be float32 of shape {lead}, not {sp.name(scale)} of shape {tuple(scale.shape)}")
-    rows = int(np.prod(lead)) if lead else 1
-    if not isinstance(x, DeviceArray) and len(shape) != 2:
+    if tuple(scale.shape) != lead or scale.dtype != sp.float32:
+        raise ValueError(f"{scale_what} must be float32 of shape {lead}, not {scale.dtype} of shape {tuple(scale.shape)}")
+    rows = math.prod(lead)
+    flat = isinstance(x, DeviceArray)
+    if not flat and len(shape) != 2:
         x = x.reshape(rows, k)
-    st = (k, 1) if isinstance(x, DeviceArray) else sp.strides(x)
+    st = (k, 1) if flat else sp.strides(x)
     if (k > 1 and st[1] != 1) or (rows > 1 and st[0] < k):  # columns apart, or rows that share memory
         x = sp.dense(x)
         st = sp.strides(x)
-    ld = max(st[0], k) if rows > 1 else max(_up16(k), k) if sp.room(x) >= _up16(k) else k
-    padded = ld >= _up16(k) and sp.room(x) >= (rows - 1) * ld + _up16(k)
-    return x, sp.dense(scale), lead, rows, k, ld, padded
+    if k & 15:
+        up = _up16(k)
+        room = sp.room(x)
+        ld = max(st[0], k) if rows > 1 else up if room >= up else k
+        ready = ld >= up and room >= (rows - 1) * ld + up
+    else:
+        ld, ready = max(st[0], k) if rows > 1 else k, True
+    return x, sp.dense(scale), lead, rows, k, ld, ready
 
 
 def _bias(sp, bias, n, kind):
     if bias is None:
         return None, 0
     bias = sp.take(bias, "bias")
-    code = _float_type(sp.name(bias), "bias")
+    code = _kind(sp, bias, "bias")
     if tuple(bias.shape) != (n,) or code not in (0, kind):
-        raise ValueError(f"bias must have shape ({n},) and be float32 or of the result's type, not {sp.name(bias)} of shape {tuple(bias.shape)}")
+        raise ValueError(f"bias must have shape ({n},) and be float32 or of the result's type, not {bias.dtype} of shape {tuple(bias.shape)}")
     return sp.dense(bias), code
 
 
@@ -294,12 +313,12 @@ def quantize_rows(x, ctx: Context | None = None):
     bytes (its last axis is dense, its rows may have gaps): that is how ``int8_matmul`` and ``int8_linear`` read them without a copy."""
     sp = _space(x, ctx)
     x, lead, rows, k, rs, cs, kind = _float_rows(sp, x, "x")
-    lib = sp.begin()
+    stream = sp.begin()
     ld = _up16(k)
     held, q = sp.rows(rows, k, ld, lead)
-    scale = sp.empty(lead, "float32")
+    scale = sp.empty(lead, sp.float32)
     if rows:
-        _call(sp.ctx, lib.nls_quantize_rows, sp.ptr(x), kind, rows, k, rs, cs, sp.ptr(held), ld, sp.ptr(scale), sp.stream)
+        _call(sp.ctx, sp.ctx.lib.nls_quantize_rows, sp.ptr(x), kind, rows, k, rs, cs, sp.ptr(held), ld, sp.ptr(scale), stream)
     return sp.done((q, scale))
 
 
@@ -310,23 +329,26 @@ def int8_matmul(a, a_scale, b, b_scale, bias=None, dtype="float32", ctx: Context
     (k <= 131071), the rest is float32, rounded once.  Rows that do not start at multiples of 16 bytes are copied first; ``quantize_rows`` lays them
     out so that they do."""
     sp = _space(a, ctx)
-    kind = _float_type(dtype, "dtype")
-    if kind == 2 and isinstance(sp, _Arrays):
+    kind = _kind_of(dtype, "dtype")
+    if kind >= len(sp.types):
         raise ValueError("dtype: NumPy arrays and DeviceArrays have no bfloat16")
-    a, a_scale, lead, m, k, lda, apad = _int8_rows(sp, a, "a", a_scale, "a_scale")
-    b, b_scale, blead, n, kb, ldb, bpad = _int8_rows(sp, b, "b", b_scale, "b_scale")
-    if len(blead) != 1 or kb != k:
-        raise ValueError(f"b must be a matrix with rows of {k} elements, not of shape {(*blead, kb)}")
+    a, a_scale, lead, m, k, lda, a_ready = _int8_rows(sp, a, "a", a_scale, "a_scale")
+    b, b_scale, b_lead, n, kb, ldb, b_ready = _int8_rows(sp, b, "b", b_scale, "b_scale")
+    if len(b_lead) != 1 or kb != k:
+        raise ValueError(f"b must be a matrix with rows of {k} elements, not of shape {(*b_lead, kb)}")
     bias, bias_kind = _bias(sp, bias, n, kind)
-    lib = sp.begin()
-    y = sp.empty((*lead, n), _NAMES[kind])
+    stream = sp.begin()
+    y = sp.empty((*lead, n), sp.types[kind])
     if m and n:
+        lib = sp.ctx.lib
+        pa, pb = sp.ptr(a), sp.ptr(b)
+        flags = (_A_PADDED if a_ready else 0) | (_B_PADDED if b_ready else 0)
         need = C.c_size_t()
-        lib.nls_int8_matmul_workspace(m, n, k, C.byref(need))
-        ws = sp.scratch(need.value)
+        lib.nls_int8_matmul_workspace(pa, lda, pb, ldb, m, n, k, flags, need)
+        ws = sp.scratch(need.value) if need.value else None
         _call(
-            sp.ctx, lib.nls_int8_matmul, sp.ptr(a), lda, sp.ptr(a_scale), sp.ptr(b), ldb, sp.ptr(b_scale), None if bias is None else sp.ptr(bias),
-            bias_kind, m, n, k, sp.ptr(y), kind, (_A_PADDED if apad else 0) | (_B_PADDED if bpad else 0), sp.ptr(ws), need.value, sp.stream,
+            sp.ctx, lib.nls_int8_matmul, pa, lda, sp.ptr(a_scale), pb, ldb, sp.ptr(b_scale), None if bias is None else sp.ptr(bias), bias_kind,
+            m, n, k, sp.ptr(y), kind, flags, None if ws is None else sp.ptr(ws), need.value, stream,
         )  # fmt: skip
     return sp.done(y)
 
@@ -335,19 +357,22 @@ def int8_linear(x, b, b_scale, bias=None, ctx: Context | None = None):
     """``int8_matmul(*quantize_rows(x), b, b_scale, bias, dtype=x.dtype)`` in one call: ``x`` (..., k) in 16 or 32 bits against rows held in 8."""
     sp = _space(x, ctx)
     x, lead, m, k, rs, cs, kind = _float_rows(sp, x, "x")
-    b, b_scale, blead, n, kb, ldb, bpad = _int8_rows(sp, b, "b", b_scale, "b_scale")
-    if len(blead) != 1 or kb != k:
-        raise ValueError(f"b must be a matrix with rows of {k} elements, not of shape {(*blead, kb)}")
+    b, b_scale, b_lead, n, kb, ldb, b_ready = _int8_rows(sp, b, "b", b_scale, "b_scale")
+    if len(b_lead) != 1 or kb != k:
+        raise ValueError(f"b must be a matrix with rows of {k} elements, not of shape {(*b_lead, kb)}")
     bias, bias_kind = _bias(sp, bias, n, kind)
-    lib = sp.begin()
-    y = sp.empty((*lead, n), _NAMES[kind])
+    stream = sp.begin()
+    y = sp.empty((*lead, n), sp.types[kind])
     if m and n:
+        lib = sp.ctx.lib
+        pb = sp.ptr(b)
+        flags = _B_PADDED if b_ready else 0
         need = C.c_size_t()
-        lib.nls_int8_linear_workspace(m, n, k, C.byref(need))
-        ws = sp.scratch(need.value)
+        lib.nls_int8_linear_workspace(pb, ldb, m, n, k, flags, need)
+        ws = sp.scratch(need.value) if need.value else None
         _call(
-            sp.ctx, lib.nls_int8_linear, sp.ptr(x), kind, rs, cs, sp.ptr(b), ldb, sp.ptr(b_scale), None if bias is None else sp.ptr(bias), bias_kind,
-            m, n, k, sp.ptr(y), _B_PADDED if bpad else 0, sp.ptr(ws), need.value, sp.stream,
+            sp.ctx, lib.nls_int8_linear, sp.ptr(x), kind, rs, cs, pb, ldb, sp.ptr(b_scale), None if bias is None else sp.ptr(bias), bias_kind, m, n, k,
+            sp.ptr(y), flags, None if ws is None else sp.ptr(ws), need.value, stream,
         )  # fmt: skip
     return sp.done(y)
 
@@ -366,7 +391,7 @@ def orthogonalize(g, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: float = 1e
     shape = tuple(g.shape)
     if len(shape) < 2:
         raise ValueError("g must be a matrix or a batch of matrices")
-    kind = _float_type(sp.name(g), "g")
+    kind = _kind(sp, g, "g")
     if isinstance(steps, bool) or int(steps) != steps or not 1 <= steps <= 64:
         raise ValueError("steps must be a whole number from 1 to 64")
     steps = int(steps)
@@ -381,20 +406,24 @@ def orthogonalize(g, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: float = 1e
         raise ValueError("eps must be a number >= 0")
     table = (C.c_double * (3 * steps))(*(v for row in rows for v in row))
     m, n = shape[-2:]
-    batch = int(np.prod(shape[:-2])) if len(shape) > 2 else 1
+    batch = math.prod(shape[:-2])
     if isinstance(g, DeviceArray):
         st = (m * n, n, 1)
+    elif len(shape) == 2:
+        st = (0, *sp.strides(g))
     else:
         if len(shape) != 3:
             g = g.reshape(batch, m, n)
         st = sp.strides(g)
-    lib = sp.begin()
-    out = sp.empty(shape, _NAMES[kind])
+    stream = sp.begin()
+    lib = sp.ctx.lib
+    out = sp.empty(shape, sp.types[kind])
     need = C.c_size_t()
-    lib.nls_orthogonalize_workspace(batch, m, n, C.byref(need))
-    ws = sp.scratch(need.value) if batch and m and n else None
+    empty = not (batch and m and n)
+    lib.nls_orthogonalize_workspace(batch, m, n, need)
+    ws = None if empty else sp.scratch(need.value)
     _call(
-        sp.ctx, lib.nls_orthogonalize, sp.ptr(g) if ws is not None else None, kind, batch, m, n, *st, table, steps, eps, sp.ptr(out),
-        None if ws is None else sp.ptr(ws), need.value if ws is not None else 0, sp.stream,
+        sp.ctx, lib.nls_orthogonalize, None if empty else sp.ptr(g), kind, batch, m, n, *st, table, steps, eps, sp.ptr(out),
+        None if empty else sp.ptr(ws), need.value, stream,
     )  # fmt: skip
     return sp.done(out)
