@@ -477,7 +477,7 @@ int nls_int8_linear(nls_ctx* ctx, const void* x, int type, int64_t row_stride, i
  * j col_stride; out: batch x m x n without gaps, of `type`, not overlapping G.  Each matrix has its own norm; one that holds a NaN or an infinity
  * comes out as NaN, one of zeros as zeros.  Products and sums carry 22 bits or more; for 16-bit results the early steps carry 11 (error of the result
  * against 64 bits below its own rounding).  The coefficients may not let a singular value of X pass 1e6. */
-int nls_orthogonalize_workspace(int64_t batch, int64_t m, int64_t n, size_t* bytes);
+int nls_orthogonalize_workspace(int64_t batch, int64_t m, int64_t n, int64_t row_stride, int64_t col_stride, size_t* bytes);
 int nls_orthogonalize(nls_ctx* ctx, const void* g, int type, int64_t batch, int64_t m, int64_t n, int64_t batch_stride, int64_t row_stride,
                       int64_t col_stride, const double* coefficients, int steps, double eps, void* out, void* workspace, size_t workspace_bytes,
                       void* stream);

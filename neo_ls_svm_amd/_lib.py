@@ -239,7 +239,7 @@ SIGNATURES = {
         [C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int]
         + [C.c_int64] * 3 + [C.c_void_p, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p],
     ),
-    "nls_orthogonalize_workspace": (C.c_int, [C.c_int64] * 3 + [C.POINTER(C.c_size_t)]),
+    "nls_orthogonalize_workspace": (C.c_int, [C.c_int64] * 5 + [C.POINTER(C.c_size_t)]),
     "nls_orthogonalize": (
         C.c_int,
         [C.c_void_p, C.c_void_p, C.c_int] + [C.c_int64] * 6 + [C.c_void_p, C.c_int, C.c_double, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p],

@@ -33,7 +33,7 @@ struct DeviceGuard {
     if (e__ != hipSuccess) return fail(ctx, NLS_ERR_HIP, "%s: launch failed: %s", what, hipGetErrorString(e__)); \
   } while (0)
 
-// Dynamic LDS beyond 64 KB has to be asked for once per kernel and device; asking again costs a table lookup.
+// Dynamic LDS beyond 64 KB has to be asked for once per kernel and device.
 template <class F>
 int ask_lds(nls_ctx* ctx, F f, int bytes) {
   if (bytes > 65536) HIPCHK(ctx, hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
@@ -158,14 +158,21 @@ int operand(nls_ctx* ctx, const int8_t* p, long rows, long k, long ld, bool read
 }
 
 // ---- Newton-Schulz ----
+// Matrices one workgroup holds: X in 64 registers of 8 waves and once in LDS; it reads them with 32-bit offsets.
+bool ns_is_small(long p, long q, long row_stride, long col_stride) {
+  if (!((p <= 128 && q <= 256) || (p <= 64 && q <= 512) || (p <= 32 && q <= 1024))) return false;
+  const long reach = 1l << 28;
+  return row_stride >= 0 && col_stride >= 0 && (p + 32) * row_stride + (q + 256) * col_stride < reach;
+}
 struct NsPlan {
   long p, q;
   size_t x, xt, a, parts, scales, batch_bytes, total;
 };
-NsPlan ns_plan(long m, long n, long batch) {
-  NsPlan w;
+NsPlan ns_plan(long m, long n, long batch, long row_stride, long col_stride) {
+  NsPlan w{};
   w.p = std::min(m, n);
   w.q = std::max(m, n);
+  if (ns_is_small(w.p, w.q, m > n ? col_stride : row_stride, m > n ? row_stride : col_stride)) return w;
   w.x = (size_t)w.p * pair_ld(w.q);
   w.xt = (size_t)w.q * pair_ld(w.p);
   w.a = (size_t)w.p * pair_ld(w.p);
@@ -197,8 +204,37 @@ int ns_product(nls_ctx* ctx, const NsArgs& g, bool pairs, long batch, hipStream_
   return pairs ? ns_product_tile<KIND, T, MODE_F16PAIR, 64, 2>(ctx, g, batch, st) : ns_product_tile<KIND, T, MODE_F16, 64, 2>(ctx, g, batch, st);
 }
 
+template <class T, int PB, int CB>
+int ns_small(nls_ctx* ctx, const NsMatrix& w, bool tall, long batch, const NsCoef& cf, int steps, int exact, double eps, T* out, hipStream_t st) {
+  const int lds = NsSmall<PB, CB>::lds((int)w.q);
+  NLSCHK(ask_lds(ctx, k_ns_small<T, PB, CB>, lds));
+  k_ns_small<T, PB, CB><<<dim3((unsigned)batch), 512, lds, st>>>(w, cf, steps, exact, eps, out, tall);
+  LAUNCHED(ctx, "orthogonalize");
+  return NLS_OK;
+}
+template <class T>
+int ns_small_any(nls_ctx* ctx, const NsMatrix& w, bool tall, long batch, const NsCoef& cf, int steps, int exact, double eps, T* out, hipStream_t st) {
+#define NS_SMALL(PB, CB) return ns_small<T, PB, CB>(ctx, w, tall, batch, cf, steps, exact, eps, out, st)
+  if (w.q <= 256) {
+    if (w.p <= 32) NS_SMALL(1, 1);
+    if (w.p <= 64) NS_SMALL(2, 1);
+    if (w.p <= 96) NS_SMALL(3, 1);
+    NS_SMALL(4, 1);
+  }
+  if (w.q <= 512) {
+    if (w.p <= 32) NS_SMALL(1, 2);
+    NS_SMALL(2, 2);
+  }
+  NS_SMALL(1, 4);
+#undef NS_SMALL
+}
+
 template <class T>
 int orthogonalize(nls_ctx* ctx, const NsMatrix& w, const NsPlan& plan, bool tall, long batch, const NsCoef& cf, int steps, double eps, T* out, char* ws, hipStream_t st) {
+  // The first steps may work on the hi halves alone where the result has few bits: what a rounding to 11 bits does to an early iterate is carried
+  // along as a slightly different matrix would be, and the steps after it pull its singular values to the same curve.
+  const int exact = sizeof(T) == 4 ? steps : std::is_same<T, __bf16>::value ? 2 : 3;
+  if (plan.total == 0) return ns_small_any(ctx, w, tall, batch, cf, steps, exact, eps, out, st);
   double* parts = (double*)ws;
   NsScales* scales = (NsScales*)(ws + plan.parts);
   char* base = ws + plan.parts + plan.scales;
@@ -208,9 +244,6 @@ int orthogonalize(nls_ctx* ctx, const NsMatrix& w, const NsPlan& plan, bool tall
   k_ns_scales<<<dim3((unsigned)batch), 64, 0, st>>>(parts, count, eps, cf, steps, scales);
   k_ns_pack<T><<<dim3((unsigned)((w.q + 63) / 64), (unsigned)((w.p + 63) / 64), (unsigned)batch), 256, 0, st>>>(w, scales, X, XT, plan.batch_bytes);
   LAUNCHED(ctx, "orthogonalize");
-  // The first steps may work on the hi halves alone where the result has few bits: what a rounding to 11 bits does to an early iterate is carried
-  // along as a slightly different matrix would be, and the steps after it pull its singular values to the same curve.
-  const int exact = sizeof(T) == 4 ? steps : std::is_same<T, __bf16>::value ? 2 : 3;
   NsArgs g{};
   g.scales = scales;
   g.batch_bytes = plan.batch_bytes;
@@ -359,9 +392,9 @@ extern "C" int nls_int8_linear(nls_ctx* ctx, const void* x, int type, int64_t ro
   return int8_product_any(ctx, g, type, st);
 }
 
-extern "C" int nls_orthogonalize_workspace(int64_t batch, int64_t m, int64_t n, size_t* bytes) {
+extern "C" int nls_orthogonalize_workspace(int64_t batch, int64_t m, int64_t n, int64_t row_stride, int64_t col_stride, size_t* bytes) {
   if (!bytes || batch < 0 || m < 0 || n < 0) return NLS_ERR_ARG;
-  *bytes = ns_plan(m, n, batch).total;
+  *bytes = ns_plan(m, n, batch, row_stride, col_stride).total;
   return NLS_OK;
 }
 
@@ -385,8 +418,8 @@ extern "C" int nls_orthogonalize(nls_ctx* ctx, const void* g, int type, int64_t 
   }
   if (m > (1 << 20) || n > (1 << 20) || batch > 65535) return fail(ctx, NLS_ERR_ARG, "orthogonalize: at most 2^20 rows and columns and 65535 matrices");
   if (batch == 0 || m == 0 || n == 0) return NLS_OK;
-  if (!g || !out || !workspace) return fail(ctx, NLS_ERR_ARG, "orthogonalize: null pointer");
-  const NsPlan plan = ns_plan(m, n, batch);
+  const NsPlan plan = ns_plan(m, n, batch, row_stride, col_stride);
+  if (!g || !out || (plan.total && !workspace)) return fail(ctx, NLS_ERR_ARG, "orthogonalize: null pointer");
   if (workspace_bytes < plan.total) return fail(ctx, NLS_ERR_ARG, "orthogonalize: workspace of %zu bytes, %zu needed", workspace_bytes, plan.total);
   if ((uintptr_t)workspace % 256) return fail(ctx, NLS_ERR_ARG, "orthogonalize: the workspace must be aligned to 256 bytes");
   DeviceGuard dev(ctx->device);

@@ -86,14 +86,9 @@ __device__ __forceinline__ int ns_exponent(double v) {
   return 15 - e;
 }
 
-__global__ __launch_bounds__(64) void k_ns_scales(const double* parts, int count, double eps, NsCoef cf, int steps, NsScales* out) {
-  double s = 0.0;
-  for (int i = threadIdx.x; i < count; i += 64) s += parts[(size_t)blockIdx.x * NS_PARTS + i];
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-  if (threadIdx.x != 0) return;
-  NsScales& z = out[blockIdx.x];
-  const double norm = sqrt(s);
+// squares: |G|_F^2
+__device__ __forceinline__ void ns_scales(double squares, double eps, const NsCoef& cf, int steps, NsScales& z) {
+  const double norm = sqrt(squares);
   const bool fine = norm < 1e300;
   z.inv = fine ? (norm + eps > 0.0 ? 1.0 / (norm + eps) : 0.0) : __longlong_as_double(0x7ff8000000000000ll);
   double u = fine ? norm * z.inv * (1.0 + 1e-3) : 1.0;  // |X_0| <= |X_0|_F
@@ -104,6 +99,14 @@ __global__ __launch_bounds__(64) void k_ns_scales(const double* parts, int count
     u = ns_peak_x(cf.a[t], cf.b[t], cf.c[t], u) * (1.0 + 1e-3);
   }
   z.ex[steps] = ns_exponent(u);
+}
+
+__global__ __launch_bounds__(64) void k_ns_scales(const double* parts, int count, double eps, NsCoef cf, int steps, NsScales* out) {
+  double s = 0.0;
+  for (int i = threadIdx.x; i < count; i += 64) s += parts[(size_t)blockIdx.x * NS_PARTS + i];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+  if (threadIdx.x == 0) ns_scales(s, eps, cf, steps, out[blockIdx.x]);
 }
 
 __device__ __forceinline__ void split(float v, _Float16* hi, _Float16* lo) {
@@ -290,6 +293,261 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_ns_product(NsArgs g) {
         }
       }
     }
+  }
+}
+
+// ---- small matrices ---------------------------------------------------------------------------------------------------------------------------
+// One workgroup does all steps of a matrix of up to 32 PB x 256 CB (padded to blocks of 32).  X stays in registers in float32, in the places the matrix
+// instruction leaves its results in: lane l has column l % 32 of a block, registers r the rows 8 (r / 4) + 4 (l / 32) + r % 4.  Wave w has the column
+// blocks w, w + 8, ...
+//   A = X X^T contracts over columns, which lie across lanes: X goes through LDS once a step, as rows of fp16 (hi and lo planes).
+//   B X contracts over rows, which lie along registers: registers 8 s .. 8 s + 7 of a block ARE a fragment of the 32 x 32 x 16 instruction if k runs in the
+//   order 16 s + {4 h, 4 h + 1, .., 4 h + 3, 8 + 4 h, ..} for lane half h - so B is laid out in LDS with its columns in that order and X is never moved.
+// Rows of LDS planes are 16 bytes longer than their numbers: eight neighbouring rows start in different banks.
+// A step is a chain of three short products; what bounds it is latency (barriers, LDS round trips), not a rate.
+// What a general path costs instead is three launches a step.
+template <int PB, int CB>
+struct NsSmall {
+  static constexpr int P = 32 * PB, Q = 256 * CB;
+  static constexpr int BLOCKS = PB * PB;
+  static constexpr int OWN = (BLOCKS + 7) / 8;              // blocks of A a wave has
+  static constexpr int KS = BLOCKS >= 8 ? 1 : PB == 2 ? 2 : 8;  // waves that share a block's columns
+  static constexpr int PITCH_A = P * 2 + 16;
+  // LDS for the columns that are there
+  __host__ __device__ static int pitch_x(int q) { return (q + 31) / 32 * 64 + 16; }
+  __host__ __device__ static int lds(int q) {
+    const int x = 2 * P * pitch_x(q), a = 2 * P * PITCH_A, parts = KS > 1 ? 8 * 4096 : 0;
+    const int m = x > a ? x : a;
+    return m > parts ? m : parts;
+  }
+};
+
+template <class T, int PB, int CB>
+__global__ __launch_bounds__(512) void k_ns_small(NsMatrix m, NsCoef cf, int steps, int exact, double eps, T* out, int tall) {
+  using S = NsSmall<PB, CB>;
+  extern __shared__ char lds[];
+  __shared__ NsScales z;
+  __shared__ double part[8];
+  const int l = (int)(threadIdx.x & 63), w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int h = l >> 5, c32 = l & 31;
+  const int p = (int)m.p, q = (int)m.q;
+  const int cols = (q + 31) / 32;  // column blocks
+  const T* g = (const T*)m.g + blockIdx.x * m.batch_stride;
+  float x[CB][PB][16];
+  double sum = 0.0;
+#pragma unroll
+  for (int c = 0; c < CB; ++c) {
+    const int j = (w + 8 * c) * 32 + c32;
+    // (32-bit offsets within the matrix: the host sees to it)
+    const unsigned at = (unsigned)(4 * h * (int)m.row_stride + j * (int)m.col_stride) * (unsigned)sizeof(T);
+#pragma unroll
+    for (int a = 0; a < PB; ++a)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int iu = 32 * a + 8 * (r >> 2) + (r & 3);
+        const char* row = (const char*)(g + iu * m.row_stride);
+        x[c][a][r] = (iu + 4 * h < p && j < q) ? to_f32(*(const T*)(row + at)) : 0.0f;
+      }
+  }
+#pragma unroll
+  for (int c = 0; c < CB; ++c)
+#pragma unroll
+    for (int a = 0; a < PB; ++a)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sum += (double)x[c][a][r] * (double)x[c][a][r];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+  if (l == 0) part[w] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double s = 0.0;
+    for (int i = 0; i < 8; ++i) s += part[i];
+    ns_scales(s, eps, cf, steps, z);
+  }
+  __syncthreads();
+  {
+    const double f = ldexp(z.inv, z.ex[0]);
+#pragma unroll
+    for (int c = 0; c < CB; ++c)
+#pragma unroll
+      for (int a = 0; a < PB; ++a)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[c][a][r] = (float)((double)x[c][a][r] * f);
+  }
+  const int pitch = S::pitch_x(q);
+  for (int t = 0; t < steps; ++t) {
+    const bool pairs = t >= steps - exact;
+    const int ex = z.ex[t], ea = z.ea[t], eb = z.eb[t], en = z.ex[t + 1];
+    const float ca = (float)cf.a[t], cb = (float)cf.b[t], cc = (float)cf.c[t];
+    // X to LDS, hi plane then lo plane
+#pragma unroll
+    for (int c = 0; c < CB; ++c)
+      if (w + 8 * c < cols) {
+#pragma unroll
+        for (int a = 0; a < PB; ++a)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            char* at = lds + (32 * a + 8 * (r >> 2) + 4 * h + (r & 3)) * pitch + ((w + 8 * c) * 32 + c32) * 2;
+            _Float16 hi, lo;
+            split(x[c][a][r], &hi, &lo);
+            *(_Float16*)at = hi;
+            if (pairs) *(_Float16*)(at + S::P * pitch) = lo;
+          }
+      }
+    __syncthreads();
+    // A: block (bi, bj) of wave w % blocks, KS waves share its columns
+    f32x16 acc[S::OWN];
+#pragma unroll
+    for (int o = 0; o < S::OWN; ++o) {
+      acc[o] = f32x16{};
+      const int blk = S::KS > 1 ? w % S::BLOCKS : w + 8 * o;
+      if (blk < S::BLOCKS) {
+        const char* pi = lds + (blk / PB * 32 + c32) * pitch + h * 16;
+        const char* pj = lds + (blk % PB * 32 + c32) * pitch + h * 16;
+        for (int k = S::KS > 1 ? w / S::BLOCKS : 0; k < 2 * cols; k += S::KS) {
+          const f16x8 ih = *(const f16x8*)(pi + k * 32), jh = *(const f16x8*)(pj + k * 32);
+          acc[o] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ih, jh, acc[o], 0, 0, 0);
+          if (pairs) {
+            const f16x8 il = *(const f16x8*)(pi + S::P * pitch + k * 32), jl = *(const f16x8*)(pj + S::P * pitch + k * 32);
+            acc[o] = __builtin_amdgcn_mfma_f32_32x32x16_f16(il, jh, acc[o], 0, 0, 0);
+            acc[o] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ih, jl, acc[o], 0, 0, 0);
+          }
+        }
+      }
+    }
+    __syncthreads();
+    if constexpr (S::KS > 1) {
+      float* mine = (float*)lds + w * 1024 + l;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mine[r * 64] = acc[0][r];
+      __syncthreads();
+      if (w < S::BLOCKS) {
+#pragma unroll
+        for (int o = 1; o < S::KS; ++o)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[0][r] += mine[o * S::BLOCKS * 1024 + r * 64];
+      }
+      __syncthreads();
+    }
+    // A as pairs; it is symmetric, so the lane's column is a row and its four neighbouring rows are four neighbours in it
+#pragma unroll
+    for (int o = 0; o < S::OWN; ++o) {
+      const int blk = w + 8 * o;
+      if (blk < S::BLOCKS) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[o][r] = ldexpf(acc[o][r], ea - 2 * ex);
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+          char* at = lds + (blk % PB * 32 + c32) * S::PITCH_A + (blk / PB * 32 + 2 * r + 4 * h) * 2;
+          f16x4 hi, lo;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            _Float16 u, v;
+            split(acc[o][r + e], &u, &v);
+            hi[e] = u;
+            lo[e] = v;
+          }
+          *(f16x4*)at = hi;
+          if (pairs) *(f16x4*)(at + S::P * S::PITCH_A) = lo;
+        }
+      }
+    }
+    __syncthreads();
+    // B = b A + c A A
+    f32x16 poly[S::OWN];
+#pragma unroll
+    for (int o = 0; o < S::OWN; ++o) {
+      poly[o] = f32x16{};
+      const int blk = w + 8 * o;
+      if (blk < S::BLOCKS) {
+        const char* pi = lds + (blk / PB * 32 + c32) * S::PITCH_A + h * 16;
+        const char* pj = lds + (blk % PB * 32 + c32) * S::PITCH_A + h * 16;
+#pragma unroll 2
+        for (int k = 0; k < 2 * PB; ++k) {
+          const f16x8 ih = *(const f16x8*)(pi + k * 32), jh = *(const f16x8*)(pj + k * 32);
+          poly[o] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ih, jh, poly[o], 0, 0, 0);
+          if (pairs) {
+            const f16x8 il = *(const f16x8*)(pi + S::P * S::PITCH_A + k * 32), jl = *(const f16x8*)(pj + S::P * S::PITCH_A + k * 32);
+            poly[o] = __builtin_amdgcn_mfma_f32_32x32x16_f16(il, jh, poly[o], 0, 0, 0);
+            poly[o] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ih, jl, poly[o], 0, 0, 0);
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) poly[o][r] = ldexpf(cb * acc[o][r], eb - ea) + ldexpf(cc * poly[o][r], eb - 2 * ea);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int o = 0; o < S::OWN; ++o) {
+      const int blk = w + 8 * o;
+      if (blk < S::BLOCKS) {
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+          // row (column of the block) c32, k = 8 (r / 4) + 4 h + e, at the place 16 (r / 8) + 8 h + 4 (r / 4 % 2) + e
+          char* at = lds + (blk % PB * 32 + c32) * S::PITCH_A + (blk / PB * 32 + 16 * (r >> 3) + 8 * h + 4 * ((r >> 2) & 1)) * 2;
+          f16x4 hi, lo;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            _Float16 u, v;
+            split(poly[o][r + e], &u, &v);
+            hi[e] = u;
+            lo[e] = v;
+          }
+          *(f16x4*)at = hi;
+          if (pairs) *(f16x4*)(at + S::P * S::PITCH_A) = lo;
+        }
+      }
+    }
+    __syncthreads();
+    // X <- a X + B X
+#pragma unroll
+    for (int c = 0; c < CB; ++c)
+      if (w + 8 * c < cols) {
+        f16x8 xh[2 * PB], xl[2 * PB];
+#pragma unroll
+        for (int k = 0; k < 2 * PB; ++k)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            _Float16 u, v;
+            split(x[c][k >> 1][8 * (k & 1) + e], &u, &v);
+            xh[k][e] = u;
+            xl[k][e] = v;
+          }
+#pragma unroll
+        for (int a = 0; a < PB; ++a) {
+          const char* pi = lds + (32 * a + c32) * S::PITCH_A + h * 16;
+          f32x16 s = f32x16{};
+#pragma unroll
+          for (int k = 0; k < 2 * PB; ++k) {
+            const f16x8 bh = *(const f16x8*)(pi + k * 32);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(bh, xh[k], s, 0, 0, 0);
+            if (pairs) {
+              const f16x8 bl = *(const f16x8*)(pi + S::P * S::PITCH_A + k * 32);
+              s = __builtin_amdgcn_mfma_f32_32x32x16_f16(bl, xh[k], s, 0, 0, 0);
+              s = __builtin_amdgcn_mfma_f32_32x32x16_f16(bh, xl[k], s, 0, 0, 0);
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) x[c][a][r] = ldexpf(ca * x[c][a][r], en - ex) + ldexpf(s[r], en - eb - ex);
+          __builtin_amdgcn_sched_barrier(0);  // (one row block's fragments of B at a time: registers)
+        }
+      }
+    __syncthreads();
+  }
+  T* y = out + blockIdx.x * (size_t)p * q;
+  const int en = z.ex[steps], rs = tall ? 1 : q, cs = tall ? p : 1;
+#pragma unroll
+  for (int c = 0; c < CB; ++c) {
+    const int j = (w + 8 * c) * 32 + c32;
+    const unsigned at = (unsigned)(4 * h * rs + j * cs) * (unsigned)sizeof(T);
+#pragma unroll
+    for (int a = 0; a < PB; ++a)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int iu = 32 * a + 8 * (r >> 2) + (r & 3);
+        char* row = (char*)(y + iu * rs);
+        if (iu + 4 * h < p && j < q) *(T*)(row + at) = (T)ldexpf(x[c][a][r], -en);
+      }
   }
 }
 

@@ -420,10 +420,10 @@ def orthogonalize(g, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: float = 1e
     out = sp.empty(shape, sp.types[kind])
     need = C.c_size_t()
     empty = not (batch and m and n)
-    lib.nls_orthogonalize_workspace(batch, m, n, need)
-    ws = None if empty else sp.scratch(need.value)
+    lib.nls_orthogonalize_workspace(batch, m, n, st[1], st[2], need)
+    ws = None if empty or not need.value else sp.scratch(need.value)
     _call(
         sp.ctx, lib.nls_orthogonalize, None if empty else sp.ptr(g), kind, batch, m, n, *st, table, steps, eps, sp.ptr(out),
-        None if empty else sp.ptr(ws), need.value, stream,
+        None if ws is None else sp.ptr(ws), need.value, stream,
     )  # fmt: skip
     return sp.done(out)
