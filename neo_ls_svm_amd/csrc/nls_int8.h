@@ -151,10 +151,9 @@ __device__ __forceinline__ float bias_at(const Int8Args& g, int n) {
 // (sum * a_scale) * b_scale, left to right: the product of the two scales alone may fall below the smallest float.
 __device__ __forceinline__ float scaled(int sum, float as, float bs, float bias) { return (float)sum * as * bs + bias; }
 
-// Many rows: P = b (its rows run along a lane's four consecutive registers, which are four neighbours of an output row), Q = a.
-template <class T, int BI, int BJ, int WI, int WJ>
-__global__ __launch_bounds__(64 * WI * WJ) void k_int8_tile(Int8Args g, int ti, int tj, int strip) {
-  using TL = Tile<MODE_I8, BI, BJ, WI, WJ>;
+// Many rows: P = b (its rows lie along a chunk's words, as neighbours in a row of y), Q = a.
+template <class T, class TL, int BI, int BJ>
+__global__ __launch_bounds__(TL::THREADS) void k_int8_tile(Int8Args g, int ti, int tj, int strip) {
   extern __shared__ char lds[];
   int bi, bj;
   strip_order(die_order(blockIdx.x, ti * tj), ti, tj, strip, &bi, &bj);
@@ -163,28 +162,32 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_int8_tile(Int8Args g, int ti, 
   const int steps = (g.k + 127) / 128;
   t.run(g.b, i0, g.a, j0, 0, steps, g.k - (steps - 1) * 128, lds);
   T* y = (T*)g.y;
-  const bool vec = g.n % 4 == 0;
+  // a thread has the same eight channels in all its rows
+  constexpr int ACROSS = BI / 8, ROWS = TL::THREADS / ACROSS;
+  const int iw = threadIdx.x % ACROSS * 8, n = i0 + iw, left = g.n - n;
+  float bs[8], bias[8];
 #pragma unroll
-  for (int b = 0; b < TL::MJ; ++b) {
-    const int m = j0 + TL::col_of(b);
-    if (m >= g.m) continue;
-    const float as = g.a_scale[m];
+  for (int e = 0; e < 8; ++e) {
+    bs[e] = e < left ? g.b_scale[n + e] : 0.0f;
+    bias[e] = e < left ? bias_at<T>(g, n + e) : 0.0f;
+  }
+  const bool whole = left >= 8 && g.n % (16 / (int)sizeof(T)) == 0;
 #pragma unroll
-    for (int a = 0; a < TL::MI; ++a)
+  for (int c = 0; c < TL::CHUNKS; ++c) {
+    __syncthreads();
+    t.spill(c, lds);
+    __syncthreads();
+    for (int r = threadIdx.x / ACROSS; r < TL::CHUNK; r += ROWS) {
+      const int m = j0 + TL::column(c, r);
+      if (m >= g.m || left <= 0) continue;
+      int s[8];
+      chunk_sums<TL>(lds, r, iw, s);
+      const float as = g.a_scale[m];
+      float v[8];
 #pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const int n = i0 + TL::row_of(a) + 2 * r;
-        if (vec && n < g.n) {
-          typename Vec4<T>::type v;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = (T)scaled(t.acc[a][b][r + e], as, g.b_scale[n + e], bias_at<T>(g, n + e));
-          *(typename Vec4<T>::type*)(y + (size_t)m * g.n + n) = v;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (n + e < g.n) y[(size_t)m * g.n + n + e] = (T)scaled(t.acc[a][b][r + e], as, g.b_scale[n + e], bias_at<T>(g, n + e));
-        }
-      }
+      for (int e = 0; e < 8; ++e) v[e] = scaled(s[e], as, bs[e], bias[e]);
+      store8(y + (size_t)m * g.n + n, v, left, whole);
+    }
   }
 }
 
@@ -248,15 +251,6 @@ __device__ __forceinline__ void few_quantise(const Int8Args& g, const FewX& f, s
     }
   }
   __syncthreads();
-}
-
-__device__ __forceinline__ i32x4 keep_bytes(i32x4 v, int n) {  // the first n of 16 bytes, the others zero
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const int b = n - 4 * w;
-    v[w] = b >= 4 ? v[w] : b <= 0 ? 0 : (v[w] & ((1 << (8 * b)) - 1));
-  }
-  return v;
 }
 
 template <class T, int MG, int NG, bool FUSED>

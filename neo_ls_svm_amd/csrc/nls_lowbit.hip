@@ -79,12 +79,12 @@ int quantize_any(nls_ctx* ctx, const void* x, int type, long rows, long k, long 
 }
 
 // ---- 8-bit product ----
-template <class T, int BI, int BJ, int WI, int WJ>
+template <class T, class TL, int BI, int BJ>
 int int8_tile(nls_ctx* ctx, const Int8Args& g, hipStream_t st) {
-  using TL = Tile<MODE_I8, BI, BJ, WI, WJ>;
   const int ti = (g.n + BI - 1) / BI, tj = (g.m + BJ - 1) / BJ;
-  NLSCHK(ask_lds(ctx, k_int8_tile<T, BI, BJ, WI, WJ>, TL::LDS));
-  k_int8_tile<T, BI, BJ, WI, WJ><<<dim3((unsigned)((long)ti * tj)), TL::THREADS, TL::LDS, st>>>(g, ti, tj, 8);
+  constexpr int LDS = std::max(TL::LDS, TL::SCRATCH);
+  NLSCHK(ask_lds(ctx, k_int8_tile<T, TL, BI, BJ>, LDS));
+  k_int8_tile<T, TL, BI, BJ><<<dim3((unsigned)((long)ti * tj)), TL::THREADS, LDS, st>>>(g, ti, tj, 8);
   LAUNCHED(ctx, "int8_matmul");
   return NLS_OK;
 }
@@ -109,8 +109,8 @@ int int8_product(nls_ctx* ctx, const Int8Args& g, hipStream_t st) {
   if (g.m <= 48) return int8_few<T, 3>(ctx, g, st);
   if (g.m <= 64) return int8_few<T, 4>(ctx, g, st);
   const long big = (long)((g.n + 127) / 128) * ((g.m + 127) / 128);
-  if (big >= ctx->cus) return int8_tile<T, 128, 128, 2, 2>(ctx, g, st);
-  return int8_tile<T, 64, 64, 2, 2>(ctx, g, st);
+  if (big >= ctx->cus) return int8_tile<T, Tile<MODE_I8, 128, 128, 2, 2, 2>, 128, 128>(ctx, g, st);
+  return int8_tile<T, Ring<MODE_I8, 2>, 64, 64>(ctx, g, st);
 }
 // Whether int8_linear quantises inside the product: every workgroup does all the rows of x over again, which has to stay small beside its share of b.
 bool int8_fused(long m, long k) { return m <= 4 && m * k <= 32768; }
@@ -183,25 +183,32 @@ NsPlan ns_plan(long m, long n, long batch, long row_stride, long col_stride) {
   return w;
 }
 
-template <int KIND, class T, int MODE, int B, int W>
+template <int KIND, class T, class TL, int MODE, int B>
 int ns_product_tile(nls_ctx* ctx, NsArgs g, long batch, hipStream_t st) {
-  using TL = Tile<MODE, B, B, W, W>;
-  constexpr int LDS = TL::LDS > TL::WAVES * 32 * 33 * 4 ? TL::LDS : TL::WAVES * 32 * 33 * 4;
   g.ti = (g.I + B - 1) / B;
   g.tj = (g.J + B - 1) / B;
   g.strip = 8;
   constexpr bool SYM = KIND == NS_GRAM || KIND == NS_POLY;
+  constexpr int LDS = std::max(TL::LDS, TL::SCRATCH);
   const long tiles = SYM ? (long)g.ti * (g.ti + 1) / 2 : (long)g.ti * g.tj;
-  NLSCHK(ask_lds(ctx, k_ns_product<KIND, T, MODE, B, B, W, W>, LDS));
-  k_ns_product<KIND, T, MODE, B, B, W, W><<<dim3((unsigned)tiles, 1, (unsigned)batch), TL::THREADS, LDS, st>>>(g);
+  NLSCHK(ask_lds(ctx, k_ns_product<KIND, T, TL, MODE, B, B>, LDS));
+  k_ns_product<KIND, T, TL, MODE, B, B><<<dim3((unsigned)tiles, 1, (unsigned)batch), TL::THREADS, LDS, st>>>(g);
   LAUNCHED(ctx, "orthogonalize");
   return NLS_OK;
 }
+template <int KIND, class T, int MODE>
+int ns_product(nls_ctx* ctx, const NsArgs& g, long batch, hipStream_t st) {
+  constexpr bool SYM = KIND == NS_GRAM || KIND == NS_POLY;
+  auto tiles = [&](long b) {
+    const long i = (g.I + b - 1) / b, j = (g.J + b - 1) / b;
+    return (SYM ? i * (i + 1) / 2 : i * j) * batch;
+  };
+  if (tiles(128) >= ctx->cus) return ns_product_tile<KIND, T, Tile<MODE, 128, 128, 2, 2, 2>, MODE, 128>(ctx, g, batch, st);
+  return ns_product_tile<KIND, T, Ring<MODE, 2>, MODE, 64>(ctx, g, batch, st);
+}
 template <int KIND, class T>
 int ns_product(nls_ctx* ctx, const NsArgs& g, bool pairs, long batch, hipStream_t st) {
-  const long big = (long)((g.I + 127) / 128) * ((g.J + 127) / 128) * batch;
-  if (big >= ctx->cus) return pairs ? ns_product_tile<KIND, T, MODE_F16PAIR, 128, 2>(ctx, g, batch, st) : ns_product_tile<KIND, T, MODE_F16, 128, 2>(ctx, g, batch, st);
-  return pairs ? ns_product_tile<KIND, T, MODE_F16PAIR, 64, 2>(ctx, g, batch, st) : ns_product_tile<KIND, T, MODE_F16, 64, 2>(ctx, g, batch, st);
+  return pairs ? ns_product<KIND, T, MODE_F16PAIR>(ctx, g, batch, st) : ns_product<KIND, T, MODE_F16>(ctx, g, batch, st);
 }
 
 template <class T, int PB, int CB>
@@ -251,9 +258,6 @@ int orthogonalize(nls_ctx* ctx, const NsMatrix& w, const NsPlan& plan, bool tall
   for (int t = 0; t < steps; ++t) {
     const bool pairs = t >= steps - exact;
     g.t = t;
-    g.a = (float)cf.a[t];
-    g.b = (float)cf.b[t];
-    g.c = (float)cf.c[t];
     g.P = g.Q = X;
     g.D = A;
     g.I = g.J = p;
@@ -410,10 +414,8 @@ extern "C" int nls_orthogonalize(nls_ctx* ctx, const void* g, int type, int64_t 
   NsCoef cf{};
   double u = 1.0;
   for (int t = 0; t < steps; ++t) {
-    cf.a[t] = coefficients[3 * t];
-    cf.b[t] = coefficients[3 * t + 1];
-    cf.c[t] = coefficients[3 * t + 2];
-    u = ns_peak_x(cf.a[t], cf.b[t], cf.c[t], u) * (1.0 + 1e-3);
+    ns_step(coefficients[3 * t], coefficients[3 * t + 1], coefficients[3 * t + 2], &cf.s[t]);
+    u = ns_peak_x(cf.s[t], u) * (1.0 + 1e-3);
     if (!(u < 1e6)) return fail(ctx, NLS_ERR_ARG, "orthogonalize: the coefficients let singular values grow past 1e6 in step %d", t + 1);
   }
   if (m > (1 << 20) || n > (1 << 20) || batch > 65535) return fail(ctx, NLS_ERR_ARG, "orthogonalize: at most 2^20 rows and columns and 65535 matrices");

@@ -7,19 +7,34 @@
 // the singular values (polynomial extrema, from the norm on), so that entries stay below 2^15 and neither half leaves fp16's range.  A product of
 // pairs is hi hi + lo hi + hi lo (the dropped lo lo is below 2^-22 of a term), three matrix instructions at 16 x the rate of the fp32 one.
 #pragma once
+#include <cmath>
+
 #include "nls_tile.h"
 
 namespace lb {
 
-constexpr int NS_MAX_STEPS = 64;
+constexpr int NS_MAX_STEPS = 32;
 constexpr int NS_PARTS = 256;  // partial sums of squares a matrix
 
+// X_t, A_t, B_t are held times 2^ex, 2^ea, 2^eb (of their step); what a product's sum w becomes the next held matrix with:
+struct NsFactors {
+  float gram;            // A: gram w
+  float lin, quad;       // B: lin A + quad w
+  float keep, add;       // next X: keep X + add w
+};
 struct NsScales {  // one per matrix
-  double inv;      // 1 / (|G|_F + eps); NaN when the norm is not finite: the whole result is then NaN
-  int ex[NS_MAX_STEPS + 1], ea[NS_MAX_STEPS], eb[NS_MAX_STEPS];  // X_t, A_t, B_t are held times 2^ex, 2^ea, 2^eb
+  double first;    // G to held X_0; NaN when the norm is not finite: the whole result is then NaN
+  int last;        // the result is held X times 2^last
+  NsFactors f[NS_MAX_STEPS];
+};
+// A step's polynomial a s + b s^3 + c s^5 and where it and b z + c z^2 have their extrema (host: ns_coefficients)
+struct NsStep {
+  double a, b, c;
+  double xs[2], xv[2];   // s > 0 and the absolute value there
+  double zs, zv;
 };
 struct NsCoef {
-  double a[NS_MAX_STEPS], b[NS_MAX_STEPS], c[NS_MAX_STEPS];
+  NsStep s[NS_MAX_STEPS];
 };
 
 // A matrix of fp16 pairs: granules of 32 elements, 64 bytes hi then 64 bytes lo; rows padded with zeros to 64 elements.
@@ -54,51 +69,65 @@ __global__ __launch_bounds__(256) void k_ns_norm(NsMatrix w, double* parts) {
   if (threadIdx.x == 0) parts[(size_t)blockIdx.y * NS_PARTS + blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
 }
 
-__host__ __device__ inline double ns_peak_x(double a, double b, double c, double u) {  // max |a s + b s^3 + c s^5| on [0, u]
-  auto f = [&](double s) { return fabs(s * (a + s * s * (b + c * s * s))); };
-  double top = f(u);
+inline void ns_step(double a, double b, double c, NsStep* o) {
+  *o = NsStep{a, b, c, {INFINITY, INFINITY}, {0.0, 0.0}, INFINITY, 0.0};
+  auto at = [&](int k, double z) {  // z = s^2
+    if (!(z > 0.0) || !std::isfinite(z)) return;
+    o->xs[k] = std::sqrt(z);
+    o->xv[k] = std::fabs(o->xs[k] * (a + z * (b + c * z)));
+  };
   const double d = 9.0 * b * b - 20.0 * a * c;
   if (c != 0.0 && d >= 0.0) {
-    for (int k = -1; k <= 1; k += 2) {
-      const double z = (-3.0 * b + k * sqrt(d)) / (10.0 * c);
-      if (z > 0.0 && z < u * u) top = fmax(top, f(sqrt(z)));
-    }
+    at(0, (-3.0 * b - std::sqrt(d)) / (10.0 * c));
+    at(1, (-3.0 * b + std::sqrt(d)) / (10.0 * c));
   } else if (c == 0.0 && b != 0.0) {
-    const double z = -a / (3.0 * b);
-    if (z > 0.0 && z < u * u) top = fmax(top, f(sqrt(z)));
+    at(0, -a / (3.0 * b));
   }
+  if (c != 0.0 && -b / (2.0 * c) > 0.0) {
+    o->zs = -b / (2.0 * c);
+    o->zv = std::fabs(o->zs * (b + c * o->zs));
+  }
+}
+__host__ __device__ inline double ns_peak_x(const NsStep& s, double u) {  // max |a s + b s^3 + c s^5| on [0, u]
+  double top = fabs(u * (s.a + u * u * (s.b + s.c * u * u)));
+  if (s.xs[0] < u) top = fmax(top, s.xv[0]);
+  if (s.xs[1] < u) top = fmax(top, s.xv[1]);
   return top;
 }
-__host__ __device__ inline double ns_peak_b(double b, double c, double u) {  // max |b z + c z^2| on [0, u^2]
-  auto f = [&](double z) { return fabs(z * (b + c * z)); };
-  double top = f(u * u);
-  if (c != 0.0) {
-    const double z = -b / (2.0 * c);
-    if (z > 0.0 && z < u * u) top = fmax(top, f(z));
-  }
-  return top;
+__host__ __device__ inline double ns_peak_b(const NsStep& s, double u) {  // max |b z + c z^2| on [0, u^2]
+  const double z = u * u, top = fabs(z * (s.b + s.c * z));
+  return s.zs < z ? fmax(top, s.zv) : top;
 }
 // 15 - e with |v| < 2^e: what is bounded by v is held below 2^15 (fp16 ends at 65504: a factor of two for the roundings)
 __device__ __forceinline__ int ns_exponent(double v) {
-  if (!(v > 0.0) || !(v < 1e300)) return 0;
-  int e;
-  (void)frexp(v, &e);
-  return 15 - e;
+  const int e = (int)((__double_as_longlong(v) >> 52) & 2047);  // v in [2^(e - 1023), 2^(e - 1022))
+  return e == 0 || e == 2047 ? 0 : 15 - (e - 1022);
 }
+// 2^e.  Past the ends of float32 the nearest power in it: a product that needs a smaller one has no share in a sum beside a term below 2^15.
+__device__ __forceinline__ float ns_pow2(int e) { return __int_as_float((min(max(e, -126), 127) + 127) << 23); }
 
-// squares: |G|_F^2
+// squares: |G|_F^2.  Bounds on the singular values of X_t, from |X_0| <= |X_0|_F on, choose the powers of two.
 __device__ __forceinline__ void ns_scales(double squares, double eps, const NsCoef& cf, int steps, NsScales& z) {
   const double norm = sqrt(squares);
   const bool fine = norm < 1e300;
-  z.inv = fine ? (norm + eps > 0.0 ? 1.0 / (norm + eps) : 0.0) : __longlong_as_double(0x7ff8000000000000ll);
-  double u = fine ? norm * z.inv * (1.0 + 1e-3) : 1.0;  // |X_0| <= |X_0|_F
+  const double inv = fine ? (norm + eps > 0.0 ? 1.0 / (norm + eps) : 0.0) : __longlong_as_double(0x7ff8000000000000ll);
+  double u = fine ? norm * inv * (1.0 + 1e-3) : 1.0;
+  int ex = ns_exponent(u);
+  z.first = ldexp(inv, ex);
   for (int t = 0; t < steps; ++t) {
-    z.ex[t] = ns_exponent(u);
-    z.ea[t] = ns_exponent(u * u);
-    z.eb[t] = ns_exponent(ns_peak_b(cf.b[t], cf.c[t], u));
-    u = ns_peak_x(cf.a[t], cf.b[t], cf.c[t], u) * (1.0 + 1e-3);
+    const NsStep& s = cf.s[t];
+    const int ea = ns_exponent(u * u), eb = ns_exponent(ns_peak_b(s, u));
+    u = ns_peak_x(s, u) * (1.0 + 1e-3);
+    const int en = ns_exponent(u);
+    NsFactors& f = z.f[t];
+    f.gram = ns_pow2(ea - 2 * ex);
+    f.lin = (float)s.b * ns_pow2(eb - ea);
+    f.quad = (float)s.c * ns_pow2(eb - 2 * ea);
+    f.keep = (float)s.a * ns_pow2(en - ex);
+    f.add = ns_pow2(en - eb - ex);
+    ex = en;
   }
-  z.ex[steps] = ns_exponent(u);
+  z.last = -ex;
 }
 
 __global__ __launch_bounds__(64) void k_ns_scales(const double* parts, int count, double eps, NsCoef cf, int steps, NsScales* out) {
@@ -122,7 +151,7 @@ __global__ __launch_bounds__(256) void k_ns_pack(NsMatrix w, const NsScales* sca
   x += blockIdx.z * batch_bytes;
   xt += blockIdx.z * batch_bytes;
   const NsScales& z = scales[blockIdx.z];
-  const double f = ldexp(z.inv, z.ex[0]);
+  const double f = z.first;
   const long p0 = (long)blockIdx.y * 64, q0 = (long)blockIdx.x * 64;
   const bool along_q = w.col_stride <= w.row_stride;
   const int l = threadIdx.x & 63, r = threadIdx.x >> 6;
@@ -166,24 +195,24 @@ struct NsArgs {
   int I, J, K;
   int ti, tj, strip;
   int t;                  // step
-  float a, b, c;
   int transposed;         // LAST: out is stored q x p
 };
 
-// One 32 x 32 block, value(i, j) in the accumulator's places, to row-major pairs with rows i (the transposed orientation), through the wave's own LDS.
-__device__ __forceinline__ void block_turn(const f32x16& v, float* scratch, float* line) {
-  const int l = (int)(threadIdx.x & 63);
+__device__ __forceinline__ void store_pairs(char* at, const float (&v)[8]) {  // eight neighbours of a row of pairs
+  f16x8 h, o;
 #pragma unroll
-  for (int r = 0; r < 16; ++r) scratch[(8 * (r >> 2) + 4 * (l >> 5) + (r & 3)) * 33 + (l & 31)] = v[r];
-  __builtin_amdgcn_wave_barrier();
-#pragma unroll
-  for (int e = 0; e < 16; ++e) line[e] = scratch[(l >> 1) * 33 + (l & 1) * 16 + e];
-  __builtin_amdgcn_wave_barrier();
+  for (int e = 0; e < 8; ++e) {
+    _Float16 hi, lo;
+    split(v[e], &hi, &lo);
+    h[e] = hi;
+    o[e] = lo;
+  }
+  *(f16x8*)at = h;
+  *(f16x8*)(at + 64) = o;
 }
 
-template <int KIND, class T, int MODE, int BI, int BJ, int WI, int WJ>
-__global__ __launch_bounds__(64 * WI * WJ) void k_ns_product(NsArgs g) {
-  using TL = Tile<MODE, BI, BJ, WI, WJ>;
+template <int KIND, class T, class TL, int MODE, int BI, int BJ>
+__global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
   extern __shared__ char lds[];
   constexpr bool SYM = KIND == NS_GRAM || KIND == NS_POLY;
   int bi, bj;
@@ -203,93 +232,66 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_ns_product(NsArgs g) {
   const int per = MODE == MODE_F16 ? 64 : 32;
   t.run(Operand{g.P + off, (unsigned)ldk, g.I}, i0, Operand{g.Q + off, (unsigned)ldk, g.J}, j0, 0, (g.K + per - 1) / per, 128, lds);
   const NsScales& z = g.scales[blockIdx.z];
-  const int ex = z.ex[g.t], ea = z.ea[g.t], eb = z.eb[g.t], en = z.ex[g.t + 1];
+  const NsFactors f = z.f[g.t];
+  const int last = z.last;
   const char* E = g.E + off;
   char* D = g.D + off;
-  char* DT = g.DT + off;
+  char* DT = SYM ? D : g.DT + off;
   T* out = (T*)g.out + blockIdx.z * g.out_stride;
-  __syncthreads();  // the tile's LDS becomes the waves' scratch
-  float* scratch = (float*)lds + TL::wave() * (32 * 33);
-  const int l = TL::lane();
+  const bool natural = KIND != NS_LAST || !g.transposed, turned = KIND == NS_LAST ? g.transposed != 0 : SYM ? bi != bj : true;
+  // Chunks of the tile through LDS: the result in the product's own orientation (rows j, eight neighbours i a thread), then, from the values left
+  // there, its transpose (rows i, eight neighbours j).
+  constexpr int ACROSS = BI / 8, ROWS = TL::THREADS / ACROSS;
+  const int iw = threadIdx.x % ACROSS * 8, i = i0 + iw;
+  constexpr int DOWN = TL::CHUNK / 8;
+  const int iv = threadIdx.x / DOWN, rv = threadIdx.x % DOWN * 8;
 #pragma unroll
-  for (int b = 0; b < TL::MJ; ++b) {
-    const int j = j0 + TL::col_of(b);
-#pragma unroll
-    for (int a = 0; a < TL::MI; ++a) {
-      f32x16 v = t.acc[a][b];
-      const int ib = i0 + TL::row_of(a);  // + 8 (r / 4) + r % 4
-#pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const int i = ib + 2 * r;
-        float e[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (KIND != NS_GRAM && j < g.J && i < g.I) {  // (rows of E are padded: whole groups of four)
-          const char* at = E + pair_at(j, i, ldi);
-          const f16x4 h = *(const f16x4*)at, o = *(const f16x4*)(at + 64);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) e[k] = (float)h[k] + (float)o[k];
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          float w = v[r + k];
-          if (KIND == NS_GRAM) w = ldexpf(w, ea - 2 * ex);
-          if (KIND == NS_POLY) w = ldexpf(g.b * e[k], eb - ea) + ldexpf(g.c * w, eb - 2 * ea);
-          if (KIND == NS_STEP) w = ldexpf(g.a * e[k], en - ex) + ldexpf(w, en - eb - ex);
-          if (KIND == NS_LAST) w = ldexpf(g.a * e[k] + ldexpf(w, -eb), -ex);
-          v[r + k] = (i + k < g.I && j < g.J) ? w : 0.0f;
-        }
-        if (KIND != NS_LAST) {
-          if (j < g.J && (size_t)i * 4 < ldi) {
-            f16x4 h, o;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              _Float16 hk, ok;
-              split(v[r + k], &hk, &ok);
-              h[k] = hk;
-              o[k] = ok;
-            }
-            char* at = D + pair_at(j, i, ldi);
-            *(f16x4*)at = h;
-            *(f16x4*)(at + 64) = o;
-          }
-        } else if (!g.transposed && j < g.J) {
-          if (g.I % 4 == 0 && i < g.I) {
-            typename Vec4<T>::type y;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) y[k] = (T)v[r + k];
-            *(typename Vec4<T>::type*)(out + (size_t)j * g.I + i) = y;
-          } else {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (i + k < g.I) out[(size_t)j * g.I + i + k] = (T)v[r + k];
-          }
-        }
+  for (int c = 0; c < TL::CHUNKS; ++c) {
+    __syncthreads();
+    t.spill(c, lds);
+    __syncthreads();
+    for (int r = threadIdx.x / ACROSS; r < TL::CHUNK; r += ROWS) {
+      const int j = j0 + TL::column(c, r);
+      float v[8];
+      chunk_sums<TL>(lds, r, iw, v);
+      f16x8 eh = {}, el = {};
+      const bool there = j < g.J && (size_t)i * 4 < ldi;  // (rows are padded: whole groups of eight, zeros behind the end)
+      if (KIND != NS_GRAM && there) {
+        const char* at = E + pair_at(j, i, ldi);
+        eh = *(const f16x8*)at;
+        el = *(const f16x8*)(at + 64);
       }
-      const bool turn = KIND == NS_LAST ? g.transposed != 0 : SYM ? bi != bj : true;
-      if (turn) {
-        float line[16];
-        block_turn(v, scratch, line);
-        const int i = i0 + (TL::wave() / WJ * TL::MI + a) * 32 + (l >> 1);
-        const int jb = j0 + (TL::wave() % WJ * TL::MJ + b) * 32 + (l & 1) * 16;
-        if (KIND == NS_LAST) {
-          if (i < g.I) {
 #pragma unroll
-            for (int k = 0; k < 16; ++k)
-              if (jb + k < g.J) out[(size_t)i * g.J + jb + k] = (T)line[k];
-          }
-        } else if (i < g.I && (size_t)jb * 4 < ldj) {
-          f16x8 hi[2], lo[2];
+      for (int e = 0; e < 8; ++e) {
+        const float x = (float)eh[e] + (float)el[e];
+        float w = v[e];
+        if (KIND == NS_GRAM) w = f.gram * w;
+        if (KIND == NS_POLY) w = f.lin * x + f.quad * w;
+        if (KIND == NS_STEP) w = f.keep * x + f.add * w;
+        if (KIND == NS_LAST) w = ldexpf(f.keep * x + f.add * w, last);
+        v[e] = i + e < g.I && j < g.J ? w : 0.0f;
+      }
+      if (turned)
 #pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            _Float16 h, o;
-            split(line[k], &h, &o);
-            hi[k >> 3][k & 7] = h;
-            lo[k >> 3][k & 7] = o;
-          }
-          char* at = (SYM ? D : DT) + pair_at(i, jb, ldj);
-          *(f16x8*)at = hi[0];
-          *(f16x8*)(at + 16) = hi[1];
-          *(f16x8*)(at + 64) = lo[0];
-          *(f16x8*)(at + 80) = lo[1];
+        for (int e = 0; e < 8; ++e) ((float*)lds)[r * TL::PITCH + iw + e] = v[e];
+      if (KIND != NS_LAST) {
+        if (there) store_pairs(D + pair_at(j, i, ldi), v);
+      } else if (natural && j < g.J && i < g.I) {
+        store8(out + (size_t)j * g.I + i, v, g.I - i, i + 8 <= g.I && g.I % (16 / (int)sizeof(T)) == 0);
+      }
+    }
+    if (turned) {
+      __syncthreads();
+      for (int ii = iv; ii < BI; ii += TL::THREADS / DOWN) {
+        const int irow = i0 + ii, j = j0 + TL::column(c, rv);
+        if (irow >= g.I) continue;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = ((const float*)lds)[(rv + e) * TL::PITCH + ii];
+        if (KIND != NS_LAST) {
+          if ((size_t)j * 4 < ldj) store_pairs(DT + pair_at(irow, j, ldj), v);
+        } else if (j < g.J) {
+          store8(out + (size_t)irow * g.J + j, v, g.J - j, j + 8 <= g.J && g.J % (16 / (int)sizeof(T)) == 0);
         }
       }
     }
@@ -366,7 +368,7 @@ __global__ __launch_bounds__(512) void k_ns_small(NsMatrix m, NsCoef cf, int ste
   }
   __syncthreads();
   {
-    const double f = ldexp(z.inv, z.ex[0]);
+    const double f = z.first;
 #pragma unroll
     for (int c = 0; c < CB; ++c)
 #pragma unroll
@@ -377,8 +379,7 @@ __global__ __launch_bounds__(512) void k_ns_small(NsMatrix m, NsCoef cf, int ste
   const int pitch = S::pitch_x(q);
   for (int t = 0; t < steps; ++t) {
     const bool pairs = t >= steps - exact;
-    const int ex = z.ex[t], ea = z.ea[t], eb = z.eb[t], en = z.ex[t + 1];
-    const float ca = (float)cf.a[t], cb = (float)cf.b[t], cc = (float)cf.c[t];
+    const NsFactors f = z.f[t];
     // X to LDS, hi plane then lo plane
 #pragma unroll
     for (int c = 0; c < CB; ++c)
@@ -435,7 +436,7 @@ __global__ __launch_bounds__(512) void k_ns_small(NsMatrix m, NsCoef cf, int ste
       const int blk = w + 8 * o;
       if (blk < S::BLOCKS) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[o][r] = ldexpf(acc[o][r], ea - 2 * ex);
+        for (int r = 0; r < 16; ++r) acc[o][r] *= f.gram;
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
           char* at = lds + (blk % PB * 32 + c32) * S::PITCH_A + (blk / PB * 32 + 2 * r + 4 * h) * 2;
@@ -473,7 +474,7 @@ __global__ __launch_bounds__(512) void k_ns_small(NsMatrix m, NsCoef cf, int ste
           }
         }
 #pragma unroll
-        for (int r = 0; r < 16; ++r) poly[o][r] = ldexpf(cb * acc[o][r], eb - ea) + ldexpf(cc * poly[o][r], eb - 2 * ea);
+        for (int r = 0; r < 16; ++r) poly[o][r] = f.lin * acc[o][r] + f.quad * poly[o][r];
       }
     }
     __syncthreads();
@@ -528,14 +529,14 @@ __global__ __launch_bounds__(512) void k_ns_small(NsMatrix m, NsCoef cf, int ste
             }
           }
 #pragma unroll
-          for (int r = 0; r < 16; ++r) x[c][a][r] = ldexpf(ca * x[c][a][r], en - ex) + ldexpf(s[r], en - eb - ex);
+          for (int r = 0; r < 16; ++r) x[c][a][r] = f.keep * x[c][a][r] + f.add * s[r];
           __builtin_amdgcn_sched_barrier(0);  // (one row block's fragments of B at a time: registers)
         }
       }
     __syncthreads();
   }
   T* y = out + blockIdx.x * (size_t)p * q;
-  const int en = z.ex[steps], rs = tall ? 1 : q, cs = tall ? p : 1;
+  const int last = z.last, rs = tall ? 1 : q, cs = tall ? p : 1;
 #pragma unroll
   for (int c = 0; c < CB; ++c) {
     const int j = (w + 8 * c) * 32 + c32;
@@ -546,7 +547,7 @@ __global__ __launch_bounds__(512) void k_ns_small(NsMatrix m, NsCoef cf, int ste
       for (int r = 0; r < 16; ++r) {
         const int iu = 32 * a + 8 * (r >> 2) + (r & 3);
         char* row = (char*)(y + iu * rs);
-        if (iu + 4 * h < p && j < q) *(T*)(row + at) = (T)ldexpf(x[c][a][r], -en);
+        if (iu + 4 * h < p && j < q) *(T*)(row + at) = (T)ldexpf(x[c][a][r], last);
       }
   }
 }

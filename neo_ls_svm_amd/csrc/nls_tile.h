@@ -3,7 +3,8 @@
 //
 // One K step is 128 bytes of every operand row, whatever the type: 128 int8, 64 fp16, or 32 fp16 pairs (a row holds granules of 64 bytes hi and
 // 64 bytes lo per 32 elements).  The rows travel from memory to LDS without touching registers (16 bytes a lane, a wave moves 8 whole rows =
-// eight full 128-byte lines), into the other half of a double buffer while the matrix cores work on this half.
+// eight full 128-byte lines), into the next of STAGES buffers while the matrix cores work on this one: the fewer workgroups share a compute unit, the more steps have to be
+// under way to cover the way to memory.
 //
 // LDS holds a tile row at r * 128, its 16-byte chunk c at slot c ^ (r & 7): a fragment read takes the same chunk of 32 rows, so any 8 neighbouring
 // lanes touch 8 different slots - every bank once.  The writing side needs no scatter: the lane that fills slot s simply fetches chunk s ^ (r & 7).
@@ -46,13 +47,71 @@ __device__ __forceinline__ unsigned chunk_offset(int c) {
   return MODE == MODE_F16 ? (unsigned)((c >> 2) * 128 + (c & 3) * 16) : (unsigned)(c * 16);
 }
 
+__device__ __forceinline__ i32x4 keep_bytes(i32x4 v, int n) {  // the first n of 16 bytes, the others zero
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const int b = n - 4 * w;
+    v[w] = b >= 4 ? v[w] : b <= 0 ? 0 : (v[w] & ((1 << (8 * b)) - 1));
+  }
+  return v;
+}
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
+__device__ __forceinline__ int lane_id() { return (int)(threadIdx.x & 63); }
+// 16 bytes a lane from memory to LDS (lane after lane from `lds` on)
+__device__ __forceinline__ void move16(const char* base, unsigned off, char* lds) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(base + off), (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+}
+// A move takes 8 rows: the lane's row is lane >> 3, its slot lane & 7, hence its chunk slot ^ (row & 7); moves start at multiples of 8 rows.
+__device__ __forceinline__ int move_chunk() { return (lane_id() & 7) ^ ((lane_id() >> 3) & 7); }
+// Chunks past the valid bytes of a ragged step are fetched from its start instead: how far back the lane goes.
+__device__ __forceinline__ unsigned move_back(int valid) { return move_chunk() * 16 >= valid ? (unsigned)move_chunk() * 16 : 0u; }
+
+// Fragments of one K step for MI x MJ blocks, and their products.  p, q: the lane's row (lane & 31) of the first block; blocks are 4096 bytes apart.
+template <int MODE, int MI, int MJ>
+struct Frags {
+  static constexpr int SUB = MODE == MODE_F16PAIR ? 2 : 4;  // instructions' worth of K in a step
+  static constexpr int KINDS = MODE == MODE_F16PAIR ? 2 : 1;
+  i32x4 p[SUB][KINDS][MI], q[SUB][KINDS][MJ];
+  using Acc = typename AccOf<MODE>::type;
+
+  template <bool TAIL>
+  __device__ __forceinline__ void read(int s, const char* pr, const char* qr, int valid) {
+    const int x = lane_id() & 7, h = lane_id() >> 5;
+#pragma unroll
+    for (int k = 0; k < KINDS; ++k) {
+      const int c = ((4 * k * (MODE == MODE_F16PAIR) + 2 * s + h) ^ x) * 16;
+#pragma unroll
+      for (int a = 0; a < MI; ++a) p[s][k][a] = *(const i32x4*)(pr + a * 4096 + c);
+#pragma unroll
+      for (int b = 0; b < MJ; ++b) {
+        q[s][k][b] = *(const i32x4*)(qr + b * 4096 + c);
+        if (TAIL) q[s][k][b] = keep_bytes(q[s][k][b], valid - (2 * s + h) * 16);
+      }
+    }
+  }
+  __device__ __forceinline__ static Acc product(const i32x4& u, const i32x4& v, const Acc& c) {
+    if constexpr (MODE == MODE_I8)
+      return __builtin_amdgcn_mfma_i32_32x32x32_i8(u, v, c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, u), __builtin_bit_cast(f16x8, v), c, 0, 0, 0);
+  }
+  __device__ __forceinline__ void multiply(int s, Acc (&acc)[MI][MJ]) const {
+#pragma unroll
+    for (int k = 0; k < (KINDS == 2 ? 3 : 1); ++k)  // pairs: hi hi, lo hi, hi lo
+#pragma unroll
+      for (int a = 0; a < MI; ++a)
+#pragma unroll
+        for (int b = 0; b < MJ; ++b) acc[a][b] = product(p[s][KINDS == 2 ? k == 1 : 0][a], q[s][KINDS == 2 ? k == 2 : 0][b], acc[a][b]);
+  }
+};
+
 struct Operand {
   const char* base;  // 16-byte aligned
   unsigned ld;       // bytes from row to row, a multiple of 16
   int rows;
 };
 
-template <int MODE, int BI, int BJ, int WI, int WJ>
+template <int MODE, int BI, int BJ, int WI, int WJ, int STAGES>
 struct Tile {
   static constexpr int WAVES = WI * WJ;
   static constexpr int THREADS = 64 * WAVES;
@@ -61,7 +120,9 @@ struct Tile {
   static constexpr int LOADS_P = BI / 8 / WAVES;  // 8-row moves a wave makes per step
   static constexpr int LOADS_Q = BJ / 8 / WAVES;
   static constexpr int BUF = (BI + BJ) * 128;
-  static constexpr int LDS = 2 * BUF;
+  static constexpr int LDS = STAGES * BUF;
+  static constexpr int FLIGHT = (LOADS_P + LOADS_Q) * (STAGES - 2);  // moves of a wave that may still be under way when a step begins
+  static_assert(STAGES >= 2 && FLIGHT <= 63, "the counter of moves under way ends at 63");
   static_assert(LOADS_P * 8 * WAVES == BI && LOADS_Q * 8 * WAVES == BJ && LOADS_P > 0 && LOADS_Q > 0, "tile rows must divide over the waves");
   static_assert(MI * WI * 32 == BI && MJ * WJ * 32 == BJ, "tile must divide over the waves");
   using Acc = typename AccOf<MODE>::type;
@@ -69,18 +130,9 @@ struct Tile {
   Acc acc[MI][MJ];
   unsigned offp[LOADS_P], offq[LOADS_Q];
 
-  __device__ __forceinline__ static int wave() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
-  __device__ __forceinline__ static int lane() { return (int)(threadIdx.x & 63); }
-
-  __device__ __forceinline__ static void move(const char* base, unsigned off, char* lds) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(base + off), (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
-  }
-  // The lane's place: row (lane >> 3) of the move, slot (lane & 7), hence chunk slot ^ (row & 7); moves start at multiples of 8 rows.
-  __device__ __forceinline__ static int my_chunk() { return (lane() & 7) ^ ((lane() >> 3) & 7); }
-
   __device__ __forceinline__ void start(const Operand& P, int i0, const Operand& Q, int j0) {
-    const int r = wave() * 8 + (lane() >> 3);
-    const unsigned c = chunk_offset<MODE>(my_chunk());
+    const int r = wave_id() * 8 + (lane_id() >> 3);
+    const unsigned c = chunk_offset<MODE>(move_chunk());
 #pragma unroll
     for (int l = 0; l < LOADS_P; ++l) offp[l] = (unsigned)min(l * 8 * WAVES + r, P.rows - 1 - i0) * P.ld + c;
 #pragma unroll
@@ -92,110 +144,171 @@ struct Tile {
   }
   // valid: bytes of the step that exist (>= 128: all); only 8-bit operands have ragged ends, fp16 operands are padded to whole steps
   __device__ __forceinline__ void fetch(const char* p, const char* q, char* buf, int valid) const {
-    const int w = wave();
-    unsigned back = 0;
-    if (MODE == MODE_I8 && valid < 128) back = my_chunk() * 16 >= valid ? (unsigned)my_chunk() * 16 : 0u;
+    const int w = wave_id();
+    const unsigned back = MODE == MODE_I8 && valid < 128 ? move_back(valid) : 0;
 #pragma unroll
-    for (int l = 0; l < LOADS_P; ++l) move(p, offp[l] - back, buf + (l * WAVES + w) * 1024);
+    for (int l = 0; l < LOADS_P; ++l) move16(p, offp[l] - back, buf + (l * WAVES + w) * 1024);
 #pragma unroll
-    for (int l = 0; l < LOADS_Q; ++l) move(q, offq[l] - back, buf + BI * 128 + (l * WAVES + w) * 1024);
-  }
-  __device__ __forceinline__ static i32x4 mask_bytes(i32x4 v, int n) {  // keep the first n of 16 bytes
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const int b = n - 4 * w;
-      v[w] = b >= 4 ? v[w] : b <= 0 ? 0 : (v[w] & ((1 << (8 * b)) - 1));
-    }
-    return v;
+    for (int l = 0; l < LOADS_Q; ++l) move16(q, offq[l] - back, buf + BI * 128 + (l * WAVES + w) * 1024);
   }
   template <bool TAIL>
   __device__ __forceinline__ void multiply(const char* buf, int valid) {
-    const int w = wave(), l = lane();
-    const int wi = w / WJ, wj = w % WJ;
+    const int wi = wave_id() / WJ, wj = wave_id() % WJ, l = lane_id();
     const char* p = buf + (wi * MI * 32 + (l & 31)) * 128;
     const char* q = buf + BI * 128 + (wj * MJ * 32 + (l & 31)) * 128;
-    const int x = l & 7, h = l >> 5;
-    if constexpr (MODE == MODE_F16PAIR) {
+    Frags<MODE, MI, MJ> f;
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int hi = ((2 * s + h) ^ x) * 16, lo = ((4 + 2 * s + h) ^ x) * 16;
-        f16x8 ph[MI], pl[MI], qh[MJ], ql[MJ];
-#pragma unroll
-        for (int a = 0; a < MI; ++a) ph[a] = *(const f16x8*)(p + a * 4096 + hi);
-#pragma unroll
-        for (int b = 0; b < MJ; ++b) qh[b] = *(const f16x8*)(q + b * 4096 + hi);
-#pragma unroll
-        for (int a = 0; a < MI; ++a) pl[a] = *(const f16x8*)(p + a * 4096 + lo);
-#pragma unroll
-        for (int b = 0; b < MJ; ++b) ql[b] = *(const f16x8*)(q + b * 4096 + lo);
-#pragma unroll
-        for (int a = 0; a < MI; ++a)
-#pragma unroll
-          for (int b = 0; b < MJ; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[a], qh[b], acc[a][b], 0, 0, 0);
-#pragma unroll
-        for (int a = 0; a < MI; ++a)
-#pragma unroll
-          for (int b = 0; b < MJ; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl[a], qh[b], acc[a][b], 0, 0, 0);
-#pragma unroll
-        for (int a = 0; a < MI; ++a)
-#pragma unroll
-          for (int b = 0; b < MJ; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[a], ql[b], acc[a][b], 0, 0, 0);
-      }
-    } else {
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const int c = ((2 * s + h) ^ x) * 16;
-        if constexpr (MODE == MODE_I8) {
-          i32x4 pf[MI], qf[MJ];
-#pragma unroll
-          for (int a = 0; a < MI; ++a) pf[a] = *(const i32x4*)(p + a * 4096 + c);
-#pragma unroll
-          for (int b = 0; b < MJ; ++b) {
-            qf[b] = *(const i32x4*)(q + b * 4096 + c);
-            if (TAIL) qf[b] = mask_bytes(qf[b], valid - (2 * s + h) * 16);
-          }
-#pragma unroll
-          for (int a = 0; a < MI; ++a)
-#pragma unroll
-            for (int b = 0; b < MJ; ++b) acc[a][b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(pf[a], qf[b], acc[a][b], 0, 0, 0);
-        } else {
-          f16x8 pf[MI], qf[MJ];
-#pragma unroll
-          for (int a = 0; a < MI; ++a) pf[a] = *(const f16x8*)(p + a * 4096 + c);
-#pragma unroll
-          for (int b = 0; b < MJ; ++b) qf[b] = *(const f16x8*)(q + b * 4096 + c);
-#pragma unroll
-          for (int a = 0; a < MI; ++a)
-#pragma unroll
-            for (int b = 0; b < MJ; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pf[a], qf[b], acc[a][b], 0, 0, 0);
-        }
-      }
+    for (int s = 0; s < f.SUB; ++s) {
+      f.template read<TAIL>(s, p, q, valid);
+      f.multiply(s, acc);
     }
   }
-  // steps >= 1 whole or ragged K steps from byte kb of the rows on; ragged: valid bytes of the last one (128: whole).
+  // Every wave's share of the oldest step has arrived and every wave has read what the next move overwrites.
+  template <int N>
+  __device__ __forceinline__ static void arrive() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+  }
+  // steps >= 1 whole or ragged K steps from byte kb of the rows on; last_valid: valid bytes of the last one (128: whole).
+  // STAGES - 1 steps are under way at any time; one barrier a step: behind it step t is there and the buffer of step t - 1 is free.
   __device__ __forceinline__ void run(const Operand& P, int i0, const Operand& Q, int j0, size_t kb, int steps, int last_valid, char* lds) {
     start(P, i0, Q, j0);
     const char* p = P.base + (size_t)i0 * P.ld + kb;
     const char* q = Q.base + (size_t)j0 * Q.ld + kb;
     constexpr int STEP = kstep_bytes<MODE>();
-    fetch(p, q, lds, steps == 1 ? last_valid : 128);
+    const int first = min(STAGES - 1, steps);
+    for (int t = 0; t < first; ++t) fetch(p + t * STEP, q + t * STEP, lds + t * BUF, t + 1 == steps ? last_valid : 128);
+    p += (STAGES - 1) * STEP;
+    q += (STAGES - 1) * STEP;
+    int now = 0, next = (STAGES - 1) * BUF;
     for (int t = 0; t < steps - 1; ++t) {
-      __syncthreads();  // step t has arrived (the barrier drains the moves), step t - 1 has been read
-      p += STEP;
-      q += STEP;
-      fetch(p, q, lds + ((t + 1) & 1) * BUF, t + 2 == steps ? last_valid : 128);
-      multiply<false>(lds + (t & 1) * BUF, 128);
+      if (t + STAGES - 1 <= steps)
+        arrive<FLIGHT>();
+      else
+        arrive<0>();
+      if (t + STAGES - 1 < steps) {
+        fetch(p, q, lds + next, t + STAGES == steps ? last_valid : 128);
+        p += STEP;
+        q += STEP;
+      }
+      multiply<false>(lds + now, 128);
+      now = now + BUF == LDS ? 0 : now + BUF;
+      next = next + BUF == LDS ? 0 : next + BUF;
     }
-    __syncthreads();
+    arrive<0>();
     if (MODE == MODE_I8 && last_valid < 128)
-      multiply<true>(lds + ((steps - 1) & 1) * BUF, last_valid);
+      multiply<true>(lds + now, last_valid);
     else
-      multiply<false>(lds + ((steps - 1) & 1) * BUF, 128);
+      multiply<false>(lds + now, 128);
   }
-  // Where register r (0 .. 15) of block (a, b) lies in the tile: i = row_of(a) + 8 (r / 4) + r % 4, j = col_of(b).
-  __device__ __forceinline__ static int row_of(int a) { return (wave() / WJ * MI + a) * 32 + 4 * (lane() >> 5); }
-  __device__ __forceinline__ static int col_of(int b) { return (wave() % WJ * MJ + b) * 32 + (lane() & 31); }
+  // The epilogue goes through LDS: column block b of every wave at a time, CHUNK columns of the tile as rows of PITCH words, i along the row.
+  // (PITCH = BI + 1: neighbouring rows and neighbouring words both change the bank, so both orientations are read without conflicts.)
+  static constexpr int CHUNK = 32 * WJ, CHUNKS = MJ, PARTS = 1, PITCH = BI + 1;
+  static constexpr int SCRATCH = CHUNK * PITCH * 4;
+  __device__ __forceinline__ static int column(int chunk, int r) { return ((r >> 5) * MJ + chunk) * 32 + (r & 31); }
+  __device__ __forceinline__ void spill(int chunk, char* lds) const {  // (the chunk's number picks registers: unrolled by the callers)
+    const int wi = wave_id() / WJ, wj = wave_id() % WJ, l = lane_id();
+    int* t = (int*)lds + (wj * 32 + (l & 31)) * PITCH + wi * MI * 32 + 4 * (l >> 5);
+#pragma unroll
+    for (int b = 0; b < MJ; ++b)
+      if (b == chunk)
+#pragma unroll
+        for (int a = 0; a < MI; ++a)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) t[a * 32 + 8 * (r >> 2) + (r & 3)] = __builtin_bit_cast(i32x16, acc[a][b])[r];
+  }
 };
+
+// 64 x 64 tiles for products with few of them: each of the four waves has the whole tile and every fourth K step, in buffers of its own - no barriers,
+// four independent accumulators a wave, half the LDS reads per product of four waves side by side - and the epilogue adds the four up.
+template <int MODE, int STAGES>
+struct Ring {
+  static constexpr int THREADS = 256;
+  static constexpr int BUF = 128 * 128;
+  static constexpr int LDS = 4 * STAGES * BUF;
+  using Acc = typename AccOf<MODE>::type;
+  Acc acc[2][2];
+  unsigned offp[8], offq[8];
+
+  __device__ __forceinline__ void fetch(const char* p, const char* q, char* buf, int valid) const {
+    const unsigned back = MODE == MODE_I8 && valid < 128 ? move_back(valid) : 0;
+#pragma unroll
+    for (int l = 0; l < 8; ++l) move16(p, offp[l] - back, buf + l * 1024);
+#pragma unroll
+    for (int l = 0; l < 8; ++l) move16(q, offq[l] - back, buf + 8192 + l * 1024);
+  }
+  template <bool TAIL>
+  __device__ __forceinline__ void read(Frags<MODE, 2, 2>& f, const char* buf, int valid) const {
+#pragma unroll
+    for (int s = 0; s < f.SUB; ++s) f.template read<TAIL>(s, buf + (lane_id() & 31) * 128, buf + 8192 + (lane_id() & 31) * 128, valid);
+  }
+  __device__ __forceinline__ void run(const Operand& P, int i0, const Operand& Q, int j0, size_t kb, int steps, int last_valid, char* lds) {
+    const int w = wave_id(), r = lane_id() >> 3;
+    const unsigned c = chunk_offset<MODE>(move_chunk());
+#pragma unroll
+    for (int l = 0; l < 8; ++l) {
+      offp[l] = (unsigned)min(l * 8 + r, P.rows - 1 - i0) * P.ld + c;
+      offq[l] = (unsigned)min(l * 8 + r, Q.rows - 1 - j0) * Q.ld + c;
+    }
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int b = 0; b < 2; ++b) acc[a][b] = Acc{};
+    constexpr int STEP = kstep_bytes<MODE>();
+    const char* p = P.base + (size_t)i0 * P.ld + kb + w * STEP;
+    const char* q = Q.base + (size_t)j0 * Q.ld + kb + w * STEP;
+    lds += w * STAGES * BUF;
+    const int mine = (steps - w + 3) / 4;  // steps w, w + 4, ..
+    auto valid_of = [&](int t) { return 4 * t + w + 1 == steps ? last_valid : 128; };
+    for (int t = 0; t < min(STAGES, mine); ++t) fetch(p + (size_t)t * 4 * STEP, q + (size_t)t * 4 * STEP, lds + t * BUF, valid_of(t));
+    p += (size_t)STAGES * 4 * STEP;
+    q += (size_t)STAGES * 4 * STEP;
+    int now = 0;
+    for (int t = 0; t < mine; ++t) {
+      if (t + STAGES <= mine)
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(16 * (STAGES - 1)) : "memory");
+      else
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      Frags<MODE, 2, 2> f;
+      if (MODE == MODE_I8 && valid_of(t) < 128)
+        read<true>(f, lds + now, last_valid);
+      else
+        read<false>(f, lds + now, 128);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the step is in registers, its buffer free
+      if (t + STAGES < mine) {
+        fetch(p, q, lds + now, valid_of(t + STAGES));
+        p += 4 * STEP;
+        q += 4 * STEP;
+      }
+#pragma unroll
+      for (int s = 0; s < f.SUB; ++s) f.multiply(s, acc);
+      now = now + BUF == STAGES * BUF ? 0 : now + BUF;
+    }
+  }
+  static constexpr int CHUNK = 64, CHUNKS = 1, PARTS = 4, PITCH = 65;
+  static constexpr int SCRATCH = PARTS * CHUNK * PITCH * 4;
+  __device__ __forceinline__ static int column(int, int r) { return r; }
+  __device__ __forceinline__ void spill(int, char* lds) const {
+    const int l = lane_id();
+    int* t = (int*)lds + (wave_id() * CHUNK + (l & 31)) * PITCH + 4 * (l >> 5);
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) t[b * 32 * PITCH + a * 32 + 8 * (r >> 2) + (r & 3)] = __builtin_bit_cast(i32x16, acc[a][b])[r];
+  }
+};
+
+// Eight sums of a chunk: row r, words i .. i + 7
+template <class TL, class V>
+__device__ __forceinline__ void chunk_sums(const char* lds, int r, int i, V (&v)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = ((const V*)lds)[r * TL::PITCH + i + e];
+#pragma unroll
+  for (int o = 1; o < TL::PARTS; ++o)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += ((const V*)lds)[(o * TL::CHUNK + r) * TL::PITCH + i + e];
+}
 
 // Tiles in an order that keeps the ones a die works on together: workgroups are dealt to the 8 dies in turn, so die x takes the x-th eighth of the
 // list (bijective for any count), and the list walks strips of `strip` tile rows, so that a die's tiles share operand rows in its L2.
@@ -216,19 +329,24 @@ template <class T>
 __device__ __forceinline__ float to_f32(T v) {
   return (float)v;
 }
+// Eight neighbouring results, rounded to T, to an output row: whole where it is aligned, else those below n one by one
 template <class T>
-struct Vec4;
-template <>
-struct Vec4<float> {
-  using type = f32x4;
-};
-template <>
-struct Vec4<_Float16> {
-  using type = f16x4;
-};
-template <>
-struct Vec4<__bf16> {
-  using type = bf16x4;
-};
+__device__ __forceinline__ void store8(T* at, const float (&v)[8], int n, bool whole) {
+  if (whole) {
+    typedef T V __attribute__((ext_vector_type(sizeof(T) == 2 ? 8 : 4)));
+    constexpr int N = sizeof(V) / sizeof(T);
+#pragma unroll
+    for (int e = 0; e < 8; e += N) {
+      V w;
+#pragma unroll
+      for (int k = 0; k < N; ++k) w[k] = (T)v[e + k];
+      *(V*)(at + e) = w;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) at[e] = (T)v[e];
+  }
+}
 
 }  // namespace lb

@@ -392,8 +392,8 @@ def orthogonalize(g, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: float = 1e
     if len(shape) < 2:
         raise ValueError("g must be a matrix or a batch of matrices")
     kind = _kind(sp, g, "g")
-    if isinstance(steps, bool) or int(steps) != steps or not 1 <= steps <= 64:
-        raise ValueError("steps must be a whole number from 1 to 64")
+    if isinstance(steps, bool) or int(steps) != steps or not 1 <= steps <= 32:
+        raise ValueError("steps must be a whole number from 1 to 32")
     steps = int(steps)
     try:
         rows = [tuple(float(v) for v in row) for row in coefficients] if hasattr(coefficients[0], "__len__") else [tuple(float(v) for v in coefficients)] * steps

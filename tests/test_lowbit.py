@@ -42,7 +42,7 @@ S = np.ones(3, dtype=np.float32)
         lambda: nls.orthogonalize(X.astype(np.float64)),
         lambda: nls.orthogonalize(X[0]),
         lambda: nls.orthogonalize(X, steps=0),
-        lambda: nls.orthogonalize(X, steps=65),
+        lambda: nls.orthogonalize(X, steps=33),
         lambda: nls.orthogonalize(X, steps=2.5),
         lambda: nls.orthogonalize(X, steps=3, coefficients=[(1.5, -0.5, 0.0)] * 2),
         lambda: nls.orthogonalize(X, coefficients=(1.5, -0.5)),
