@@ -212,16 +212,16 @@ int ns_product(nls_ctx* ctx, const NsArgs& g, bool pairs, long batch, hipStream_
 }
 
 template <class T, int PB, int CB>
-int ns_small(nls_ctx* ctx, const NsMatrix& w, bool tall, long batch, const NsCoef& cf, int steps, int exact, double eps, T* out, hipStream_t st) {
-  const int lds = NsSmall<PB, CB>::lds((int)w.q);
+int ns_small(nls_ctx* ctx, const NsMatrix& w, bool tall, long batch, const NsCoef& cf, int steps, double eps, T* out, hipStream_t st) {
+  constexpr int lds = NsRows<PB, CB>::LDS;
   NLSCHK(ask_lds(ctx, k_ns_small<T, PB, CB>, lds));
-  k_ns_small<T, PB, CB><<<dim3((unsigned)batch), 512, lds, st>>>(w, cf, steps, exact, eps, out, tall);
+  k_ns_small<T, PB, CB><<<dim3((unsigned)batch), 512, lds, st>>>(w, cf, steps, eps, out, tall);
   LAUNCHED(ctx, "orthogonalize");
   return NLS_OK;
 }
 template <class T>
-int ns_small_any(nls_ctx* ctx, const NsMatrix& w, bool tall, long batch, const NsCoef& cf, int steps, int exact, double eps, T* out, hipStream_t st) {
-#define NS_SMALL(PB, CB) return ns_small<T, PB, CB>(ctx, w, tall, batch, cf, steps, exact, eps, out, st)
+int ns_small_any(nls_ctx* ctx, const NsMatrix& w, bool tall, long batch, const NsCoef& cf, int steps, double eps, T* out, hipStream_t st) {
+#define NS_SMALL(PB, CB) return ns_small<T, PB, CB>(ctx, w, tall, batch, cf, steps, eps, out, st)
   if (w.q <= 256) {
     if (w.p <= 32) NS_SMALL(1, 1);
     if (w.p <= 64) NS_SMALL(2, 1);
@@ -236,12 +236,33 @@ int ns_small_any(nls_ctx* ctx, const NsMatrix& w, bool tall, long batch, const N
 #undef NS_SMALL
 }
 
+// Which steps are done in one chain: as many as let small singular values grow by no more than `most` (nls_ortho.h); one at least.
+void ns_chains(NsCoef& cf, int steps, double most) {
+  cf.ends = 0;
+  double grown = 1.0;
+  for (int t = 0; t < steps; ++t) {
+    const double g = std::max(1.0, cf.s[t].grow);
+    if (t > 0 && grown * g > most) {
+      cf.ends |= 1u << (t - 1);
+      grown = 1.0;
+    }
+    grown *= g;
+  }
+  cf.ends |= 1u << (steps - 1);
+  const double u = 1.0 + 1e-3;
+  cf.first = ns_exponent(u);
+  cf.last = -ns_factors(u, cf.s, cf.ends, steps, cf.f);
+}
 template <class T>
-int orthogonalize(nls_ctx* ctx, const NsMatrix& w, const NsPlan& plan, bool tall, long batch, const NsCoef& cf, int steps, double eps, T* out, char* ws, hipStream_t st) {
+int orthogonalize(nls_ctx* ctx, const NsMatrix& w, const NsPlan& plan, bool tall, long batch, NsCoef& cf, int steps, double eps, T* out, char* ws, hipStream_t st) {
   // The first steps may work on the hi halves alone where the result has few bits: what a rounding to 11 bits does to an early iterate is carried
   // along as a slightly different matrix would be, and the steps after it pull its singular values to the same curve.
   const int exact = sizeof(T) == 4 ? steps : std::is_same<T, __bf16>::value ? 2 : 3;
-  if (plan.total == 0) return ns_small_any(ctx, w, tall, batch, cf, steps, exact, eps, out, st);
+  if (plan.total == 0) {
+    ns_chains(cf, steps, sizeof(T) == 4 ? 0.0 : std::is_same<T, __bf16>::value ? 500.0 : 45.0);
+    return ns_small_any(ctx, w, tall, batch, cf, steps, eps, out, st);
+  }
+  ns_chains(cf, steps, 0.0);
   double* parts = (double*)ws;
   NsScales* scales = (NsScales*)(ws + plan.parts);
   char* base = ws + plan.parts + plan.scales;
@@ -412,9 +433,9 @@ extern "C" int nls_orthogonalize(nls_ctx* ctx, const void* g, int type, int64_t 
   if (!(eps >= 0.0) || !(eps < 1e30)) return fail(ctx, NLS_ERR_ARG, "orthogonalize: eps must be a number >= 0");
   if (!coefficients) return fail(ctx, NLS_ERR_ARG, "orthogonalize: null pointer");
   NsCoef cf{};
-  double u = 1.0;
+  double u = 1.0 + 1e-3;
   for (int t = 0; t < steps; ++t) {
-    ns_step(coefficients[3 * t], coefficients[3 * t + 1], coefficients[3 * t + 2], &cf.s[t]);
+    ns_step(coefficients[3 * t], coefficients[3 * t + 1], coefficients[3 * t + 2], u, &cf.s[t]);
     u = ns_peak_x(cf.s[t], u) * (1.0 + 1e-3);
     if (!(u < 1e6)) return fail(ctx, NLS_ERR_ARG, "orthogonalize: the coefficients let singular values grow past 1e6 in step %d", t + 1);
   }

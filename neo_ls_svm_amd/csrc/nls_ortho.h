@@ -16,11 +16,12 @@ namespace lb {
 constexpr int NS_MAX_STEPS = 32;
 constexpr int NS_PARTS = 256;  // partial sums of squares a matrix
 
-// X_t, A_t, B_t are held times 2^ex, 2^ea, 2^eb (of their step); what a product's sum w becomes the next held matrix with:
+// Matrices are held times a power of two.  What a step's sums w are multiplied with to become the next held matrix:
 struct NsFactors {
-  float gram;            // A: gram w
-  float lin, quad;       // B: lin A + quad w
-  float keep, add;       // next X: keep X + add w
+  float gram;               // A = X X^T: gram w
+  float unit, lin, quad;    // B = lin A + quad w;  P = unit 1 + lin A + quad w in a chain (below)
+  float keep, add;          // next X: keep X + add w
+  float half, next, chain;  // a chain: R = P A: half w;  A <- P R: next w;  Q <- P Q: chain w
 };
 struct NsScales {  // one per matrix
   double first;    // G to held X_0; NaN when the norm is not finite: the whole result is then NaN
@@ -32,9 +33,13 @@ struct NsStep {
   double a, b, c;
   double xs[2], xv[2];   // s > 0 and the absolute value there
   double zs, zv;
+  double grow;           // max |a + b z + c z^2| for the singular values the step can meet when |X_0| <= 1
 };
 struct NsCoef {
   NsStep s[NS_MAX_STEPS];
+  NsFactors f[NS_MAX_STEPS];  // for matrices whose norm is not small beside eps: |X_0|_F near 1
+  int first, last;            // their powers: X_0 is held times 2^first, the result times 2^-last
+  unsigned ends;              // bit t: a chain of steps ends with step t
 };
 
 // A matrix of fp16 pairs: granules of 32 elements, 64 bytes hi then 64 bytes lo; rows padded with zeros to 64 elements.
@@ -69,8 +74,9 @@ __global__ __launch_bounds__(256) void k_ns_norm(NsMatrix w, double* parts) {
   if (threadIdx.x == 0) parts[(size_t)blockIdx.y * NS_PARTS + blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
 }
 
-inline void ns_step(double a, double b, double c, NsStep* o) {
-  *o = NsStep{a, b, c, {INFINITY, INFINITY}, {0.0, 0.0}, INFINITY, 0.0};
+// u: bound on the singular values that enter the step
+inline void ns_step(double a, double b, double c, double u, NsStep* o) {
+  *o = NsStep{a, b, c, {INFINITY, INFINITY}, {0.0, 0.0}, INFINITY, 0.0, 0.0};
   auto at = [&](int k, double z) {  // z = s^2
     if (!(z > 0.0) || !std::isfinite(z)) return;
     o->xs[k] = std::sqrt(z);
@@ -87,6 +93,9 @@ inline void ns_step(double a, double b, double c, NsStep* o) {
     o->zs = -b / (2.0 * c);
     o->zv = std::fabs(o->zs * (b + c * o->zs));
   }
+  const double z = u * u;
+  o->grow = std::max(std::fabs(a), std::fabs(a + z * (b + c * z)));
+  if (o->zs < z) o->grow = std::max(o->grow, std::fabs(a + o->zs * (b + c * o->zs)));
 }
 __host__ __device__ inline double ns_peak_x(const NsStep& s, double u) {  // max |a s + b s^3 + c s^5| on [0, u]
   double top = fabs(u * (s.a + u * u * (s.b + s.c * u * u)));
@@ -99,48 +108,101 @@ __host__ __device__ inline double ns_peak_b(const NsStep& s, double u) {  // max
   return s.zs < z ? fmax(top, s.zv) : top;
 }
 // 15 - e with |v| < 2^e: what is bounded by v is held below 2^15 (fp16 ends at 65504: a factor of two for the roundings)
-__device__ __forceinline__ int ns_exponent(double v) {
-  const int e = (int)((__double_as_longlong(v) >> 52) & 2047);  // v in [2^(e - 1023), 2^(e - 1022))
+__host__ __device__ inline int ns_exponent(double v) {
+  const int e = (int)((__builtin_bit_cast(long long, v) >> 52) & 2047);  // v in [2^(e - 1023), 2^(e - 1022))
   return e == 0 || e == 2047 ? 0 : 15 - (e - 1022);
 }
 // 2^e.  Past the ends of float32 the nearest power in it: a product that needs a smaller one has no share in a sum beside a term below 2^15.
-__device__ __forceinline__ float ns_pow2(int e) { return __int_as_float((min(max(e, -126), 127) + 127) << 23); }
+__host__ __device__ inline float ns_pow2(int e) { return __builtin_bit_cast(float, ((e < -126 ? -126 : e > 127 ? 127 : e) + 127) << 23); }
 
-// squares: |G|_F^2.  Bounds on the singular values of X_t, from |X_0| <= |X_0|_F on, choose the powers of two.
+// The factors of all steps from a bound u on the singular values of X_0 = 2^-first held X_0; returns -last of NsScales.
+constexpr int NS_UNIT = 14;  // a chain starts with Q = 1 held as 2^14
+__host__ __device__ inline int ns_factors(double u, const NsStep* steps, unsigned ends, int count, NsFactors* out) {
+  double chain = 1.0;
+  int ex = ns_exponent(u), eq = NS_UNIT;
+  for (int t = 0; t < count; ++t) {
+    const NsStep& s = steps[t];
+    const bool begin = t == 0 || (ends >> (t - 1) & 1), end = ends >> t & 1, alone = begin && end;
+    if (begin) {
+      eq = NS_UNIT;
+      chain = 1.0;
+    }
+    const double un = ns_peak_x(s, u) * (1.0 + 1e-3);
+    chain *= s.grow * (1.0 + 1e-3);
+    const int ea = ns_exponent(u * u), en = ns_exponent(un), ean = ns_exponent(un * un);
+    const int eb = ns_exponent(alone ? ns_peak_b(s, u) : s.grow), er = ns_exponent(s.grow * u * u), eqn = ns_exponent(chain);
+    NsFactors f;
+    f.gram = ns_pow2(ea - 2 * ex);
+    f.unit = (float)s.a * ns_pow2(eb);
+    f.lin = (float)s.b * ns_pow2(eb - ea);
+    f.quad = (float)s.c * ns_pow2(eb - 2 * ea);
+    f.half = ns_pow2(er - eb - ea);
+    f.next = ns_pow2(ean - eb - er);
+    f.chain = ns_pow2(eqn - eb - eq);
+    f.keep = alone ? (float)s.a * ns_pow2(en - ex) : 0.0f;
+    f.add = ns_pow2(en - ex - (alone ? eb : eqn));
+    out[t] = f;
+    eq = eqn;
+    if (end) ex = en;
+    u = un;
+  }
+  return ex;
+}
+// squares: |G|_F^2.  Bounds on the singular values of X_t, from |X_0| <= |X_0|_F on, choose the powers of two; where |X_0|_F is near 1 (the norm is
+// large beside eps) they are known before (ns_fetch has them in place already), else they are worked out here.
 __device__ __forceinline__ void ns_scales(double squares, double eps, const NsCoef& cf, int steps, NsScales& z) {
   const double norm = sqrt(squares);
   const bool fine = norm < 1e300;
   const double inv = fine ? (norm + eps > 0.0 ? 1.0 / (norm + eps) : 0.0) : __longlong_as_double(0x7ff8000000000000ll);
-  double u = fine ? norm * inv * (1.0 + 1e-3) : 1.0;
-  int ex = ns_exponent(u);
-  z.first = ldexp(inv, ex);
-  for (int t = 0; t < steps; ++t) {
-    const NsStep& s = cf.s[t];
-    const int ea = ns_exponent(u * u), eb = ns_exponent(ns_peak_b(s, u));
-    u = ns_peak_x(s, u) * (1.0 + 1e-3);
-    const int en = ns_exponent(u);
-    NsFactors& f = z.f[t];
-    f.gram = ns_pow2(ea - 2 * ex);
-    f.lin = (float)s.b * ns_pow2(eb - ea);
-    f.quad = (float)s.c * ns_pow2(eb - 2 * ea);
-    f.keep = (float)s.a * ns_pow2(en - ex);
-    f.add = ns_pow2(en - eb - ex);
-    ex = en;
+  const double u = norm * inv;
+  int first = cf.first, last = cf.last;
+  if (u < 0.25) {
+    const double v = u * (1.0 + 1e-3);
+    first = ns_exponent(v);
+    last = -ns_factors(v, cf.s, cf.ends, steps, z.f);
   }
-  z.last = -ex;
+  z.first = ldexp(inv, first);
+  z.last = last;
 }
 
+// The steps' tables from the kernel's arguments, all at once: read one by one they are a chain of misses.  A barrier has to follow.
+__device__ __forceinline__ void ns_fetch(const NsCoef& cf, int steps, NsCoef* to, NsFactors* f) {
+  for (int i = threadIdx.x; i < steps * (int)(sizeof(NsStep) / 4); i += blockDim.x) ((int*)to->s)[i] = ((const int*)cf.s)[i];
+  for (int i = threadIdx.x; i < steps * (int)(sizeof(NsFactors) / 4); i += blockDim.x) ((int*)f)[i] = ((const int*)cf.f)[i];
+  if (threadIdx.x == 0) {
+    to->ends = cf.ends;
+    to->first = cf.first;
+    to->last = cf.last;
+  }
+}
 __global__ __launch_bounds__(64) void k_ns_scales(const double* parts, int count, double eps, NsCoef cf, int steps, NsScales* out) {
+  __shared__ NsCoef mine;
+  ns_fetch(cf, steps, &mine, out[blockIdx.x].f);
   double s = 0.0;
   for (int i = threadIdx.x; i < count; i += 64) s += parts[(size_t)blockIdx.x * NS_PARTS + i];
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-  if (threadIdx.x == 0) ns_scales(s, eps, cf, steps, out[blockIdx.x]);
+  __syncthreads();
+  if (threadIdx.x == 0) ns_scales(s, eps, mine, steps, out[blockIdx.x]);
 }
 
-__device__ __forceinline__ void split(float v, _Float16* hi, _Float16* lo) {
-  *hi = (_Float16)v;
-  *lo = (_Float16)(v - (float)*hi);
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void split(float v, float u, f16x2* hi, f16x2* lo) {  // (two at a time: one conversion instruction)
+  *hi = __builtin_convertvector(f32x2{v, u}, f16x2);
+  *lo = __builtin_convertvector(f32x2{v - (float)(*hi)[0], u - (float)(*hi)[1]}, f16x2);
+}
+template <class V>
+__device__ __forceinline__ void split8(const V& v, int at, f16x8* hi, f16x8* lo) {  // v[at .. at + 7]
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    f16x2 h, o;
+    split(v[at + e], v[at + e + 1], &h, &o);
+    (*hi)[e] = h[0];
+    (*hi)[e + 1] = h[1];
+    (*lo)[e] = o[0];
+    (*lo)[e + 1] = o[1];
+  }
 }
 
 // G -> X_0 (p rows) and its transpose (q rows), zero-padded.  One 64 x 64 tile a workgroup.
@@ -168,13 +230,11 @@ __global__ __launch_bounds__(256) void k_ns_pack(NsMatrix w, const NsScales* sca
     char* base = turn ? xt + pair_at(q0 + row, p0 + part, ldt) : x + pair_at(p0 + row, q0 + part, ldx);
     if (turn ? q0 + row >= w.q : p0 + row >= w.p) continue;
     f16x8 hi[2], lo[2];
+    float v[16];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      _Float16 h, o;
-      split(turn ? tile[part + e][row] : tile[row][part + e], &h, &o);
-      hi[e >> 3][e & 7] = h;
-      lo[e >> 3][e & 7] = o;
-    }
+    for (int e = 0; e < 16; ++e) v[e] = turn ? tile[part + e][row] : tile[row][part + e];
+    split8(v, 0, &hi[0], &lo[0]);
+    split8(v, 8, &hi[1], &lo[1]);
     *(f16x8*)base = hi[0];
     *(f16x8*)(base + 16) = hi[1];
     *(f16x8*)(base + 64) = lo[0];
@@ -200,13 +260,7 @@ struct NsArgs {
 
 __device__ __forceinline__ void store_pairs(char* at, const float (&v)[8]) {  // eight neighbours of a row of pairs
   f16x8 h, o;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    _Float16 hi, lo;
-    split(v[e], &hi, &lo);
-    h[e] = hi;
-    o[e] = lo;
-  }
+  split8(v, 0, &h, &o);
   *(f16x8*)at = h;
   *(f16x8*)(at + 64) = o;
 }
@@ -298,65 +352,300 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
   }
 }
 
-// ---- small matrices ---------------------------------------------------------------------------------------------------------------------------
-// One workgroup does all steps of a matrix of up to 32 PB x 256 CB (padded to blocks of 32).  X stays in registers in float32, in the places the matrix
-// instruction leaves its results in: lane l has column l % 32 of a block, registers r the rows 8 (r / 4) + 4 (l / 32) + r % 4.  Wave w has the column
-// blocks w, w + 8, ...
-//   A = X X^T contracts over columns, which lie across lanes: X goes through LDS once a step, as rows of fp16 (hi and lo planes).
-//   B X contracts over rows, which lie along registers: registers 8 s .. 8 s + 7 of a block ARE a fragment of the 32 x 32 x 16 instruction if k runs in the
-//   order 16 s + {4 h, 4 h + 1, .., 4 h + 3, 8 + 4 h, ..} for lane half h - so B is laid out in LDS with its columns in that order and X is never moved.
+// ---- up to 128 rows -----------------------------------------------------------------------------------------------------------------------------
+// Everything p x p fits one workgroup; X is dealt out to the waves by columns and stays in registers in float32, in the places the matrix instruction
+// leaves its results in: a wave has column blocks of 32, lane l the column l % 32, registers r of row block a the rows 32 a + 8 (r / 4) + 4 (l / 32) + r % 4.
+//   S X for symmetric S contracts over rows, which lie along registers: registers 8 s .. 8 s + 7 of a block ARE a fragment of the 32 x 32 x 16 instruction
+//   if k runs in the order 16 s + {4 h .. 4 h + 3, 8 + 4 h .. 8 + 4 h + 3} for lane half h.  So S lies in LDS with its columns in that order (an "image",
+//   hi and lo planes) and X never moves (ns_times).
+//   A = X X^T contracts over columns, which lie across lanes: X goes through LDS as rows (ns_gram).
 // Rows of LDS planes are 16 bytes longer than their numbers: eight neighbouring rows start in different banks.
-// A step is a chain of three short products; what bounds it is latency (barriers, LDS round trips), not a rate.
-// What a general path costs instead is three launches a step.
-template <int PB, int CB>
-struct NsSmall {
-  static constexpr int P = 32 * PB, Q = 256 * CB;
-  static constexpr int BLOCKS = PB * PB;
-  static constexpr int OWN = (BLOCKS + 7) / 8;              // blocks of A a wave has
-  static constexpr int KS = BLOCKS >= 8 ? 1 : PB == 2 ? 2 : 8;  // waves that share a block's columns
-  static constexpr int PITCH_A = P * 2 + 16;
-  // LDS for the columns that are there
-  __host__ __device__ static int pitch_x(int q) { return (q + 31) / 32 * 64 + 16; }
-  __host__ __device__ static int lds(int q) {
-    const int x = 2 * P * pitch_x(q), a = 2 * P * PITCH_A, parts = KS > 1 ? 8 * 4096 : 0;
-    const int m = x > a ? x : a;
-    return m > parts ? m : parts;
-  }
+//
+// Chains: with P_t = a + b A_t + c A_t A_t the iterates are X_t+1 = P_t X_t and A_t+1 = P_t A_t P_t, so steps t .. t' can be done on p x p matrices
+// alone, Q <- P Q, and X is multiplied once, by Q.  What it costs is accuracy: A's roundings are relative to its LARGEST eigenvalue, and Q amplifies
+// what they do to small ones by the square of the polynomials' slope.  Measured against 64 bits (five standard steps, Gaussian, 1 / k and exponential
+// spectra, low rank + noise; 64 .. 512 rows): relative error of the result up to 4e-4 in one chain, 2e-5 in chains of 3 + 2, 9e-6 without (as
+// float32 products: 9e-6).  So bfloat16 results (rounding 1.7e-3) take chains of growth up to 500, float16 (2e-4) up to 45, float32 none.
+// Bound by latency for one small matrix (a chain's step is three dependent products and two barriers), by the matrix cores for batches.
+template <int PB, int CB = 1>
+struct NsRows {
+  static constexpr int P = 32 * PB;
+  static constexpr int PITCH = P * 2 + 16, IMAGE = 2 * P * PITCH;
+  static constexpr int KS = 8 / PB < 4 ? 8 / PB : 4;          // most waves that share a column block of A
+  // Adding shares up costs about as much as 2 .. 4 of the K steps it saves: measured, from these lengths on it pays.
+  __device__ static int shares(int cols) { return min(KS, max(1, cols / (PB <= 2 ? 4 : PB == 3 ? 3 : 2))); }
+  static constexpr int PARTS = (KS - 1) * PB * PB * 4096;     // what they add up through LDS
+  static constexpr int PITCH_X = CB * 512 + 16, X = 2 * P * PITCH_X;  // rows of X (a constant pitch: their addresses are then offsets of one)
+  static constexpr int LDS = X > 2 * IMAGE ? (X > PARTS ? X : PARTS) : (2 * IMAGE > PARTS ? 2 * IMAGE : PARTS);
 };
+template <int PB>
+using NsCols = float[PB][16];  // a column block of a p-row matrix
 
-template <class T, int PB, int CB>
-__global__ __launch_bounds__(512) void k_ns_small(NsMatrix m, NsCoef cf, int steps, int exact, double eps, T* out, int tall) {
-  using S = NsSmall<PB, CB>;
-  extern __shared__ char lds[];
-  __shared__ NsScales z;
-  __shared__ double part[8];
-  const int l = (int)(threadIdx.x & 63), w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int h = l >> 5, c32 = l & 31;
-  const int p = (int)m.p, q = (int)m.q;
-  const int cols = (q + 31) / 32;  // column blocks
-  const T* g = (const T*)m.g + blockIdx.x * m.batch_stride;
-  float x[CB][PB][16];
-  double sum = 0.0;
+// y = S x, S an image.  One fragment of x at a time is split and met by all row blocks: PB (for one block: three) independent accumulators.
+template <int PB>
+__device__ __forceinline__ void ns_times(const char* image, const NsCols<PB>& x, NsCols<PB>& y) {
+  using S = NsRows<PB>;
+  const int l = lane_id();
+  const char* at = image + (l & 31) * S::PITCH + (l >> 5) * 16;
+  constexpr int APART = PB == 1 ? 3 : 1;
+  f32x16 acc[PB * APART];
 #pragma unroll
-  for (int c = 0; c < CB; ++c) {
-    const int j = (w + 8 * c) * 32 + c32;
-    // (32-bit offsets within the matrix: the host sees to it)
-    const unsigned at = (unsigned)(4 * h * (int)m.row_stride + j * (int)m.col_stride) * (unsigned)sizeof(T);
+  for (int a = 0; a < PB * APART; ++a) acc[a] = f32x16{};
+#pragma unroll
+  for (int k = 0; k < 2 * PB; ++k) {
+    f16x8 xh, xl, bh[PB], bl[PB];
+#pragma unroll
+    for (int a = 0; a < PB; ++a) {
+      bh[a] = *(const f16x8*)(at + a * 32 * S::PITCH + k * 32);
+      bl[a] = *(const f16x8*)(at + (a * 32 + S::P) * S::PITCH + k * 32);
+    }
+    split8(x[k >> 1], 8 * (k & 1), &xh, &xl);
+#pragma unroll
+    for (int a = 0; a < PB; ++a) acc[a * APART] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bh[a], xh, acc[a * APART], 0, 0, 0);
+#pragma unroll
+    for (int a = 0; a < PB; ++a) acc[a * APART + APART / 2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bl[a], xh, acc[a * APART + APART / 2], 0, 0, 0);
+#pragma unroll
+    for (int a = 0; a < PB; ++a) acc[a * APART + APART - 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bh[a], xl, acc[a * APART + APART - 1], 0, 0, 0);
+    if (PB > 1) {  // one step's fragments at a time: all of them would not fit the registers
+#pragma unroll
+      for (int a = 0; a < PB; ++a) asm volatile("" : "+v"(acc[a]));
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+#pragma unroll
+  for (int a = 0; a < PB; ++a)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) y[a][r] = APART == 1 ? acc[a][r] : (acc[a * APART + 1][r] + acc[a * APART + APART - 1][r]) + acc[a * APART][r];
+}
+// A column block to rows of LDS (hi plane, lo plane `plane` bytes on): the lane's column is at byte `at`, rows are `pitch` apart.  Neighbouring lanes swap
+// halves of two rows, so that each writes two neighbours of one.
+template <int PB>
+__device__ __forceinline__ void ns_scatter(char* lds, int pitch, int plane, int at, const NsCols<PB>& x) {
+  const int l = lane_id(), h = l >> 5;
+  const bool odd = l & 1;
+  char* base = lds + (4 * h + odd) * pitch + at - 2 * odd;
+  const unsigned pick = odd ? 0x03020706u : 0x05040100u;  // bytes of (mine, the neighbour's): even lanes the lower halves, odd lanes the upper ones
+#pragma unroll
+  for (int a = 0; a < PB; ++a)
+#pragma unroll
+    for (int r = 0; r < 16; r += 2) {
+      f16x2 hi, lo;
+      split(x[a][r], x[a][r + 1], &hi, &lo);
+      char* to = base + (32 * a + 8 * (r >> 2) + (r & 3)) * pitch;
+      const unsigned mh = __builtin_bit_cast(unsigned, hi), ml = __builtin_bit_cast(unsigned, lo);
+      const unsigned nh = (unsigned)__builtin_amdgcn_mov_dpp((int)mh, 0xb1, 0xf, 0xf, true);  // lanes 1 0 3 2
+      const unsigned nl = (unsigned)__builtin_amdgcn_mov_dpp((int)ml, 0xb1, 0xf, 0xf, true);
+      *(unsigned*)to = __builtin_amdgcn_perm(nh, mh, pick);
+      *(unsigned*)(to + plane) = __builtin_amdgcn_perm(nl, ml, pick);
+      if (r % 8 == 6) __builtin_amdgcn_sched_barrier(0);
+    }
+}
+// Column block b of a p x p matrix into an image.  (Row i of the image is row i: the matrices of a chain are symmetric but for their roundings, and an
+// image of the transpose would make those grow - the products of a chain commute only as long as all are polynomials of the SAME A.)
+template <int PB>
+__device__ __forceinline__ void ns_put(char* image, int b, const NsCols<PB>& x) {
+  using S = NsRows<PB>;
+  const int c = lane_id() & 31;
+  ns_scatter<PB>(image, S::PITCH, S::P * S::PITCH, 64 * b + 32 * (c >> 4) + 16 * ((c >> 2) & 1) + 8 * ((c >> 3) & 1) + 2 * (c & 3), x);
+}
+// Column block number c of X to rows
+template <int PB, int CB>
+__device__ __forceinline__ void ns_rows(char* lds, int c, const NsCols<PB>& x) {
+  using S = NsRows<PB, CB>;
+  ns_scatter<PB>(lds, S::PITCH_X, S::P * S::PITCH_X, 64 * c + 2 * (lane_id() & 31), x);
+}
+// Column block w % PB of X X^T from the rows in LDS, wave w's share w / PB of the K range (added up by ns_gather)
+template <int PB, int CB>
+__device__ __forceinline__ void ns_gram(const char* lds, int cols, NsCols<PB>& m) {
+  using S = NsRows<PB, CB>;
+  constexpr int pitch = S::PITCH_X;
+  const int w = wave_id(), l = lane_id();
+  f32x16 acc[PB];
+#pragma unroll
+  for (int a = 0; a < PB; ++a) acc[a] = f32x16{};
+  const int shares = S::shares(cols);
+  if (w < PB * shares) {
+    const char* at = lds + (l & 31) * pitch + (l >> 5) * 16;
+    const int j = w % PB * 32;
+    for (int k = w / PB; k < 2 * cols; k += shares) {
+      const f16x8 jh = *(const f16x8*)(at + j * pitch + k * 32), jl = *(const f16x8*)(at + (j + S::P) * pitch + k * 32);
+      f16x8 ih[PB], il[PB];
+#pragma unroll
+      for (int a = 0; a < PB; ++a) {
+        ih[a] = *(const f16x8*)(at + 32 * a * pitch + k * 32);
+        il[a] = *(const f16x8*)(at + (32 * a + S::P) * pitch + k * 32);
+      }
+#pragma unroll
+      for (int a = 0; a < PB; ++a) acc[a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ih[a], jh, acc[a], 0, 0, 0);
+#pragma unroll
+      for (int a = 0; a < PB; ++a) acc[a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(il[a], jh, acc[a], 0, 0, 0);
+#pragma unroll
+      for (int a = 0; a < PB; ++a) acc[a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ih[a], jl, acc[a], 0, 0, 0);
+    }
+  }
+#pragma unroll
+  for (int a = 0; a < PB; ++a)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) m[a][r] = acc[a][r];
+}
+// Adds the shares up: afterwards waves 0 .. PB - 1 have the column blocks.  The first barrier is for the rows, which have been read.
+template <int PB>
+__device__ __forceinline__ void ns_gather(char* lds, int cols, NsCols<PB>& m) {
+  using S = NsRows<PB>;
+  const int w = wave_id(), l = lane_id();
+  const int shares = S::shares(cols);
+  __syncthreads();
+  if (shares == 1) return;
+  if (w >= PB && w < PB * shares) {
+    float* mine = (float*)lds + (w - PB) * PB * 1024 + l;
 #pragma unroll
     for (int a = 0; a < PB; ++a)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int iu = 32 * a + 8 * (r >> 2) + (r & 3);
-        const char* row = (const char*)(g + iu * m.row_stride);
-        x[c][a][r] = (iu + 4 * h < p && j < q) ? to_f32(*(const T*)(row + at)) : 0.0f;
-      }
+      for (int r = 0; r < 16; ++r) mine[(a * 16 + r) * 64] = m[a][r];
   }
+  __syncthreads();
+  if (w < PB) {
+    for (int o = 1; o < shares; ++o) {
+      const float* its = (const float*)lds + (o * PB + w - PB) * PB * 1024 + l;
+#pragma unroll
+      for (int a = 0; a < PB; ++a)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) m[a][r] += its[(a * 16 + r) * 64];
+    }
+  }
+  __syncthreads();
+}
+// From A (waves 0 .. PB - 1: its column blocks, as summed) the image that X is multiplied with: B of a single step, or Q of the chain t .. end.
+// Images at lds and lds + IMAGE; returns the one that holds it; a barrier has passed.
+template <int PB>
+__device__ __forceinline__ char* ns_chain(char* lds, NsCols<PB>& m, const NsScales& z, int t, int end) {
+  using S = NsRows<PB>;
+  const int w = wave_id(), l = lane_id();
+  const bool a_wave = w < PB, q_wave = w >= 4 && w < 4 + PB;
+  char *ia = lds, *ip = lds + S::IMAGE;
+  const float gram = z.f[t].gram;
+#pragma unroll
+  for (int a = 0; a < PB; ++a) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) m[a][r] = q_wave ? 0.0f : gram * m[a][r];
+    if (a == w - 4)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (8 * (r >> 2) + 4 * (l >> 5) + (r & 3) == (l & 31)) m[a][r] = (float)(1 << NS_UNIT);
+  }
+  const bool alone = t == end;
+  for (;; ++t) {
+    const NsFactors f = z.f[t];
+    if (a_wave) ns_put<PB>(ia, w, m);
+    __syncthreads();
+    if (a_wave) {
+      NsCols<PB> p;
+      ns_times<PB>(ia, m, p);
+#pragma unroll
+      for (int a = 0; a < PB; ++a) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) p[a][r] = f.lin * m[a][r] + f.quad * p[a][r];
+        if (!alone && a == w)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (8 * (r >> 2) + 4 * (l >> 5) + (r & 3) == (l & 31)) p[a][r] += f.unit;
+      }
+      ns_put<PB>(ip, w, p);
+    }
+    __syncthreads();
+    if (alone) return ip;
+    const bool on = a_wave && t != end;
+    if (on || q_wave) {  // R = P A, Q <- P Q
+      NsCols<PB> y;
+      ns_times<PB>(ip, m, y);
+      const float by = a_wave ? f.half : f.chain;
+#pragma unroll
+      for (int a = 0; a < PB; ++a)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) m[a][r] = by * y[a][r];
+    }
+    if (t == end) break;
+    if (on) {
+      NsCols<PB> y;
+      ns_times<PB>(ip, m, y);
+#pragma unroll
+      for (int a = 0; a < PB; ++a)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) m[a][r] = f.next * y[a][r];
+    }
+  }
+  if (q_wave) ns_put<PB>(ia, w - 4, m);
+  __syncthreads();
+  return ia;
+}
+// Column block number c of G times f.  (32-bit offsets within the matrix: the host sees to it.)
+template <class T, int PB>
+__device__ __forceinline__ void ns_load(const T* g, const NsMatrix& m, long j0, int c, NsCols<PB>& x) {
+  const int l = lane_id(), h = l >> 5;
+  const long j = j0 + 32 * c + (l & 31);
+  const char* col = (const char*)(g + (j0 + 32 * c) * m.col_stride);
+  const unsigned rs = (unsigned)m.row_stride * (unsigned)sizeof(T);
+  const int rows = j < m.q ? (int)m.p - 4 * h : 0;
+  // rows past the end are read from the last one, columns past it from the first, and count as zeros: all loads are under way together
+  const unsigned side = (j < m.q ? l & 31 : 0) * (unsigned)m.col_stride * (unsigned)sizeof(T);
+  const unsigned end = ((unsigned)m.p - 1) * rs + side;
+  unsigned at = 4 * h * rs + side;
+  const char* from = m.q > j0 + 32 * c ? col : (const char*)g;
+  T v[PB][16];
+#pragma unroll
+  for (int a = 0; a < PB; ++a)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      v[a][r] = *(const T*)(from + min(at, end));
+      at += (r & 3) == 3 ? 5 * rs : rs;  // rows 0 1 2 3, 8 9 10 11, ..
+    }
+#pragma unroll
+  for (int a = 0; a < PB; ++a)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[a][r] = 32 * a + 8 * (r >> 2) + (r & 3) < rows ? to_f32(v[a][r]) : 0.0f;
+}
+template <class T, int PB>
+__device__ __forceinline__ void ns_store(T* out, const NsMatrix& m, long j0, int c, const NsCols<PB>& x, int last, bool tall) {
+  const int l = lane_id(), h = l >> 5;
+  const long j = j0 + 32 * c + (l & 31);
+  const long rs = tall ? 1 : m.q, cs = tall ? m.p : 1;
+  char* col = (char*)(out + (j0 + 32 * c) * cs);
+  const unsigned step = (unsigned)rs * (unsigned)sizeof(T);
+  int rows = j < m.q ? (int)m.p - 4 * h : 0;
+  asm volatile("" : "+v"(rows));  // (compare again: the 16 PB masks of the load are not worth keeping in scalar registers until here)
+  unsigned at = 4 * h * step + (l & 31) * (unsigned)cs * (unsigned)sizeof(T);
+#pragma unroll
+  for (int a = 0; a < PB; ++a)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      if (32 * a + 8 * (r >> 2) + (r & 3) < rows) *(T*)(col + at) = (T)ldexpf(x[a][r], last);
+      at += (r & 3) == 3 ? 5 * step : step;
+    }
+}
+
+// One workgroup does a whole matrix of up to 32 PB x 256 CB.
+template <class T, int PB, int CB>
+__global__ __launch_bounds__(512) void k_ns_small(NsMatrix m, NsCoef cf, int steps, double eps, T* out, int tall) {
+  extern __shared__ char lds[];
+  __shared__ NsScales z;
+  __shared__ NsCoef mine;
+  __shared__ double part[8];
+  const int l = lane_id(), w = wave_id();
+  ns_fetch(cf, steps, &mine, z.f);
+  const int cols = (int)((m.q + 31) / 32);
+  const T* g = (const T*)m.g + blockIdx.x * m.batch_stride;
+  NsCols<PB> x[CB];
+  double sum = 0.0;
+#pragma unroll
+  for (int c = 0; c < CB; ++c) ns_load<T, PB>(g, m, 0, w + 8 * c, x[c]);
 #pragma unroll
   for (int c = 0; c < CB; ++c)
 #pragma unroll
-    for (int a = 0; a < PB; ++a)
+    for (int a = 0; a < PB; ++a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) sum += (double)x[c][a][r] * (double)x[c][a][r];
+      __builtin_amdgcn_sched_barrier(0);
+    }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
   if (l == 0) part[w] = sum;
@@ -364,192 +653,46 @@ __global__ __launch_bounds__(512) void k_ns_small(NsMatrix m, NsCoef cf, int ste
   if (threadIdx.x == 0) {
     double s = 0.0;
     for (int i = 0; i < 8; ++i) s += part[i];
-    ns_scales(s, eps, cf, steps, z);
+    ns_scales(s, eps, mine, steps, z);
   }
   __syncthreads();
-  {
-    const double f = z.first;
+  const double first = z.first;
+#pragma unroll
+  for (int c = 0; c < CB; ++c)
+#pragma unroll
+    for (int a = 0; a < PB; ++a) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[c][a][r] = (float)((double)x[c][a][r] * first);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  for (int t = 0; t < steps;) {
+    int end = t;
+    while (!(mine.ends >> end & 1)) ++end;
 #pragma unroll
     for (int c = 0; c < CB; ++c)
-#pragma unroll
-      for (int a = 0; a < PB; ++a)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) x[c][a][r] = (float)((double)x[c][a][r] * f);
-  }
-  const int pitch = S::pitch_x(q);
-  for (int t = 0; t < steps; ++t) {
-    const bool pairs = t >= steps - exact;
-    const NsFactors f = z.f[t];
-    // X to LDS, hi plane then lo plane
-#pragma unroll
-    for (int c = 0; c < CB; ++c)
-      if (w + 8 * c < cols) {
-#pragma unroll
-        for (int a = 0; a < PB; ++a)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            char* at = lds + (32 * a + 8 * (r >> 2) + 4 * h + (r & 3)) * pitch + ((w + 8 * c) * 32 + c32) * 2;
-            _Float16 hi, lo;
-            split(x[c][a][r], &hi, &lo);
-            *(_Float16*)at = hi;
-            if (pairs) *(_Float16*)(at + S::P * pitch) = lo;
-          }
-      }
+      if (w + 8 * c < cols) ns_rows<PB, CB>(lds, w + 8 * c, x[c]);
     __syncthreads();
-    // A: block (bi, bj) of wave w % blocks, KS waves share its columns
-    f32x16 acc[S::OWN];
-#pragma unroll
-    for (int o = 0; o < S::OWN; ++o) {
-      acc[o] = f32x16{};
-      const int blk = S::KS > 1 ? w % S::BLOCKS : w + 8 * o;
-      if (blk < S::BLOCKS) {
-        const char* pi = lds + (blk / PB * 32 + c32) * pitch + h * 16;
-        const char* pj = lds + (blk % PB * 32 + c32) * pitch + h * 16;
-        for (int k = S::KS > 1 ? w / S::BLOCKS : 0; k < 2 * cols; k += S::KS) {
-          const f16x8 ih = *(const f16x8*)(pi + k * 32), jh = *(const f16x8*)(pj + k * 32);
-          acc[o] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ih, jh, acc[o], 0, 0, 0);
-          if (pairs) {
-            const f16x8 il = *(const f16x8*)(pi + S::P * pitch + k * 32), jl = *(const f16x8*)(pj + S::P * pitch + k * 32);
-            acc[o] = __builtin_amdgcn_mfma_f32_32x32x16_f16(il, jh, acc[o], 0, 0, 0);
-            acc[o] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ih, jl, acc[o], 0, 0, 0);
-          }
-        }
-      }
-    }
-    __syncthreads();
-    if constexpr (S::KS > 1) {
-      float* mine = (float*)lds + w * 1024 + l;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) mine[r * 64] = acc[0][r];
-      __syncthreads();
-      if (w < S::BLOCKS) {
-#pragma unroll
-        for (int o = 1; o < S::KS; ++o)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) acc[0][r] += mine[o * S::BLOCKS * 1024 + r * 64];
-      }
-      __syncthreads();
-    }
-    // A as pairs; it is symmetric, so the lane's column is a row and its four neighbouring rows are four neighbours in it
-#pragma unroll
-    for (int o = 0; o < S::OWN; ++o) {
-      const int blk = w + 8 * o;
-      if (blk < S::BLOCKS) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[o][r] *= f.gram;
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-          char* at = lds + (blk % PB * 32 + c32) * S::PITCH_A + (blk / PB * 32 + 2 * r + 4 * h) * 2;
-          f16x4 hi, lo;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            _Float16 u, v;
-            split(acc[o][r + e], &u, &v);
-            hi[e] = u;
-            lo[e] = v;
-          }
-          *(f16x4*)at = hi;
-          if (pairs) *(f16x4*)(at + S::P * S::PITCH_A) = lo;
-        }
-      }
-    }
-    __syncthreads();
-    // B = b A + c A A
-    f32x16 poly[S::OWN];
-#pragma unroll
-    for (int o = 0; o < S::OWN; ++o) {
-      poly[o] = f32x16{};
-      const int blk = w + 8 * o;
-      if (blk < S::BLOCKS) {
-        const char* pi = lds + (blk / PB * 32 + c32) * S::PITCH_A + h * 16;
-        const char* pj = lds + (blk % PB * 32 + c32) * S::PITCH_A + h * 16;
-#pragma unroll 2
-        for (int k = 0; k < 2 * PB; ++k) {
-          const f16x8 ih = *(const f16x8*)(pi + k * 32), jh = *(const f16x8*)(pj + k * 32);
-          poly[o] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ih, jh, poly[o], 0, 0, 0);
-          if (pairs) {
-            const f16x8 il = *(const f16x8*)(pi + S::P * S::PITCH_A + k * 32), jl = *(const f16x8*)(pj + S::P * S::PITCH_A + k * 32);
-            poly[o] = __builtin_amdgcn_mfma_f32_32x32x16_f16(il, jh, poly[o], 0, 0, 0);
-            poly[o] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ih, jl, poly[o], 0, 0, 0);
-          }
-        }
-#pragma unroll
-        for (int r = 0; r < 16; ++r) poly[o][r] = f.lin * acc[o][r] + f.quad * poly[o][r];
-      }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int o = 0; o < S::OWN; ++o) {
-      const int blk = w + 8 * o;
-      if (blk < S::BLOCKS) {
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-          // row (column of the block) c32, k = 8 (r / 4) + 4 h + e, at the place 16 (r / 8) + 8 h + 4 (r / 4 % 2) + e
-          char* at = lds + (blk % PB * 32 + c32) * S::PITCH_A + (blk / PB * 32 + 16 * (r >> 3) + 8 * h + 4 * ((r >> 2) & 1)) * 2;
-          f16x4 hi, lo;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            _Float16 u, v;
-            split(poly[o][r + e], &u, &v);
-            hi[e] = u;
-            lo[e] = v;
-          }
-          *(f16x4*)at = hi;
-          if (pairs) *(f16x4*)(at + S::P * S::PITCH_A) = lo;
-        }
-      }
-    }
-    __syncthreads();
-    // X <- a X + B X
+    NsCols<PB> a;
+    ns_gram<PB, CB>(lds, cols, a);
+    ns_gather<PB>(lds, cols, a);
+    const char* image = ns_chain<PB>(lds, a, z, t, end);
+    const float keep = z.f[end].keep, add = z.f[end].add;
 #pragma unroll
     for (int c = 0; c < CB; ++c)
       if (w + 8 * c < cols) {
-        f16x8 xh[2 * PB], xl[2 * PB];
+        NsCols<PB> y;
+        ns_times<PB>(image, x[c], y);
 #pragma unroll
-        for (int k = 0; k < 2 * PB; ++k)
+        for (int b = 0; b < PB; ++b)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            _Float16 u, v;
-            split(x[c][k >> 1][8 * (k & 1) + e], &u, &v);
-            xh[k][e] = u;
-            xl[k][e] = v;
-          }
-#pragma unroll
-        for (int a = 0; a < PB; ++a) {
-          const char* pi = lds + (32 * a + c32) * S::PITCH_A + h * 16;
-          f32x16 s = f32x16{};
-#pragma unroll
-          for (int k = 0; k < 2 * PB; ++k) {
-            const f16x8 bh = *(const f16x8*)(pi + k * 32);
-            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(bh, xh[k], s, 0, 0, 0);
-            if (pairs) {
-              const f16x8 bl = *(const f16x8*)(pi + S::P * S::PITCH_A + k * 32);
-              s = __builtin_amdgcn_mfma_f32_32x32x16_f16(bl, xh[k], s, 0, 0, 0);
-              s = __builtin_amdgcn_mfma_f32_32x32x16_f16(bh, xl[k], s, 0, 0, 0);
-            }
-          }
-#pragma unroll
-          for (int r = 0; r < 16; ++r) x[c][a][r] = f.keep * x[c][a][r] + f.add * s[r];
-          __builtin_amdgcn_sched_barrier(0);  // (one row block's fragments of B at a time: registers)
-        }
+          for (int r = 0; r < 16; ++r) x[c][b][r] = keep * x[c][b][r] + add * y[b][r];
       }
-    __syncthreads();
+    t = end + 1;
+    if (t < steps) __syncthreads();
   }
-  T* y = out + blockIdx.x * (size_t)p * q;
-  const int last = z.last, rs = tall ? 1 : q, cs = tall ? p : 1;
+  T* y = out + blockIdx.x * (size_t)(m.p * m.q);
 #pragma unroll
-  for (int c = 0; c < CB; ++c) {
-    const int j = (w + 8 * c) * 32 + c32;
-    const unsigned at = (unsigned)(4 * h * rs + j * cs) * (unsigned)sizeof(T);
-#pragma unroll
-    for (int a = 0; a < PB; ++a)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int iu = 32 * a + 8 * (r >> 2) + (r & 3);
-        char* row = (char*)(y + iu * rs);
-        if (iu + 4 * h < p && j < q) *(T*)(row + at) = (T)ldexpf(x[c][a][r], last);
-      }
-  }
+  for (int c = 0; c < CB; ++c) ns_store<T, PB>(y, m, 0, w + 8 * c, x[c], z.last, tall);
 }
 
 }  // namespace lb
