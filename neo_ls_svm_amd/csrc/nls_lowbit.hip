@@ -158,21 +158,39 @@ int operand(nls_ctx* ctx, const int8_t* p, long rows, long k, long ld, bool read
 }
 
 // ---- Newton-Schulz ----
-// Matrices one workgroup holds: X in 64 registers of 8 waves and once in LDS; it reads them with 32-bit offsets.
-bool ns_is_small(long p, long q, long row_stride, long col_stride) {
-  if (!((p <= 128 && q <= 256) || (p <= 64 && q <= 512) || (p <= 32 && q <= 1024))) return false;
+// Matrices of at most 128 rows (nls_ortho.h): NS_SMALL, one workgroup holds X in registers and in LDS; NS_SLABS, workgroups share its columns.  Both
+// read a matrix with 32-bit offsets.  NS_TILES: all others.
+enum NsPath { NS_SMALL, NS_SLABS, NS_TILES };
+NsPath ns_path(long p, long q, long row_stride, long col_stride) {
   const long reach = 1l << 28;
-  return row_stride >= 0 && col_stride >= 0 && (p + 32) * row_stride + (q + 256) * col_stride < reach;
+  if (p > 128 || row_stride < 0 || col_stride < 0 || row_stride >= reach || col_stride >= reach || (p + 32) * row_stride + 16 * col_stride >= reach) return NS_TILES;
+  return (q <= 256 || (p <= 64 && q <= 512) || (p <= 32 && q <= 1024)) ? NS_SMALL : NS_SLABS;
 }
 struct NsPlan {
+  NsPath path;
   long p, q;
   size_t x, xt, a, parts, scales, batch_bytes, total;
 };
+NsPlan ns_slab_plan(long p, long q, long batch) {
+  NsPlan w{};
+  w.p = p;
+  w.q = q;
+  const size_t rows = (size_t)(p + 31) / 32 * 32, slabs = (size_t)(q + NS_SLAB - 1) / NS_SLAB;
+  w.x = slabs * NS_SLAB * rows * 4;
+  w.a = slabs * rows * rows * 4;
+  w.parts = up256((size_t)batch * NS_PARTS * sizeof(double));
+  w.scales = up256((size_t)batch * sizeof(NsScales));
+  w.total = w.parts + w.scales + (size_t)batch * (w.x + w.a);
+  return w;
+}
 NsPlan ns_plan(long m, long n, long batch, long row_stride, long col_stride) {
   NsPlan w{};
   w.p = std::min(m, n);
   w.q = std::max(m, n);
-  if (ns_is_small(w.p, w.q, m > n ? col_stride : row_stride, m > n ? row_stride : col_stride)) return w;
+  const NsPath path = ns_path(w.p, w.q, m > n ? col_stride : row_stride, m > n ? row_stride : col_stride);
+  if (path == NS_SLABS) w = ns_slab_plan(w.p, w.q, batch);
+  w.path = path;
+  if (path != NS_TILES) return w;
   w.x = (size_t)w.p * pair_ld(w.q);
   w.xt = (size_t)w.q * pair_ld(w.p);
   w.a = (size_t)w.p * pair_ld(w.p);
@@ -213,7 +231,7 @@ int ns_product(nls_ctx* ctx, const NsArgs& g, bool pairs, long batch, hipStream_
 
 template <class T, int PB, int CB>
 int ns_small(nls_ctx* ctx, const NsMatrix& w, bool tall, long batch, const NsCoef& cf, int steps, double eps, T* out, hipStream_t st) {
-  constexpr int lds = NsRows<PB, CB>::LDS;
+  constexpr int lds = NsLds<PB, CB>::BYTES;
   NLSCHK(ask_lds(ctx, k_ns_small<T, PB, CB>, lds));
   k_ns_small<T, PB, CB><<<dim3((unsigned)batch), 512, lds, st>>>(w, cf, steps, eps, out, tall);
   LAUNCHED(ctx, "orthogonalize");
@@ -221,19 +239,61 @@ int ns_small(nls_ctx* ctx, const NsMatrix& w, bool tall, long batch, const NsCoe
 }
 template <class T>
 int ns_small_any(nls_ctx* ctx, const NsMatrix& w, bool tall, long batch, const NsCoef& cf, int steps, double eps, T* out, hipStream_t st) {
-#define NS_SMALL(PB, CB) return ns_small<T, PB, CB>(ctx, w, tall, batch, cf, steps, eps, out, st)
+#define NS_SMALL_OF(PB, CB) return ns_small<T, PB, CB>(ctx, w, tall, batch, cf, steps, eps, out, st)
+  if (w.q <= 128) {
+    if (w.p <= 32) NS_SMALL_OF(1, 1);
+    if (w.p <= 64) NS_SMALL_OF(2, 1);
+    if (w.p <= 96) NS_SMALL_OF(3, 1);
+    NS_SMALL_OF(4, 1);
+  }
   if (w.q <= 256) {
-    if (w.p <= 32) NS_SMALL(1, 1);
-    if (w.p <= 64) NS_SMALL(2, 1);
-    if (w.p <= 96) NS_SMALL(3, 1);
-    NS_SMALL(4, 1);
+    if (w.p <= 32) NS_SMALL_OF(1, 2);
+    if (w.p <= 64) NS_SMALL_OF(2, 2);
+    if (w.p <= 96) NS_SMALL_OF(3, 2);
+    NS_SMALL_OF(4, 2);
   }
   if (w.q <= 512) {
-    if (w.p <= 32) NS_SMALL(1, 2);
-    NS_SMALL(2, 2);
+    if (w.p <= 32) NS_SMALL_OF(1, 4);
+    NS_SMALL_OF(2, 4);
   }
-  NS_SMALL(1, 4);
-#undef NS_SMALL
+  NS_SMALL_OF(1, 8);
+#undef NS_SMALL_OF
+}
+
+// p <= 128, more columns than one workgroup holds.  Up to four slabs' shares of A are added up by every workgroup, more by a launch of their own.
+template <class T, int PB>
+int ns_slabs(nls_ctx* ctx, const NsMatrix& w, bool tall, long batch, const NsCoef& cf, int steps, double eps, T* out, char* ws, hipStream_t st) {
+  constexpr int P = 32 * PB, lds = NsLds<PB, NS_SLAB / 128>::BYTES;
+  NLSCHK(ask_lds(ctx, k_ns_slab<T, PB, true>, lds));
+  NLSCHK(ask_lds(ctx, k_ns_slab<T, PB, false>, lds));
+  NsSlabs g{};
+  g.m = w;
+  g.count = (int)std::min<long>(NS_PARTS, (std::max(w.p, w.q) + 3) / 4);
+  g.eps = eps;
+  g.steps = steps;
+  g.out = out;
+  g.tall = tall;
+  g.slabs = (int)((w.q + NS_SLAB - 1) / NS_SLAB);
+  const NsPlan plan = ns_slab_plan(w.p, w.q, batch);
+  g.parts = (const double*)ws;
+  g.scales = (NsScales*)(ws + plan.parts);
+  g.x = (float*)(ws + plan.parts + plan.scales);
+  g.a = (float*)(ws + plan.parts + plan.scales + batch * plan.x);
+  g.x_batch = plan.x / 4;
+  g.a_batch = plan.a / 4;
+  const dim3 grid((unsigned)g.slabs, (unsigned)batch);
+  k_ns_norm<T><<<dim3(g.count, (unsigned)batch), 256, 0, st>>>(w, (double*)ws);
+  k_ns_slab<T, PB, true><<<grid, 512, lds, st>>>(g, cf);
+  const bool sum = g.slabs > 4;
+  g.shares = sum ? 1 : g.slabs;
+  for (g.t = 0; g.t < steps; g.t = g.end + 1) {
+    g.end = g.t;
+    while (!(cf.ends >> g.end & 1)) ++g.end;
+    if (sum) k_ns_sum<<<dim3(P * P / 256, (unsigned)batch), 64, 0, st>>>(g.a, g.a_batch, P * P, g.slabs);
+    k_ns_slab<T, PB, false><<<grid, 512, lds, st>>>(g, cf);
+  }
+  LAUNCHED(ctx, "orthogonalize");
+  return NLS_OK;
 }
 
 // Which steps are done in one chain: as many as let small singular values grow by no more than `most` (nls_ortho.h); one at least.
@@ -258,9 +318,13 @@ int orthogonalize(nls_ctx* ctx, const NsMatrix& w, const NsPlan& plan, bool tall
   // The first steps may work on the hi halves alone where the result has few bits: what a rounding to 11 bits does to an early iterate is carried
   // along as a slightly different matrix would be, and the steps after it pull its singular values to the same curve.
   const int exact = sizeof(T) == 4 ? steps : std::is_same<T, __bf16>::value ? 2 : 3;
-  if (plan.total == 0) {
+  if (plan.path != NS_TILES) {
     ns_chains(cf, steps, sizeof(T) == 4 ? 0.0 : std::is_same<T, __bf16>::value ? 500.0 : 45.0);
-    return ns_small_any(ctx, w, tall, batch, cf, steps, eps, out, st);
+    if (plan.path == NS_SMALL) return ns_small_any(ctx, w, tall, batch, cf, steps, eps, out, st);
+    if (w.p <= 32) return ns_slabs<T, 1>(ctx, w, tall, batch, cf, steps, eps, out, ws, st);
+    if (w.p <= 64) return ns_slabs<T, 2>(ctx, w, tall, batch, cf, steps, eps, out, ws, st);
+    if (w.p <= 96) return ns_slabs<T, 3>(ctx, w, tall, batch, cf, steps, eps, out, ws, st);
+    return ns_slabs<T, 4>(ctx, w, tall, batch, cf, steps, eps, out, ws, st);
   }
   ns_chains(cf, steps, 0.0);
   double* parts = (double*)ws;

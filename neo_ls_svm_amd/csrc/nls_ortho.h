@@ -192,12 +192,11 @@ __device__ __forceinline__ void split(float v, float u, f16x2* hi, f16x2* lo) { 
   *hi = __builtin_convertvector(f32x2{v, u}, f16x2);
   *lo = __builtin_convertvector(f32x2{v - (float)(*hi)[0], u - (float)(*hi)[1]}, f16x2);
 }
-template <class V>
-__device__ __forceinline__ void split8(const V& v, int at, f16x8* hi, f16x8* lo) {  // v[at .. at + 7]
+__device__ __forceinline__ void split8(const float* v, f16x8* hi, f16x8* lo) {
 #pragma unroll
   for (int e = 0; e < 8; e += 2) {
     f16x2 h, o;
-    split(v[at + e], v[at + e + 1], &h, &o);
+    split(v[e], v[e + 1], &h, &o);
     (*hi)[e] = h[0];
     (*hi)[e + 1] = h[1];
     (*lo)[e] = o[0];
@@ -233,8 +232,8 @@ __global__ __launch_bounds__(256) void k_ns_pack(NsMatrix w, const NsScales* sca
     float v[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) v[e] = turn ? tile[part + e][row] : tile[row][part + e];
-    split8(v, 0, &hi[0], &lo[0]);
-    split8(v, 8, &hi[1], &lo[1]);
+    split8(v, &hi[0], &lo[0]);
+    split8(v + 8, &hi[1], &lo[1]);
     *(f16x8*)base = hi[0];
     *(f16x8*)(base + 16) = hi[1];
     *(f16x8*)(base + 64) = lo[0];
@@ -260,7 +259,7 @@ struct NsArgs {
 
 __device__ __forceinline__ void store_pairs(char* at, const float (&v)[8]) {  // eight neighbours of a row of pairs
   f16x8 h, o;
-  split8(v, 0, &h, &o);
+  split8(v, &h, &o);
   *(f16x8*)at = h;
   *(f16x8*)(at + 64) = o;
 }
@@ -353,12 +352,12 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
 }
 
 // ---- up to 128 rows -----------------------------------------------------------------------------------------------------------------------------
-// Everything p x p fits one workgroup; X is dealt out to the waves by columns and stays in registers in float32, in the places the matrix instruction
-// leaves its results in: a wave has column blocks of 32, lane l the column l % 32, registers r of row block a the rows 32 a + 8 (r / 4) + 4 (l / 32) + r % 4.
-//   S X for symmetric S contracts over rows, which lie along registers: registers 8 s .. 8 s + 7 of a block ARE a fragment of the 32 x 32 x 16 instruction
-//   if k runs in the order 16 s + {4 h .. 4 h + 3, 8 + 4 h .. 8 + 4 h + 3} for lane half h.  So S lies in LDS with its columns in that order (an "image",
-//   hi and lo planes) and X never moves (ns_times).
-//   A = X X^T contracts over columns, which lie across lanes: X goes through LDS as rows (ns_gram).
+// Everything p x p fits one workgroup of eight waves; X is dealt out to the waves by columns and stays in registers in float32, in the places the matrix
+// instruction leaves its results in: a wave has column blocks of 16, lane l the column l % 16, register r of row block a the row 16 a + 4 (l / 16) + r.
+//   S X for a p x p matrix S contracts over rows, which lie along registers: the registers of two neighbouring row blocks ARE a fragment of the
+//   16 x 16 x 32 instruction if k runs in the order {4 g .. 4 g + 3, 16 + 4 g .. 16 + 4 g + 3} for quarter g of the lanes.  So S lies in LDS with its columns
+//   in that order (an "image", hi and lo planes) and X never moves (ns_times).
+//   A = X X^T contracts over columns, which lie across lanes: X goes through LDS as rows (ns_rows, ns_gram).
 // Rows of LDS planes are 16 bytes longer than their numbers: eight neighbouring rows start in different banks.
 //
 // Chains: with P_t = a + b A_t + c A_t A_t the iterates are X_t+1 = P_t X_t and A_t+1 = P_t A_t P_t, so steps t .. t' can be done on p x p matrices
@@ -366,78 +365,107 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
 // what they do to small ones by the square of the polynomials' slope.  Measured against 64 bits (five standard steps, Gaussian, 1 / k and exponential
 // spectra, low rank + noise; 64 .. 512 rows): relative error of the result up to 4e-4 in one chain, 2e-5 in chains of 3 + 2, 9e-6 without (as
 // float32 products: 9e-6).  So bfloat16 results (rounding 1.7e-3) take chains of growth up to 500, float16 (2e-4) up to 45, float32 none.
-// Bound by latency for one small matrix (a chain's step is three dependent products and two barriers), by the matrix cores for batches.
-template <int PB, int CB = 1>
+// Bound by latency and by vector instructions (roundings to pairs) for few matrices: a step is a chain of dependent products, LDS round trips and
+// barriers.  Column blocks of 32 and the 32 x 32 x 16 instruction read half as much LDS but keep half as many waves busy: 64 x 64 26 us, 128 x 128 63 us
+// for five float32 steps; blocks of 16: see k_ns_small.
+template <int PB>
 struct NsRows {
-  static constexpr int P = 32 * PB;
+  static constexpr int P = 32 * PB, RB = 2 * PB;              // rows, row blocks
   static constexpr int PITCH = P * 2 + 16, IMAGE = 2 * P * PITCH;
-  static constexpr int KS = 8 / PB < 4 ? 8 / PB : 4;          // most waves that share a column block of A
-  // Adding shares up costs about as much as 2 .. 4 of the K steps it saves: measured, from these lengths on it pays.
-  __device__ static int shares(int cols) { return min(KS, max(1, cols / (PB <= 2 ? 4 : PB == 3 ? 3 : 2))); }
-  static constexpr int PARTS = (KS - 1) * PB * PB * 4096;     // what they add up through LDS
-  static constexpr int PITCH_X = CB * 512 + 16, X = 2 * P * PITCH_X;  // rows of X (a constant pitch: their addresses are then offsets of one)
-  static constexpr int LDS = X > 2 * IMAGE ? (X > PARTS ? X : PARTS) : (2 * IMAGE > PARTS ? 2 * IMAGE : PARTS);
+  static constexpr bool BOTH = PB > 2;                        // A's and Q's column blocks on the same waves, else A on the first four, Q on the others
+  static constexpr int KS = 8 / RB;                           // most waves that share a column block of A
+  static constexpr int PARTS = KS > 1 ? (KS - 1) * P * P * 4 : 0;
+  // Adding shares up costs about as much as the K steps it saves for short rows.  blocks: column blocks of X
+  __device__ static int shares(int blocks) { return KS == 1 ? 1 : min(KS, max(1, blocks / 8)); }
+};
+template <int PB, int CB>
+struct NsLds {  // X of 128 CB columns as rows (a constant pitch: their addresses are offsets of one another), or two images, or the shares
+  using S = NsRows<PB>;
+  static constexpr int PITCH = CB * 256 + 16, X = 2 * S::P * PITCH;
+  static constexpr int IMAGES = X > 2 * S::IMAGE ? X : 2 * S::IMAGE;
+  static constexpr int BYTES = IMAGES > S::PARTS ? IMAGES : S::PARTS;
 };
 template <int PB>
-using NsCols = float[PB][16];  // a column block of a p-row matrix
+using NsCols = float[2 * PB][4];  // a column block of a p-row matrix
 
-// y = S x, S an image.  One fragment of x at a time is split and met by all row blocks: PB (for one block: three) independent accumulators.
-template <int PB>
-__device__ __forceinline__ void ns_times(const char* image, const NsCols<PB>& x, NsCols<PB>& y) {
+// y = S x for N column blocks, S an image: every wave reads all of S, so blocks done together share what bounds it, the reads of LDS.  One fragment of x
+// at a time is split and met by all row blocks.
+template <int PB, int N>
+__device__ __forceinline__ void ns_times(const char* image, const NsCols<PB>* const (&x)[N], NsCols<PB>* const (&y)[N]) {
   using S = NsRows<PB>;
   const int l = lane_id();
-  const char* at = image + (l & 31) * S::PITCH + (l >> 5) * 16;
-  constexpr int APART = PB == 1 ? 3 : 1;
-  f32x16 acc[PB * APART];
+  const char* at = image + (l & 15) * S::PITCH + (l >> 4) * 16;
+  constexpr int APART = N == 1 && PB <= 2 ? 2 : 1;  // few accumulators: the small products in ones of their own
+  f32x4 acc[N][APART][S::RB];
 #pragma unroll
-  for (int a = 0; a < PB * APART; ++a) acc[a] = f32x16{};
+  for (int n = 0; n < N; ++n)
 #pragma unroll
-  for (int k = 0; k < 2 * PB; ++k) {
-    f16x8 xh, xl, bh[PB], bl[PB];
+    for (int o = 0; o < APART; ++o)
 #pragma unroll
-    for (int a = 0; a < PB; ++a) {
-      bh[a] = *(const f16x8*)(at + a * 32 * S::PITCH + k * 32);
-      bl[a] = *(const f16x8*)(at + (a * 32 + S::P) * S::PITCH + k * 32);
+      for (int a = 0; a < S::RB; ++a) acc[n][o][a] = f32x4{};
+#pragma unroll
+  for (int k = 0; k < PB; ++k) {
+    f16x8 xh[N], xl[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const NsCols<PB>& c = *x[n];
+      const float v[8] = {c[2 * k][0], c[2 * k][1], c[2 * k][2], c[2 * k][3], c[2 * k + 1][0], c[2 * k + 1][1], c[2 * k + 1][2], c[2 * k + 1][3]};
+      split8(v, &xh[n], &xl[n]);
     }
-    split8(x[k >> 1], 8 * (k & 1), &xh, &xl);
 #pragma unroll
-    for (int a = 0; a < PB; ++a) acc[a * APART] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bh[a], xh, acc[a * APART], 0, 0, 0);
+    for (int a = 0; a < S::RB; ++a) {
+      const f16x8 bh = *(const f16x8*)(at + a * 16 * S::PITCH + k * 64), bl = *(const f16x8*)(at + (a * 16 + S::P) * S::PITCH + k * 64);
 #pragma unroll
-    for (int a = 0; a < PB; ++a) acc[a * APART + APART / 2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bl[a], xh, acc[a * APART + APART / 2], 0, 0, 0);
+      for (int n = 0; n < N; ++n) acc[n][0][a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bh, xh[n], acc[n][0][a], 0, 0, 0);
 #pragma unroll
-    for (int a = 0; a < PB; ++a) acc[a * APART + APART - 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bh[a], xl, acc[a * APART + APART - 1], 0, 0, 0);
+      for (int n = 0; n < N; ++n) acc[n][APART - 1][a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bl, xh[n], acc[n][APART - 1][a], 0, 0, 0);
+#pragma unroll
+      for (int n = 0; n < N; ++n) acc[n][APART - 1][a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bh, xl[n], acc[n][APART - 1][a], 0, 0, 0);
+      if (PB > 2 && a % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+    }
     if (PB > 1) {  // one step's fragments at a time: all of them would not fit the registers
 #pragma unroll
-      for (int a = 0; a < PB; ++a) asm volatile("" : "+v"(acc[a]));
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int o = 0; o < APART; ++o)
+#pragma unroll
+          for (int a = 0; a < S::RB; ++a) asm volatile("" : "+v"(acc[n][o][a]));
       __builtin_amdgcn_sched_barrier(0);
     }
   }
 #pragma unroll
-  for (int a = 0; a < PB; ++a)
+  for (int n = 0; n < N; ++n)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) y[a][r] = APART == 1 ? acc[a][r] : (acc[a * APART + 1][r] + acc[a * APART + APART - 1][r]) + acc[a * APART][r];
+    for (int a = 0; a < S::RB; ++a)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) (*y[n])[a][r] = APART == 1 ? acc[n][0][a][r] : acc[n][0][a][r] + acc[n][APART - 1][a][r];
+}
+template <int PB>
+__device__ __forceinline__ void ns_times(const char* image, const NsCols<PB>& x, NsCols<PB>& y) {
+  const NsCols<PB>* const from[1] = {&x};
+  NsCols<PB>* const to[1] = {&y};
+  ns_times<PB, 1>(image, from, to);
 }
 // A column block to rows of LDS (hi plane, lo plane `plane` bytes on): the lane's column is at byte `at`, rows are `pitch` apart.  Neighbouring lanes swap
 // halves of two rows, so that each writes two neighbours of one.
 template <int PB>
 __device__ __forceinline__ void ns_scatter(char* lds, int pitch, int plane, int at, const NsCols<PB>& x) {
-  const int l = lane_id(), h = l >> 5;
+  const int l = lane_id();
   const bool odd = l & 1;
-  char* base = lds + (4 * h + odd) * pitch + at - 2 * odd;
+  char* base = lds + (4 * (l >> 4) + odd) * pitch + at - 2 * odd;
   const unsigned pick = odd ? 0x03020706u : 0x05040100u;  // bytes of (mine, the neighbour's): even lanes the lower halves, odd lanes the upper ones
 #pragma unroll
-  for (int a = 0; a < PB; ++a)
+  for (int a = 0; a < 2 * PB; ++a)
 #pragma unroll
-    for (int r = 0; r < 16; r += 2) {
+    for (int r = 0; r < 4; r += 2) {
       f16x2 hi, lo;
       split(x[a][r], x[a][r + 1], &hi, &lo);
-      char* to = base + (32 * a + 8 * (r >> 2) + (r & 3)) * pitch;
+      char* to = base + (16 * a + r) * pitch;
       const unsigned mh = __builtin_bit_cast(unsigned, hi), ml = __builtin_bit_cast(unsigned, lo);
       const unsigned nh = (unsigned)__builtin_amdgcn_mov_dpp((int)mh, 0xb1, 0xf, 0xf, true);  // lanes 1 0 3 2
       const unsigned nl = (unsigned)__builtin_amdgcn_mov_dpp((int)ml, 0xb1, 0xf, 0xf, true);
       *(unsigned*)to = __builtin_amdgcn_perm(nh, mh, pick);
       *(unsigned*)(to + plane) = __builtin_amdgcn_perm(nl, ml, pick);
-      if (r % 8 == 6) __builtin_amdgcn_sched_barrier(0);
     }
 }
 // Column block b of a p x p matrix into an image.  (Row i of the image is row i: the matrices of a chain are symmetric but for their roundings, and an
@@ -445,95 +473,103 @@ __device__ __forceinline__ void ns_scatter(char* lds, int pitch, int plane, int 
 template <int PB>
 __device__ __forceinline__ void ns_put(char* image, int b, const NsCols<PB>& x) {
   using S = NsRows<PB>;
-  const int c = lane_id() & 31;
-  ns_scatter<PB>(image, S::PITCH, S::P * S::PITCH, 64 * b + 32 * (c >> 4) + 16 * ((c >> 2) & 1) + 8 * ((c >> 3) & 1) + 2 * (c & 3), x);
+  const int c = lane_id() & 15;
+  ns_scatter<PB>(image, S::PITCH, S::P * S::PITCH, 64 * (b >> 1) + 16 * (c >> 2) + 8 * (b & 1) + 2 * (c & 3), x);
 }
 // Column block number c of X to rows
 template <int PB, int CB>
 __device__ __forceinline__ void ns_rows(char* lds, int c, const NsCols<PB>& x) {
-  using S = NsRows<PB, CB>;
-  ns_scatter<PB>(lds, S::PITCH_X, S::P * S::PITCH_X, 64 * c + 2 * (lane_id() & 31), x);
+  using L = NsLds<PB, CB>;
+  ns_scatter<PB>(lds, L::PITCH, NsRows<PB>::P * L::PITCH, 32 * c + 2 * (lane_id() & 15), x);
 }
-// Column block w % PB of X X^T from the rows in LDS, wave w's share w / PB of the K range (added up by ns_gather)
+// Column block w % RB of X X^T from the rows in LDS, wave w's share w / RB of the K range, then the shares added up: waves 0 .. RB - 1 have the result.
+// blocks: an even number of column blocks of X.  All rows have been read when this returns (a barrier).
 template <int PB, int CB>
-__device__ __forceinline__ void ns_gram(const char* lds, int cols, NsCols<PB>& m) {
-  using S = NsRows<PB, CB>;
-  constexpr int pitch = S::PITCH_X;
-  const int w = wave_id(), l = lane_id();
-  f32x16 acc[PB];
+__device__ __forceinline__ void ns_gram(char* lds, int blocks, NsCols<PB>& m) {
+  using S = NsRows<PB>;
+  constexpr int pitch = NsLds<PB, CB>::PITCH;
+  const int w = wave_id(), l = lane_id(), shares = S::shares(blocks);
+  constexpr int APART = PB <= 2 ? 2 : 1;
+  f32x4 acc[APART][S::RB];
 #pragma unroll
-  for (int a = 0; a < PB; ++a) acc[a] = f32x16{};
-  const int shares = S::shares(cols);
-  if (w < PB * shares) {
-    const char* at = lds + (l & 31) * pitch + (l >> 5) * 16;
-    const int j = w % PB * 32;
-    for (int k = w / PB; k < 2 * cols; k += shares) {
-      const f16x8 jh = *(const f16x8*)(at + j * pitch + k * 32), jl = *(const f16x8*)(at + (j + S::P) * pitch + k * 32);
-      f16x8 ih[PB], il[PB];
+  for (int o = 0; o < APART; ++o)
 #pragma unroll
-      for (int a = 0; a < PB; ++a) {
-        ih[a] = *(const f16x8*)(at + 32 * a * pitch + k * 32);
-        il[a] = *(const f16x8*)(at + (32 * a + S::P) * pitch + k * 32);
+    for (int a = 0; a < S::RB; ++a) acc[o][a] = f32x4{};
+  if (w < S::RB * shares) {
+    const char* at = lds + (l & 15) * pitch + (l >> 4) * 16;
+    const int j = w % S::RB * 16;
+    for (int k = w / S::RB; 2 * k < blocks; k += shares) {
+      const f16x8 jh = *(const f16x8*)(at + j * pitch + k * 64), jl = *(const f16x8*)(at + (j + S::P) * pitch + k * 64);
+#pragma unroll
+      for (int a = 0; a < S::RB; ++a) {
+        const f16x8 ih = *(const f16x8*)(at + 16 * a * pitch + k * 64), il = *(const f16x8*)(at + (16 * a + S::P) * pitch + k * 64);
+        acc[0][a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ih, jh, acc[0][a], 0, 0, 0);
+        acc[APART - 1][a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(il, jh, acc[APART - 1][a], 0, 0, 0);
+        acc[APART - 1][a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ih, jl, acc[APART - 1][a], 0, 0, 0);
+        if (PB > 2 && a % 4 == 3) __builtin_amdgcn_sched_barrier(0);
       }
-#pragma unroll
-      for (int a = 0; a < PB; ++a) acc[a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ih[a], jh, acc[a], 0, 0, 0);
-#pragma unroll
-      for (int a = 0; a < PB; ++a) acc[a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(il[a], jh, acc[a], 0, 0, 0);
-#pragma unroll
-      for (int a = 0; a < PB; ++a) acc[a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ih[a], jl, acc[a], 0, 0, 0);
     }
   }
 #pragma unroll
-  for (int a = 0; a < PB; ++a)
+  for (int a = 0; a < S::RB; ++a)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) m[a][r] = acc[a][r];
-}
-// Adds the shares up: afterwards waves 0 .. PB - 1 have the column blocks.  The first barrier is for the rows, which have been read.
-template <int PB>
-__device__ __forceinline__ void ns_gather(char* lds, int cols, NsCols<PB>& m) {
-  using S = NsRows<PB>;
-  const int w = wave_id(), l = lane_id();
-  const int shares = S::shares(cols);
+    for (int r = 0; r < 4; ++r) m[a][r] = APART == 1 ? acc[0][a][r] : acc[0][a][r] + acc[APART - 1][a][r];
   __syncthreads();
   if (shares == 1) return;
-  if (w >= PB && w < PB * shares) {
-    float* mine = (float*)lds + (w - PB) * PB * 1024 + l;
+  if (w >= S::RB && w < S::RB * shares) {
+    f32x4* mine = (f32x4*)lds + (w - S::RB) * S::RB * 64 + l;
 #pragma unroll
-    for (int a = 0; a < PB; ++a)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) mine[(a * 16 + r) * 64] = m[a][r];
+    for (int a = 0; a < S::RB; ++a) mine[a * 64] = f32x4{m[a][0], m[a][1], m[a][2], m[a][3]};
   }
   __syncthreads();
-  if (w < PB) {
+  if (w < S::RB) {
     for (int o = 1; o < shares; ++o) {
-      const float* its = (const float*)lds + (o * PB + w - PB) * PB * 1024 + l;
+      const f32x4* its = (const f32x4*)lds + (o * S::RB + w - S::RB) * S::RB * 64 + l;
 #pragma unroll
-      for (int a = 0; a < PB; ++a)
+      for (int a = 0; a < S::RB; ++a)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) m[a][r] += its[(a * 16 + r) * 64];
+        for (int r = 0; r < 4; ++r) m[a][r] += its[a * 64][r];
     }
   }
   __syncthreads();
 }
-// From A (waves 0 .. PB - 1: its column blocks, as summed) the image that X is multiplied with: B of a single step, or Q of the chain t .. end.
+// m[row][column] += v where they are equal; b: the column block
+template <int PB>
+__device__ __forceinline__ void ns_diagonal(int b, float v, NsCols<PB>& m) {
+  const int l = lane_id();
+#pragma unroll
+  for (int a = 0; a < 2 * PB; ++a)
+    if (a == b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (4 * (l >> 4) + r == (l & 15)) m[a][r] += v;
+}
+template <int PB>
+__device__ __forceinline__ void ns_scale(float v, NsCols<PB>& m) {
+#pragma unroll
+  for (int a = 0; a < 2 * PB; ++a)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) m[a][r] *= v;
+}
+// From A (waves 0 .. RB - 1: its column blocks, as summed) the image that X is multiplied with: B of a single step, or Q of the chain t .. end.
 // Images at lds and lds + IMAGE; returns the one that holds it; a barrier has passed.
 template <int PB>
 __device__ __forceinline__ char* ns_chain(char* lds, NsCols<PB>& m, const NsScales& z, int t, int end) {
   using S = NsRows<PB>;
-  const int w = wave_id(), l = lane_id();
-  const bool a_wave = w < PB, q_wave = w >= 4 && w < 4 + PB;
+  const int w = wave_id(), first_q = S::BOTH ? 0 : 4;
+  const bool a_wave = w < S::RB, q_wave = w >= first_q && w < first_q + S::RB;
   char *ia = lds, *ip = lds + S::IMAGE;
-  const float gram = z.f[t].gram;
-#pragma unroll
-  for (int a = 0; a < PB; ++a) {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) m[a][r] = q_wave ? 0.0f : gram * m[a][r];
-    if (a == w - 4)
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (8 * (r >> 2) + 4 * (l >> 5) + (r & 3) == (l & 31)) m[a][r] = (float)(1 << NS_UNIT);
-  }
+  NsCols<PB> own;  // Q's column block, where the wave has A's too
+  NsCols<PB>& q = S::BOTH ? own : m;
+  ns_scale<PB>(z.f[t].gram, m);
   const bool alone = t == end;
+  if (!alone && q_wave) {
+#pragma unroll
+    for (int a = 0; a < S::RB; ++a)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) q[a][r] = 0.0f;
+    ns_diagonal<PB>(w - first_q, (float)(1 << NS_UNIT), q);
+  }
   for (;; ++t) {
     const NsFactors f = z.f[t];
     if (a_wave) ns_put<PB>(ia, w, m);
@@ -542,88 +578,127 @@ __device__ __forceinline__ char* ns_chain(char* lds, NsCols<PB>& m, const NsScal
       NsCols<PB> p;
       ns_times<PB>(ia, m, p);
 #pragma unroll
-      for (int a = 0; a < PB; ++a) {
+      for (int a = 0; a < S::RB; ++a)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) p[a][r] = f.lin * m[a][r] + f.quad * p[a][r];
-        if (!alone && a == w)
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (8 * (r >> 2) + 4 * (l >> 5) + (r & 3) == (l & 31)) p[a][r] += f.unit;
-      }
+        for (int r = 0; r < 4; ++r) p[a][r] = f.lin * m[a][r] + f.quad * p[a][r];
+      if (!alone) ns_diagonal<PB>(w, f.unit, p);
       ns_put<PB>(ip, w, p);
     }
     __syncthreads();
     if (alone) return ip;
-    const bool on = a_wave && t != end;
-    if (on || q_wave) {  // R = P A, Q <- P Q
+    // Q <- P Q; R = P A, A <- P R
+    if (S::BOTH && a_wave && t != end) {
+      NsCols<PB> r, y;
+      const NsCols<PB>* const from[2] = {&m, &q};
+      NsCols<PB>* const to[2] = {&r, &y};
+      ns_times<PB, 2>(ip, from, to);
+      ns_scale<PB>(f.half, r);
+#pragma unroll
+      for (int a = 0; a < S::RB; ++a)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[a][e] = f.chain * y[a][e];
+      ns_times<PB>(ip, r, m);
+      ns_scale<PB>(f.next, m);
+      continue;
+    }
+    if (q_wave) {
       NsCols<PB> y;
-      ns_times<PB>(ip, m, y);
-      const float by = a_wave ? f.half : f.chain;
+      ns_times<PB>(ip, q, y);
 #pragma unroll
-      for (int a = 0; a < PB; ++a)
+      for (int a = 0; a < S::RB; ++a)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) m[a][r] = by * y[a][r];
+        for (int r = 0; r < 4; ++r) q[a][r] = f.chain * y[a][r];
     }
     if (t == end) break;
-    if (on) {
-      NsCols<PB> y;
-      ns_times<PB>(ip, m, y);
-#pragma unroll
-      for (int a = 0; a < PB; ++a)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) m[a][r] = f.next * y[a][r];
+    if (!S::BOTH && a_wave) {
+      NsCols<PB> r;
+      ns_times<PB>(ip, m, r);
+      ns_scale<PB>(f.half, r);
+      ns_times<PB>(ip, r, m);
+      ns_scale<PB>(f.next, m);
     }
   }
-  if (q_wave) ns_put<PB>(ia, w - 4, m);
+  if (q_wave) ns_put<PB>(ia, w - first_q, q);
   __syncthreads();
   return ia;
 }
-// Column block number c of G times f.  (32-bit offsets within the matrix: the host sees to it.)
+// Column block number c of G, from column j0 on.  (32-bit offsets within the matrix: the host sees to it.)
+// Rows past the end are read from the last one, columns past it from the first, and count as zeros: all loads are under way together.
 template <class T, int PB>
 __device__ __forceinline__ void ns_load(const T* g, const NsMatrix& m, long j0, int c, NsCols<PB>& x) {
-  const int l = lane_id(), h = l >> 5;
-  const long j = j0 + 32 * c + (l & 31);
-  const char* col = (const char*)(g + (j0 + 32 * c) * m.col_stride);
+  const int l = lane_id();
+  const long jb = j0 + 16 * c, j = jb + (l & 15);
+  const char* from = (const char*)(jb < m.q ? g + jb * m.col_stride : g);
   const unsigned rs = (unsigned)m.row_stride * (unsigned)sizeof(T);
-  const int rows = j < m.q ? (int)m.p - 4 * h : 0;
-  // rows past the end are read from the last one, columns past it from the first, and count as zeros: all loads are under way together
-  const unsigned side = (j < m.q ? l & 31 : 0) * (unsigned)m.col_stride * (unsigned)sizeof(T);
+  const unsigned side = (j < m.q ? l & 15 : 0) * (unsigned)m.col_stride * (unsigned)sizeof(T);
+  const int rows = j < m.q ? (int)m.p - 4 * (l >> 4) : 0;
   const unsigned end = ((unsigned)m.p - 1) * rs + side;
-  unsigned at = 4 * h * rs + side;
-  const char* from = m.q > j0 + 32 * c ? col : (const char*)g;
-  T v[PB][16];
+  unsigned at = 4 * (l >> 4) * rs + side;
+  T v[2 * PB][4];
 #pragma unroll
-  for (int a = 0; a < PB; ++a)
+  for (int a = 0; a < 2 * PB; ++a)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
+    for (int r = 0; r < 4; ++r) {
       v[a][r] = *(const T*)(from + min(at, end));
-      at += (r & 3) == 3 ? 5 * rs : rs;  // rows 0 1 2 3, 8 9 10 11, ..
+      at += r == 3 ? 13 * rs : rs;  // rows 0 1 2 3, 16 17 18 19, ..
     }
 #pragma unroll
-  for (int a = 0; a < PB; ++a)
+  for (int a = 0; a < 2 * PB; ++a)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) x[a][r] = 32 * a + 8 * (r >> 2) + (r & 3) < rows ? to_f32(v[a][r]) : 0.0f;
+    for (int r = 0; r < 4; ++r) x[a][r] = 16 * a + r < rows ? to_f32(v[a][r]) : 0.0f;
 }
 template <class T, int PB>
 __device__ __forceinline__ void ns_store(T* out, const NsMatrix& m, long j0, int c, const NsCols<PB>& x, int last, bool tall) {
-  const int l = lane_id(), h = l >> 5;
-  const long j = j0 + 32 * c + (l & 31);
+  const int l = lane_id();
+  const long j = j0 + 16 * c + (l & 15);
   const long rs = tall ? 1 : m.q, cs = tall ? m.p : 1;
-  char* col = (char*)(out + (j0 + 32 * c) * cs);
+  char* col = (char*)(out + (j0 + 16 * c) * cs);
   const unsigned step = (unsigned)rs * (unsigned)sizeof(T);
-  int rows = j < m.q ? (int)m.p - 4 * h : 0;
-  asm volatile("" : "+v"(rows));  // (compare again: the 16 PB masks of the load are not worth keeping in scalar registers until here)
-  unsigned at = 4 * h * step + (l & 31) * (unsigned)cs * (unsigned)sizeof(T);
+  int rows = j < m.q ? (int)m.p - 4 * (l >> 4) : 0;
+  asm volatile("" : "+v"(rows));  // (compare again: the masks of the load are not worth keeping in scalar registers until here)
+  unsigned at = 4 * (l >> 4) * step + (l & 15) * (unsigned)cs * (unsigned)sizeof(T);
 #pragma unroll
-  for (int a = 0; a < PB; ++a)
+  for (int a = 0; a < 2 * PB; ++a)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      if (32 * a + 8 * (r >> 2) + (r & 3) < rows) *(T*)(col + at) = (T)ldexpf(x[a][r], last);
-      at += (r & 3) == 3 ? 5 * step : step;
+    for (int r = 0; r < 4; ++r) {
+      if (16 * a + r < rows) *(T*)(col + at) = (T)ldexpf(x[a][r], last);
+      at += r == 3 ? 13 * step : step;
+    }
+}
+template <int PB>
+__device__ __forceinline__ void ns_first(double first, NsCols<PB>& x) {
+#pragma unroll
+  for (int a = 0; a < 2 * PB; ++a)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x[a][r] = (float)((double)x[a][r] * first);
+}
+// X <- keep X + add S X for the wave's column blocks w, w + 8, .. below `blocks`, two at a time
+template <int PB, int CB>
+__device__ __forceinline__ void ns_advance(const char* image, float keep, float add, int blocks, NsCols<PB> (&x)[CB]) {
+  const int w = wave_id();
+  constexpr int N = CB > 1 ? 2 : 1;
+#pragma unroll
+  for (int c = 0; c < CB; c += N)
+    if (w + 8 * c < blocks) {
+      NsCols<PB> y[N];
+      const NsCols<PB>* from[N];
+      NsCols<PB>* to[N];
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        from[n] = &x[c + n];
+        to[n] = &y[n];
+      }
+      ns_times<PB, N>(image, from, to);
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int a = 0; a < 2 * PB; ++a)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[c + n][a][r] = keep * x[c + n][a][r] + add * y[n][a][r];
     }
 }
 
-// One workgroup does a whole matrix of up to 32 PB x 256 CB.
+// One workgroup does a whole matrix of up to 32 PB x 128 CB.
 template <class T, int PB, int CB>
 __global__ __launch_bounds__(512) void k_ns_small(NsMatrix m, NsCoef cf, int steps, double eps, T* out, int tall) {
   extern __shared__ char lds[];
@@ -632,7 +707,7 @@ __global__ __launch_bounds__(512) void k_ns_small(NsMatrix m, NsCoef cf, int ste
   __shared__ double part[8];
   const int l = lane_id(), w = wave_id();
   ns_fetch(cf, steps, &mine, z.f);
-  const int cols = (int)((m.q + 31) / 32);
+  const int blocks = (int)((m.q + 31) / 32) * 2;
   const T* g = (const T*)m.g + blockIdx.x * m.batch_stride;
   NsCols<PB> x[CB];
   double sum = 0.0;
@@ -641,11 +716,9 @@ __global__ __launch_bounds__(512) void k_ns_small(NsMatrix m, NsCoef cf, int ste
 #pragma unroll
   for (int c = 0; c < CB; ++c)
 #pragma unroll
-    for (int a = 0; a < PB; ++a) {
+    for (int a = 0; a < 2 * PB; ++a)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sum += (double)x[c][a][r] * (double)x[c][a][r];
-      __builtin_amdgcn_sched_barrier(0);
-    }
+      for (int r = 0; r < 4; ++r) sum += (double)x[c][a][r] * (double)x[c][a][r];
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
   if (l == 0) part[w] = sum;
@@ -656,43 +729,143 @@ __global__ __launch_bounds__(512) void k_ns_small(NsMatrix m, NsCoef cf, int ste
     ns_scales(s, eps, mine, steps, z);
   }
   __syncthreads();
-  const double first = z.first;
 #pragma unroll
-  for (int c = 0; c < CB; ++c)
-#pragma unroll
-    for (int a = 0; a < PB; ++a) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) x[c][a][r] = (float)((double)x[c][a][r] * first);
-      __builtin_amdgcn_sched_barrier(0);
-    }
+  for (int c = 0; c < CB; ++c) ns_first<PB>(z.first, x[c]);
   for (int t = 0; t < steps;) {
     int end = t;
     while (!(mine.ends >> end & 1)) ++end;
 #pragma unroll
     for (int c = 0; c < CB; ++c)
-      if (w + 8 * c < cols) ns_rows<PB, CB>(lds, w + 8 * c, x[c]);
+      if (w + 8 * c < blocks) ns_rows<PB, CB>(lds, w + 8 * c, x[c]);
     __syncthreads();
     NsCols<PB> a;
-    ns_gram<PB, CB>(lds, cols, a);
-    ns_gather<PB>(lds, cols, a);
+    ns_gram<PB, CB>(lds, blocks, a);
     const char* image = ns_chain<PB>(lds, a, z, t, end);
-    const float keep = z.f[end].keep, add = z.f[end].add;
-#pragma unroll
-    for (int c = 0; c < CB; ++c)
-      if (w + 8 * c < cols) {
-        NsCols<PB> y;
-        ns_times<PB>(image, x[c], y);
-#pragma unroll
-        for (int b = 0; b < PB; ++b)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) x[c][b][r] = keep * x[c][b][r] + add * y[b][r];
-      }
+    ns_advance<PB, CB>(image, z.f[end].keep, z.f[end].add, blocks, x);
     t = end + 1;
     if (t < steps) __syncthreads();
   }
   T* y = out + blockIdx.x * (size_t)(m.p * m.q);
 #pragma unroll
   for (int c = 0; c < CB; ++c) ns_store<T, PB>(y, m, 0, w + 8 * c, x[c], z.last, tall);
+}
+
+// ---- up to 128 rows, any number of columns --------------------------------------------------------------------------------------------------------
+// Workgroups take slabs of 256 columns.  One launch a chain of steps: every workgroup adds the slabs' shares of A up (k_ns_sum has done so before where
+// there are many), works the chain out for itself - all do the same, the result does not have to travel - multiplies its slab and leaves its share
+// of the next A.  Between launches X lies in the workspace as the registers had it.
+struct NsSlabs {
+  NsMatrix m;
+  const double* parts;   // sums of squares (k_ns_norm)
+  int count;
+  double eps;
+  NsScales* scales;
+  float *x, *a;          // a matrix's X; its slabs' shares of A (32 PB x 32 PB floats each, in register order)
+  size_t x_batch, a_batch;  // floats from matrix to matrix
+  int slabs, shares;     // shares of A to add up
+  int steps, t, end;     // the chain; first launch: t < 0
+  void* out;
+  int tall;
+};
+constexpr int NS_SLAB = 256;
+
+template <class T, int PB, bool FIRST>
+__global__ __launch_bounds__(512) void k_ns_slab(NsSlabs g, NsCoef cf) {
+  using S = NsRows<PB>;
+  constexpr int CB = NS_SLAB / 128, FLOATS = S::RB * 4 * 64;  // of a column block
+  extern __shared__ char lds[];
+  __shared__ NsScales z;
+  __shared__ NsCoef mine;
+  const int l = lane_id(), w = wave_id();
+  const long j0 = (long)blockIdx.x * NS_SLAB;
+  const int blocks = (int)((min((long)NS_SLAB, g.m.q - j0) + 31) / 32) * 2;
+  float* xs = g.x + blockIdx.y * g.x_batch + ((size_t)blockIdx.x * 8 + w) * CB * FLOATS + l * 4;
+  float* as = g.a + blockIdx.y * g.a_batch;
+  const T* from = (const T*)g.m.g + blockIdx.y * g.m.batch_stride;
+  const bool fresh = FIRST || g.t == 0;  // X_0 comes from G
+  const bool last = !FIRST && g.end + 1 == g.steps;
+  NsCols<PB> x[CB], m;
+  if (fresh) {
+#pragma unroll
+    for (int c = 0; c < CB; ++c) ns_load<T, PB>(from, g.m, j0, w + 8 * c, x[c]);
+  } else {
+#pragma unroll
+    for (int c = 0; c < CB; ++c)
+#pragma unroll
+      for (int a = 0; a < S::RB; ++a) {
+        const f32x4 v = *(const f32x4*)(xs + c * FLOATS + a * 256);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[c][a][r] = v[r];
+      }
+  }
+  if constexpr (FIRST) {
+    ns_fetch(cf, g.steps, &mine, z.f);
+    double s = 0.0;
+    if (w == 0)
+      for (int i = l; i < g.count; i += 64) s += g.parts[(size_t)blockIdx.y * NS_PARTS + i];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+    __syncthreads();
+    if (threadIdx.x == 0) ns_scales(s, g.eps, mine, g.steps, z);
+    __syncthreads();
+    if (blockIdx.x == 0)
+      for (int i = threadIdx.x; i < (int)(sizeof(NsScales) / 4); i += 512) ((int*)(g.scales + blockIdx.y))[i] = ((const int*)&z)[i];
+  } else {
+    for (int i = threadIdx.x; i < (int)(sizeof(NsScales) / 4); i += 512) ((int*)&z)[i] = ((const int*)(g.scales + blockIdx.y))[i];
+    if (w < S::RB) {
+      const float* at = as + w * FLOATS + l * 4;
+#pragma unroll
+      for (int a = 0; a < S::RB; ++a)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) m[a][r] = 0.0f;
+      for (int o = 0; o < g.shares; ++o, at += S::P * S::P)
+#pragma unroll
+        for (int a = 0; a < S::RB; ++a) {
+          const f32x4 v = *(const f32x4*)(at + a * 256);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) m[a][r] += v[r];
+        }
+    }
+    __syncthreads();
+  }
+  if (fresh) {
+#pragma unroll
+    for (int c = 0; c < CB; ++c) ns_first<PB>(z.first, x[c]);
+  }
+  if constexpr (!FIRST) {
+    const char* image = ns_chain<PB>(lds, m, z, g.t, g.end);
+    ns_advance<PB, CB>(image, z.f[g.end].keep, z.f[g.end].add, blocks, x);
+    if (last) {
+      T* y = (T*)g.out + blockIdx.y * (size_t)(g.m.p * g.m.q);
+#pragma unroll
+      for (int c = 0; c < CB; ++c) ns_store<T, PB>(y, g.m, j0, w + 8 * c, x[c], z.last, g.tall);
+      return;
+    }
+#pragma unroll
+    for (int c = 0; c < CB; ++c)
+#pragma unroll
+      for (int a = 0; a < S::RB; ++a) *(f32x4*)(xs + c * FLOATS + a * 256) = f32x4{x[c][a][0], x[c][a][1], x[c][a][2], x[c][a][3]};
+    __syncthreads();  // the image has been read
+  }
+#pragma unroll
+  for (int c = 0; c < CB; ++c)
+    if (w + 8 * c < blocks) ns_rows<PB, CB>(lds, w + 8 * c, x[c]);
+  __syncthreads();
+  ns_gram<PB, CB>(lds, blocks, m);
+  if (w < S::RB) {
+    float* at = as + (size_t)blockIdx.x * S::P * S::P + w * FLOATS + l * 4;
+#pragma unroll
+    for (int a = 0; a < S::RB; ++a) *(f32x4*)(at + a * 256) = f32x4{m[a][0], m[a][1], m[a][2], m[a][3]};
+  }
+}
+
+// The slabs' shares of A added up into the first, in order: one thread four numbers, from all slabs
+__global__ __launch_bounds__(64) void k_ns_sum(float* a, size_t a_batch, int floats, int slabs) {
+  float* at = a + blockIdx.y * a_batch + ((size_t)blockIdx.x * 64 + threadIdx.x) * 4;
+  f32x4 s = *(const f32x4*)at;
+#pragma unroll 8
+  for (int o = 1; o < slabs; ++o) s += *(const f32x4*)(at + (size_t)o * floats);
+  *(f32x4*)at = s;
 }
 
 }  // namespace lb

@@ -235,7 +235,7 @@ def gradient(rng, m, n):
 
 @pytest.mark.parametrize("name", sorted(DTYPES))
 @pytest.mark.parametrize(
-    "m,n", [(1, 1), (1, 7), (300, 1), (2, 3), (31, 33), (32, 64), (63, 64), (64, 128), (65, 64), (128, 128), (100, 333), (129, 130), (257, 190), (64, 2000), (700, 512), (1025, 1100)]
+    "m,n", [(1, 1), (1, 7), (300, 1), (2, 3), (31, 33), (32, 64), (63, 64), (64, 128), (65, 64), (128, 128), (100, 333), (129, 130), (257, 190), (64, 2000), (700, 512), (1025, 1100), (5, 1100), (1200, 20), (31, 1025), (64, 513), (90, 1500), (128, 257), (128, 3001), (97, 300), (129, 300)]
 )
 def test_orthogonalize(m, n, name):
     rng = np.random.default_rng(m * 17 + n)
@@ -245,7 +245,7 @@ def test_orthogonalize(m, n, name):
     newton_schulz_check(out, host(g), nls.NEWTON_SCHULZ, 5, 1e-7, name, m + n)
 
 
-@pytest.mark.parametrize("batch,m,n", [(1, 64, 64), (5, 48, 80), (33, 80, 48), (3, 200, 260), (2, 1, 9)])
+@pytest.mark.parametrize("batch,m,n", [(1, 64, 64), (5, 48, 80), (33, 80, 48), (3, 200, 260), (2, 1, 9), (3, 120, 700), (4, 1300, 10), (2, 128, 128)])
 def test_orthogonalize_batches(batch, m, n):
     rng = np.random.default_rng(batch + m)
     g = np.stack([10.0 ** (2 * i - 4) * gradient(rng, m, n) for i in range(batch)]) if batch < 8 else np.stack([gradient(rng, m, n) for _ in range(batch)])
