@@ -122,14 +122,20 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const T* x, long rows, lo
   }
 }
 
-// Rows of 8-bit numbers that do not start at multiples of 16 bytes, laid out again so that they do (padding: zeros).
-__global__ __launch_bounds__(256) void k_align_rows(const signed char* x, long rows, long k, long ld, signed char* y, long ldy) {
+// Rows of 8-bit numbers that do not start at multiples of 16 bytes, laid out again so that they do (padding: zeros): one or two matrices a launch.
+struct AlignRows {
+  const signed char* x;
+  signed char* y;
+  long rows, ld;
+};
+__global__ __launch_bounds__(256) void k_align_rows(AlignRows a, AlignRows b, long k, long ldy) {
+  const AlignRows g = blockIdx.y ? b : a;
   const long per = ldy / 4;
-  for (long t = (long)blockIdx.x * 256 + threadIdx.x; t < rows * per; t += (long)gridDim.x * 256) {
+  for (long t = (long)blockIdx.x * 256 + threadIdx.x; t < g.rows * per; t += (long)gridDim.x * 256) {
     const long r = t / per, c = (t - r * per) * 4;
     int v[4];
-    for (int e = 0; e < 4; ++e) v[e] = c + e < k ? x[r * ld + c + e] : 0;
-    *(unsigned*)(y + r * ldy + c) = pack4(v[0], v[1], v[2], v[3]);
+    for (int e = 0; e < 4; ++e) v[e] = c + e < k ? g.x[r * g.ld + c + e] : 0;
+    *(unsigned*)(g.y + r * ldy + c) = pack4(v[0], v[1], v[2], v[3]);
   }
 }
 
@@ -151,6 +157,39 @@ __device__ __forceinline__ float bias_at(const Int8Args& g, int n) {
 // (sum * a_scale) * b_scale, left to right: the product of the two scales alone may fall below the smallest float.
 __device__ __forceinline__ float scaled(int sum, float as, float bs, float bias) { return (float)sum * as * bs + bias; }
 
+// The tile's sums, scaled, to y.  A thread has the same N channels in all its rows.
+template <class T, class TL, int BI, int N>
+__device__ __forceinline__ void int8_write(const TL& t, const Int8Args& g, int i0, int j0, char* lds) {
+  typedef T V __attribute__((ext_vector_type(N)));
+  constexpr int ACROSS = BI / N, ROWS = TL::THREADS / ACROSS;
+  T* y = (T*)g.y;
+  const int iw = threadIdx.x % ACROSS * N, n = i0 + iw;
+  const bool there = n < g.n;
+  float bs[N], bias[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    bs[e] = there ? g.b_scale[n + e] : 0.0f;
+    bias[e] = there ? bias_at<T>(g, n + e) : 0.0f;
+  }
+#pragma unroll
+  for (int c = 0; c < TL::CHUNKS; ++c) {
+    __syncthreads();
+    t.spill(c, lds);
+    __syncthreads();
+    for (int r = threadIdx.x / ACROSS; r < TL::CHUNK; r += ROWS) {
+      const int m = j0 + TL::column(c, r);
+      if (m >= g.m || !there) continue;
+      int s[N];
+      chunk_sums<TL, N>(lds, r, iw, s);
+      const float as = g.a_scale[m];
+      V v;
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[e] = (T)scaled(s[e], as, bs[e], bias[e]);
+      *(V*)(y + (size_t)m * g.n + n) = v;
+    }
+  }
+}
+
 // Many rows: P = b (its rows lie along a chunk's words, as neighbours in a row of y), Q = a.
 template <class T, class TL, int BI, int BJ>
 __global__ __launch_bounds__(TL::THREADS) void k_int8_tile(Int8Args g, int ti, int tj, int strip) {
@@ -161,34 +200,11 @@ __global__ __launch_bounds__(TL::THREADS) void k_int8_tile(Int8Args g, int ti, i
   TL t;
   const int steps = (g.k + 127) / 128;
   t.run(g.b, i0, g.a, j0, 0, steps, g.k - (steps - 1) * 128, lds);
-  T* y = (T*)g.y;
-  // a thread has the same eight channels in all its rows
-  constexpr int ACROSS = BI / 8, ROWS = TL::THREADS / ACROSS;
-  const int iw = threadIdx.x % ACROSS * 8, n = i0 + iw, left = g.n - n;
-  float bs[8], bias[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    bs[e] = e < left ? g.b_scale[n + e] : 0.0f;
-    bias[e] = e < left ? bias_at<T>(g, n + e) : 0.0f;
-  }
-  const bool whole = left >= 8 && g.n % (16 / (int)sizeof(T)) == 0;
-#pragma unroll
-  for (int c = 0; c < TL::CHUNKS; ++c) {
-    __syncthreads();
-    t.spill(c, lds);
-    __syncthreads();
-    for (int r = threadIdx.x / ACROSS; r < TL::CHUNK; r += ROWS) {
-      const int m = j0 + TL::column(c, r);
-      if (m >= g.m || left <= 0) continue;
-      int s[8];
-      chunk_sums<TL>(lds, r, iw, s);
-      const float as = g.a_scale[m];
-      float v[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = scaled(s[e], as, bs[e], bias[e]);
-      store8(y + (size_t)m * g.n + n, v, left, whole);
-    }
-  }
+  // 16 bytes of a row of y a thread where rows start at such multiples, else one element: neighbouring threads neighbouring columns in both
+  if (g.n % (16 / (int)sizeof(T)) == 0)
+    int8_write<T, TL, BI, 16 / sizeof(T)>(t, g, i0, j0, lds);
+  else
+    int8_write<T, TL, BI, 1>(t, g, i0, j0, lds);
 }
 
 // ---- few rows ------------------------------------------------------------------------------------------------------------------------------

@@ -142,18 +142,32 @@ int check_int8(nls_ctx* ctx, const char* what, int64_t m, int64_t n, int64_t k, 
   return NLS_OK;
 }
 
-// a and b as the kernels take them: laid out again in the workspace where the caller's rows do not start at multiples of 16 bytes.
-int operand(nls_ctx* ctx, const int8_t* p, long rows, long k, long ld, bool ready, char** ws, Operand* out, hipStream_t st) {
-  if (ready) {
-    *out = Operand{(const char*)p, (unsigned)ld, (int)rows};
-    return NLS_OK;
-  }
+// a and b as the kernels take them: laid out again in the workspace, in one launch, where the caller's rows do not start at multiples of 16 bytes.
+struct Int8Rows {
+  const int8_t* p;
+  long rows, ld;
+  bool ready;
+};
+int operands(nls_ctx* ctx, const Int8Rows& a, const Int8Rows& b, long k, char* ws, Operand* oa, Operand* ob, hipStream_t st) {
+  AlignRows todo[2] = {};
+  int count = 0;
+  long most = 0;
   const long ldy = up16(k);
-  const long work = rows * (ldy / 4);
-  k_align_rows<<<dim3((unsigned)std::min<long>((work + 255) / 256, 65536)), 256, 0, st>>>((const signed char*)p, rows, k, ld, (signed char*)*ws, ldy);
+  for (int i = 0; i < 2; ++i) {
+    const Int8Rows& r = i ? b : a;
+    Operand* o = i ? ob : oa;
+    if (r.ready) {
+      *o = Operand{(const char*)r.p, (unsigned)r.ld, (int)r.rows};
+      continue;
+    }
+    todo[count++] = AlignRows{(const signed char*)r.p, (signed char*)ws, r.rows, r.ld};
+    *o = Operand{ws, (unsigned)ldy, (int)r.rows};
+    ws += up256((size_t)r.rows * ldy);
+    most = std::max(most, r.rows * (ldy / 4));
+  }
+  if (!count) return NLS_OK;
+  k_align_rows<<<dim3((unsigned)std::min<long>((most + 255) / 256, 32768), (unsigned)count), 256, 0, st>>>(todo[0], todo[1], k, ldy);
   LAUNCHED(ctx, "int8_matmul (alignment)");
-  *out = Operand{*ws, (unsigned)ldy, (int)rows};
-  *ws += up256((size_t)rows * ldy);
   return NLS_OK;
 }
 
@@ -416,10 +430,9 @@ extern "C" int nls_int8_matmul(nls_ctx* ctx, const int8_t* a, int64_t lda, const
   DeviceGuard dev(ctx->device);
   HIPCHK(ctx, dev.err);
   hipStream_t st = (hipStream_t)stream;
-  char* ws = (char*)workspace;
   Int8Args g{};
-  NLSCHK(operand(ctx, a, m, k, lda, aligned_rows(a, lda, k, flags, NLS_INT8_A_PADDED), &ws, &g.a, st));
-  NLSCHK(operand(ctx, b, n, k, ldb, aligned_rows(b, ldb, k, flags, NLS_INT8_B_PADDED), &ws, &g.b, st));
+  NLSCHK(operands(ctx, {a, m, lda, aligned_rows(a, lda, k, flags, NLS_INT8_A_PADDED)}, {b, n, ldb, aligned_rows(b, ldb, k, flags, NLS_INT8_B_PADDED)}, k,
+                  (char*)workspace, &g.a, &g.b, st));
   g.a_scale = a_scale;
   g.b_scale = b_scale;
   g.bias = bias;
@@ -462,7 +475,9 @@ extern "C" int nls_int8_linear(nls_ctx* ctx, const void* x, int type, int64_t ro
   g.n = (int)n;
   g.k = (int)k;
   g.y = y;
-  NLSCHK(operand(ctx, b, n, k, ldb, aligned_rows(b, ldb, k, flags, NLS_INT8_B_PADDED), &ws, &g.b, st));
+  const bool b_ready = aligned_rows(b, ldb, k, flags, NLS_INT8_B_PADDED);
+  NLSCHK(operands(ctx, {nullptr, 0, 0, true}, {b, n, ldb, b_ready}, k, ws, &g.a, &g.b, st));
+  if (!b_ready) ws += up256((size_t)n * up16(k));
   if (int8_fused(m, k)) {
     const int size = type_size(type);
     const FewX f{x, row_stride, col_stride, col_stride == 1 && (uintptr_t)x % (8 * size) == 0 && (m == 1 || row_stride % 8 == 0)};

@@ -306,7 +306,7 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
     for (int r = threadIdx.x / ACROSS; r < TL::CHUNK; r += ROWS) {
       const int j = j0 + TL::column(c, r);
       float v[8];
-      chunk_sums<TL>(lds, r, iw, v);
+      chunk_sums<TL, 8>(lds, r, iw, v);
       f16x8 eh = {}, el = {};
       const bool there = j < g.J && (size_t)i * 4 < ldi;  // (rows are padded: whole groups of eight, zeros behind the end)
       if (KIND != NS_GRAM && there) {

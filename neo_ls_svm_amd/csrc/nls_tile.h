@@ -299,15 +299,15 @@ struct Ring {
   }
 };
 
-// Eight sums of a chunk: row r, words i .. i + 7
-template <class TL, class V>
-__device__ __forceinline__ void chunk_sums(const char* lds, int r, int i, V (&v)[8]) {
+// Sums of a chunk: row r, words i .. i + N - 1
+template <class TL, int N, class V>
+__device__ __forceinline__ void chunk_sums(const char* lds, int r, int i, V (&v)[N]) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = ((const V*)lds)[r * TL::PITCH + i + e];
+  for (int e = 0; e < N; ++e) v[e] = ((const V*)lds)[r * TL::PITCH + i + e];
 #pragma unroll
   for (int o = 1; o < TL::PARTS; ++o)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] += ((const V*)lds)[(o * TL::CHUNK + r) * TL::PITCH + i + e];
+    for (int e = 0; e < N; ++e) v[e] += ((const V*)lds)[(o * TL::CHUNK + r) * TL::PITCH + i + e];
 }
 
 // Tiles in an order that keeps the ones a die works on together: workgroups are dealt to the 8 dies in turn, so die x takes the x-th eighth of the

@@ -63,6 +63,7 @@ class _Tensors:
         self.kinds = {getattr(lib, name): i for i, name in enumerate(_NAMES)}
         self.types = tuple(getattr(lib, name) for name in _NAMES)
         self.int8, self.float32, self.uint8, self.strided, self.Tensor = lib.int8, lib.float32, lib.uint8, lib.strided, lib.Tensor
+        self._empty = lib.empty
         self._raw_stream = getattr(lib._C, "_cuda_getCurrentRawStream", None)
 
     def begin(self):
@@ -99,11 +100,31 @@ class _Tensors:
         return x.untyped_storage().nbytes() - x.storage_offset() * x.element_size()
 
     def empty(self, shape, dtype):
-        return self.lib.empty(shape, dtype=dtype, device=self.device)
+        return self._empty(*shape, dtype=dtype, device=self.device) if shape else self._empty((), dtype=dtype, device=self.device)
 
     def rows(self, rows, k, ld, lead):
-        held = self.lib.empty((*lead, ld), dtype=self.int8, device=self.device)
+        held = self._empty(*lead, ld, dtype=self.int8, device=self.device)
         return held, held if ld == k else held[..., :k]
+
+    # The usual arguments - dense matrices - in the few checks they need; all others, wrong ones among them, the long way.
+    def float_rows(self, x, what):
+        if isinstance(x, self.Tensor) and x.get_device() == self.index and x.layout is self.strided and x.is_contiguous() and not x.requires_grad and not x.is_neg():
+            shape, kind = x.shape, self.kinds.get(x.dtype)
+            if kind is not None and len(shape) == 2 and shape[1] > 0:
+                return x, shape[:1], shape[0], shape[1], shape[1], 1, kind
+        return _float_rows(self, x, what)
+
+    def int8_rows(self, x, what, scale, scale_what):
+        T, strided = self.Tensor, self.strided
+        if (
+            isinstance(x, T) and isinstance(scale, T) and x.dtype is self.int8 and scale.dtype is self.float32
+            and x.get_device() == self.index == scale.get_device() and x.layout is strided is scale.layout
+            and x.is_contiguous() and scale.is_contiguous() and not scale.requires_grad and not scale.is_neg()
+        ):  # fmt: skip
+            shape = x.shape
+            if len(shape) == 2 and scale.shape == shape[:1] and 0 < shape[1] <= MAX_K and not shape[1] & 15:
+                return x, scale, shape[:1], shape[0], shape[1], shape[1], True
+        return _int8_rows(self, x, what, scale, scale_what)
 
     def scratch(self, nbytes):
         return self.lib.empty(nbytes, dtype=self.uint8, device=self.device)
@@ -161,6 +182,12 @@ class _Arrays:
     @staticmethod
     def room(x):
         return x.nbytes
+
+    def float_rows(self, x, what):
+        return _float_rows(self, x, what)
+
+    def int8_rows(self, x, what, scale, scale_what):
+        return _int8_rows(self, x, what, scale, scale_what)
 
     def empty(self, shape, dtype):
         return DeviceArray(self.ctx, shape, dtype=dtype)
@@ -312,7 +339,7 @@ def quantize_rows(x, ctx: Context | None = None):
     scale 0; a row with a NaN or an infinity has that for its scale and zeros in ``q``.  The rows of a ``q`` on the GPU start at multiples of 16
     bytes (its last axis is dense, its rows may have gaps): that is how ``int8_matmul`` and ``int8_linear`` read them without a copy."""
     sp = _space(x, ctx)
-    x, lead, rows, k, rs, cs, kind = _float_rows(sp, x, "x")
+    x, lead, rows, k, rs, cs, kind = sp.float_rows(x, "x")
     stream = sp.begin()
     ld = _up16(k)
     held, q = sp.rows(rows, k, ld, lead)
@@ -332,8 +359,8 @@ def int8_matmul(a, a_scale, b, b_scale, bias=None, dtype="float32", ctx: Context
     kind = _kind_of(dtype, "dtype")
     if kind >= len(sp.types):
         raise ValueError("dtype: NumPy arrays and DeviceArrays have no bfloat16")
-    a, a_scale, lead, m, k, lda, a_ready = _int8_rows(sp, a, "a", a_scale, "a_scale")
-    b, b_scale, b_lead, n, kb, ldb, b_ready = _int8_rows(sp, b, "b", b_scale, "b_scale")
+    a, a_scale, lead, m, k, lda, a_ready = sp.int8_rows(a, "a", a_scale, "a_scale")
+    b, b_scale, b_lead, n, kb, ldb, b_ready = sp.int8_rows(b, "b", b_scale, "b_scale")
     if len(b_lead) != 1 or kb != k:
         raise ValueError(f"b must be a matrix with rows of {k} elements, not of shape {(*b_lead, kb)}")
     bias, bias_kind = _bias(sp, bias, n, kind)
@@ -343,12 +370,15 @@ def int8_matmul(a, a_scale, b, b_scale, bias=None, dtype="float32", ctx: Context
         lib = sp.ctx.lib
         pa, pb = sp.ptr(a), sp.ptr(b)
         flags = (_A_PADDED if a_ready else 0) | (_B_PADDED if b_ready else 0)
-        need = C.c_size_t()
-        lib.nls_int8_matmul_workspace(pa, lda, pb, ldb, m, n, k, flags, need)
-        ws = sp.scratch(need.value) if need.value else None
+        nbytes, ws = 0, None
+        if not (a_ready and b_ready) or (pa | pb | lda | ldb) & 15:  # rows that have to be laid out again
+            need = C.c_size_t()
+            lib.nls_int8_matmul_workspace(pa, lda, pb, ldb, m, n, k, flags, need)
+            nbytes = need.value
+            ws = sp.scratch(nbytes) if nbytes else None
         _call(
             sp.ctx, lib.nls_int8_matmul, pa, lda, sp.ptr(a_scale), pb, ldb, sp.ptr(b_scale), None if bias is None else sp.ptr(bias), bias_kind,
-            m, n, k, sp.ptr(y), kind, flags, None if ws is None else sp.ptr(ws), need.value, stream,
+            m, n, k, sp.ptr(y), kind, flags, None if ws is None else sp.ptr(ws), nbytes, stream,
         )  # fmt: skip
     return sp.done(y)
 
@@ -356,8 +386,8 @@ def int8_matmul(a, a_scale, b, b_scale, bias=None, dtype="float32", ctx: Context
 def int8_linear(x, b, b_scale, bias=None, ctx: Context | None = None):
     """``int8_matmul(*quantize_rows(x), b, b_scale, bias, dtype=x.dtype)`` in one call: ``x`` (..., k) in 16 or 32 bits against rows held in 8."""
     sp = _space(x, ctx)
-    x, lead, m, k, rs, cs, kind = _float_rows(sp, x, "x")
-    b, b_scale, b_lead, n, kb, ldb, b_ready = _int8_rows(sp, b, "b", b_scale, "b_scale")
+    x, lead, m, k, rs, cs, kind = sp.float_rows(x, "x")
+    b, b_scale, b_lead, n, kb, ldb, b_ready = sp.int8_rows(b, "b", b_scale, "b_scale")
     if len(b_lead) != 1 or kb != k:
         raise ValueError(f"b must be a matrix with rows of {k} elements, not of shape {(*b_lead, kb)}")
     bias, bias_kind = _bias(sp, bias, n, kind)
@@ -396,15 +426,19 @@ def orthogonalize(g, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: float = 1e
         raise ValueError("steps must be a whole number from 1 to 32")
     steps = int(steps)
     try:
-        rows = [tuple(float(v) for v in row) for row in coefficients] if hasattr(coefficients[0], "__len__") else [tuple(float(v) for v in coefficients)] * steps
-    except (TypeError, ValueError, IndexError):
-        rows = []
-    if len(rows) != steps or any(len(row) != 3 or not all(math.isfinite(v) for v in row) for row in rows):
+        flat = [float(v) for v in coefficients] if len(coefficients) == 3 and not hasattr(coefficients[0], "__len__") else None
+        if flat is None:
+            flat = [float(v) for row in coefficients for v in row] if len(coefficients) == steps and all(len(row) == 3 for row in coefficients) else []
+        else:
+            flat *= steps
+    except TypeError:
+        flat = []
+    if len(flat) != 3 * steps or not all(map(math.isfinite, flat)):
         raise ValueError(f"coefficients must be three finite numbers, or three for each of the {steps} steps")
     eps = float(eps)
     if not 0.0 <= eps < 1e30:
         raise ValueError("eps must be a number >= 0")
-    table = (C.c_double * (3 * steps))(*(v for row in rows for v in row))
+    table = (C.c_double * (3 * steps))(*flat)
     m, n = shape[-2:]
     batch = math.prod(shape[:-2])
     if isinstance(g, DeviceArray):
