@@ -157,10 +157,19 @@ __device__ __forceinline__ float bias_at(const Int8Args& g, int n) {
 // (sum * a_scale) * b_scale, left to right: the product of the two scales alone may fall below the smallest float.
 __device__ __forceinline__ float scaled(int sum, float as, float bs, float bias) { return (float)sum * as * bs + bias; }
 
-// The tile's sums, scaled, to y.  A thread has the same N channels in all its rows.
-template <class T, class TL, int BI, int N>
-__device__ __forceinline__ void int8_write(const TL& t, const Int8Args& g, int i0, int j0, char* lds) {
+// Many rows: P = b (its rows lie along a chunk's words, as neighbours in a row of y), Q = a.
+// N: elements of a row of y a thread writes at once - 16 bytes where the rows start at such multiples, else one; neighbouring threads neighbouring
+// columns in both.  A thread has the same channels in all its rows.
+template <class T, class TL, int BI, int BJ, int N>
+__global__ __launch_bounds__(TL::THREADS) void k_int8_tile(Int8Args g, int ti, int tj, int strip) {
   typedef T V __attribute__((ext_vector_type(N)));
+  extern __shared__ char lds[];
+  int bi, bj;
+  strip_order(die_order(blockIdx.x, ti * tj), ti, tj, strip, &bi, &bj);
+  const int i0 = bi * BI, j0 = bj * BJ;
+  TL t;
+  const int steps = (g.k + 127) / 128;
+  t.run(g.b, i0, g.a, j0, 0, steps, g.k - (steps - 1) * 128, lds);
   constexpr int ACROSS = BI / N, ROWS = TL::THREADS / ACROSS;
   T* y = (T*)g.y;
   const int iw = threadIdx.x % ACROSS * N, n = i0 + iw;
@@ -188,23 +197,6 @@ __device__ __forceinline__ void int8_write(const TL& t, const Int8Args& g, int i
       *(V*)(y + (size_t)m * g.n + n) = v;
     }
   }
-}
-
-// Many rows: P = b (its rows lie along a chunk's words, as neighbours in a row of y), Q = a.
-template <class T, class TL, int BI, int BJ>
-__global__ __launch_bounds__(TL::THREADS) void k_int8_tile(Int8Args g, int ti, int tj, int strip) {
-  extern __shared__ char lds[];
-  int bi, bj;
-  strip_order(die_order(blockIdx.x, ti * tj), ti, tj, strip, &bi, &bj);
-  const int i0 = bi * BI, j0 = bj * BJ;
-  TL t;
-  const int steps = (g.k + 127) / 128;
-  t.run(g.b, i0, g.a, j0, 0, steps, g.k - (steps - 1) * 128, lds);
-  // 16 bytes of a row of y a thread where rows start at such multiples, else one element: neighbouring threads neighbouring columns in both
-  if (g.n % (16 / (int)sizeof(T)) == 0)
-    int8_write<T, TL, BI, 16 / sizeof(T)>(t, g, i0, j0, lds);
-  else
-    int8_write<T, TL, BI, 1>(t, g, i0, j0, lds);
 }
 
 // ---- few rows ------------------------------------------------------------------------------------------------------------------------------

@@ -33,10 +33,14 @@ struct DeviceGuard {
     if (e__ != hipSuccess) return fail(ctx, NLS_ERR_HIP, "%s: launch failed: %s", what, hipGetErrorString(e__)); \
   } while (0)
 
-// Dynamic LDS beyond 64 KB has to be asked for once per kernel and device.
-template <class F>
-int ask_lds(nls_ctx* ctx, F f, int bytes) {
-  if (bytes > 65536) HIPCHK(ctx, hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+// Dynamic LDS beyond 64 KB has to be asked for, once per kernel and device.
+template <auto F>
+int ask_lds(nls_ctx* ctx, int bytes) {
+  static std::atomic<unsigned long long> asked{0};  // a bit a device (the first 64; asking again does no harm)
+  const unsigned long long bit = ctx->device < 64 ? 1ull << ctx->device : 0;
+  if (bytes <= 65536 || (asked.load(std::memory_order_relaxed) & bit)) return NLS_OK;
+  HIPCHK(ctx, hipFuncSetAttribute(reinterpret_cast<const void*>(F), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  asked.fetch_or(bit, std::memory_order_relaxed);
   return NLS_OK;
 }
 
@@ -79,14 +83,21 @@ int quantize_any(nls_ctx* ctx, const void* x, int type, long rows, long k, long 
 }
 
 // ---- 8-bit product ----
-template <class T, class TL, int BI, int BJ>
+template <class T, class TL, int BI, int BJ, int N>
 int int8_tile(nls_ctx* ctx, const Int8Args& g, hipStream_t st) {
   const int ti = (g.n + BI - 1) / BI, tj = (g.m + BJ - 1) / BJ;
   constexpr int LDS = std::max(TL::LDS, TL::SCRATCH);
-  NLSCHK(ask_lds(ctx, k_int8_tile<T, TL, BI, BJ>, LDS));
-  k_int8_tile<T, TL, BI, BJ><<<dim3((unsigned)((long)ti * tj)), TL::THREADS, LDS, st>>>(g, ti, tj, 8);
+  NLSCHK((ask_lds<&k_int8_tile<T, TL, BI, BJ, N>>(ctx, LDS)));
+  k_int8_tile<T, TL, BI, BJ, N><<<dim3((unsigned)((long)ti * tj)), TL::THREADS, LDS, st>>>(g, ti, tj, 8);
   LAUNCHED(ctx, "int8_matmul");
   return NLS_OK;
+}
+template <class T, int N>
+int int8_tile(nls_ctx* ctx, const Int8Args& g, hipStream_t st) {
+  auto tiles = [&](long i, long j) { return ((g.n + i - 1) / i) * ((g.m + j - 1) / j); };
+  if (tiles(256, 256) >= ctx->cus) return int8_tile<T, Tile<MODE_I8, 256, 256, 2, 4, 2>, 256, 256, N>(ctx, g, st);
+  if (tiles(128, 128) >= ctx->cus) return int8_tile<T, Tile<MODE_I8, 128, 128, 2, 2, 2>, 128, 128, N>(ctx, g, st);
+  return int8_tile<T, Ring<MODE_I8, 2>, 64, 64, N>(ctx, g, st);
 }
 template <class T, int MG, int NG, bool FUSED>
 int int8_few(nls_ctx* ctx, const Int8Args& g, const FewX& f, hipStream_t st) {
@@ -108,9 +119,7 @@ int int8_product(nls_ctx* ctx, const Int8Args& g, hipStream_t st) {
   if (g.m <= 32) return int8_few<T, 2>(ctx, g, st);
   if (g.m <= 48) return int8_few<T, 3>(ctx, g, st);
   if (g.m <= 64) return int8_few<T, 4>(ctx, g, st);
-  const long big = (long)((g.n + 127) / 128) * ((g.m + 127) / 128);
-  if (big >= ctx->cus) return int8_tile<T, Tile<MODE_I8, 128, 128, 2, 2, 2>, 128, 128>(ctx, g, st);
-  return int8_tile<T, Ring<MODE_I8, 2>, 64, 64>(ctx, g, st);
+  return g.n % (16 / (int)sizeof(T)) == 0 ? int8_tile<T, 16 / sizeof(T)>(ctx, g, st) : int8_tile<T, 1>(ctx, g, st);
 }
 // Whether int8_linear quantises inside the product: every workgroup does all the rows of x over again, which has to stay small beside its share of b.
 bool int8_fused(long m, long k) { return m <= 4 && m * k <= 32768; }
@@ -223,7 +232,7 @@ int ns_product_tile(nls_ctx* ctx, NsArgs g, long batch, hipStream_t st) {
   constexpr bool SYM = KIND == NS_GRAM || KIND == NS_POLY;
   constexpr int LDS = std::max(TL::LDS, TL::SCRATCH);
   const long tiles = SYM ? (long)g.ti * (g.ti + 1) / 2 : (long)g.ti * g.tj;
-  NLSCHK(ask_lds(ctx, k_ns_product<KIND, T, TL, MODE, B, B>, LDS));
+  NLSCHK((ask_lds<&k_ns_product<KIND, T, TL, MODE, B, B>>(ctx, LDS)));
   k_ns_product<KIND, T, TL, MODE, B, B><<<dim3((unsigned)tiles, 1, (unsigned)batch), TL::THREADS, LDS, st>>>(g);
   LAUNCHED(ctx, "orthogonalize");
   return NLS_OK;
@@ -235,6 +244,7 @@ int ns_product(nls_ctx* ctx, const NsArgs& g, long batch, hipStream_t st) {
     const long i = (g.I + b - 1) / b, j = (g.J + b - 1) / b;
     return (SYM ? i * (i + 1) / 2 : i * j) * batch;
   };
+  if (tiles(256) * 2 >= ctx->cus) return ns_product_tile<KIND, T, Tile<MODE, 256, 256, 2, 4, 2>, MODE, 256>(ctx, g, batch, st);
   if (tiles(128) >= ctx->cus) return ns_product_tile<KIND, T, Tile<MODE, 128, 128, 2, 2, 2>, MODE, 128>(ctx, g, batch, st);
   return ns_product_tile<KIND, T, Ring<MODE, 2>, MODE, 64>(ctx, g, batch, st);
 }
@@ -246,7 +256,7 @@ int ns_product(nls_ctx* ctx, const NsArgs& g, bool pairs, long batch, hipStream_
 template <class T, int PB, int CB>
 int ns_small(nls_ctx* ctx, const NsMatrix& w, bool tall, long batch, const NsCoef& cf, int steps, double eps, T* out, hipStream_t st) {
   constexpr int lds = NsLds<PB, CB>::BYTES;
-  NLSCHK(ask_lds(ctx, k_ns_small<T, PB, CB>, lds));
+  NLSCHK((ask_lds<&k_ns_small<T, PB, CB>>(ctx, lds)));
   k_ns_small<T, PB, CB><<<dim3((unsigned)batch), 512, lds, st>>>(w, cf, steps, eps, out, tall);
   LAUNCHED(ctx, "orthogonalize");
   return NLS_OK;
@@ -278,8 +288,8 @@ int ns_small_any(nls_ctx* ctx, const NsMatrix& w, bool tall, long batch, const N
 template <class T, int PB>
 int ns_slabs(nls_ctx* ctx, const NsMatrix& w, bool tall, long batch, const NsCoef& cf, int steps, double eps, T* out, char* ws, hipStream_t st) {
   constexpr int P = 32 * PB, lds = NsLds<PB, NS_SLAB / 128>::BYTES;
-  NLSCHK(ask_lds(ctx, k_ns_slab<T, PB, true>, lds));
-  NLSCHK(ask_lds(ctx, k_ns_slab<T, PB, false>, lds));
+  NLSCHK((ask_lds<&k_ns_slab<T, PB, true>>(ctx, lds)));
+  NLSCHK((ask_lds<&k_ns_slab<T, PB, false>>(ctx, lds)));
   NsSlabs g{};
   g.m = w;
   g.count = (int)std::min<long>(NS_PARTS, (std::max(w.p, w.q) + 3) / 4);

@@ -195,10 +195,7 @@ struct Tile {
       next = next + BUF == LDS ? 0 : next + BUF;
     }
     arrive<0>();
-    if (MODE == MODE_I8 && last_valid < 128)
-      multiply<true>(lds + now, last_valid);
-    else
-      multiply<false>(lds + now, 128);
+    multiply<MODE == MODE_I8>(lds + now, last_valid);  // (masked whether ragged or not: two ways to the accumulators' end would double their registers)
   }
   // The epilogue goes through LDS: column block b of every wave at a time, CHUNK columns of the tile as rows of PITCH words, i along the row.
   // (PITCH = BI + 1: neighbouring rows and neighbouring words both change the bank, so both orientations are read without conflicts.)
