@@ -169,7 +169,7 @@ __global__ __launch_bounds__(TL::THREADS) void k_int8_tile(Int8Args g, int ti, i
   const int i0 = bi * BI, j0 = bj * BJ;
   TL t;
   const int steps = (g.k + 127) / 128;
-  t.run(g.b, i0, g.a, j0, 0, steps, g.k - (steps - 1) * 128, lds);
+  t.run(g.b, i0, g.a, j0, steps, g.k - (steps - 1) * 128, lds);
   constexpr int ACROSS = BI / N, ROWS = TL::THREADS / ACROSS;
   T* y = (T*)g.y;
   const int iw = threadIdx.x % ACROSS * N, n = i0 + iw;

@@ -46,6 +46,23 @@ int ask_lds(nls_ctx* ctx, int bytes) {
 
 int type_size(int t) { return t == NLS_TYPE_F32 ? 4 : (t == NLS_TYPE_F16 || t == NLS_TYPE_BF16) ? 2 : 0; }
 
+// The tile a product is cut into.  Measured (int8 and fp16 products of 300 .. 8192 rows and columns, 10 .. 256 K steps):
+//   256 x 256 (8 waves, two steps held) reads the least and is first once its tiles keep more than half of the compute units busy: 4096^2 pairs 355 us
+//     against 387 with 128 x 128; int8 4096^3 73 / 84;
+//   128 x 128, four waves, two workgroups a unit, when there are more of them than units: 2048 x 8192 pairs 203 us against 218 with eight waves;
+//   128 x 128, eight waves, three steps held, when they cover 0.6 .. 1 of the units: 2048^2 pairs 59 us against 67 (four waves) and 70 (64 x 64);
+//   64 x 64, four waves side by side, three workgroups a unit: more of them than units, or few K steps: 1536^2 symmetric 26 us against 36 (128 x 128);
+//   64 x 64 with the K steps dealt out over the waves otherwise: 512 rows, K = 2048 pairs: 16 us against 23 (side by side) and 44 (128 x 128).
+enum TileKind { TILE_256, TILE_128, TILE_128_DEEP, TILE_64, TILE_64_RING };
+template <class F>
+TileKind tile_kind(const nls_ctx* ctx, F tiles, int steps) {
+  const long cus = ctx->cus;
+  if (20 * tiles(256) > 11 * cus) return TILE_256;
+  if (tiles(128) > cus) return TILE_128;
+  if (5 * tiles(128) >= 3 * cus) return TILE_128_DEEP;
+  return tiles(64) > cus || steps < 20 ? TILE_64 : TILE_64_RING;
+}
+
 // ---- quantise ----
 // Short rows: a wave each; others: a workgroup.  The number of pieces a thread holds follows from the length; rows past 8 pieces are read twice.
 template <class T, bool VEC>
@@ -94,10 +111,14 @@ int int8_tile(nls_ctx* ctx, const Int8Args& g, hipStream_t st) {
 }
 template <class T, int N>
 int int8_tile(nls_ctx* ctx, const Int8Args& g, hipStream_t st) {
-  auto tiles = [&](long i, long j) { return ((g.n + i - 1) / i) * ((g.m + j - 1) / j); };
-  if (tiles(256, 256) >= ctx->cus) return int8_tile<T, Tile<MODE_I8, 256, 256, 2, 4, 2>, 256, 256, N>(ctx, g, st);
-  if (tiles(128, 128) >= ctx->cus) return int8_tile<T, Tile<MODE_I8, 128, 128, 2, 2, 2>, 128, 128, N>(ctx, g, st);
-  return int8_tile<T, Ring<MODE_I8, 2>, 64, 64, N>(ctx, g, st);
+  auto tiles = [&](long b) { return ((g.n + b - 1) / b) * ((g.m + b - 1) / b); };
+  switch (tile_kind(ctx, tiles, (g.k + 127) / 128)) {
+    case TILE_256: return int8_tile<T, Tile<MODE_I8, 256, 256, 2, 4, 2>, 256, 256, N>(ctx, g, st);
+    case TILE_128: return int8_tile<T, Tile<MODE_I8, 128, 128, 2, 2, 2>, 128, 128, N>(ctx, g, st);
+    case TILE_128_DEEP: return int8_tile<T, Tile<MODE_I8, 128, 128, 4, 2, 3>, 128, 128, N>(ctx, g, st);
+    case TILE_64: return int8_tile<T, Tile<MODE_I8, 64, 64, 2, 2, 3>, 64, 64, N>(ctx, g, st);
+    default: return int8_tile<T, Ring<MODE_I8, 2>, 64, 64, N>(ctx, g, st);
+  }
 }
 template <class T, int MG, int NG, bool FUSED>
 int int8_few(nls_ctx* ctx, const Int8Args& g, const FewX& f, hipStream_t st) {
@@ -189,6 +210,9 @@ NsPath ns_path(long p, long q, long row_stride, long col_stride) {
   if (p > 128 || row_stride < 0 || col_stride < 0 || row_stride >= reach || col_stride >= reach || (p + 32) * row_stride + 16 * col_stride >= reach) return NS_TILES;
   return (q <= 256 || (p <= 64 && q <= 512) || (p <= 32 && q <= 1024)) ? NS_SMALL : NS_SLABS;
 }
+// Workgroups that sum squares: four rows (of the direction that is dense in memory) each
+int ns_parts(const NsMatrix& w) { return (int)std::min<long>(NS_PARTS, ((w.col_stride <= w.row_stride ? w.p : w.q) + 3) / 4); }
+
 struct NsPlan {
   NsPath path;
   long p, q;
@@ -244,9 +268,13 @@ int ns_product(nls_ctx* ctx, const NsArgs& g, long batch, hipStream_t st) {
     const long i = (g.I + b - 1) / b, j = (g.J + b - 1) / b;
     return (SYM ? i * (i + 1) / 2 : i * j) * batch;
   };
-  if (tiles(256) * 2 >= ctx->cus) return ns_product_tile<KIND, T, Tile<MODE, 256, 256, 2, 4, 2>, MODE, 256>(ctx, g, batch, st);
-  if (tiles(128) >= ctx->cus) return ns_product_tile<KIND, T, Tile<MODE, 128, 128, 2, 2, 2>, MODE, 128>(ctx, g, batch, st);
-  return ns_product_tile<KIND, T, Ring<MODE, 2>, MODE, 64>(ctx, g, batch, st);
+  switch (tile_kind(ctx, tiles, (g.K + (MODE == MODE_F16 ? 63 : 31)) / (MODE == MODE_F16 ? 64 : 32))) {
+    case TILE_256: return ns_product_tile<KIND, T, Tile<MODE, 256, 256, 2, 4, 2>, MODE, 256>(ctx, g, batch, st);
+    case TILE_128: return ns_product_tile<KIND, T, Tile<MODE, 128, 128, 2, 2, 2>, MODE, 128>(ctx, g, batch, st);
+    case TILE_128_DEEP: return ns_product_tile<KIND, T, Tile<MODE, 128, 128, 4, 2, 3>, MODE, 128>(ctx, g, batch, st);
+    case TILE_64: return ns_product_tile<KIND, T, Tile<MODE, 64, 64, 2, 2, 3>, MODE, 64>(ctx, g, batch, st);
+    default: return ns_product_tile<KIND, T, Ring<MODE, 2>, MODE, 64>(ctx, g, batch, st);
+  }
 }
 template <int KIND, class T>
 int ns_product(nls_ctx* ctx, const NsArgs& g, bool pairs, long batch, hipStream_t st) {
@@ -292,7 +320,7 @@ int ns_slabs(nls_ctx* ctx, const NsMatrix& w, bool tall, long batch, const NsCoe
   NLSCHK((ask_lds<&k_ns_slab<T, PB, false>>(ctx, lds)));
   NsSlabs g{};
   g.m = w;
-  g.count = (int)std::min<long>(NS_PARTS, (std::max(w.p, w.q) + 3) / 4);
+  g.count = ns_parts(w);
   g.eps = eps;
   g.steps = steps;
   g.out = out;
@@ -355,7 +383,7 @@ int orthogonalize(nls_ctx* ctx, const NsMatrix& w, const NsPlan& plan, bool tall
   NsScales* scales = (NsScales*)(ws + plan.parts);
   char* base = ws + plan.parts + plan.scales;
   char *X = base, *XT = X + plan.x, *XU = XT + plan.xt, *A = XU + plan.xt, *B = A + plan.a;
-  const int count = (int)std::min<long>(NS_PARTS, (std::max(w.p, w.q) + 3) / 4);
+  const int count = ns_parts(w);
   k_ns_norm<T><<<dim3(count, (unsigned)batch), 256, 0, st>>>(w, parts);
   k_ns_scales<<<dim3((unsigned)batch), 64, 0, st>>>(parts, count, eps, cf, steps, scales);
   k_ns_pack<T><<<dim3((unsigned)((w.q + 63) / 64), (unsigned)((w.p + 63) / 64), (unsigned)batch), 256, 0, st>>>(w, scales, X, XT, plan.batch_bytes);
@@ -383,6 +411,7 @@ int orthogonalize(nls_ctx* ctx, const NsMatrix& w, const NsPlan& plan, bool tall
     if (t + 1 < steps) {
       g.D = X;
       g.DT = XU;
+      g.next_pairs = t + 1 >= steps - exact;
       NLSCHK((ns_product<NS_STEP, float>(ctx, g, pairs, batch, st)));
       std::swap(XT, XU);
     } else {

@@ -14,7 +14,7 @@
 namespace lb {
 
 constexpr int NS_MAX_STEPS = 32;
-constexpr int NS_PARTS = 256;  // partial sums of squares a matrix
+constexpr int NS_PARTS = 1024;  // partial sums of squares a matrix, at most
 
 // Matrices are held times a power of two.  What a step's sums w are multiplied with to become the next held matrix:
 struct NsFactors {
@@ -42,9 +42,10 @@ struct NsCoef {
   unsigned ends;              // bit t: a chain of steps ends with step t
 };
 
-// A matrix of fp16 pairs: granules of 32 elements, 64 bytes hi then 64 bytes lo; rows padded with zeros to 64 elements.
+// A matrix of fp16 pairs: granules of 64 elements, 128 bytes hi then 128 bytes lo; rows padded with zeros to whole granules.
 __host__ __device__ inline size_t pair_ld(long k) { return (size_t)((k + 63) / 64 * 64) * 4; }
-__device__ __forceinline__ size_t pair_at(size_t row, size_t k, size_t ld) { return row * ld + (k >> 5) * 128 + (k & 31) * 2; }
+__device__ __forceinline__ size_t pair_at(size_t row, size_t k, size_t ld) { return row * ld + (k >> 6) * 256 + (k & 63) * 2; }
+constexpr int PAIR_LO = 128;  // bytes from a hi half to its lo half
 
 struct NsMatrix {
   const void* g;
@@ -52,24 +53,44 @@ struct NsMatrix {
   long row_stride, col_stride, batch_stride;  // in elements
 };
 
+// Sums of squares, a part a workgroup.  Sixteen bytes a thread and turn along the direction whose neighbours are neighbours in memory, where they are
+// aligned; bound by memory (4096 x 4096 float32 was 103 us with one element a thread and 256 workgroups).
 template <class T>
 __global__ __launch_bounds__(256) void k_ns_norm(NsMatrix w, double* parts) {
+  constexpr int N = 16 / (int)sizeof(T);
+  typedef T V __attribute__((ext_vector_type(N)));
   const T* g = (const T*)w.g + blockIdx.y * w.batch_stride;
-  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
-  double s = 0.0;
-  // lanes along the direction whose neighbours are neighbours in memory
+  double s[2] = {0.0, 0.0};
   const bool along_q = w.col_stride <= w.row_stride;
   const long outer = along_q ? w.p : w.q, inner = along_q ? w.q : w.p;
   const long os = along_q ? w.row_stride : w.col_stride, is = along_q ? w.col_stride : w.row_stride;
-  for (long o = (long)blockIdx.x * 4 + y; o < outer; o += (long)gridDim.x * 4)
-    for (long i = x; i < inner; i += 64) {
-      const double v = (double)to_f32(g[o * os + i * is]);
-      s += v * v;
-    }
+  const bool whole = is == 1 && (size_t)g % 16 == 0 && (outer == 1 || os % N == 0);
+  // 64 threads along a row, four rows at a time
+  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
+  for (long o = (long)blockIdx.x * 4 + y; o < outer; o += (long)gridDim.x * 4) {
+    const T* row = g + o * os;
+    long i = x * N;
+    if (whole)
+#pragma unroll 4
+      for (; i + N <= inner; i += 64 * N) {
+        const V v = *(const V*)(row + i);
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+        for (int e = 0; e < N; ++e) {
+          const double d = (double)to_f32(v[e]);
+          s[e & 1] += d * d;
+        }
+      }
+    for (; i < inner; i += 64 * N)
+      for (int e = 0; e < N && i + e < inner; ++e) {
+        const double d = (double)to_f32(row[(i + e) * is]);
+        s[e & 1] += d * d;
+      }
+  }
+  double sum = s[0] + s[1];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
   __shared__ double part[4];
-  if (x == 0) part[y] = s;
+  if (x == 0) part[y] = sum;
   __syncthreads();
   if (threadIdx.x == 0) parts[(size_t)blockIdx.y * NS_PARTS + blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
 }
@@ -236,8 +257,8 @@ __global__ __launch_bounds__(256) void k_ns_pack(NsMatrix w, const NsScales* sca
     split8(v + 8, &hi[1], &lo[1]);
     *(f16x8*)base = hi[0];
     *(f16x8*)(base + 16) = hi[1];
-    *(f16x8*)(base + 64) = lo[0];
-    *(f16x8*)(base + 80) = lo[1];
+    *(f16x8*)(base + PAIR_LO) = lo[0];
+    *(f16x8*)(base + PAIR_LO + 16) = lo[1];
   }
 }
 
@@ -255,13 +276,14 @@ struct NsArgs {
   int ti, tj, strip;
   int t;                  // step
   int transposed;         // LAST: out is stored q x p
+  int next_pairs;         // STEP: the next step's products are of pairs
 };
 
-__device__ __forceinline__ void store_pairs(char* at, const float (&v)[8]) {  // eight neighbours of a row of pairs
+__device__ __forceinline__ void store_pairs(char* at, const float (&v)[8], bool low) {  // eight neighbours of a row of pairs
   f16x8 h, o;
   split8(v, &h, &o);
   *(f16x8*)at = h;
-  *(f16x8*)(at + 64) = o;
+  if (low) *(f16x8*)(at + PAIR_LO) = o;
 }
 
 template <int KIND, class T, class TL, int MODE, int BI, int BJ>
@@ -283,7 +305,7 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
   const size_t ldk = pair_ld(g.K), ldi = pair_ld(g.I), ldj = pair_ld(g.J);
   TL t;
   const int per = MODE == MODE_F16 ? 64 : 32;
-  t.run(Operand{g.P + off, (unsigned)ldk, g.I}, i0, Operand{g.Q + off, (unsigned)ldk, g.J}, j0, 0, (g.K + per - 1) / per, 128, lds);
+  t.run(Operand{g.P + off, (unsigned)ldk, g.I}, i0, Operand{g.Q + off, (unsigned)ldk, g.J}, j0, (g.K + per - 1) / per, 128, lds);
   const NsScales& z = g.scales[blockIdx.z];
   const NsFactors f = z.f[g.t];
   const int last = z.last;
@@ -291,6 +313,8 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
   char* D = g.D + off;
   char* DT = SYM ? D : g.DT + off;
   T* out = (T*)g.out + blockIdx.z * g.out_stride;
+  // Lo halves nobody reads are not written: of A and B where the step's products are single ones, of the transpose of X where the next step's are.
+  const bool low_e = KIND != NS_POLY || MODE == MODE_F16PAIR, low_d = !SYM || MODE == MODE_F16PAIR, low_t = SYM ? low_d : g.next_pairs != 0;
   const bool natural = KIND != NS_LAST || !g.transposed, turned = KIND == NS_LAST ? g.transposed != 0 : SYM ? bi != bj : true;
   // Chunks of the tile through LDS: the result in the product's own orientation (rows j, eight neighbours i a thread), then, from the values left
   // there, its transpose (rows i, eight neighbours j).
@@ -312,7 +336,7 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
       if (KIND != NS_GRAM && there) {
         const char* at = E + pair_at(j, i, ldi);
         eh = *(const f16x8*)at;
-        el = *(const f16x8*)(at + 64);
+        if (low_e) el = *(const f16x8*)(at + PAIR_LO);
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -328,7 +352,7 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) ((float*)lds)[r * TL::PITCH + iw + e] = v[e];
       if (KIND != NS_LAST) {
-        if (there) store_pairs(D + pair_at(j, i, ldi), v);
+        if (there) store_pairs(D + pair_at(j, i, ldi), v, low_d);
       } else if (natural && j < g.J && i < g.I) {
         store8(out + (size_t)j * g.I + i, v, g.I - i, i + 8 <= g.I && g.I % (16 / (int)sizeof(T)) == 0);
       }
@@ -342,7 +366,7 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = ((const float*)lds)[(rv + e) * TL::PITCH + ii];
         if (KIND != NS_LAST) {
-          if ((size_t)j * 4 < ldj) store_pairs(DT + pair_at(irow, j, ldj), v);
+          if ((size_t)j * 4 < ldj) store_pairs(DT + pair_at(irow, j, ldj), v, low_t);
         } else if (j < g.J) {
           store8(out + (size_t)irow * g.J + j, v, g.J - j, j + 8 <= g.J && g.J % (16 / (int)sizeof(T)) == 0);
         }

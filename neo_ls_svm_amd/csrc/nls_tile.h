@@ -1,8 +1,9 @@
 // Matrix-core tile engine of the few-bit operators (nls_lowbit.hip): D[i][j] = sum_k P[i][k] Q[j][k], both operands row-major with k running
 // along the row, in 8-bit integers, in fp16, or in fp16 pairs (hi + lo).
 //
-// One K step is 128 bytes of every operand row, whatever the type: 128 int8, 64 fp16, or 32 fp16 pairs (a row holds granules of 64 bytes hi and
-// 64 bytes lo per 32 elements).  The rows travel from memory to LDS without touching registers (16 bytes a lane, a wave moves 8 whole rows =
+// One K step is 128 bytes of every operand row, whatever the type: 128 int8, 64 fp16, or 32 fp16 pairs.  A row of pairs holds 128 bytes hi and 128 bytes
+// lo for every 64 elements, so that a step of the hi halves alone is a whole line (granules of 64 + 64 bytes cost single steps a third: half of each
+// line fetched was not read); a step of pairs takes half of two lines, the next step the other halves.  The rows travel from memory to LDS without touching registers (16 bytes a lane, a wave moves 8 whole rows =
 // eight full 128-byte lines), into the next of STAGES buffers while the matrix cores work on this one: the fewer workgroups share a compute unit, the more steps have to be
 // under way to cover the way to memory.
 //
@@ -36,15 +37,15 @@ struct AccOf<MODE_I8> {
   using type = i32x16;
 };
 
-// Bytes an operand row advances per K step.
+// Where K step t of an operand row begins.
 template <int MODE>
-constexpr int kstep_bytes() {
-  return MODE == MODE_F16 ? 256 : 128;
+__device__ __forceinline__ size_t step_at(int t) {
+  return MODE == MODE_I8 ? (size_t)t * 128 : MODE == MODE_F16 ? (size_t)t * 256 : (size_t)(t >> 1) * 256 + (t & 1) * 64;
 }
-// Byte offset, within a K step, of 16-byte chunk c: fp16 alone reads the hi half of two granules.
+// Byte offset, within a K step, of 16-byte chunk c.
 template <int MODE>
 __device__ __forceinline__ unsigned chunk_offset(int c) {
-  return MODE == MODE_F16 ? (unsigned)((c >> 2) * 128 + (c & 3) * 16) : (unsigned)(c * 16);
+  return MODE == MODE_F16PAIR ? (unsigned)((c >> 2) * 128 + (c & 3) * 16) : (unsigned)(c * 16);
 }
 
 __device__ __forceinline__ i32x4 keep_bytes(i32x4 v, int n) {  // the first n of 16 bytes, the others zero
@@ -168,28 +169,22 @@ struct Tile {
   __device__ __forceinline__ static void arrive() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
   }
-  // steps >= 1 whole or ragged K steps from byte kb of the rows on; last_valid: valid bytes of the last one (128: whole).
+  // steps >= 1 K steps; last_valid: valid bytes of the last one (128: whole).
   // STAGES - 1 steps are under way at any time; one barrier a step: behind it step t is there and the buffer of step t - 1 is free.
-  __device__ __forceinline__ void run(const Operand& P, int i0, const Operand& Q, int j0, size_t kb, int steps, int last_valid, char* lds) {
+  __device__ __forceinline__ void run(const Operand& P, int i0, const Operand& Q, int j0, int steps, int last_valid, char* lds) {
     start(P, i0, Q, j0);
-    const char* p = P.base + (size_t)i0 * P.ld + kb;
-    const char* q = Q.base + (size_t)j0 * Q.ld + kb;
-    constexpr int STEP = kstep_bytes<MODE>();
+    const char* p = P.base + (size_t)i0 * P.ld;
+    const char* q = Q.base + (size_t)j0 * Q.ld;
     const int first = min(STAGES - 1, steps);
-    for (int t = 0; t < first; ++t) fetch(p + t * STEP, q + t * STEP, lds + t * BUF, t + 1 == steps ? last_valid : 128);
-    p += (STAGES - 1) * STEP;
-    q += (STAGES - 1) * STEP;
+    for (int t = 0; t < first; ++t) fetch(p + step_at<MODE>(t), q + step_at<MODE>(t), lds + t * BUF, t + 1 == steps ? last_valid : 128);
     int now = 0, next = (STAGES - 1) * BUF;
     for (int t = 0; t < steps - 1; ++t) {
       if (t + STAGES - 1 <= steps)
         arrive<FLIGHT>();
       else
         arrive<0>();
-      if (t + STAGES - 1 < steps) {
-        fetch(p, q, lds + next, t + STAGES == steps ? last_valid : 128);
-        p += STEP;
-        q += STEP;
-      }
+      const int ahead = t + STAGES - 1;
+      if (ahead < steps) fetch(p + step_at<MODE>(ahead), q + step_at<MODE>(ahead), lds + next, ahead + 1 == steps ? last_valid : 128);
       multiply<false>(lds + now, 128);
       now = now + BUF == LDS ? 0 : now + BUF;
       next = next + BUF == LDS ? 0 : next + BUF;
@@ -238,7 +233,7 @@ struct Ring {
 #pragma unroll
     for (int s = 0; s < f.SUB; ++s) f.template read<TAIL>(s, buf + (lane_id() & 31) * 128, buf + 8192 + (lane_id() & 31) * 128, valid);
   }
-  __device__ __forceinline__ void run(const Operand& P, int i0, const Operand& Q, int j0, size_t kb, int steps, int last_valid, char* lds) {
+  __device__ __forceinline__ void run(const Operand& P, int i0, const Operand& Q, int j0, int steps, int last_valid, char* lds) {
     const int w = wave_id(), r = lane_id() >> 3;
     const unsigned c = chunk_offset<MODE>(move_chunk());
 #pragma unroll
@@ -250,15 +245,12 @@ struct Ring {
     for (int a = 0; a < 2; ++a)
 #pragma unroll
       for (int b = 0; b < 2; ++b) acc[a][b] = Acc{};
-    constexpr int STEP = kstep_bytes<MODE>();
-    const char* p = P.base + (size_t)i0 * P.ld + kb + w * STEP;
-    const char* q = Q.base + (size_t)j0 * Q.ld + kb + w * STEP;
+    const char* p = P.base + (size_t)i0 * P.ld;
+    const char* q = Q.base + (size_t)j0 * Q.ld;
     lds += w * STAGES * BUF;
     const int mine = (steps - w + 3) / 4;  // steps w, w + 4, ..
     auto valid_of = [&](int t) { return 4 * t + w + 1 == steps ? last_valid : 128; };
-    for (int t = 0; t < min(STAGES, mine); ++t) fetch(p + (size_t)t * 4 * STEP, q + (size_t)t * 4 * STEP, lds + t * BUF, valid_of(t));
-    p += (size_t)STAGES * 4 * STEP;
-    q += (size_t)STAGES * 4 * STEP;
+    for (int t = 0; t < min(STAGES, mine); ++t) fetch(p + step_at<MODE>(4 * t + w), q + step_at<MODE>(4 * t + w), lds + t * BUF, valid_of(t));
     int now = 0;
     for (int t = 0; t < mine; ++t) {
       if (t + STAGES <= mine)
@@ -271,11 +263,8 @@ struct Ring {
       else
         read<false>(f, lds + now, 128);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the step is in registers, its buffer free
-      if (t + STAGES < mine) {
-        fetch(p, q, lds + now, valid_of(t + STAGES));
-        p += 4 * STEP;
-        q += 4 * STEP;
-      }
+      const int ahead = t + STAGES;
+      if (ahead < mine) fetch(p + step_at<MODE>(4 * ahead + w), q + step_at<MODE>(4 * ahead + w), lds + now, valid_of(ahead));
 #pragma unroll
       for (int s = 0; s < f.SUB; ++s) f.multiply(s, acc);
       now = now + BUF == STAGES * BUF ? 0 : now + BUF;
