@@ -42,10 +42,13 @@ struct NsCoef {
   unsigned ends;              // bit t: a chain of steps ends with step t
 };
 
-// A matrix of fp16 pairs: granules of 64 elements, 128 bytes hi then 128 bytes lo; rows padded with zeros to whole granules.
+// A matrix of fp16 pairs: rows padded with zeros to 64 elements, 4 bytes an element; hi and lo halves lie in blocks of 32 or 64 elements by the kind of
+// product that reads them (nls_tile.h).
 __host__ __device__ inline size_t pair_ld(long k) { return (size_t)((k + 63) / 64 * 64) * 4; }
-__device__ __forceinline__ size_t pair_at(size_t row, size_t k, size_t ld) { return row * ld + (k >> 6) * 256 + (k & 63) * 2; }
-constexpr int PAIR_LO = 128;  // bytes from a hi half to its lo half
+__device__ __forceinline__ size_t pair_at(size_t row, size_t k, size_t ld, bool for_pairs) {
+  return row * ld + (k >> 6) * 256 + (for_pairs ? (k >> 5 & 1) * 128 + (k & 31) * 2 : (k & 63) * 2);
+}
+__device__ __forceinline__ int pair_lo(bool for_pairs) { return for_pairs ? 64 : 128; }  // bytes from a hi half to its lo half
 
 struct NsMatrix {
   const void* g;
@@ -227,7 +230,7 @@ __device__ __forceinline__ void split8(const float* v, f16x8* hi, f16x8* lo) {
 
 // G -> X_0 (p rows) and its transpose (q rows), zero-padded.  One 64 x 64 tile a workgroup.
 template <class T>
-__global__ __launch_bounds__(256) void k_ns_pack(NsMatrix w, const NsScales* scales, char* x, char* xt, size_t batch_bytes) {
+__global__ __launch_bounds__(256) void k_ns_pack(NsMatrix w, const NsScales* scales, char* x, char* xt, size_t batch_bytes, int for_pairs) {
   __shared__ float tile[64][65];
   const T* g = (const T*)w.g + blockIdx.z * w.batch_stride;
   x += blockIdx.z * batch_bytes;
@@ -247,7 +250,7 @@ __global__ __launch_bounds__(256) void k_ns_pack(NsMatrix w, const NsScales* sca
   const size_t ldx = pair_ld(w.q), ldt = pair_ld(w.p);
   const int row = threadIdx.x >> 2, part = (threadIdx.x & 3) * 16;
   for (int turn = 0; turn < 2; ++turn) {
-    char* base = turn ? xt + pair_at(q0 + row, p0 + part, ldt) : x + pair_at(p0 + row, q0 + part, ldx);
+    char* base = turn ? xt + pair_at(q0 + row, p0 + part, ldt, for_pairs) : x + pair_at(p0 + row, q0 + part, ldx, for_pairs);
     if (turn ? q0 + row >= w.q : p0 + row >= w.p) continue;
     f16x8 hi[2], lo[2];
     float v[16];
@@ -257,8 +260,8 @@ __global__ __launch_bounds__(256) void k_ns_pack(NsMatrix w, const NsScales* sca
     split8(v + 8, &hi[1], &lo[1]);
     *(f16x8*)base = hi[0];
     *(f16x8*)(base + 16) = hi[1];
-    *(f16x8*)(base + PAIR_LO) = lo[0];
-    *(f16x8*)(base + PAIR_LO + 16) = lo[1];
+    *(f16x8*)(base + pair_lo(for_pairs)) = lo[0];
+    *(f16x8*)(base + pair_lo(for_pairs) + 16) = lo[1];
   }
 }
 
@@ -279,11 +282,11 @@ struct NsArgs {
   int next_pairs;         // STEP: the next step's products are of pairs
 };
 
-__device__ __forceinline__ void store_pairs(char* at, const float (&v)[8], bool low) {  // eight neighbours of a row of pairs
+__device__ __forceinline__ void store_pairs(char* at, const float (&v)[8], int lo) {  // eight neighbours of a row of pairs; lo: where their lo halves go, 0: nowhere
   f16x8 h, o;
   split8(v, &h, &o);
   *(f16x8*)at = h;
-  if (low) *(f16x8*)(at + PAIR_LO) = o;
+  if (lo) *(f16x8*)(at + lo) = o;
 }
 
 template <int KIND, class T, class TL, int MODE, int BI, int BJ>
@@ -314,8 +317,13 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
   char* DT = SYM ? D : g.DT + off;
   T* out = (T*)g.out + blockIdx.z * g.out_stride;
   // Lo halves nobody reads are not written: of A and B where the step's products are single ones, of the transpose of X where the next step's are.
-  const bool low_e = KIND != NS_POLY || MODE == MODE_F16PAIR, low_d = !SYM || MODE == MODE_F16PAIR, low_t = SYM ? low_d : g.next_pairs != 0;
+  constexpr bool PAIRS = MODE == MODE_F16PAIR;
+  const bool to_pairs = SYM ? PAIRS : g.next_pairs != 0;  // the products that will read D and DT
+  const bool low_e = KIND != NS_POLY || PAIRS;
+  const int lo_d = !SYM || PAIRS ? pair_lo(to_pairs) : 0, lo_t = to_pairs ? pair_lo(true) : 0;
   const bool natural = KIND != NS_LAST || !g.transposed, turned = KIND == NS_LAST ? g.transposed != 0 : SYM ? bi != bj : true;
+  // (STEP writes X where it reads it, perhaps in the other layout: the 64 elements that share 256 bytes are eight neighbouring lanes' of one wave,
+  // which have read them all before the first is written.)
   // Chunks of the tile through LDS: the result in the product's own orientation (rows j, eight neighbours i a thread), then, from the values left
   // there, its transpose (rows i, eight neighbours j).
   constexpr int ACROSS = BI / 8, ROWS = TL::THREADS / ACROSS;
@@ -334,9 +342,9 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
       f16x8 eh = {}, el = {};
       const bool there = j < g.J && (size_t)i * 4 < ldi;  // (rows are padded: whole groups of eight, zeros behind the end)
       if (KIND != NS_GRAM && there) {
-        const char* at = E + pair_at(j, i, ldi);
+        const char* at = E + pair_at(j, i, ldi, PAIRS);
         eh = *(const f16x8*)at;
-        if (low_e) el = *(const f16x8*)(at + PAIR_LO);
+        if (low_e) el = *(const f16x8*)(at + pair_lo(PAIRS));
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -352,7 +360,7 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) ((float*)lds)[r * TL::PITCH + iw + e] = v[e];
       if (KIND != NS_LAST) {
-        if (there) store_pairs(D + pair_at(j, i, ldi), v, low_d);
+        if (there) store_pairs(D + pair_at(j, i, ldi, to_pairs), v, lo_d);
       } else if (natural && j < g.J && i < g.I) {
         store8(out + (size_t)j * g.I + i, v, g.I - i, i + 8 <= g.I && g.I % (16 / (int)sizeof(T)) == 0);
       }
@@ -366,7 +374,7 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = ((const float*)lds)[(rv + e) * TL::PITCH + ii];
         if (KIND != NS_LAST) {
-          if ((size_t)j * 4 < ldj) store_pairs(DT + pair_at(irow, j, ldj), v, low_t);
+          if ((size_t)j * 4 < ldj) store_pairs(DT + pair_at(irow, j, ldj, to_pairs), v, lo_t);
         } else if (j < g.J) {
           store8(out + (size_t)irow * g.J + j, v, g.J - j, j + 8 <= g.J && g.J % (16 / (int)sizeof(T)) == 0);
         }

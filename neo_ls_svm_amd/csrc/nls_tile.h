@@ -1,11 +1,12 @@
 // Matrix-core tile engine of the few-bit operators (nls_lowbit.hip): D[i][j] = sum_k P[i][k] Q[j][k], both operands row-major with k running
 // along the row, in 8-bit integers, in fp16, or in fp16 pairs (hi + lo).
 //
-// One K step is 128 bytes of every operand row, whatever the type: 128 int8, 64 fp16, or 32 fp16 pairs.  A row of pairs holds 128 bytes hi and 128 bytes
-// lo for every 64 elements, so that a step of the hi halves alone is a whole line (granules of 64 + 64 bytes cost single steps a third: half of each
-// line fetched was not read); a step of pairs takes half of two lines, the next step the other halves.  The rows travel from memory to LDS without touching registers (16 bytes a lane, a wave moves 8 whole rows =
-// eight full 128-byte lines), into the next of STAGES buffers while the matrix cores work on this one: the fewer workgroups share a compute unit, the more steps have to be
-// under way to cover the way to memory.
+// One K step is 128 bytes of every operand row, one whole line, whatever the type: 128 int8, 64 fp16 (hi halves alone), or 32 fp16 pairs.  Rows of pairs
+// are laid out for the products that read them: 64 bytes hi and 64 bytes lo for every 32 elements where those are of pairs, 128 and 128 bytes for every 64
+// where they are single.  (Each read from the other's layout costs a tenth to a third: half of every line fetched lies idle.)
+// The rows travel from memory to LDS without touching registers (16 bytes a lane, a wave moves 8 whole rows = eight full lines), into the next of STAGES
+// buffers while the matrix cores work on this one: the fewer workgroups share a compute unit, the more steps have to be under way to cover the way
+// to memory.
 //
 // LDS holds a tile row at r * 128, its 16-byte chunk c at slot c ^ (r & 7): a fragment read takes the same chunk of 32 rows, so any 8 neighbouring
 // lanes touch 8 different slots - every bank once.  The writing side needs no scatter: the lane that fills slot s simply fetches chunk s ^ (r & 7).
@@ -40,12 +41,7 @@ struct AccOf<MODE_I8> {
 // Where K step t of an operand row begins.
 template <int MODE>
 __device__ __forceinline__ size_t step_at(int t) {
-  return MODE == MODE_I8 ? (size_t)t * 128 : MODE == MODE_F16 ? (size_t)t * 256 : (size_t)(t >> 1) * 256 + (t & 1) * 64;
-}
-// Byte offset, within a K step, of 16-byte chunk c.
-template <int MODE>
-__device__ __forceinline__ unsigned chunk_offset(int c) {
-  return MODE == MODE_F16PAIR ? (unsigned)((c >> 2) * 128 + (c & 3) * 16) : (unsigned)(c * 16);
+  return (size_t)t * (MODE == MODE_F16 ? 256 : 128);
 }
 
 __device__ __forceinline__ i32x4 keep_bytes(i32x4 v, int n) {  // the first n of 16 bytes, the others zero
@@ -133,7 +129,7 @@ struct Tile {
 
   __device__ __forceinline__ void start(const Operand& P, int i0, const Operand& Q, int j0) {
     const int r = wave_id() * 8 + (lane_id() >> 3);
-    const unsigned c = chunk_offset<MODE>(move_chunk());
+    const unsigned c = move_chunk() * 16;
 #pragma unroll
     for (int l = 0; l < LOADS_P; ++l) offp[l] = (unsigned)min(l * 8 * WAVES + r, P.rows - 1 - i0) * P.ld + c;
 #pragma unroll
@@ -235,7 +231,7 @@ struct Ring {
   }
   __device__ __forceinline__ void run(const Operand& P, int i0, const Operand& Q, int j0, int steps, int last_valid, char* lds) {
     const int w = wave_id(), r = lane_id() >> 3;
-    const unsigned c = chunk_offset<MODE>(move_chunk());
+    const unsigned c = move_chunk() * 16;
 #pragma unroll
     for (int l = 0; l < 8; ++l) {
       offp[l] = (unsigned)min(l * 8 + r, P.rows - 1 - i0) * P.ld + c;
