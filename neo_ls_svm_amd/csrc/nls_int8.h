@@ -6,18 +6,10 @@ namespace lb {
 
 // ---- quantise rows --------------------------------------------------------------------------------------------------------------------------
 // scale = max|x| / 127, q = 127 x / max|x| to the nearest integer, ties to even, decided as if in exact arithmetic:
-// r = x * inv with inv = fl(127 / max|x|) is off by less than 127 * 2^-23 + (its own rounding) < 2^-15.9; only where r lies that near to a half is
-// the quotient formed in 64 bits - 127 x is exact there and a quotient of a 31-bit by a 24-bit number that is no half is at least 2^-26 away from one.
+// r = x * inv with inv = fl(127 / max|x|) is off by less than 127 * 2^-23 = 1.5e-5; only where a piece of the row has an r that near to a half is the
+// quotient formed in 64 bits - 127 x is exact there, and a quotient of a 31-bit by a 24-bit number that is no half is at least 2^-26 away from one.
+// Adding 1.5 * 2^23 rounds r and leaves the integer in the sum's low byte.
 // A row with a NaN or an infinity gets that as its scale and zeros as q (the product then gives NaN in the whole row); a row of zeros, scale 0.
-__device__ __forceinline__ int quantise_exact(float x, float top) {
-  return (int)__builtin_rint((double)x * 127.0 / (double)top);
-}
-__device__ __forceinline__ int quantise_one(float x, float top, float inv) {
-  const float r = x * inv;
-  const float n = __builtin_rintf(r);
-  if (__builtin_expect(fabsf(fabsf(r - n) - 0.5f) < 2.0e-5f, 0)) return quantise_exact(x, top);
-  return (int)n;
-}
 struct RowScale {
   float top, inv;
   int kind;  // 0: the usual row; 1: all through 64 bits (127 / top is out of range); 2: zeros
@@ -29,31 +21,81 @@ __device__ __forceinline__ RowScale row_scale(unsigned topbits) {
   s.inv = s.kind == 0 ? 127.0f / s.top : 0.0f;
   return s;
 }
-__device__ __forceinline__ int quantise(float x, const RowScale& s) {
-  return s.kind == 0 ? quantise_one(x, s.top, s.inv) : s.kind == 1 ? quantise_exact(x, s.top) : 0;
+__device__ __forceinline__ unsigned low_bytes(unsigned a, unsigned b, unsigned c, unsigned d) {
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0400u), __builtin_amdgcn_perm(b, a, 0x0c0c0400u), 0x05040100u);
 }
-__device__ __forceinline__ unsigned magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }  // orders |x|, infinity, NaN
-__device__ __forceinline__ unsigned pack4(int a, int b, int c, int d) {
-  return (unsigned)(a & 255) | (unsigned)(b & 255) << 8 | (unsigned)(c & 255) << 16 | (unsigned)d << 24;
-}
-__device__ __forceinline__ unsigned wave_max(unsigned v) {
+__device__ __forceinline__ unsigned exact4(const float* x, float top) {
+  unsigned q[4];
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, o));
-  return v;
+  for (int e = 0; e < 4; ++e) q[e] = (unsigned)(int)__builtin_rint((double)x[e] * 127.0 / (double)top);
+  return low_bytes(q[0], q[1], q[2], q[3]);
+}
+// N (a multiple of four) elements to their bytes
+template <int N>
+__device__ __forceinline__ void quantise(const float (&x)[N], const RowScale& s, unsigned (&q)[N / 4]) {
+  constexpr float ROUND = 12582912.0f;
+  float far = 0.0f;
+  unsigned bits[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const float r = x[e] * s.inv, n = r + ROUND;
+    bits[e] = __float_as_uint(n);
+    far = fmaxf(far, fabsf(r - (n - ROUND)));
+  }
+#pragma unroll
+  for (int e = 0; e < N; e += 4) q[e / 4] = low_bytes(bits[e], bits[e + 1], bits[e + 2], bits[e + 3]);
+  if (__builtin_expect(far > 0.49998f || s.kind != 0, 0)) {
+#pragma unroll
+    for (int e = 0; e < N; e += 4) q[e / 4] = s.kind == 2 ? 0u : exact4(x + e, s.top);
+  }
+}
+// The largest magnitude of a piece, as bits that order |x|, infinity, NaN: of the type itself for 16 bits (two at a time), float32's else
+template <class T, int N>
+__device__ __forceinline__ unsigned most_bits(const T __attribute__((ext_vector_type(N))) v, unsigned top) {
+  if constexpr (sizeof(T) == 2) {
+    typedef unsigned short U2 __attribute__((ext_vector_type(2)));
+    typedef unsigned W __attribute__((ext_vector_type(N / 2)));
+    const W w = __builtin_bit_cast(W, v) & 0x7fff7fffu;
+    U2 t = __builtin_bit_cast(U2, top);
+#pragma unroll
+    for (int e = 0; e < N / 2; ++e) t = __builtin_elementwise_max(t, __builtin_bit_cast(U2, (unsigned)w[e]));
+    return __builtin_bit_cast(unsigned, t);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+    return top;
+  }
+}
+// .. of all the pieces a wave has seen, as float32's bits
+template <class T>
+__device__ __forceinline__ unsigned wave_most(unsigned top) {
+  if constexpr (sizeof(T) == 2) top = max(top & 0xffffu, top >> 16);
+  unsigned o;
+#define NLS_MOST(ctrl) o = (unsigned)__builtin_amdgcn_mov_dpp((int)top, ctrl, 0xf, 0xf, true), top = max(top, o)
+  NLS_MOST(0xb1);   // lanes 1 0 3 2
+  NLS_MOST(0x4e);   // lanes 2 3 0 1
+  NLS_MOST(0x141);  // half rows mirrored
+  NLS_MOST(0x140);  // rows mirrored
+#undef NLS_MOST
+  top = max(max((unsigned)__builtin_amdgcn_readlane((int)top, 0), (unsigned)__builtin_amdgcn_readlane((int)top, 16)),
+            max((unsigned)__builtin_amdgcn_readlane((int)top, 32), (unsigned)__builtin_amdgcn_readlane((int)top, 48)));
+  if constexpr (sizeof(T) == 2) top = __float_as_uint(to_f32(__builtin_bit_cast(T, (unsigned short)top)));
+  return top;
 }
 
-// Elements a thread takes at once: 16 bytes where the rows are dense and their starts aligned to that, else four elements one by one.
+// Elements a thread takes at once: 16 bytes where the rows are dense (such a load may begin at any element), else four elements one by one.
 template <class T, bool VEC>
 struct Few {
   static constexpr int N = VEC ? 16 / (int)sizeof(T) : 4;
   typedef T type __attribute__((ext_vector_type(N)));
+  typedef T loose __attribute__((ext_vector_type(N), aligned(sizeof(T))));
 };
 template <class T, bool VEC>
 __device__ __forceinline__ typename Few<T, VEC>::type few_at(const T* x, long c, long k, long col_stride) {
   constexpr int N = Few<T, VEC>::N;
   typename Few<T, VEC>::type v = {};
   if (VEC && c + N <= k) {
-    v = *(const typename Few<T, VEC>::type*)(x + c);
+    v = *(const typename Few<T, VEC>::loose*)(x + c);
   } else {
 #pragma unroll
     for (int e = 0; e < N; ++e)
@@ -63,13 +105,15 @@ __device__ __forceinline__ typename Few<T, VEC>::type few_at(const T* x, long c,
 }
 template <int N, class V>
 __device__ __forceinline__ void quantise_store(const V& v, const RowScale& s, signed char* at) {
-  unsigned w[N / 4];
+  float x[N];
+  unsigned q[N / 4];
 #pragma unroll
-  for (int e = 0; e < N; e += 4) w[e / 4] = pack4(quantise(to_f32(v[e]), s), quantise(to_f32(v[e + 1]), s), quantise(to_f32(v[e + 2]), s), quantise(to_f32(v[e + 3]), s));
+  for (int e = 0; e < N; ++e) x[e] = to_f32(v[e]);
+  quantise<N>(x, s, q);
   if constexpr (N == 8)
-    *(i32x2*)at = i32x2{(int)w[0], (int)w[1]};
+    *(i32x2*)at = i32x2{(int)q[0], (int)q[1]};
   else
-    *(unsigned*)at = w[0];
+    *(unsigned*)at = q[0];
 }
 
 // A group of G threads takes a row.  HELD > 0: the row fits into HELD pieces a thread, is read once and stays in registers between the maximum and
@@ -89,17 +133,11 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const T* x, long rows, lo
 #pragma unroll
     for (int h = 0; h < HELD; ++h) held[h] = few_at<T, VEC>(xr, (long)N * (g + G * h), k, col_stride);
 #pragma unroll
-    for (int h = 0; h < HELD; ++h)
-#pragma unroll
-      for (int e = 0; e < N; ++e) top = max(top, magnitude(to_f32(held[h][e])));
+    for (int h = 0; h < HELD; ++h) top = most_bits<T, N>(held[h], top);
   } else {
-    for (long c = N * g; c < k; c += N * G) {
-      const typename F::type v = few_at<T, VEC>(xr, c, k, col_stride);
-#pragma unroll
-      for (int e = 0; e < N; ++e) top = max(top, magnitude(to_f32(v[e])));
-    }
+    for (long c = N * g; c < k; c += N * G) top = most_bits<T, N>(few_at<T, VEC>(xr, c, k, col_stride), top);
   }
-  top = wave_max(top);
+  top = wave_most<T>(top);
   if (G > 64) {
     __shared__ unsigned part[4];
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
@@ -122,6 +160,16 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const T* x, long rows, lo
   }
 }
 
+// n (up to 16) bytes from anywhere, the others zero
+typedef int i32x4_loose __attribute__((ext_vector_type(4), aligned(1)));
+__device__ __forceinline__ i32x4 loose_bytes(const signed char* p, int n) {
+  if (n >= 16) return *(const i32x4_loose*)p;
+  i32x4 v = {};
+#pragma unroll
+  for (int e = 0; e < 15; ++e)
+    if (e < n) v[e >> 2] |= (int)((unsigned)(unsigned char)p[e] << (8 * (e & 3)));
+  return v;
+}
 // Rows of 8-bit numbers that do not start at multiples of 16 bytes, laid out again so that they do (padding: zeros): one or two matrices a launch.
 struct AlignRows {
   const signed char* x;
@@ -130,12 +178,10 @@ struct AlignRows {
 };
 __global__ __launch_bounds__(256) void k_align_rows(AlignRows a, AlignRows b, long k, long ldy) {
   const AlignRows g = blockIdx.y ? b : a;
-  const long per = ldy / 4;
+  const long per = ldy / 16;
   for (long t = (long)blockIdx.x * 256 + threadIdx.x; t < g.rows * per; t += (long)gridDim.x * 256) {
-    const long r = t / per, c = (t - r * per) * 4;
-    int v[4];
-    for (int e = 0; e < 4; ++e) v[e] = c + e < k ? g.x[r * g.ld + c + e] : 0;
-    *(unsigned*)(g.y + r * ldy + c) = pack4(v[0], v[1], v[2], v[3]);
+    const long r = t / per, c = (t - r * per) * 16;
+    *(i32x4*)(g.y + r * ldy + c) = loose_bytes(g.x + r * g.ld + c, (int)min(k - c, 16l));
   }
 }
 
@@ -203,61 +249,64 @@ __global__ __launch_bounds__(TL::THREADS) void k_int8_tile(Int8Args g, int ti, i
 // Up to 64 rows of a against all of b: bound by reading b once.  A workgroup takes 16 NG rows of b; its eight waves deal the K range out among
 // themselves in pairs of 64 bytes (a wave reads 128 bytes of 16 rows: whole lines) straight into the fragments of the 16 x 16 x 64 instruction,
 // U loads under way before the first is used, and add their sums up in LDS - integers, so the order does not matter.  No second launch, no scratch memory.
-// a comes from L2 for every workgroup: MG fragments for NG of b.
+// a comes from L2 for every workgroup: MG fragments for NG of b.  Rows of a and b may start anywhere (a load may); a last chunk is read byte by byte where
+// the bytes behind it may not be there.
 // FUSED: a is not there yet - the workgroup quantises the rows of x into LDS itself while the first reads of b are under way (rows, k as the caller
 // allows them: see the host code).
 constexpr int FEW_U = 8;
 
-struct FewX {  // FUSED: the rows to quantise
-  const void* x;
+struct FewX {
+  const void* x;  // FUSED: the rows to quantise
   long row_stride, col_stride;
   int vec;
+  int a_padded, b_padded;  // a row's last chunk may be read whole
 };
 
+constexpr int FEW_ROWS = 4;  // FUSED: at most
+
+// All 512 threads share a row: the piece of eight elements number threadIdx.x, + 512, ..; the rows' reads are under way together, and the first piece
+// stays in registers between the maximum and the rounding.
 template <class TX>
 __device__ __forceinline__ void few_quantise(const Int8Args& g, const FewX& f, signed char* rows, long ld, float* scales, unsigned* parts) {
-  // all 512 threads share a row: piece of eight elements number threadIdx.x, + 512, ...
-  const int w = threadIdx.x >> 6;
-  for (int m = 0; m < g.m; ++m) {
+  typedef TX V __attribute__((ext_vector_type(8)));
+  typedef TX Loose __attribute__((ext_vector_type(8), aligned(sizeof(TX))));
+  const int w = threadIdx.x >> 6, c0 = 8 * threadIdx.x;
+  auto piece = [&](int m, int c) {
     const TX* x = (const TX*)f.x + m * f.row_stride;
-    unsigned top = 0;
-    for (int c = 8 * threadIdx.x; c < g.k; c += 8 * 512) {
-      typedef TX V __attribute__((ext_vector_type(8)));
-      V v = {};
-      if (f.vec && c + 8 <= g.k) {
-        v = *(const V*)(x + c);
-      } else {
+    V v = {};
+    if (f.vec && c + 8 <= g.k) {
+      v = *(const Loose*)(x + c);
+    } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (c + e < g.k) v[e] = x[(c + e) * f.col_stride];
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) top = max(top, magnitude(to_f32(v[e])));
+      for (int e = 0; e < 8; ++e)
+        if (c + e < g.k) v[e] = x[(c + e) * f.col_stride];
     }
-    top = wave_max(top);
-    if ((threadIdx.x & 63) == 0) parts[m * 8 + w] = top;
-  }
+    return v;
+  };
+  V held[FEW_ROWS];
+#pragma unroll
+  for (int m = 0; m < FEW_ROWS; ++m)
+    if (m < g.m) held[m] = piece(m, c0);
+#pragma unroll
+  for (int m = 0; m < FEW_ROWS; ++m)
+    if (m < g.m) {
+      unsigned top = most_bits<TX, 8>(held[m], 0);
+      for (int c = c0 + 8 * 512; c < g.k; c += 8 * 512) top = most_bits<TX, 8>(piece(m, c), top);
+      top = wave_most<TX>(top);
+      if ((threadIdx.x & 63) == 0) parts[m * 8 + w] = top;
+    }
   __syncthreads();
-  for (int m = 0; m < g.m; ++m) {
-    unsigned top = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, parts[m * 8 + i]);
-    const RowScale s = row_scale(top);
-    if (threadIdx.x == 0) scales[m] = s.top / 127.0f;
-    const TX* x = (const TX*)f.x + m * f.row_stride;
-    for (int c = 8 * threadIdx.x; c < ld - 16; c += 8 * 512) {
-      typedef TX V __attribute__((ext_vector_type(8)));
-      V v = {};
-      if (f.vec && c + 8 <= g.k) {
-        v = *(const V*)(x + c);
-      } else {
+  for (int m = 0; m < FEW_ROWS; ++m)
+    if (m < g.m) {
+      unsigned top = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (c + e < g.k) v[e] = x[(c + e) * f.col_stride];
-      }
-      quantise_store<8>(v, s, rows + m * ld + c);
+      for (int i = 0; i < 8; ++i) top = max(top, parts[m * 8 + i]);
+      const RowScale s = row_scale(top);
+      if (threadIdx.x == 0) scales[m] = s.top / 127.0f;
+      if (c0 < ld - 16) quantise_store<8>(held[m], s, rows + m * ld + c0);
+      for (int c = c0 + 8 * 512; c < ld - 16; c += 8 * 512) quantise_store<8>(piece(m, c), s, rows + m * ld + c);
     }
-  }
   __syncthreads();
 }
 
@@ -288,9 +337,9 @@ __global__ __launch_bounds__(512) void k_int8_few(Int8Args g, FewX f) {
 #pragma unroll
     for (int j = 0; j < NG; ++j) acc[i][j] = i32x4{};
 
-  // block u of round s: the wave's pairs are s * U / 2 + u / 2, dealt out over the waves
-  const int rounds = (blocks + 8 * FEW_U - 1) / (8 * FEW_U);
-  const int up = (g.k + 15) / 16 * 16;
+  // block u of round s: the wave's pairs are s * U / 2 + u / 2, dealt out over the waves.  All of a round's reads, of a too, are under way together;
+  // blocks past the end are zeros of b.
+  const int whole = g.k / 64, rounds = (whole + 8 * FEW_U - 1) / (8 * FEW_U);
   auto block_of = [&](int s, int u) { return ((s * (FEW_U / 2) + u / 2) * 8 + w) * 2 + (u & 1); };
   auto load_b = [&](int s, i32x4 (&v)[FEW_U][NG]) {
 #pragma unroll
@@ -298,39 +347,52 @@ __global__ __launch_bounds__(512) void k_int8_few(Int8Args g, FewX f) {
       const int b = block_of(s, u);
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
-        if (b * 64 + 64 <= g.k) {
-          v[u][j] = *(const i32x4*)(pb[j] + (size_t)b * 64);
-        } else {
-          v[u][j] = i32x4{};
-          const int c = b * 64 + quarter * 16;
-          if (c < up) v[u][j] = keep_bytes(*(const i32x4*)(pb[j] + (size_t)b * 64), g.k - c);
-        }
+        v[u][j] = i32x4{};
+        if (b < whole) v[u][j] = *(const i32x4_loose*)(pb[j] + (size_t)b * 64);
       }
     }
   };
-  auto multiply = [&](int s, i32x4 (&v)[FEW_U][NG]) {
+  auto load_a = [&](int s, i32x4 (&v)[FEW_U][MG]) {
 #pragma unroll
     for (int u = 0; u < FEW_U; ++u) {
       const int b = block_of(s, u);
-      if (b < blocks) {
-        const bool there = FUSED || b * 64 + quarter * 16 < up;
-        i32x4 a[MG];
+      if (b < whole)
 #pragma unroll
-        for (int i = 0; i < MG; ++i) a[i] = *(const i32x4*)(pa[i] + (there ? (size_t)b * 64 : 0));  // (what stands in for a missing chunk meets zeros)
-#pragma unroll
-        for (int i = 0; i < MG; ++i)
-#pragma unroll
-          for (int j = 0; j < NG; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(v[u][j], a[i], acc[i][j], 0, 0, 0);
-      }
+        for (int i = 0; i < MG; ++i) v[u][i] = *(const i32x4_loose*)(pa[i] + (size_t)b * 64);
     }
   };
-  i32x4 v[FEW_U][NG];
+  i32x4 v[FEW_U][NG], a[FEW_U][MG] = {};
   load_b(0, v);
   if constexpr (FUSED) few_quantise<T>(g, f, rows, ldf, scales, parts);
-  for (int s = 0;;) {
-    multiply(s, v);
-    if (++s == rounds) break;
-    load_b(s, v);
+  for (int s = 0; s < rounds;) {
+    load_a(s, a);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < FEW_U; ++u)
+#pragma unroll
+      for (int i = 0; i < MG; ++i)
+#pragma unroll
+        for (int j = 0; j < NG; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(v[u][j], a[u][i], acc[i][j], 0, 0, 0);
+    if (++s < rounds) load_b(s, v);
+  }
+  if (whole < blocks && w == whole % 8) {  // the ragged block
+    const int left = g.k - whole * 64 - quarter * 16;  // bytes of the lane's chunk
+    auto chunk = [&](const char* row, int padded) {
+      const signed char* p = (const signed char*)row + (size_t)whole * 64;
+      return left <= 0 ? i32x4{} : keep_bytes(left >= 16 || padded ? (i32x4)(*(const i32x4_loose*)p) : loose_bytes(p, left), left);
+    };
+    i32x4 at[MG];
+#pragma unroll
+    for (int i = 0; i < MG; ++i) at[i] = chunk(pa[i], FUSED || f.a_padded);
+#pragma unroll 1
+    for (int j = 0; j < NG; ++j) {
+      const i32x4 bt = chunk(j ? pb[NG - 1] : pb[0], f.b_padded);
+#pragma unroll
+      for (int i = 0; i < MG; ++i) {
+        if (j == 0) acc[i][0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bt, at[i], acc[i][0], 0, 0, 0);
+        if (NG > 1 && j == 1) acc[i][NG - 1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bt, at[i], acc[i][NG - 1], 0, 0, 0);
+      }
+    }
   }
 
   __syncthreads();  // (FUSED: the rows are read no more)

@@ -88,8 +88,7 @@ int quantize(nls_ctx* ctx, const T* x, long rows, long k, long rs, long cs, sign
 }
 template <class T>
 int quantize(nls_ctx* ctx, const T* x, long rows, long k, long rs, long cs, signed char* q, long ldq, float* scale, hipStream_t st) {
-  const bool vec = cs == 1 && (uintptr_t)x % 16 == 0 && (rows == 1 || rs * sizeof(T) % 16 == 0);
-  return vec ? quantize<T, true>(ctx, x, rows, k, rs, cs, q, ldq, scale, st) : quantize<T, false>(ctx, x, rows, k, rs, cs, q, ldq, scale, st);
+  return cs == 1 ? quantize<T, true>(ctx, x, rows, k, rs, cs, q, ldq, scale, st) : quantize<T, false>(ctx, x, rows, k, rs, cs, q, ldq, scale, st);
 }
 int quantize_any(nls_ctx* ctx, const void* x, int type, long rows, long k, long rs, long cs, signed char* q, long ldq, float* scale, hipStream_t st) {
   switch (type) {
@@ -130,37 +129,43 @@ int int8_few(nls_ctx* ctx, const Int8Args& g, const FewX& f, hipStream_t st) {
 }
 // Two row groups of b a workgroup halve what is read of a; taken where that leaves a workgroup for every compute unit.
 template <class T, int MG>
-int int8_few(nls_ctx* ctx, const Int8Args& g, hipStream_t st) {
-  if (MG > 1 && (g.n + 31) / 32 >= ctx->cus) return int8_few<T, MG, 2, false>(ctx, g, FewX{}, st);
-  return int8_few<T, MG, 1, false>(ctx, g, FewX{}, st);
+int int8_few(nls_ctx* ctx, const Int8Args& g, const FewX& f, hipStream_t st) {
+  if (MG > 1 && (g.n + 31) / 32 >= ctx->cus) return int8_few<T, MG, 2, false>(ctx, g, f, st);
+  return int8_few<T, MG, 1, false>(ctx, g, f, st);
 }
+// Few rows of a: fragments straight from memory, or tiles.  Measured: 16 x 4096 x 4096 8.2 us against 11.3 with tiles, 48 x 4096 x 4096 12.4 / 12.8,
+// 64 x 4096 x 4096 14.4 / 13.5; 16 x 8192 x 8192 21 / 21, 48 x 8192 x 8192 28 / 24 (128 tiles keep enough of the card busy).
+bool int8_is_few(long m, long n) { return m <= 16 || (m <= 48 && n < 8192); }
 template <class T>
-int int8_product(nls_ctx* ctx, const Int8Args& g, hipStream_t st) {
-  if (g.m <= 16) return int8_few<T, 1>(ctx, g, st);
-  if (g.m <= 32) return int8_few<T, 2>(ctx, g, st);
-  if (g.m <= 48) return int8_few<T, 3>(ctx, g, st);
-  if (g.m <= 64) return int8_few<T, 4>(ctx, g, st);
+int int8_product(nls_ctx* ctx, const Int8Args& g, const FewX& f, hipStream_t st) {
+  if (int8_is_few(g.m, g.n)) return g.m <= 16 ? int8_few<T, 1>(ctx, g, f, st) : g.m <= 32 ? int8_few<T, 2>(ctx, g, f, st) : int8_few<T, 3>(ctx, g, f, st);
   return g.n % (16 / (int)sizeof(T)) == 0 ? int8_tile<T, 16 / sizeof(T)>(ctx, g, st) : int8_tile<T, 1>(ctx, g, st);
 }
 // Whether int8_linear quantises inside the product: every workgroup does all the rows of x over again, which has to stay small beside its share of b.
-bool int8_fused(long m, long k) { return m <= 4 && m * k <= 32768; }
+// Measured: one row always (1 x 4096 x 4096 8.0 us against 9.8 in two launches, 8192 x 8192 19.1 / 20.8), four of small products (4096 x 4096 11.4 / 10.3 and a
+// launch less to make, 8192 x 8192 28 / 21).
+bool int8_fused(long m, long n, long k) { return m * k <= 32768 && (m <= 2 || (m <= FEW_ROWS && n * k <= 1l << 24)); }
 template <class T>
 int int8_fused_product(nls_ctx* ctx, const Int8Args& g, const FewX& f, hipStream_t st) {
   return int8_few<T, 1, 1, true>(ctx, g, f, st);
 }
-int int8_product_any(nls_ctx* ctx, const Int8Args& g, int type, hipStream_t st) {
+int int8_product_any(nls_ctx* ctx, const Int8Args& g, const FewX& f, int type, hipStream_t st) {
   switch (type) {
-    case NLS_TYPE_F32: return int8_product<float>(ctx, g, st);
-    case NLS_TYPE_F16: return int8_product<_Float16>(ctx, g, st);
-    default: return int8_product<__bf16>(ctx, g, st);
+    case NLS_TYPE_F32: return int8_product<float>(ctx, g, f, st);
+    case NLS_TYPE_F16: return int8_product<_Float16>(ctx, g, f, st);
+    default: return int8_product<__bf16>(ctx, g, f, st);
   }
 }
 
 long up16(long k) { return (k + 15) / 16 * 16; }
 size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 
-bool aligned_rows(const void* p, long ld, long k, int flags, int flag) {
-  return (uintptr_t)p % 16 == 0 && ld % 16 == 0 && ld >= up16(k) && (k % 16 == 0 || (flags & flag));
+// Rows that the product can read where they are.  Tiles: those that start at multiples of 16 bytes and may be read up to one.  Few rows: any start for up
+// to 16 of them (1 x 4097 x 4099 from odd addresses 10 us), multiples of 16 bytes for more (48 x 4097 x 4099: 43 us from odd addresses, 22 us aligned).
+bool rows_ready(long m, long n, const void* p, long ld, long k, int flags, int flag) {
+  const bool aligned = (uintptr_t)p % 16 == 0 && ld % 16 == 0;
+  if (int8_is_few(m, n)) return m <= 16 || aligned;
+  return aligned && ld >= up16(k) && (k % 16 == 0 || (flags & flag));
 }
 
 int check_int8(nls_ctx* ctx, const char* what, int64_t m, int64_t n, int64_t k, int type, int bias_type, const void* bias) {
@@ -193,7 +198,7 @@ int operands(nls_ctx* ctx, const Int8Rows& a, const Int8Rows& b, long k, char* w
     todo[count++] = AlignRows{(const signed char*)r.p, (signed char*)ws, r.rows, r.ld};
     *o = Operand{ws, (unsigned)ldy, (int)r.rows};
     ws += up256((size_t)r.rows * ldy);
-    most = std::max(most, r.rows * (ldy / 4));
+    most = std::max(most, r.rows * (ldy / 16));
   }
   if (!count) return NLS_OK;
   k_align_rows<<<dim3((unsigned)std::min<long>((most + 255) / 256, 32768), (unsigned)count), 256, 0, st>>>(todo[0], todo[1], k, ldy);
@@ -450,8 +455,8 @@ extern "C" int nls_quantize_rows(nls_ctx* ctx, const void* x, int type, int64_t 
 extern "C" int nls_int8_matmul_workspace(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, int64_t m, int64_t n, int64_t k, int flags,
                                          size_t* bytes) {
   if (!bytes || m < 0 || n < 0 || k < 1) return NLS_ERR_ARG;
-  *bytes = (aligned_rows(a, lda, k, flags, NLS_INT8_A_PADDED) ? 0 : up256((size_t)m * up16(k))) +
-           (aligned_rows(b, ldb, k, flags, NLS_INT8_B_PADDED) ? 0 : up256((size_t)n * up16(k)));
+  *bytes = (rows_ready(m, n, a, lda, k, flags, NLS_INT8_A_PADDED) ? 0 : up256((size_t)m * up16(k))) +
+           (rows_ready(m, n, b, ldb, k, flags, NLS_INT8_B_PADDED) ? 0 : up256((size_t)n * up16(k)));
   return NLS_OK;
 }
 
@@ -471,7 +476,7 @@ extern "C" int nls_int8_matmul(nls_ctx* ctx, const int8_t* a, int64_t lda, const
   HIPCHK(ctx, dev.err);
   hipStream_t st = (hipStream_t)stream;
   Int8Args g{};
-  NLSCHK(operands(ctx, {a, m, lda, aligned_rows(a, lda, k, flags, NLS_INT8_A_PADDED)}, {b, n, ldb, aligned_rows(b, ldb, k, flags, NLS_INT8_B_PADDED)}, k,
+  NLSCHK(operands(ctx, {a, m, lda, rows_ready(m, n, a, lda, k, flags, NLS_INT8_A_PADDED)}, {b, n, ldb, rows_ready(m, n, b, ldb, k, flags, NLS_INT8_B_PADDED)}, k,
                   (char*)workspace, &g.a, &g.b, st));
   g.a_scale = a_scale;
   g.b_scale = b_scale;
@@ -481,13 +486,16 @@ extern "C" int nls_int8_matmul(nls_ctx* ctx, const int8_t* a, int64_t lda, const
   g.n = (int)n;
   g.k = (int)k;
   g.y = y;
-  return int8_product_any(ctx, g, type, st);
+  FewX f{};
+  f.a_padded = flags & NLS_INT8_A_PADDED;
+  f.b_padded = flags & NLS_INT8_B_PADDED;
+  return int8_product_any(ctx, g, f, type, st);
 }
 
 extern "C" int nls_int8_linear_workspace(const int8_t* b, int64_t ldb, int64_t m, int64_t n, int64_t k, int flags, size_t* bytes) {
   if (!bytes || m < 0 || n < 0 || k < 1) return NLS_ERR_ARG;
-  *bytes = (int8_fused(m, k) ? 0 : up256((size_t)m * up16(k)) + up256((size_t)m * 4)) +
-           (aligned_rows(b, ldb, k, flags, NLS_INT8_B_PADDED) ? 0 : up256((size_t)n * up16(k)));
+  *bytes = (int8_fused(m, n, k) ? 0 : up256((size_t)m * up16(k)) + up256((size_t)m * 4)) +
+           (rows_ready(m, n, b, ldb, k, flags, NLS_INT8_B_PADDED) ? 0 : up256((size_t)n * up16(k)));
   return NLS_OK;
 }
 
@@ -515,12 +523,12 @@ extern "C" int nls_int8_linear(nls_ctx* ctx, const void* x, int type, int64_t ro
   g.n = (int)n;
   g.k = (int)k;
   g.y = y;
-  const bool b_ready = aligned_rows(b, ldb, k, flags, NLS_INT8_B_PADDED);
+  const bool b_ready = rows_ready(m, n, b, ldb, k, flags, NLS_INT8_B_PADDED);
   NLSCHK(operands(ctx, {nullptr, 0, 0, true}, {b, n, ldb, b_ready}, k, ws, &g.a, &g.b, st));
   if (!b_ready) ws += up256((size_t)n * up16(k));
-  if (int8_fused(m, k)) {
-    const int size = type_size(type);
-    const FewX f{x, row_stride, col_stride, col_stride == 1 && (uintptr_t)x % (8 * size) == 0 && (m == 1 || row_stride % 8 == 0)};
+  const int b_padded = flags & NLS_INT8_B_PADDED;
+  if (int8_fused(m, n, k)) {
+    const FewX f{x, row_stride, col_stride, col_stride == 1, 0, b_padded};
     switch (type) {
       case NLS_TYPE_F32: return int8_fused_product<float>(ctx, g, f, st);
       case NLS_TYPE_F16: return int8_fused_product<_Float16>(ctx, g, f, st);
@@ -533,7 +541,10 @@ extern "C" int nls_int8_linear(nls_ctx* ctx, const void* x, int type, int64_t ro
   NLSCHK(quantize_any(ctx, x, type, m, k, row_stride, col_stride, q, ldq, scale, st));
   g.a = Operand{(const char*)q, (unsigned)ldq, (int)m};
   g.a_scale = scale;
-  return int8_product_any(ctx, g, type, st);
+  FewX f{};
+  f.a_padded = 1;
+  f.b_padded = b_padded;
+  return int8_product_any(ctx, g, f, type, st);
 }
 
 extern "C" int nls_orthogonalize_workspace(int64_t batch, int64_t m, int64_t n, int64_t row_stride, int64_t col_stride, size_t* bytes) {
