@@ -390,9 +390,8 @@ int orthogonalize(nls_ctx* ctx, const NsMatrix& w, const NsPlan& plan, bool tall
   char *X = base, *XT = X + plan.x, *XU = XT + plan.xt, *A = XU + plan.xt, *B = A + plan.a;
   const int count = ns_parts(w);
   k_ns_norm<T><<<dim3(count, (unsigned)batch), 256, 0, st>>>(w, parts);
-  k_ns_scales<<<dim3((unsigned)batch), 64, 0, st>>>(parts, count, eps, cf, steps, scales);
-  k_ns_pack<T><<<dim3((unsigned)((w.q + 63) / 64), (unsigned)((w.p + 63) / 64), (unsigned)batch), 256, 0, st>>>(w, scales, X, XT, plan.batch_bytes,
-                                                                                                                                   steps <= exact);
+  k_ns_pack<T><<<dim3((unsigned)((w.q + 63) / 64), (unsigned)((w.p + 63) / 64), (unsigned)batch), 256, 0, st>>>(w, parts, count, eps, cf, steps, scales, X, XT,
+                                                                                                              plan.batch_bytes, steps <= exact);
   LAUNCHED(ctx, "orthogonalize");
   NsArgs g{};
   g.scales = scales;

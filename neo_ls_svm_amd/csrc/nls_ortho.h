@@ -199,17 +199,6 @@ __device__ __forceinline__ void ns_fetch(const NsCoef& cf, int steps, NsCoef* to
     to->last = cf.last;
   }
 }
-__global__ __launch_bounds__(64) void k_ns_scales(const double* parts, int count, double eps, NsCoef cf, int steps, NsScales* out) {
-  __shared__ NsCoef mine;
-  ns_fetch(cf, steps, &mine, out[blockIdx.x].f);
-  double s = 0.0;
-  for (int i = threadIdx.x; i < count; i += 64) s += parts[(size_t)blockIdx.x * NS_PARTS + i];
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-  __syncthreads();
-  if (threadIdx.x == 0) ns_scales(s, eps, mine, steps, out[blockIdx.x]);
-}
-
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void split(float v, float u, f16x2* hi, f16x2* lo) {  // (two at a time: one conversion instruction)
@@ -228,36 +217,56 @@ __device__ __forceinline__ void split8(const float* v, f16x8* hi, f16x8* lo) {
   }
 }
 
-// G -> X_0 (p rows) and its transpose (q rows), zero-padded.  One 64 x 64 tile a workgroup.
+// G -> X_0 (p rows) and its transpose (q rows), zero-padded.  One 64 x 64 tile a workgroup; each adds the parts of the norm up for itself while its
+// elements are on the way (a launch of its own for that took 4 us), the first of a matrix leaves the factors for the products.
 template <class T>
-__global__ __launch_bounds__(256) void k_ns_pack(NsMatrix w, const NsScales* scales, char* x, char* xt, size_t batch_bytes, int for_pairs) {
+__global__ __launch_bounds__(256) void k_ns_pack(NsMatrix w, const double* parts, int count, double eps, NsCoef cf, int steps, NsScales* scales, char* x,
+                                                 char* xt, size_t batch_bytes, int for_pairs) {
   __shared__ float tile[64][65];
+  __shared__ NsCoef mine;
+  __shared__ NsScales z;
+  __shared__ double part[4];
   const T* g = (const T*)w.g + blockIdx.z * w.batch_stride;
   x += blockIdx.z * batch_bytes;
   xt += blockIdx.z * batch_bytes;
-  const NsScales& z = scales[blockIdx.z];
-  const double f = z.first;
   const long p0 = (long)blockIdx.y * 64, q0 = (long)blockIdx.x * 64;
   const bool along_q = w.col_stride <= w.row_stride;
   const int l = threadIdx.x & 63, r = threadIdx.x >> 6;
-  for (int o = r; o < 64; o += 4) {
-    const int pi = along_q ? o : l, qi = along_q ? l : o;
-    float v = 0.0f;
-    if (p0 + pi < w.p && q0 + qi < w.q) v = (float)((double)to_f32(g[(p0 + pi) * w.row_stride + (q0 + qi) * w.col_stride]) * f);
-    tile[pi][qi] = v;
+  T v[16];
+#pragma unroll
+  for (int u = 0; u < 16; ++u) {
+    const int o = r + 4 * u, pi = along_q ? o : l, qi = along_q ? l : o;
+    v[u] = p0 + pi < w.p && q0 + qi < w.q ? g[(p0 + pi) * w.row_stride + (q0 + qi) * w.col_stride] : (T)0.0f;
+  }
+  ns_fetch(cf, steps, &mine, z.f);
+  double s = 0.0;
+  for (int i = threadIdx.x; i < count; i += 256) s += parts[(size_t)blockIdx.z * NS_PARTS + i];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+  if (l == 0) part[r] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) ns_scales((part[0] + part[1]) + (part[2] + part[3]), eps, mine, steps, z);
+  __syncthreads();
+  if (blockIdx.x == 0 && blockIdx.y == 0)
+    for (int i = threadIdx.x; i < (int)(sizeof(NsScales) / 4); i += 256) ((int*)(scales + blockIdx.z))[i] = ((const int*)&z)[i];
+  const double f = z.first;
+#pragma unroll
+  for (int u = 0; u < 16; ++u) {
+    const int o = r + 4 * u;
+    tile[along_q ? o : l][along_q ? l : o] = (float)((double)to_f32(v[u]) * f);
   }
   __syncthreads();
   const size_t ldx = pair_ld(w.q), ldt = pair_ld(w.p);
-  const int row = threadIdx.x >> 2, part = (threadIdx.x & 3) * 16;
+  const int row = threadIdx.x >> 2, from = (threadIdx.x & 3) * 16;
   for (int turn = 0; turn < 2; ++turn) {
-    char* base = turn ? xt + pair_at(q0 + row, p0 + part, ldt, for_pairs) : x + pair_at(p0 + row, q0 + part, ldx, for_pairs);
+    char* base = turn ? xt + pair_at(q0 + row, p0 + from, ldt, for_pairs) : x + pair_at(p0 + row, q0 + from, ldx, for_pairs);
     if (turn ? q0 + row >= w.q : p0 + row >= w.p) continue;
     f16x8 hi[2], lo[2];
-    float v[16];
+    float e[16];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) v[e] = turn ? tile[part + e][row] : tile[row][part + e];
-    split8(v, &hi[0], &lo[0]);
-    split8(v + 8, &hi[1], &lo[1]);
+    for (int k = 0; k < 16; ++k) e[k] = turn ? tile[from + k][row] : tile[row][from + k];
+    split8(e, &hi[0], &lo[0]);
+    split8(e + 8, &hi[1], &lo[1]);
     *(f16x8*)base = hi[0];
     *(f16x8*)(base + 16) = hi[1];
     *(f16x8*)(base + pair_lo(for_pairs)) = lo[0];
@@ -306,28 +315,42 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
   const int i0 = bi * BI, j0 = bj * BJ;
   const size_t off = blockIdx.z * g.batch_bytes;
   const size_t ldk = pair_ld(g.K), ldi = pair_ld(g.I), ldj = pair_ld(g.J);
-  TL t;
-  const int per = MODE == MODE_F16 ? 64 : 32;
-  t.run(Operand{g.P + off, (unsigned)ldk, g.I}, i0, Operand{g.Q + off, (unsigned)ldk, g.J}, j0, (g.K + per - 1) / per, 128, lds);
   const NsScales& z = g.scales[blockIdx.z];
   const NsFactors f = z.f[g.t];
   const int last = z.last;
   const char* E = g.E + off;
+  constexpr bool PAIRS = MODE == MODE_F16PAIR;
+  constexpr int ACROSS = BI / 8, ROWS = TL::THREADS / ACROSS, TURNS = TL::CHUNK / ROWS;
+  const int iw = threadIdx.x % ACROSS * 8, i = i0 + iw;
+  auto addend = [&](int j, f16x8* h, f16x8* o) {  // eight elements of E; rows are padded: whole groups of eight, zeros behind the end
+    *h = *o = f16x8{};
+    if (j < g.J && (size_t)i * 4 < ldi) {
+      const char* at = E + pair_at(j, i, ldi, PAIRS);
+      *h = *(const f16x8*)at;
+      if (KIND != NS_POLY || PAIRS) *o = *(const f16x8*)(at + pair_lo(PAIRS));
+    }
+  };
+  // Small tiles fetch what the epilogue adds before the product: for small matrices every launch is a chain of misses, this one is then off it.
+  constexpr bool EARLY = KIND != NS_GRAM && TL::CHUNKS == 1 && TURNS <= 2;
+  f16x8 eh[EARLY ? TURNS : 1], el[EARLY ? TURNS : 1];
+  if constexpr (EARLY) {
+#pragma unroll
+    for (int u = 0; u < TURNS; ++u) addend(j0 + TL::column(0, threadIdx.x / ACROSS + u * ROWS), &eh[u], &el[u]);
+  }
+  TL t;
+  const int per = MODE == MODE_F16 ? 64 : 32;
+  t.run(Operand{g.P + off, (unsigned)ldk, g.I}, i0, Operand{g.Q + off, (unsigned)ldk, g.J}, j0, (g.K + per - 1) / per, 128, lds);
   char* D = g.D + off;
   char* DT = SYM ? D : g.DT + off;
   T* out = (T*)g.out + blockIdx.z * g.out_stride;
   // Lo halves nobody reads are not written: of A and B where the step's products are single ones, of the transpose of X where the next step's are.
-  constexpr bool PAIRS = MODE == MODE_F16PAIR;
   const bool to_pairs = SYM ? PAIRS : g.next_pairs != 0;  // the products that will read D and DT
-  const bool low_e = KIND != NS_POLY || PAIRS;
   const int lo_d = !SYM || PAIRS ? pair_lo(to_pairs) : 0, lo_t = to_pairs ? pair_lo(true) : 0;
   const bool natural = KIND != NS_LAST || !g.transposed, turned = KIND == NS_LAST ? g.transposed != 0 : SYM ? bi != bj : true;
   // (STEP writes X where it reads it, perhaps in the other layout: the 64 elements that share 256 bytes are eight neighbouring lanes' of one wave,
   // which have read them all before the first is written.)
   // Chunks of the tile through LDS: the result in the product's own orientation (rows j, eight neighbours i a thread), then, from the values left
   // there, its transpose (rows i, eight neighbours j).
-  constexpr int ACROSS = BI / 8, ROWS = TL::THREADS / ACROSS;
-  const int iw = threadIdx.x % ACROSS * 8, i = i0 + iw;
   constexpr int DOWN = TL::CHUNK / 8;
   const int iv = threadIdx.x / DOWN, rv = threadIdx.x % DOWN * 8;
 #pragma unroll
@@ -335,20 +358,21 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
     __syncthreads();
     t.spill(c, lds);
     __syncthreads();
-    for (int r = threadIdx.x / ACROSS; r < TL::CHUNK; r += ROWS) {
-      const int j = j0 + TL::column(c, r);
+#pragma unroll EARLY ? TURNS : 1
+    for (int u = 0; u < TURNS; ++u) {
+      const int r = threadIdx.x / ACROSS + u * ROWS, j = j0 + TL::column(c, r);
       float v[8];
       chunk_sums<TL, 8>(lds, r, iw, v);
-      f16x8 eh = {}, el = {};
-      const bool there = j < g.J && (size_t)i * 4 < ldi;  // (rows are padded: whole groups of eight, zeros behind the end)
-      if (KIND != NS_GRAM && there) {
-        const char* at = E + pair_at(j, i, ldi, PAIRS);
-        eh = *(const f16x8*)at;
-        if (low_e) el = *(const f16x8*)(at + pair_lo(PAIRS));
+      f16x8 h = {}, o = {};
+      if constexpr (EARLY) {
+        h = eh[u];
+        o = el[u];
+      } else if (KIND != NS_GRAM) {
+        addend(j, &h, &o);
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float x = (float)eh[e] + (float)el[e];
+        const float x = (float)h[e] + (float)o[e];
         float w = v[e];
         if (KIND == NS_GRAM) w = f.gram * w;
         if (KIND == NS_POLY) w = f.lin * x + f.quad * w;
@@ -360,7 +384,7 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) ((float*)lds)[r * TL::PITCH + iw + e] = v[e];
       if (KIND != NS_LAST) {
-        if (there) store_pairs(D + pair_at(j, i, ldi, to_pairs), v, lo_d);
+        if (j < g.J && (size_t)i * 4 < ldi) store_pairs(D + pair_at(j, i, ldi, to_pairs), v, lo_d);
       } else if (natural && j < g.J && i < g.I) {
         store8(out + (size_t)j * g.I + i, v, g.I - i, i + 8 <= g.I && g.I % (16 / (int)sizeof(T)) == 0);
       }

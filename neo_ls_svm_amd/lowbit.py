@@ -119,11 +119,19 @@ class _Tensors:
         if (
             isinstance(x, T) and isinstance(scale, T) and x.dtype is self.int8 and scale.dtype is self.float32
             and x.get_device() == self.index == scale.get_device() and x.layout is strided is scale.layout
-            and x.is_contiguous() and scale.is_contiguous() and not scale.requires_grad and not scale.is_neg()
+            and scale.is_contiguous() and not scale.requires_grad and not scale.is_neg()
         ):  # fmt: skip
             shape = x.shape
-            if len(shape) == 2 and scale.shape == shape[:1] and 0 < shape[1] <= MAX_K and not shape[1] & 15:
-                return x, scale, shape[:1], shape[0], shape[1], shape[1], True
+            if len(shape) == 2 and scale.shape == shape[:1] and 0 < shape[1] <= MAX_K:
+                rows, k = shape
+                ld, dense = x.stride()
+                if dense == 1 and rows > 1 and ld >= k:
+                    if not k & 15:
+                        return x, scale, shape[:1], rows, k, ld, True
+                    up = (k + 15) & -16
+                    return x, scale, shape[:1], rows, k, ld, ld >= up and self.room(x) >= (rows - 1) * ld + up
+                if dense == 1 and not k & 15:
+                    return x, scale, shape[:1], rows, k, k, True
         return _int8_rows(self, x, what, scale, scale_what)
 
     def scratch(self, nbytes):
