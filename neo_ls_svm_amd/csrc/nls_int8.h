@@ -204,11 +204,10 @@ __device__ __forceinline__ float bias_at(const Int8Args& g, int n) {
 __device__ __forceinline__ float scaled(int sum, float as, float bs, float bias) { return (float)sum * as * bs + bias; }
 
 // Many rows: P = b (its rows lie along a chunk's words, as neighbours in a row of y), Q = a.
-// N: elements of a row of y a thread writes at once - 16 bytes where the rows start at such multiples, else one; neighbouring threads neighbouring
-// columns in both.  A thread has the same channels in all its rows.
-template <class T, class TL, int BI, int BJ, int N>
+// A thread writes 16 bytes of a row of y at once, wherever the row starts (a store may begin at any element), and has the same channels in all its rows.
+template <class T, class TL, int BI, int BJ>
 __global__ __launch_bounds__(TL::THREADS) void k_int8_tile(Int8Args g, int ti, int tj, int strip) {
-  typedef T V __attribute__((ext_vector_type(N)));
+  constexpr int N = 16 / (int)sizeof(T);
   extern __shared__ char lds[];
   int bi, bj;
   strip_order(die_order(blockIdx.x, ti * tj), ti, tj, strip, &bi, &bj);
@@ -218,13 +217,12 @@ __global__ __launch_bounds__(TL::THREADS) void k_int8_tile(Int8Args g, int ti, i
   t.run(g.b, i0, g.a, j0, steps, g.k - (steps - 1) * 128, lds);
   constexpr int ACROSS = BI / N, ROWS = TL::THREADS / ACROSS;
   T* y = (T*)g.y;
-  const int iw = threadIdx.x % ACROSS * N, n = i0 + iw;
-  const bool there = n < g.n;
+  const int iw = threadIdx.x % ACROSS * N, n = i0 + iw, left = g.n - n;
   float bs[N], bias[N];
 #pragma unroll
   for (int e = 0; e < N; ++e) {
-    bs[e] = there ? g.b_scale[n + e] : 0.0f;
-    bias[e] = there ? bias_at<T>(g, n + e) : 0.0f;
+    bs[e] = e < left ? g.b_scale[n + e] : 0.0f;
+    bias[e] = e < left ? bias_at<T>(g, n + e) : 0.0f;
   }
 #pragma unroll
   for (int c = 0; c < TL::CHUNKS; ++c) {
@@ -233,14 +231,14 @@ __global__ __launch_bounds__(TL::THREADS) void k_int8_tile(Int8Args g, int ti, i
     __syncthreads();
     for (int r = threadIdx.x / ACROSS; r < TL::CHUNK; r += ROWS) {
       const int m = j0 + TL::column(c, r);
-      if (m >= g.m || !there) continue;
+      if (m >= g.m || left <= 0) continue;
       int s[N];
       chunk_sums<TL, N>(lds, r, iw, s);
       const float as = g.a_scale[m];
-      V v;
+      float v[N];
 #pragma unroll
-      for (int e = 0; e < N; ++e) v[e] = (T)scaled(s[e], as, bs[e], bias[e]);
-      *(V*)(y + (size_t)m * g.n + n) = v;
+      for (int e = 0; e < N; ++e) v[e] = scaled(s[e], as, bs[e], bias[e]);
+      store_some<T, N>(y + (size_t)m * g.n + n, v, left);
     }
   }
 }

@@ -60,7 +60,7 @@ TileKind tile_kind(const nls_ctx* ctx, F tiles, int steps) {
   if (20 * tiles(256) > 11 * cus) return TILE_256;
   if (tiles(128) > cus) return TILE_128;
   if (5 * tiles(128) >= 3 * cus) return TILE_128_DEEP;
-  return tiles(64) > cus || steps < 20 ? TILE_64 : TILE_64_RING;
+  return tiles(64) > cus || steps < 16 ? TILE_64 : TILE_64_RING;
 }
 
 // ---- quantise ----
@@ -99,24 +99,24 @@ int quantize_any(nls_ctx* ctx, const void* x, int type, long rows, long k, long 
 }
 
 // ---- 8-bit product ----
-template <class T, class TL, int BI, int BJ, int N>
+template <class T, class TL, int BI, int BJ>
 int int8_tile(nls_ctx* ctx, const Int8Args& g, hipStream_t st) {
   const int ti = (g.n + BI - 1) / BI, tj = (g.m + BJ - 1) / BJ;
   constexpr int LDS = std::max(TL::LDS, TL::SCRATCH);
-  NLSCHK((ask_lds<&k_int8_tile<T, TL, BI, BJ, N>>(ctx, LDS)));
-  k_int8_tile<T, TL, BI, BJ, N><<<dim3((unsigned)((long)ti * tj)), TL::THREADS, LDS, st>>>(g, ti, tj, 8);
+  NLSCHK((ask_lds<&k_int8_tile<T, TL, BI, BJ>>(ctx, LDS)));
+  k_int8_tile<T, TL, BI, BJ><<<dim3((unsigned)((long)ti * tj)), TL::THREADS, LDS, st>>>(g, ti, tj, 8);
   LAUNCHED(ctx, "int8_matmul");
   return NLS_OK;
 }
-template <class T, int N>
+template <class T>
 int int8_tile(nls_ctx* ctx, const Int8Args& g, hipStream_t st) {
   auto tiles = [&](long b) { return ((g.n + b - 1) / b) * ((g.m + b - 1) / b); };
   switch (tile_kind(ctx, tiles, (g.k + 127) / 128)) {
-    case TILE_256: return int8_tile<T, Tile<MODE_I8, 256, 256, 2, 4, 2>, 256, 256, N>(ctx, g, st);
-    case TILE_128: return int8_tile<T, Tile<MODE_I8, 128, 128, 2, 2, 2>, 128, 128, N>(ctx, g, st);
-    case TILE_128_DEEP: return int8_tile<T, Tile<MODE_I8, 128, 128, 4, 2, 3>, 128, 128, N>(ctx, g, st);
-    case TILE_64: return int8_tile<T, Tile<MODE_I8, 64, 64, 2, 2, 3>, 64, 64, N>(ctx, g, st);
-    default: return int8_tile<T, Ring<MODE_I8, 2>, 64, 64, N>(ctx, g, st);
+    case TILE_256: return int8_tile<T, Tile<MODE_I8, 256, 256, 2, 4, 2>, 256, 256>(ctx, g, st);
+    case TILE_128: return int8_tile<T, Tile<MODE_I8, 128, 128, 2, 2, 2>, 128, 128>(ctx, g, st);
+    case TILE_128_DEEP: return int8_tile<T, Tile<MODE_I8, 128, 128, 4, 2, 3>, 128, 128>(ctx, g, st);
+    case TILE_64: return int8_tile<T, Tile<MODE_I8, 64, 64, 2, 2, 3>, 64, 64>(ctx, g, st);
+    default: return int8_tile<T, Ring<MODE_I8, 2>, 64, 64>(ctx, g, st);
   }
 }
 template <class T, int MG, int NG, bool FUSED>
@@ -139,7 +139,7 @@ bool int8_is_few(long m, long n) { return m <= 16 || (m <= 48 && n < 8192); }
 template <class T>
 int int8_product(nls_ctx* ctx, const Int8Args& g, const FewX& f, hipStream_t st) {
   if (int8_is_few(g.m, g.n)) return g.m <= 16 ? int8_few<T, 1>(ctx, g, f, st) : g.m <= 32 ? int8_few<T, 2>(ctx, g, f, st) : int8_few<T, 3>(ctx, g, f, st);
-  return g.n % (16 / (int)sizeof(T)) == 0 ? int8_tile<T, 16 / sizeof(T)>(ctx, g, st) : int8_tile<T, 1>(ctx, g, st);
+  return int8_tile<T>(ctx, g, st);
 }
 // Whether int8_linear quantises inside the product: every workgroup does all the rows of x over again, which has to stay small beside its share of b.
 // Measured: one row always (1 x 4096 x 4096 8.0 us against 9.8 in two launches, 8192 x 8192 19.1 / 20.8), four of small products (4096 x 4096 11.4 / 10.3 and a

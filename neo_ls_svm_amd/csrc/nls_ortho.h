@@ -386,7 +386,7 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
       if (KIND != NS_LAST) {
         if (j < g.J && (size_t)i * 4 < ldi) store_pairs(D + pair_at(j, i, ldi, to_pairs), v, lo_d);
       } else if (natural && j < g.J && i < g.I) {
-        store8(out + (size_t)j * g.I + i, v, g.I - i, i + 8 <= g.I && g.I % (16 / (int)sizeof(T)) == 0);
+        store_some<T, 8>(out + (size_t)j * g.I + i, v, g.I - i);
       }
     }
     if (turned) {
@@ -400,7 +400,7 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
         if (KIND != NS_LAST) {
           if ((size_t)j * 4 < ldj) store_pairs(DT + pair_at(irow, j, ldj, to_pairs), v, lo_t);
         } else if (j < g.J) {
-          store8(out + (size_t)irow * g.J + j, v, g.J - j, j + 8 <= g.J && g.J % (16 / (int)sizeof(T)) == 0);
+          store_some<T, 8>(out + (size_t)irow * g.J + j, v, g.J - j);
         }
       }
     }

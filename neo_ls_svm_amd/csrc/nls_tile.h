@@ -311,23 +311,24 @@ template <class T>
 __device__ __forceinline__ float to_f32(T v) {
   return (float)v;
 }
-// Eight neighbouring results, rounded to T, to an output row: whole where it is aligned, else those below n one by one
-template <class T>
-__device__ __forceinline__ void store8(T* at, const float (&v)[8], int n, bool whole) {
-  if (whole) {
-    typedef T V __attribute__((ext_vector_type(sizeof(T) == 2 ? 8 : 4)));
-    constexpr int N = sizeof(V) / sizeof(T);
+// N neighbouring results, rounded to T, to an output row: 16 bytes at a time wherever they fall, at the row's end one by one
+template <class T, int N>
+__device__ __forceinline__ void store_some(T* at, const float (&v)[N], int left) {
+  constexpr int W = 16 / (int)sizeof(T);
+  static_assert(N % W == 0, "whole stores");
+  typedef T V __attribute__((ext_vector_type(W), aligned(sizeof(T))));
+  if (left >= N) {
 #pragma unroll
-    for (int e = 0; e < 8; e += N) {
+    for (int e = 0; e < N; e += W) {
       V w;
 #pragma unroll
-      for (int k = 0; k < N; ++k) w[k] = (T)v[e + k];
+      for (int k = 0; k < W; ++k) w[k] = (T)v[e + k];
       *(V*)(at + e) = w;
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < n) at[e] = (T)v[e];
+    for (int e = 0; e < N; ++e)
+      if (e < left) at[e] = (T)v[e];
   }
 }
 

@@ -31,6 +31,7 @@ NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
 MAX_K = 131071  # NLS_INT8_MAX_K
 _A_PADDED, _B_PADDED = 1, 2
 _NAMES = ("float32", "float16", "bfloat16")  # the position is the type's number in the C ABI
+_NAMED = {name: i for i, name in enumerate(_NAMES)}
 
 
 def _kind_of(dtype, what) -> int:
@@ -61,6 +62,8 @@ class _Tensors:
         self.lib, self.index, self.ctx = lib, index, ctx
         self.device = lib.device("cuda", index)
         self.kinds = {getattr(lib, name): i for i, name in enumerate(_NAMES)}
+        self.named = {**self.kinds, **_NAMED}
+        self.ptr, self.strides, self.dense = lib.Tensor.data_ptr, lib.Tensor.stride, lib.Tensor.contiguous
         self.types = tuple(getattr(lib, name) for name in _NAMES)
         self.int8, self.float32, self.uint8, self.strided, self.Tensor = lib.int8, lib.float32, lib.uint8, lib.strided, lib.Tensor
         self._empty = lib.empty
@@ -81,18 +84,6 @@ class _Tensors:
         if x.requires_grad and self.lib.is_grad_enabled():
             raise ValueError(f"{what} asks for gradients, which this operator does not give: detach it, or call under no_grad")
         return x.resolve_neg() if x.is_neg() else x
-
-    @staticmethod
-    def ptr(x):
-        return x.data_ptr()
-
-    @staticmethod
-    def strides(x):
-        return x.stride()
-
-    @staticmethod
-    def dense(x):
-        return x.contiguous()
 
     @staticmethod
     def room(x):
@@ -146,6 +137,7 @@ class _Arrays:
     """NumPy arrays and DeviceArrays, on the context's own stream; results come back as what went in."""
 
     kinds = {np.dtype("float32"): 0, np.dtype("float16"): 1}
+    named = _NAMED
     types = (np.dtype("float32"), np.dtype("float16"))
     int8, float32 = np.dtype("int8"), np.dtype("float32")
 
@@ -364,7 +356,9 @@ def int8_matmul(a, a_scale, b, b_scale, bias=None, dtype="float32", ctx: Context
     (k <= 131071), the rest is float32, rounded once.  Rows that do not start at multiples of 16 bytes are copied first; ``quantize_rows`` lays them
     out so that they do."""
     sp = _space(a, ctx)
-    kind = _kind_of(dtype, "dtype")
+    kind = sp.named.get(dtype) if dtype.__hash__ is not None else None
+    if kind is None:
+        kind = _kind_of(dtype, "dtype")
     if kind >= len(sp.types):
         raise ValueError("dtype: NumPy arrays and DeviceArrays have no bfloat16")
     a, a_scale, lead, m, k, lda, a_ready = sp.int8_rows(a, "a", a_scale, "a_scale")
