@@ -273,6 +273,9 @@ int ns_product(nls_ctx* ctx, const NsArgs& g, long batch, hipStream_t st) {
     const long i = (g.I + b - 1) / b, j = (g.J + b - 1) / b;
     return (SYM ? i * (i + 1) / 2 : i * j) * batch;
   };
+  // 192 x 192, four waves with a SIMD each, where they cover the card in one go and 128 x 128 in more than one: symmetric 4096^2 pairs 230 us against 280
+  // (128 x 128: 528 tiles for 512 places) and 287 (256 x 256: 136 tiles), single 95 against 117 and 114.
+  if (tiles(128) > 2 * ctx->cus && tiles(192) <= ctx->cus) return ns_product_tile<KIND, T, Tile<MODE, 192, 192, 2, 2, 3>, MODE, 192>(ctx, g, batch, st);
   switch (tile_kind(ctx, tiles, (g.K + (MODE == MODE_F16 ? 63 : 31)) / (MODE == MODE_F16 ? 64 : 32))) {
     case TILE_256: return ns_product_tile<KIND, T, Tile<MODE, 256, 256, 2, 4, 2>, MODE, 256>(ctx, g, batch, st);
     case TILE_128: return ns_product_tile<KIND, T, Tile<MODE, 128, 128, 2, 2, 2>, MODE, 128>(ctx, g, batch, st);

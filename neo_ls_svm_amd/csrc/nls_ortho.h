@@ -320,9 +320,16 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
   const int last = z.last;
   const char* E = g.E + off;
   constexpr bool PAIRS = MODE == MODE_F16PAIR;
-  constexpr int ACROSS = BI / 8, ROWS = TL::THREADS / ACROSS, TURNS = TL::CHUNK / ROWS;
-  const int iw = threadIdx.x % ACROSS * 8, i = i0 + iw;
-  auto addend = [&](int j, f16x8* h, f16x8* o) {  // eight elements of E; rows are padded: whole groups of eight, zeros behind the end
+  // A chunk's groups of eight elements, TURNS a thread: row r, words iw .. iw + 7
+  constexpr int ACROSS = BI / 8, TURNS = TL::CHUNK * ACROSS / TL::THREADS;
+  static_assert(TURNS * TL::THREADS == TL::CHUNK * ACROSS, "chunks must divide over the threads");
+  auto place = [&](int u, int* r, int* iw) {
+    const bool straight = TL::THREADS % ACROSS == 0;  // (iw is the same in all turns)
+    const int at = straight ? threadIdx.x : threadIdx.x + u * TL::THREADS;
+    *r = at / ACROSS + (straight ? u * (TL::THREADS / ACROSS) : 0);
+    *iw = at % ACROSS * 8;
+  };
+  auto addend = [&](int i, int j, f16x8* h, f16x8* o) {  // eight elements of E; rows are padded: whole groups of eight, zeros behind the end
     *h = *o = f16x8{};
     if (j < g.J && (size_t)i * 4 < ldi) {
       const char* at = E + pair_at(j, i, ldi, PAIRS);
@@ -335,7 +342,11 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
   f16x8 eh[EARLY ? TURNS : 1], el[EARLY ? TURNS : 1];
   if constexpr (EARLY) {
 #pragma unroll
-    for (int u = 0; u < TURNS; ++u) addend(j0 + TL::column(0, threadIdx.x / ACROSS + u * ROWS), &eh[u], &el[u]);
+    for (int u = 0; u < TURNS; ++u) {
+      int r, iw;
+      place(u, &r, &iw);
+      addend(i0 + iw, j0 + TL::column(0, r), &eh[u], &el[u]);
+    }
   }
   TL t;
   const int per = MODE == MODE_F16 ? 64 : 32;
@@ -360,7 +371,9 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
     __syncthreads();
 #pragma unroll EARLY ? TURNS : 1
     for (int u = 0; u < TURNS; ++u) {
-      const int r = threadIdx.x / ACROSS + u * ROWS, j = j0 + TL::column(c, r);
+      int r, iw;
+      place(u, &r, &iw);
+      const int i = i0 + iw, j = j0 + TL::column(c, r);
       float v[8];
       chunk_sums<TL, 8>(lds, r, iw, v);
       f16x8 h = {}, o = {};
@@ -368,7 +381,7 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
         h = eh[u];
         o = el[u];
       } else if (KIND != NS_GRAM) {
-        addend(j, &h, &o);
+        addend(i, j, &h, &o);
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {

@@ -165,27 +165,62 @@ struct Tile {
   __device__ __forceinline__ static void arrive() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
   }
+  // Waves with many blocks have the first fragments of a step in registers when the last products of the step before begin: the reads behind the
+  // barrier are then off the matrix cores' path.  (256 x 256, int8 8192^3: 499 us against 520 .. 541, 8192 x 8192 x 2048 176 / 183, K = 512 92 / 90; fp16
+  // symmetric 4096^2 114 / 145.  128 x 128 with eight waves, two workgroups' worth of waves to fill the gaps: pairs 2048^2 52 against 47.5.)
+  static constexpr bool AHEAD = MI * MJ >= 8;
   // steps >= 1 K steps; last_valid: valid bytes of the last one (128: whole).
-  // STAGES - 1 steps are under way at any time; one barrier a step: behind it step t is there and the buffer of step t - 1 is free.
+  // STAGES - 1 steps are under way at any time; one barrier a step: behind it the next step is there and a buffer that all have read is free.
   __device__ __forceinline__ void run(const Operand& P, int i0, const Operand& Q, int j0, int steps, int last_valid, char* lds) {
     start(P, i0, Q, j0);
     const char* p = P.base + (size_t)i0 * P.ld;
     const char* q = Q.base + (size_t)j0 * Q.ld;
-    const int first = min(STAGES - 1, steps);
-    for (int t = 0; t < first; ++t) fetch(p + step_at<MODE>(t), q + step_at<MODE>(t), lds + t * BUF, t + 1 == steps ? last_valid : 128);
-    int now = 0, next = (STAGES - 1) * BUF;
-    for (int t = 0; t < steps - 1; ++t) {
-      if (t + STAGES - 1 <= steps)
-        arrive<FLIGHT>();
+    auto move = [&](int t, char* buf) { fetch(p + step_at<MODE>(t), q + step_at<MODE>(t), buf, t + 1 == steps ? last_valid : 128); };
+    constexpr int FIRST = AHEAD ? STAGES : STAGES - 1;
+    for (int t = 0; t < min(FIRST, steps); ++t) move(t, lds + t * BUF);
+    int now = 0;
+    if constexpr (AHEAD) {
+      const int wi = wave_id() / WJ, wj = wave_id() % WJ, l = lane_id();
+      const int at_p = (wi * MI * 32 + (l & 31)) * 128, at_q = BI * 128 + (wj * MJ * 32 + (l & 31)) * 128;
+      if (steps >= STAGES)
+        arrive<FLIGHT + LOADS_P + LOADS_Q>();
       else
         arrive<0>();
-      const int ahead = t + STAGES - 1;
-      if (ahead < steps) fetch(p + step_at<MODE>(ahead), q + step_at<MODE>(ahead), lds + next, ahead + 1 == steps ? last_valid : 128);
-      multiply<false>(lds + now, 128);
-      now = now + BUF == LDS ? 0 : now + BUF;
-      next = next + BUF == LDS ? 0 : next + BUF;
+      Frags<MODE, MI, MJ> f;
+      f.template read<false>(0, lds + at_p, lds + at_q, 128);
+      for (int t = 0; t < steps - 1; ++t) {
+        const int next = now + BUF == LDS ? 0 : now + BUF;
+#pragma unroll
+        for (int s = 0; s < f.SUB; ++s) {
+          if (s + 1 < f.SUB) {
+            f.template read<false>(s + 1, lds + now + at_p, lds + now + at_q, 128);
+          } else {  // all of step t is in registers
+            if (t + STAGES <= steps)
+              arrive<FLIGHT>();
+            else
+              arrive<0>();
+            if (t + STAGES < steps) move(t + STAGES, lds + now);
+            f.template read<false>(0, lds + next + at_p, lds + next + at_q, 128);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+          f.multiply(s, acc);
+        }
+        now = next;
+      }
+    } else {
+      int next = (STAGES - 1) * BUF;
+      for (int t = 0; t < steps - 1; ++t) {
+        if (t + STAGES - 1 <= steps)
+          arrive<FLIGHT>();
+        else
+          arrive<0>();
+        if (t + STAGES - 1 < steps) move(t + STAGES - 1, lds + next);
+        multiply<false>(lds + now, 128);
+        now = now + BUF == LDS ? 0 : now + BUF;
+        next = next + BUF == LDS ? 0 : next + BUF;
+      }
+      arrive<0>();
     }
-    arrive<0>();
     multiply<MODE == MODE_I8>(lds + now, last_valid);  // (masked whether ragged or not: two ways to the accumulators' end would double their registers)
   }
   // The epilogue goes through LDS: column block b of every wave at a time, CHUNK columns of the tile as rows of PITCH words, i along the row.
