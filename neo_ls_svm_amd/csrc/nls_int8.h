@@ -124,7 +124,7 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const T* x, long rows, lo
   using F = Few<T, VEC>;
   constexpr int N = F::N;
   const int g = threadIdx.x % G;
-  const long row = (long)blockIdx.x * (256 / G) + threadIdx.x / G;
+  const long row = group_id() * (256 / G) + threadIdx.x / G;
   const bool live = row < rows;
   const T* xr = x + (live ? row : rows - 1) * row_stride;
   unsigned top = 0;
@@ -313,7 +313,8 @@ __global__ __launch_bounds__(512) void k_int8_few(Int8Args g, FewX f) {
   extern __shared__ char lds[];
   const int l = (int)(threadIdx.x & 63), w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int row = l & 15, quarter = l >> 4;
-  const int n0 = blockIdx.x * 16 * NG;
+  if (group_id() * 16 * NG >= g.n) return;
+  const int n0 = (int)group_id() * 16 * NG;
   const int blocks = (g.k + 63) / 64;
   const char* pb[NG];
 #pragma unroll

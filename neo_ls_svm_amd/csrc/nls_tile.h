@@ -327,6 +327,11 @@ __device__ __forceinline__ void chunk_sums(const char* lds, int r, int i, V (&v)
     for (int e = 0; e < N; ++e) v[e] += ((const V*)lds)[(o * TL::CHUNK + r) * TL::PITCH + i + e];
 }
 
+// Workgroups of a launch in two dimensions: threads of one dimension are counted in 32 bits.
+constexpr long GRID_X = 1l << 22;
+inline dim3 grid_of(long groups) { return dim3((unsigned)(groups < GRID_X ? groups : GRID_X), (unsigned)((groups + GRID_X - 1) / GRID_X)); }
+__device__ __forceinline__ long group_id() { return blockIdx.y * GRID_X + blockIdx.x; }
+
 // Tiles in an order that keeps the ones a die works on together: workgroups are dealt to the 8 dies in turn, so die x takes the x-th eighth of the
 // list (bijective for any count), and the list walks strips of `strip` tile rows, so that a die's tiles share operand rows in its L2.
 __device__ __forceinline__ int die_order(int id, int total) {

@@ -29,6 +29,7 @@ __all__ = ["NEWTON_SCHULZ", "quantize_rows", "int8_matmul", "int8_linear", "orth
 NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
 
 MAX_K = 131071  # NLS_INT8_MAX_K
+_MAX_LD = (2**32 - 1) // 512  # the longest way from an 8-bit row to the next that the kernels take
 _A_PADDED, _B_PADDED = 1, 2
 _NAMES = ("float32", "float16", "bfloat16")  # the position is the type's number in the C ABI
 _NAMED = {name: i for i, name in enumerate(_NAMES)}
@@ -116,12 +117,12 @@ class _Tensors:
             if len(shape) == 2 and scale.shape == shape[:1] and 0 < shape[1] <= MAX_K:
                 rows, k = shape
                 ld, dense = x.stride()
-                if dense == 1 and rows > 1 and ld >= k:
+                if dense == 1 and rows > 1 and k <= ld <= _MAX_LD:
                     if not k & 15:
                         return x, scale, shape[:1], rows, k, ld, True
                     up = (k + 15) & -16
                     return x, scale, shape[:1], rows, k, ld, ld >= up and self.room(x) >= (rows - 1) * ld + up
-                if dense == 1 and not k & 15:
+                if dense == 1 and rows == 1 and not k & 15:
                     return x, scale, shape[:1], rows, k, k, True
         return _int8_rows(self, x, what, scale, scale_what)
 
@@ -158,7 +159,7 @@ class _Arrays:
             raise ValueError(f"{what} must be an array like the other arguments, not {type(x).__name__}")
         if not self.host and x.ctx.device != self.ctx.device:
             raise ValueError(f"{what} is on GPU {x.ctx.device}, the context on GPU {self.ctx.device}")
-        return x
+        return x.astype(x.dtype.newbyteorder("=")) if self.host and not x.dtype.isnative else x
 
     def ptr(self, x):
         if isinstance(x, DeviceArray):
@@ -250,6 +251,8 @@ def _space(first, ctx):
             return _Tensors(lib, index, ctx)
         sp = _on_device.get(index)
         if sp is None or sp.ctx is not _default_ctx.get(index):
+            if index not in _default_ctx and lib.cuda.is_current_stream_capturing():
+                raise RuntimeError("a device's first call creates its context, which cannot be done in a graph: call once before the capture")
             with lib.cuda.device(index):  # (the first use of a device creates its context, which makes that device the current one)
                 sp = _on_device[index] = _Tensors(lib, index, default_context(index))
         return sp
@@ -309,7 +312,7 @@ def _int8_rows(sp, x, what, scale, scale_what):
     if not flat and len(shape) != 2:
         x = x.reshape(rows, k)
     st = (k, 1) if flat else sp.strides(x)
-    if (k > 1 and st[1] != 1) or (rows > 1 and st[0] < k):  # columns apart, or rows that share memory
+    if (k > 1 and st[1] != 1) or (rows > 1 and not k <= st[0] <= _MAX_LD):  # columns apart, rows that share memory, or further apart than the kernels count
         x = sp.dense(x)
         st = sp.strides(x)
     if k & 15:

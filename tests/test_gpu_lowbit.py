@@ -169,6 +169,79 @@ def test_int8_matmul(m, n, k, tight):
             product_check(y, a, a_scale, b, b_scale, None if bias is None else host(tbias), name)
 
 
+@pytest.mark.parametrize("m,n,k", [(200, 333, 5001), (1300, 1700, 140), (2300, 2100, 257), (3100, 3100, 700), (3100, 3105, 64), (2500, 4100, 2050)])
+def test_int8_matmul_in_every_tile(m, n, k):
+    rng = np.random.default_rng(m + n + k)
+    a, b = eight_bits(rng, m, k), eight_bits(rng, n, k)
+    a_scale, b_scale = rng.uniform(1e-3, 1e-2, m).astype(np.float32), rng.uniform(1e-3, 1e-2, n).astype(np.float32)
+    ta, tb, tsa, tsb = (torch.tensor(v).cuda() for v in (a, b, a_scale, b_scale))
+    room = torch.full((n, -(-k // 16) * 16 + 16), 99, dtype=torch.int8, device="cuda")
+    room[:, :k] = tb
+    for name in ("float32", "bfloat16"):
+        y = nls.int8_matmul(ta, tsa, tb, tsb, dtype=name)
+        product_check(y, a, a_scale, b, b_scale, None, name)
+        assert torch.equal(nls.int8_matmul(ta, tsa, room[:, :k], tsb, dtype=name), y)
+
+
+@pytest.mark.parametrize("m", [2, 4, 16, 33, 48])
+@pytest.mark.parametrize("k", [40, 63, 1000, 4097])
+def test_few_rows_from_any_address(m, k):
+    """Rows of a and b that start anywhere and end where their memory ends."""
+    rng = np.random.default_rng(m + k)
+    n = 70
+    a, b = eight_bits(rng, m, k), eight_bits(rng, n, k)
+    a_scale, b_scale = rng.uniform(1e-3, 1e-2, m).astype(np.float32), rng.uniform(1e-3, 1e-2, n).astype(np.float32)
+    tsa, tsb = torch.tensor(a_scale).cuda(), torch.tensor(b_scale).cuda()
+    x = torch.tensor(activations(rng, m, k), dtype=torch.float32).cuda().half()
+    q, scale = quantize_oracle(host(x))
+    for off in (0, 1, 7):
+
+        def held(v):
+            flat = torch.empty(v.size + off, dtype=torch.int8, device="cuda")
+            flat[off:] = torch.tensor(v.ravel()).cuda()
+            return flat[off:].view(v.shape)
+
+        product_check(nls.int8_matmul(held(a), tsa, held(b), tsb), a, a_scale, b, b_scale, None, "float32")
+        product_check(nls.int8_linear(x, held(b), tsb), q, scale, b, b_scale, None, "float16")
+
+
+def test_rows_with_a_nan_or_an_infinity_spoil_their_results_only():
+    for m, k in ((1, 512), (3, 100), (20, 300), (130, 300)):
+        x = torch.randn(m, k, device="cuda", generator=torch.Generator("cuda").manual_seed(m))
+        q, s = nls.quantize_rows(torch.randn(90, k, device="cuda", generator=torch.Generator("cuda").manual_seed(k)))
+        want = nls.int8_linear(x, q, s)
+        for bad in (float("nan"), float("inf"), -float("inf")):
+            y = x.clone()
+            y[m // 2, k - 1] = bad
+            got = nls.int8_linear(y, q, s)
+            assert torch.isnan(got[m // 2]).all()
+            got[m // 2] = want[m // 2]
+            assert torch.equal(got, want)
+
+
+def test_more_rows_than_one_dimension_of_a_launch_counts():
+    rows = 2**26 + 5
+    value = torch.arange(rows, device="cuda") % 2001 - 1000
+    x = value.half().view(rows, 1)
+    q, scale = nls.quantize_rows(x)
+    want = torch.tensor(np.arange(1001, dtype=np.float32) / np.float32(127)).cuda()  # (torch divides by a number as a product with its inverse)
+    assert torch.equal(q[:, 0].float(), torch.sign(x[:, 0]).float() * 127) and torch.equal(scale, want[value.abs()])
+    del q, scale, x, value
+    n = 2**27 + 40
+    b = (torch.arange(n, device="cuda") % 255 - 127).to(torch.int8).view(n, 1).expand(n, 16).contiguous()
+    y = nls.int8_matmul(torch.ones(1, 16, dtype=torch.int8, device="cuda"), torch.ones(1, device="cuda"), b, torch.ones(n, device="cuda"), dtype="float16")
+    assert torch.equal(y[0], (16 * b[:, 0].to(torch.int16)).half())
+
+
+def test_rows_further_apart_than_the_kernels_count():
+    rng = np.random.default_rng(0)
+    a, b = eight_bits(rng, 3, 32), eight_bits(rng, 20, 32)
+    far = torch.zeros(3, 9_000_000, dtype=torch.int8, device="cuda")
+    far[:, :32] = torch.tensor(a).cuda()
+    one, many = torch.ones(3, device="cuda"), torch.ones(20, device="cuda")
+    product_check(nls.int8_matmul(far[:, :32], one, torch.tensor(b).cuda(), many), a, np.ones(3, np.float32), b, np.ones(20, np.float32), None, "float32")
+
+
 def test_int8_matmul_sums_to_the_end_of_32_bits():
     k = 131071
     a = torch.full((2, k), -128, dtype=torch.int8, device="cuda")
@@ -200,6 +273,8 @@ def test_int8_matmul_views_and_leading_axes():
     assert one.shape == (40,) and torch.equal(one, want[5])
     same = ta[3:4].expand(24, 96)
     assert torch.equal(nls.int8_matmul(same, tsa[3:4].expand(24), tb, tsb), want[3:4].expand(24, 40))
+    assert torch.equal(nls.int8_matmul(same, tsa[3:4].expand(24).contiguous(), tb, tsb), want[3:4].expand(24, 40))
+    assert torch.equal(nls.int8_matmul(tb[:0], tsb[:0], tb, tsb), want[:0])
 
 
 @pytest.mark.parametrize("name", sorted(DTYPES))
@@ -256,6 +331,25 @@ def test_orthogonalize_batches(batch, m, n):
     assert torch.equal(nls.orthogonalize(t.view(1, batch, m, n))[0], out)
 
 
+@pytest.mark.parametrize("name", sorted(DTYPES))
+@pytest.mark.parametrize("batch,m,n", [(25, 700, 720), (8, 690, 700), (5, 700, 700), (3, 1000, 130)])
+def test_orthogonalize_in_every_tile(batch, m, n, name):
+    rng = np.random.default_rng(batch)
+    g = torch.tensor(np.stack([gradient(rng, m, n)] * 2), dtype=torch.float32)
+    g[1] *= 1e-3
+    t = torch.stack([g[i % 2] for i in range(batch)]).to(DTYPES[name]).cuda()
+    out = nls.orthogonalize(t)
+    for i in range(2):
+        newton_schulz_check(out[i], host(t[i]), nls.NEWTON_SCHULZ, 5, 1e-7, name, i)
+        assert all(torch.equal(out[j], out[i]) for j in range(i, batch, 2))
+
+
+@pytest.mark.parametrize("m,n", [(40, 50), (100, 900), (150, 140)])
+def test_orthogonalize_as_many_steps_as_there_may_be(m, n):
+    g = torch.tensor(gradient(np.random.default_rng(m), m, n), dtype=torch.float32).cuda()
+    newton_schulz_check(nls.orthogonalize(g, steps=32, coefficients=CUBIC), host(g), CUBIC, 32, 1e-7, "float32", m)
+
+
 @pytest.mark.parametrize("steps,coefficients", [(1, nls.NEWTON_SCHULZ), (2, CUBIC), (9, CUBIC), (8, [nls.NEWTON_SCHULZ] * 5 + [(1.875, -1.25, 0.375)] * 3), (3, (0.5, 0.0, 0.0)), (4, (-1.5, 0.5, 0.0)), (12, nls.NEWTON_SCHULZ)])
 @pytest.mark.parametrize("name", sorted(DTYPES))
 def test_orthogonalize_polynomials(steps, coefficients, name):
@@ -307,6 +401,8 @@ def test_arrays_of_the_framework():
     assert np.array_equal(nls.int8_linear(x, hq, hs), y.cpu().numpy())
     assert np.array_equal(nls.int8_matmul(xq, xs, hq, hs), y.cpu().numpy())
     assert np.array_equal(nls.orthogonalize(w), o.cpu().numpy())
+    assert np.array_equal(nls.orthogonalize(w.astype(">f4")), o.cpu().numpy())
+    assert np.array_equal(nls.int8_linear(x.astype(">f4"), hq, hs.astype(">f4")), y.cpu().numpy())
     assert np.array_equal(nls.int8_linear(x.astype(np.float16), hq, hs), nls.int8_linear(torch.tensor(x).half().cuda(), q, s).cpu().numpy())
     ctx = nls.default_context()
     dx, dw = ctx.to_device(x, dtype=np.float32), ctx.to_device(w, dtype=np.float32)
@@ -356,6 +452,88 @@ def test_streams_graphs_and_repeats():
         for out, w in zip(outs, want):
             assert all(torch.equal(t, u) for t, u in zip(out, w)), turn
         assert all(torch.equal(t, u) for t, u in zip(passes(*data[0]), want[0]))
+
+
+def test_threads_with_streams_of_their_own():
+    import threading
+
+    rng = np.random.default_rng(5)
+    data = []
+    for m, n, k in ((3, 128, 200), (70, 256, 320), (300, 64, 96)):
+        x = torch.tensor(activations(rng, m, k), dtype=torch.float32).cuda().half()
+        q, s = nls.quantize_rows(torch.tensor(rng.standard_normal((n, k)), dtype=torch.float32).cuda())
+        data.append((x, q, s, nls.int8_linear(x, q, s), nls.orthogonalize(x)))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(x, q, s, want, ortho):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                y, o = nls.int8_linear(x, q, s), nls.orthogonalize(x)
+                torch.cuda.current_stream().synchronize()
+                if not (torch.equal(y, want) and torch.equal(o, ortho)):
+                    wrong.append(x.shape)
+
+    threads = [threading.Thread(target=work, args=d) for d in data]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+def test_a_context_is_not_made_in_a_capture(monkeypatch):
+    from neo_ls_svm_amd import lowbit
+
+    x = torch.ones(4, 32, device="cuda")
+    nls.quantize_rows(x)
+    with monkeypatch.context() as patch:
+        patch.setattr(lowbit, "_default_ctx", {})
+        patch.setattr(lowbit, "_on_device", {})
+        with pytest.raises(RuntimeError, match="before the capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                x.add_(1.0)
+                nls.quantize_rows(x)
+    assert nls.quantize_rows(x)[0].shape == (4, 32)
+
+
+def test_arguments_the_c_calls_refuse():
+    """What the Python entry points never pass: workspaces, types, strides and sizes that are checked before anything is launched."""
+    import ctypes as C
+
+    ctx = nls.default_context()
+    x, q, s, y = torch.ones(64, 48, device="cuda"), torch.ones(64, 48, dtype=torch.int8, device="cuda"), torch.ones(64, device="cuda"), torch.zeros(64, 64, device="cuda")
+    ws = torch.zeros(1 << 22, dtype=torch.uint8, device="cuda")
+    lib, h, p = ctx.lib, ctx.handle, torch.Tensor.data_ptr
+    table = (C.c_double * 3)(1.5, -0.5, 0.0)
+    need = C.c_size_t()
+
+    def refused(rc, text):
+        with pytest.raises(ValueError, match=text):
+            ctx._check(rc)
+
+    refused(lib.nls_quantize_rows(h, p(x), 7, 64, 48, 48, 1, p(q), 48, p(s), None), "type")
+    refused(lib.nls_quantize_rows(h, p(x), 0, 64, 40, 48, 1, p(q), 40, p(s), None), "multiples of 16")
+    refused(lib.nls_quantize_rows(h, p(x), 0, 64, 48, 48, 1, p(q) + 1, 48, p(s), None), "multiples of 16")
+    refused(lib.nls_quantize_rows(h, None, 0, 64, 48, 48, 1, p(q), 48, p(s), None), "null")
+    matmul = lambda lda, n_ws, at=0, bias_type=0, m=64: lib.nls_int8_matmul(  # noqa: E731
+        h, p(q), lda, p(s), p(q), 48, p(s), p(s), bias_type, m, 64, 47, p(y), 0, 0, p(ws) + at, n_ws, None
+    )
+    assert lib.nls_int8_matmul_workspace(p(q), 48, p(q), 48, 64, 64, 47, 0, C.byref(need)) == 0 and need.value == 2 * 64 * 48
+    refused(matmul(48, need.value - 1), "workspace of")
+    refused(matmul(48, need.value, at=16), "aligned")
+    refused(matmul(40, need.value), "row strides")
+    refused(matmul(48, need.value, bias_type=1), "bias")
+    refused(matmul(48, need.value, m=-1), "negative")
+    assert matmul(48, need.value) == 0
+    lib.nls_orthogonalize_workspace(1, 200, 200, 200, 1, C.byref(need))
+    ortho = lambda m, batch, n_ws, steps=1: lib.nls_orthogonalize(h, p(ws), 0, batch, m, 200, m * 200, 200, 1, table, steps, 1e-7, p(ws), p(ws), n_ws, None)  # noqa: E731
+    refused(ortho(200, 1, need.value - 1), "workspace of")
+    refused(ortho(2**20 + 1, 1, need.value), "2\\^20")
+    refused(ortho(200, 65536, need.value), "65535")
+    refused(ortho(200, 1, need.value, steps=0), "steps")
+    torch.cuda.synchronize()
+    assert torch.equal(y, torch.full_like(y, 48.0))  # (47 products and a bias of one)
 
 
 def test_gradients_are_refused_not_lost():

@@ -79,3 +79,11 @@ def test_sixty_four_bits_decide_a_quotient_next_to_a_half():
         r = Fraction(float(xi)) * 127 / Fraction(float(ti))
         assert round(r) == int(wi)  # (Fraction rounds ties to even)
         assert abs(Fraction(float(fi)) - r) < Fraction(2, 100000)
+
+
+def test_arrays_of_the_other_byte_order_are_turned():
+    from neo_ls_svm_amd import lowbit
+
+    other = X.dtype.newbyteorder()
+    turned = lowbit._Arrays(X, None).take(X.astype(other), "x")
+    assert turned.dtype == np.float32 and turned.dtype.isnative and np.array_equal(turned, X)
