@@ -102,7 +102,7 @@ int quantize_any(nls_ctx* ctx, const void* x, int type, long rows, long k, long 
 template <class T, class TL, int BI, int BJ>
 int int8_tile(nls_ctx* ctx, const Int8Args& g, hipStream_t st) {
   const int ti = (g.n + BI - 1) / BI, tj = (g.m + BJ - 1) / BJ;
-  constexpr int LDS = std::max(TL::LDS, TL::SCRATCH);
+  constexpr int LDS = tile_bytes<TL>() + BJ * 4;
   NLSCHK((ask_lds<&k_int8_tile<T, TL, BI, BJ>>(ctx, LDS)));
   k_int8_tile<T, TL, BI, BJ><<<dim3((unsigned)((long)ti * tj)), TL::THREADS, LDS, st>>>(g, ti, tj, 8);
   LAUNCHED(ctx, "int8_matmul");

@@ -337,17 +337,21 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
       if (KIND != NS_POLY || PAIRS) *o = *(const f16x8*)(at + pair_lo(PAIRS));
     }
   };
-  // Small tiles fetch what the epilogue adds before the product: for small matrices every launch is a chain of misses, this one is then off it.
+  // What the epilogue adds is fetched in batches: for tiles of one chunk before the product, else before the chunk goes to LDS, four turns at a time.
+  // (A fetch a turn, each waited for, was 5 .. 10 us of a product.)
   constexpr bool EARLY = KIND != NS_GRAM && TL::CHUNKS == 1 && TURNS <= 2;
-  f16x8 eh[EARLY ? TURNS : 1], el[EARLY ? TURNS : 1];
-  if constexpr (EARLY) {
+  constexpr int BATCH = TURNS % 4 == 0 ? 4 : TURNS % 3 == 0 ? 3 : TURNS;
+  f16x8 eh[BATCH], el[BATCH];
+  auto batch = [&](int c, int u0) {
+    if (KIND == NS_GRAM) return;
 #pragma unroll
-    for (int u = 0; u < TURNS; ++u) {
+    for (int u = 0; u < BATCH; ++u) {
       int r, iw;
-      place(u, &r, &iw);
-      addend(i0 + iw, j0 + TL::column(0, r), &eh[u], &el[u]);
+      place(u0 + u, &r, &iw);
+      addend(i0 + iw, j0 + TL::column(c, r), &eh[u], &el[u]);
     }
-  }
+  };
+  if constexpr (EARLY) batch(0, 0);
   TL t;
   const int per = MODE == MODE_F16 ? 64 : 32;
   t.run(Operand{g.P + off, (unsigned)ldk, g.I}, i0, Operand{g.Q + off, (unsigned)ldk, g.J}, j0, (g.K + per - 1) / per, 128, lds);
@@ -366,26 +370,23 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
   const int iv = threadIdx.x / DOWN, rv = threadIdx.x % DOWN * 8;
 #pragma unroll
   for (int c = 0; c < TL::CHUNKS; ++c) {
+    if constexpr (!EARLY) batch(c, 0);
     __syncthreads();
     t.spill(c, lds);
     __syncthreads();
-#pragma unroll EARLY ? TURNS : 1
-    for (int u = 0; u < TURNS; ++u) {
+#pragma unroll 1
+    for (int u0 = 0; u0 < TURNS; u0 += BATCH) {
+    if (u0) batch(c, u0);
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
       int r, iw;
-      place(u, &r, &iw);
+      place(u0 + u, &r, &iw);
       const int i = i0 + iw, j = j0 + TL::column(c, r);
       float v[8];
       chunk_sums<TL, 8>(lds, r, iw, v);
-      f16x8 h = {}, o = {};
-      if constexpr (EARLY) {
-        h = eh[u];
-        o = el[u];
-      } else if (KIND != NS_GRAM) {
-        addend(i, j, &h, &o);
-      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float x = (float)h[e] + (float)o[e];
+        const float x = KIND == NS_GRAM ? 0.0f : (float)eh[u][e] + (float)el[u][e];
         float w = v[e];
         if (KIND == NS_GRAM) w = f.gram * w;
         if (KIND == NS_POLY) w = f.lin * x + f.quad * w;
@@ -401,6 +402,7 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
       } else if (natural && j < g.J && i < g.I) {
         store_some<T, 8>(out + (size_t)j * g.I + i, v, g.I - i);
       }
+    }
     }
     if (turned) {
       __syncthreads();
