@@ -204,10 +204,6 @@ __device__ __forceinline__ float bias_at(const Int8Args& g, int n) {
 __device__ __forceinline__ float scaled(int sum, float as, float bs, float bias) { return (float)sum * as * bs + bias; }
 
 // Many rows: P = b (its rows lie along a chunk's words, as neighbours in a row of y), Q = a.
-template <class TL>
-__host__ __device__ constexpr int tile_bytes() {
-  return TL::LDS > TL::SCRATCH ? TL::LDS : TL::SCRATCH;
-}
 // A thread writes 16 bytes of a row of y at once, wherever the row starts (a store may begin at any element), and has the same channels in all its rows.
 template <class T, class TL, int BI, int BJ>
 __global__ __launch_bounds__(TL::THREADS) void k_int8_tile(Int8Args g, int ti, int tj, int strip) {
@@ -217,11 +213,11 @@ __global__ __launch_bounds__(TL::THREADS) void k_int8_tile(Int8Args g, int ti, i
   strip_order(die_order(blockIdx.x, ti * tj), ti, tj, strip, &bi, &bj);
   const int i0 = bi * BI, j0 = bj * BJ;
   // What the epilogue needs is on its way before the product begins: a_scale to LDS behind the tile, b_scale and the bias to registers.
-  constexpr int ACROSS = BI / N, ROWS = TL::THREADS / ACROSS, TURNS = TL::CHUNK / ROWS;
-  static_assert(TURNS * ROWS == TL::CHUNK, "chunks must divide over the threads");
+  constexpr int ACROSS = TL::W / N, STEP = TL::TEAM / ACROSS, TURNS = TL::ROWS / STEP;
+  static_assert(STEP * ACROSS == TL::TEAM && TURNS * STEP == TL::ROWS, "chunks must divide over the threads");
   float* a_scale = (float*)(lds + tile_bytes<TL>());
   for (int r = threadIdx.x; r < BJ; r += TL::THREADS) a_scale[r] = g.a_scale[min(j0 + r, g.m - 1)];
-  const int iw = threadIdx.x % ACROSS * N, n = i0 + iw, left = g.n - n;
+  const int iw = TL::who() % ACROSS * N, n = i0 + TL::row0() + iw, left = g.n - n;
   float bs[N], bias[N];
 #pragma unroll
   for (int e = 0; e < N; ++e) {
@@ -232,17 +228,17 @@ __global__ __launch_bounds__(TL::THREADS) void k_int8_tile(Int8Args g, int ti, i
   const int steps = (g.k + 127) / 128;
   t.run(g.b, i0, g.a, j0, steps, g.k - (steps - 1) * 128, lds);
   T* y = (T*)g.y;
+  char* mine = TL::part(lds);
+  __syncthreads();
 #pragma unroll
   for (int c = 0; c < TL::CHUNKS; ++c) {
-    __syncthreads();
-    t.spill(c, lds);
-    __syncthreads();
+    t.spill(c, mine);
 #pragma unroll 4
     for (int u = 0; u < TURNS; ++u) {
-      const int r = threadIdx.x / ACROSS + u * ROWS, j = TL::column(c, r), m = j0 + j;
+      const int r = TL::who() / ACROSS + u * STEP, j = TL::column0(c) + r, m = j0 + j;
       if (m >= g.m || left <= 0) continue;
       int s[N];
-      chunk_sums<TL, N>(lds, r, iw, s);
+      chunk_sums<TL, N>(mine, r, iw, s);
       const float as = a_scale[j];
       float v[N];
 #pragma unroll

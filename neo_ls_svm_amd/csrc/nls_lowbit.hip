@@ -221,7 +221,7 @@ int ns_parts(const NsMatrix& w) { return (int)std::min<long>(NS_PARTS, ((w.col_s
 struct NsPlan {
   NsPath path;
   long p, q;
-  size_t x, xt, a, parts, scales, batch_bytes, total;
+  size_t x, xt, a, parts, scales, batch_bytes, total;  // (NS_TILES: two X, two X^T, A and B a matrix)
 };
 NsPlan ns_slab_plan(long p, long q, long batch) {
   NsPlan w{};
@@ -246,7 +246,7 @@ NsPlan ns_plan(long m, long n, long batch, long row_stride, long col_stride) {
   w.x = (size_t)w.p * pair_ld(w.q);
   w.xt = (size_t)w.q * pair_ld(w.p);
   w.a = (size_t)w.p * pair_ld(w.p);
-  w.batch_bytes = w.x + 2 * w.xt + 2 * w.a;
+  w.batch_bytes = 2 * w.x + 2 * w.xt + 2 * w.a;
   w.parts = up256((size_t)batch * NS_PARTS * sizeof(double));
   w.scales = up256((size_t)batch * sizeof(NsScales));
   w.total = w.parts + w.scales + (size_t)batch * w.batch_bytes;
@@ -259,7 +259,7 @@ int ns_product_tile(nls_ctx* ctx, NsArgs g, long batch, hipStream_t st) {
   g.tj = (g.J + B - 1) / B;
   g.strip = 8;
   constexpr bool SYM = KIND == NS_GRAM || KIND == NS_POLY;
-  constexpr int LDS = std::max(TL::LDS, TL::SCRATCH);
+  constexpr int LDS = tile_bytes<TL>();
   const long tiles = SYM ? (long)g.ti * (g.ti + 1) / 2 : (long)g.ti * g.tj;
   NLSCHK((ask_lds<&k_ns_product<KIND, T, TL, MODE, B, B>>(ctx, LDS)));
   k_ns_product<KIND, T, TL, MODE, B, B><<<dim3((unsigned)tiles, 1, (unsigned)batch), TL::THREADS, LDS, st>>>(g);
@@ -390,7 +390,7 @@ int orthogonalize(nls_ctx* ctx, const NsMatrix& w, const NsPlan& plan, bool tall
   double* parts = (double*)ws;
   NsScales* scales = (NsScales*)(ws + plan.parts);
   char* base = ws + plan.parts + plan.scales;
-  char *X = base, *XT = X + plan.x, *XU = XT + plan.xt, *A = XU + plan.xt, *B = A + plan.a;
+  char *X = base, *XV = X + plan.x, *XT = XV + plan.x, *XU = XT + plan.xt, *A = XU + plan.xt, *B = A + plan.a;
   const int count = ns_parts(w);
   k_ns_norm<T><<<dim3(count, (unsigned)batch), 256, 0, st>>>(w, parts);
   k_ns_pack<T><<<dim3((unsigned)((w.q + 63) / 64), (unsigned)((w.p + 63) / 64), (unsigned)batch), 256, 0, st>>>(w, parts, count, eps, cf, steps, scales, X, XT,
@@ -417,9 +417,10 @@ int orthogonalize(nls_ctx* ctx, const NsMatrix& w, const NsPlan& plan, bool tall
     g.E = X;
     g.I = q;
     if (t + 1 < steps) {
+      g.next_pairs = t + 1 >= steps - exact;
+      if (g.next_pairs != pairs) std::swap(X, XV);  // X stays where it is - a thread reads what it writes - but where its layout changes
       g.D = X;
       g.DT = XU;
-      g.next_pairs = t + 1 >= steps - exact;
       NLSCHK((ns_product<NS_STEP, float>(ctx, g, pairs, batch, st)));
       std::swap(XT, XU);
     } else {

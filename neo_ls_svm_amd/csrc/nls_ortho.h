@@ -321,12 +321,12 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
   const char* E = g.E + off;
   constexpr bool PAIRS = MODE == MODE_F16PAIR;
   // A chunk's groups of eight elements, TURNS a thread: row r, words iw .. iw + 7
-  constexpr int ACROSS = BI / 8, TURNS = TL::CHUNK * ACROSS / TL::THREADS;
-  static_assert(TURNS * TL::THREADS == TL::CHUNK * ACROSS, "chunks must divide over the threads");
+  constexpr int ACROSS = TL::W / 8, TURNS = TL::ROWS * ACROSS / TL::TEAM;
+  static_assert(TURNS * TL::TEAM == TL::ROWS * ACROSS, "chunks must divide over the threads");
   auto place = [&](int u, int* r, int* iw) {
-    const bool straight = TL::THREADS % ACROSS == 0;  // (iw is the same in all turns)
-    const int at = straight ? threadIdx.x : threadIdx.x + u * TL::THREADS;
-    *r = at / ACROSS + (straight ? u * (TL::THREADS / ACROSS) : 0);
+    const bool straight = TL::TEAM % ACROSS == 0;  // (iw is the same in all turns)
+    const int at = straight ? TL::who() : TL::who() + u * TL::TEAM;
+    *r = at / ACROSS + (straight ? u * (TL::TEAM / ACROSS) : 0);
     *iw = at % ACROSS * 8;
   };
   auto addend = [&](int i, int j, f16x8* h, f16x8* o) {  // eight elements of E; rows are padded: whole groups of eight, zeros behind the end
@@ -339,7 +339,7 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
   };
   // What the epilogue adds is fetched in batches: for tiles of one chunk before the product, else before the chunk goes to LDS, four turns at a time.
   // (A fetch a turn, each waited for, was 5 .. 10 us of a product.)
-  constexpr bool EARLY = KIND != NS_GRAM && TL::CHUNKS == 1 && TURNS <= 2;
+  constexpr bool EARLY = KIND != NS_GRAM && TL::CHUNKS == 1;
   constexpr int BATCH = TURNS % 4 == 0 ? 4 : TURNS % 3 == 0 ? 3 : TURNS;
   f16x8 eh[BATCH], el[BATCH];
   auto batch = [&](int c, int u0) {
@@ -348,7 +348,7 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
     for (int u = 0; u < BATCH; ++u) {
       int r, iw;
       place(u0 + u, &r, &iw);
-      addend(i0 + iw, j0 + TL::column(c, r), &eh[u], &el[u]);
+      addend(i0 + TL::row0() + iw, j0 + TL::column0(c) + r, &eh[u], &el[u]);
     }
   };
   if constexpr (EARLY) batch(0, 0);
@@ -362,18 +362,15 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
   const bool to_pairs = SYM ? PAIRS : g.next_pairs != 0;  // the products that will read D and DT
   const int lo_d = !SYM || PAIRS ? pair_lo(to_pairs) : 0, lo_t = to_pairs ? pair_lo(true) : 0;
   const bool natural = KIND != NS_LAST || !g.transposed, turned = KIND == NS_LAST ? g.transposed != 0 : SYM ? bi != bj : true;
-  // (STEP writes X where it reads it, perhaps in the other layout: the 64 elements that share 256 bytes are eight neighbouring lanes' of one wave,
-  // which have read them all before the first is written.)
   // Chunks of the tile through LDS: the result in the product's own orientation (rows j, eight neighbours i a thread), then, from the values left
   // there, its transpose (rows i, eight neighbours j).
-  constexpr int DOWN = TL::CHUNK / 8;
-  const int iv = threadIdx.x / DOWN, rv = threadIdx.x % DOWN * 8;
+  constexpr int DOWN = TL::ROWS / 8;
+  char* mine = TL::part(lds);
+  __syncthreads();
 #pragma unroll
   for (int c = 0; c < TL::CHUNKS; ++c) {
     if constexpr (!EARLY) batch(c, 0);
-    __syncthreads();
-    t.spill(c, lds);
-    __syncthreads();
+    t.spill(c, mine);
 #pragma unroll 1
     for (int u0 = 0; u0 < TURNS; u0 += BATCH) {
     if (u0) batch(c, u0);
@@ -381,9 +378,9 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
     for (int u = 0; u < BATCH; ++u) {
       int r, iw;
       place(u0 + u, &r, &iw);
-      const int i = i0 + iw, j = j0 + TL::column(c, r);
+      const int i = i0 + TL::row0() + iw, j = j0 + TL::column0(c) + r;
       float v[8];
-      chunk_sums<TL, 8>(lds, r, iw, v);
+      chunk_sums<TL, 8>(mine, r, iw, v);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float x = KIND == NS_GRAM ? 0.0f : (float)eh[u][e] + (float)el[u][e];
@@ -396,7 +393,7 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
       }
       if (turned)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ((float*)lds)[r * TL::PITCH + iw + e] = v[e];
+        for (int e = 0; e < 8; e += 4) *(f32x4*)((float*)mine + r * TL::PITCH + iw + e) = f32x4{v[e], v[e + 1], v[e + 2], v[e + 3]};
       if (KIND != NS_LAST) {
         if (j < g.J && (size_t)i * 4 < ldi) store_pairs(D + pair_at(j, i, ldi, to_pairs), v, lo_d);
       } else if (natural && j < g.J && i < g.I) {
@@ -405,13 +402,14 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
     }
     }
     if (turned) {
-      __syncthreads();
-      for (int ii = iv; ii < BI; ii += TL::THREADS / DOWN) {
-        const int irow = i0 + ii, j = j0 + TL::column(c, rv);
+      TL::settle();
+      for (int at = TL::who(); at < TL::W * DOWN; at += TL::TEAM) {
+        const int ii = at / DOWN, rv = at % DOWN * 8;
+        const int irow = i0 + TL::row0() + ii, j = j0 + TL::column0(c) + rv;
         if (irow >= g.I) continue;
         float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = ((const float*)lds)[(rv + e) * TL::PITCH + ii];
+        for (int e = 0; e < 8; ++e) v[e] = ((const float*)mine)[(rv + e) * TL::PITCH + ii];
         if (KIND != NS_LAST) {
           if ((size_t)j * 4 < ldj) store_pairs(DT + pair_at(irow, j, ldj, to_pairs), v, lo_t);
         } else if (j < g.J) {

@@ -223,21 +223,32 @@ struct Tile {
     }
     multiply<MODE == MODE_I8>(lds + now, last_valid);  // (masked whether ragged or not: two ways to the accumulators' end would double their registers)
   }
-  // The epilogue goes through LDS: column block b of every wave at a time, CHUNK columns of the tile as rows of PITCH words, i along the row.
-  // (PITCH = BI + 1: neighbouring rows and neighbouring words both change the bank, so both orientations are read without conflicts.)
-  static constexpr int CHUNK = 32 * WJ, CHUNKS = MJ, PARTS = 1, PITCH = BI + 1;
-  static constexpr int SCRATCH = CHUNK * PITCH * 4;
-  __device__ __forceinline__ static int column(int chunk, int r) { return ((r >> 5) * MJ + chunk) * 32 + (r & 31); }
-  __device__ __forceinline__ void spill(int chunk, char* lds) const {  // (the chunk's number picks registers: unrolled by the callers)
-    const int wi = wave_id() / WJ, wj = wave_id() % WJ, l = lane_id();
-    int* t = (int*)lds + (wj * 32 + (l & 31)) * PITCH + wi * MI * 32 + 4 * (l >> 5);
+  // The epilogue goes through LDS, every wave for itself: column block c of its results, ROWS columns of the tile as rows of W words (i along the row)
+  // that its 64 lanes read as whole lines.  No barriers but the one in front: the waves' parts overlie the tile's buffers.
+  static constexpr int TEAM = 64, ROWS = 32, CHUNKS = MJ, PARTS = 1, W = 32 * MI, PITCH = W + 4;
+  static constexpr int SCRATCH = WAVES * ROWS * PITCH * 4;
+  __device__ __forceinline__ static int who() { return lane_id(); }
+  __device__ __forceinline__ static char* part(char* lds) { return lds + wave_id() * (ROWS * PITCH * 4); }
+  __device__ __forceinline__ static int row0() { return wave_id() / WJ * W; }
+  __device__ __forceinline__ static int column0(int c) { return (wave_id() % WJ * MJ + c) * 32; }
+  __device__ __forceinline__ static void settle() {  // what the wave wrote is there for the wave (LDS keeps a wave's order; the compiler has to as well)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+  __device__ __forceinline__ void spill(int c, char* mine) const {  // (c picks registers: unrolled by the callers)
+    const int l = lane_id();
+    int* t = (int*)mine + (l & 31) * PITCH + 4 * (l >> 5);
+    settle();
 #pragma unroll
     for (int b = 0; b < MJ; ++b)
-      if (b == chunk)
+      if (b == c)
 #pragma unroll
-        for (int a = 0; a < MI; ++a)
+        for (int a = 0; a < MI; ++a) {
+          const i32x16 v = __builtin_bit_cast(i32x16, acc[a][b]);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) t[a * 32 + 8 * (r >> 2) + (r & 3)] = __builtin_bit_cast(i32x16, acc[a][b])[r];
+          for (int r = 0; r < 16; r += 4) *(i32x4*)(t + a * 32 + 2 * r) = i32x4{v[r], v[r + 1], v[r + 2], v[r + 3]};
+        }
+    settle();
   }
 };
 
@@ -301,30 +312,44 @@ struct Ring {
       now = now + BUF == STAGES * BUF ? 0 : now + BUF;
     }
   }
-  static constexpr int CHUNK = 64, CHUNKS = 1, PARTS = 4, PITCH = 65;
-  static constexpr int SCRATCH = PARTS * CHUNK * PITCH * 4;
-  __device__ __forceinline__ static int column(int, int r) { return r; }
+  static constexpr int TEAM = 256, ROWS = 64, CHUNKS = 1, PARTS = 4, W = 64, PITCH = W + 4;  // the epilogue: all waves together
+  static constexpr int SCRATCH = PARTS * ROWS * PITCH * 4;
+  __device__ __forceinline__ static int who() { return threadIdx.x; }
+  __device__ __forceinline__ static char* part(char* lds) { return lds; }
+  __device__ __forceinline__ static int row0() { return 0; }
+  __device__ __forceinline__ static int column0(int) { return 0; }
+  __device__ __forceinline__ static void settle() { __syncthreads(); }
   __device__ __forceinline__ void spill(int, char* lds) const {
     const int l = lane_id();
-    int* t = (int*)lds + (wave_id() * CHUNK + (l & 31)) * PITCH + 4 * (l >> 5);
+    int* t = (int*)lds + (wave_id() * ROWS + (l & 31)) * PITCH + 4 * (l >> 5);
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int a = 0; a < 2; ++a)
+      for (int a = 0; a < 2; ++a) {
+        const i32x16 v = __builtin_bit_cast(i32x16, acc[a][b]);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) t[b * 32 * PITCH + a * 32 + 8 * (r >> 2) + (r & 3)] = __builtin_bit_cast(i32x16, acc[a][b])[r];
+        for (int r = 0; r < 16; r += 4) *(i32x4*)(t + b * 32 * PITCH + a * 32 + 2 * r) = i32x4{v[r], v[r + 1], v[r + 2], v[r + 3]};
+      }
+    settle();
   }
 };
 
-// Sums of a chunk: row r, words i .. i + N - 1
+template <class TL>
+__host__ __device__ constexpr int tile_bytes() {
+  return TL::LDS > TL::SCRATCH ? TL::LDS : TL::SCRATCH;
+}
+// Sums of a chunk: row r, words i .. i + N - 1 (N and i multiples of four)
 template <class TL, int N, class V>
-__device__ __forceinline__ void chunk_sums(const char* lds, int r, int i, V (&v)[N]) {
+__device__ __forceinline__ void chunk_sums(const char* mine, int r, int i, V (&v)[N]) {
+  typedef V V4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-  for (int e = 0; e < N; ++e) v[e] = ((const V*)lds)[r * TL::PITCH + i + e];
+  for (int e = 0; e < N; e += 4) {
+    V4 s = *(const V4*)((const V*)mine + r * TL::PITCH + i + e);
 #pragma unroll
-  for (int o = 1; o < TL::PARTS; ++o)
+    for (int o = 1; o < TL::PARTS; ++o) s += *(const V4*)((const V*)mine + (o * TL::ROWS + r) * TL::PITCH + i + e);
 #pragma unroll
-    for (int e = 0; e < N; ++e) v[e] += ((const V*)lds)[(o * TL::CHUNK + r) * TL::PITCH + i + e];
+    for (int k = 0; k < 4; ++k) v[e + k] = s[k];
+  }
 }
 
 // Workgroups of a launch in two dimensions: threads of one dimension are counted in 32 bits.
