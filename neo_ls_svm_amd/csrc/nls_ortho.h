@@ -56,24 +56,23 @@ struct NsMatrix {
   long row_stride, col_stride, batch_stride;  // in elements
 };
 
-// Sums of squares, a part a workgroup.  Sixteen bytes a thread and turn along the direction whose neighbours are neighbours in memory, where they are
-// aligned; bound by memory (4096 x 4096 float32 was 103 us with one element a thread and 256 workgroups).
+// Sums of squares, a part a workgroup.  Sixteen bytes a thread and turn along the direction whose neighbours are neighbours in memory, from any element
+// on; bound by memory (4096 x 4096 float32 was 103 us with one element a thread and 256 workgroups).
 template <class T>
 __global__ __launch_bounds__(256) void k_ns_norm(NsMatrix w, double* parts) {
   constexpr int N = 16 / (int)sizeof(T);
-  typedef T V __attribute__((ext_vector_type(N)));
+  typedef T V __attribute__((ext_vector_type(N), aligned(sizeof(T))));
   const T* g = (const T*)w.g + blockIdx.y * w.batch_stride;
   double s[2] = {0.0, 0.0};
   const bool along_q = w.col_stride <= w.row_stride;
   const long outer = along_q ? w.p : w.q, inner = along_q ? w.q : w.p;
   const long os = along_q ? w.row_stride : w.col_stride, is = along_q ? w.col_stride : w.row_stride;
-  const bool whole = is == 1 && (size_t)g % 16 == 0 && (outer == 1 || os % N == 0);
   // 64 threads along a row, four rows at a time
   const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
   for (long o = (long)blockIdx.x * 4 + y; o < outer; o += (long)gridDim.x * 4) {
     const T* row = g + o * os;
     long i = x * N;
-    if (whole)
+    if (is == 1)
 #pragma unroll 4
       for (; i + N <= inner; i += 64 * N) {
         const V v = *(const V*)(row + i);
