@@ -47,12 +47,16 @@ int ask_lds(nls_ctx* ctx, int bytes) {
 int type_size(int t) { return t == NLS_TYPE_F32 ? 4 : (t == NLS_TYPE_F16 || t == NLS_TYPE_BF16) ? 2 : 0; }
 
 // The tile a product is cut into.  Measured (int8 and fp16 products of 300 .. 8192 rows and columns, 10 .. 256 K steps):
-//   256 x 256 (8 waves, two steps held) reads the least and is first once its tiles keep more than half of the compute units busy: 4096^2 pairs 355 us
-//     against 387 with 128 x 128; int8 4096^3 73 / 84;
-//   128 x 128, four waves, two workgroups a unit, when there are more of them than units: 2048 x 8192 pairs 203 us against 218 with eight waves;
-//   128 x 128, eight waves, three steps held, when they cover 0.6 .. 1 of the units: 2048^2 pairs 59 us against 67 (four waves) and 70 (64 x 64);
-//   64 x 64, four waves side by side, three workgroups a unit: more of them than units, or few K steps: 1536^2 symmetric 26 us against 36 (128 x 128);
-//   64 x 64 with the K steps dealt out over the waves otherwise: 512 rows, K = 2048 pairs: 16 us against 23 (side by side) and 44 (128 x 128).
+//   256 x 256 (eight waves, two steps held) reads the least and is first once its tiles keep more than half of the compute units busy: int8
+//     2500 x 4096 x 4096 53 us against 59 with 128 x 128, 8192 x 8192 x 256 55 / 62;
+//   128 x 128, four waves, two workgroups a unit, when there are more of them than units: int8 2047 x 4096 x 4096 41.7 us against 51 with eight waves,
+//     52 (256 x 256) and 57 (64 x 64); 256 x 128 with eight waves 46, with four 53;
+//   128 x 128, eight waves, three steps held, when they cover 0.6 .. 1 of the units: int8 1024 x 4096 x 4096 26.7 us against 27.8 (four waves) and 33
+//     (64 x 64), pairs 2048^2 59 / 66 / 72;
+//   64 x 64, four waves side by side, three workgroups a unit: more of them than units, or few K steps: 1536^2 symmetric pairs 25 us against 34 (128 x 128)
+//     and 27 (K dealt out), int8 512 x 4096 x 4096 18.2 / 25 / 20; more than three steps held 0 .. 10 us slower (fewer workgroups a unit);
+//   64 x 64 with the K steps dealt out over the waves otherwise: X X^T of 512 x 2048 pairs 15.5 us against 22 (side by side) and 42 (128 x 128), int8
+//     256 x 4096 x 4096 11.6 / 14.5 / 24; at 16 steps (512^2 pairs, a whole call) 145 / 148, at 8 (single) 125 / 120.
 enum TileKind { TILE_256, TILE_128, TILE_128_DEEP, TILE_64, TILE_64_RING };
 template <class F>
 TileKind tile_kind(const nls_ctx* ctx, F tiles, int steps) {
@@ -133,8 +137,8 @@ int int8_few(nls_ctx* ctx, const Int8Args& g, const FewX& f, hipStream_t st) {
   if (MG > 1 && (g.n + 31) / 32 >= ctx->cus) return int8_few<T, MG, 2, false>(ctx, g, f, st);
   return int8_few<T, MG, 1, false>(ctx, g, f, st);
 }
-// Few rows of a: fragments straight from memory, or tiles.  Measured: 16 x 4096 x 4096 8.2 us against 11.3 with tiles, 48 x 4096 x 4096 12.4 / 12.8,
-// 64 x 4096 x 4096 14.4 / 13.5; 16 x 8192 x 8192 21 / 21, 48 x 8192 x 8192 28 / 24 (128 tiles keep enough of the card busy).
+// Few rows of a: fragments straight from memory, or tiles.  Measured: 16 x 4096 x 4096 8.4 us against 11.4 with tiles, 48 x 4096 x 4096 12.6 / 12.9,
+// 64 x 4096 x 4096 14.8 / 13.5; 16 x 8192 x 8192 22.1 / 22.4, 32 x 8192 x 8192 25.5 / 23.9, 48 x 8192 x 8192 29 / 25 (128 tiles keep enough of the card busy).
 bool int8_is_few(long m, long n) { return m <= 16 || (m <= 48 && n < 8192); }
 template <class T>
 int int8_product(nls_ctx* ctx, const Int8Args& g, const FewX& f, hipStream_t st) {
@@ -142,9 +146,9 @@ int int8_product(nls_ctx* ctx, const Int8Args& g, const FewX& f, hipStream_t st)
   return int8_tile<T>(ctx, g, st);
 }
 // Whether int8_linear quantises inside the product: every workgroup does all the rows of x over again, which has to stay small beside its share of b.
-// Measured: one row always (1 x 4096 x 4096 8.0 us against 9.8 in two launches, 8192 x 8192 19.1 / 20.8), four of small products (4096 x 4096 11.4 / 10.3 and a
-// launch less to make, 8192 x 8192 28 / 21).
-bool int8_fused(long m, long n, long k) { return m * k <= 32768 && (m <= 2 || (m <= FEW_ROWS && n * k <= 1l << 24)); }
+// Measured, one launch / two: 1 x 4096 x 4096 8.2 / 9.6 us, 1 x 8192 x 8192 18.9 / 20.9; 4 x 4096 x 4096 11.5 / 10.8 (and a launch less to make, which is
+// what a caller waits for there), 2 x 8192 x 8192 23.7 / 21.6, 4 x 8192 x 8192 30.6 / 22.9.
+bool int8_fused(long m, long n, long k) { return m * k <= 32768 && (m == 1 || (m <= FEW_ROWS && n * k <= 1l << 24)); }
 template <class T>
 int int8_fused_product(nls_ctx* ctx, const Int8Args& g, const FewX& f, hipStream_t st) {
   return int8_few<T, 1, 1, true>(ctx, g, f, st);
@@ -161,7 +165,8 @@ long up16(long k) { return (k + 15) / 16 * 16; }
 size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 
 // Rows that the product can read where they are.  Tiles: those that start at multiples of 16 bytes and may be read up to one.  Few rows: any start for up
-// to 16 of them (1 x 4097 x 4099 from odd addresses 10 us), multiples of 16 bytes for more (48 x 4097 x 4099: 43 us from odd addresses, 22 us aligned).
+// to 16 of them (16 x 4097 x 4099 from odd addresses 11 us, aligned 7.6), multiples of 16 bytes for more (48 x 4097 x 4099: 43 us from odd addresses, 22 us
+// with the copy, 13 aligned).
 bool rows_ready(long m, long n, const void* p, long ld, long k, int flags, int flag) {
   const bool aligned = (uintptr_t)p % 16 == 0 && ld % 16 == 0;
   if (int8_is_few(m, n)) return m <= 16 || aligned;
@@ -232,7 +237,7 @@ NsPlan ns_slab_plan(long p, long q, long batch) {
   w.a = slabs * rows * rows * 4;
   w.parts = up256((size_t)batch * NS_PARTS * sizeof(double));
   w.scales = up256((size_t)batch * sizeof(NsScales));
-  w.total = w.parts + w.scales + (size_t)batch * (w.x + w.a);
+  w.total = w.parts + w.scales + (size_t)batch * (w.x + 2 * w.a);
   return w;
 }
 NsPlan ns_plan(long m, long n, long batch, long row_stride, long col_stride) {
@@ -333,24 +338,29 @@ int ns_slabs(nls_ctx* ctx, const NsMatrix& w, bool tall, long batch, const NsCoe
   g.steps = steps;
   g.out = out;
   g.tall = tall;
-  g.slabs = (int)((w.q + NS_SLAB - 1) / NS_SLAB);
+  const int slabs = (int)((w.q + NS_SLAB - 1) / NS_SLAB);
   const NsPlan plan = ns_slab_plan(w.p, w.q, batch);
   g.parts = (const double*)ws;
   g.scales = (NsScales*)(ws + plan.parts);
   g.x = (float*)(ws + plan.parts + plan.scales);
-  g.a = (float*)(ws + plan.parts + plan.scales + batch * plan.x);
+  float* a = (float*)(ws + plan.parts + plan.scales + batch * plan.x);
+  float* next_a = a + batch * plan.a / 4;
+  g.next_a = a;
   g.x_batch = plan.x / 4;
   g.a_batch = plan.a / 4;
-  const dim3 grid((unsigned)g.slabs, (unsigned)batch);
+  const dim3 grid((unsigned)slabs, (unsigned)batch);
   k_ns_norm<T><<<dim3(g.count, (unsigned)batch), 256, 0, st>>>(w, (double*)ws);
   k_ns_slab<T, PB, true><<<grid, 512, lds, st>>>(g, cf);
-  const bool sum = g.slabs > 4;
-  g.shares = sum ? 1 : g.slabs;
+  const bool sum = slabs > 4;
+  g.shares = sum ? 1 : slabs;
   for (g.t = 0; g.t < steps; g.t = g.end + 1) {
     g.end = g.t;
     while (!(cf.ends >> g.end & 1)) ++g.end;
-    if (sum) k_ns_sum<<<dim3(P * P / 256, (unsigned)batch), 64, 0, st>>>(g.a, g.a_batch, P * P, g.slabs);
+    if (sum) k_ns_sum<<<dim3(P * P / 256, (unsigned)batch), 64, 0, st>>>(a, g.a_batch, P * P, slabs);
+    g.a = a;
+    g.next_a = next_a;
     k_ns_slab<T, PB, false><<<grid, 512, lds, st>>>(g, cf);
+    std::swap(a, next_a);
   }
   LAUNCHED(ctx, "orthogonalize");
   return NLS_OK;

@@ -434,8 +434,8 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
 // spectra, low rank + noise; 64 .. 512 rows): relative error of the result up to 4e-4 in one chain, 2e-5 in chains of 3 + 2, 9e-6 without (as
 // float32 products: 9e-6).  So bfloat16 results (rounding 1.7e-3) take chains of growth up to 500, float16 (2e-4) up to 45, float32 none.
 // Bound by latency and by vector instructions (roundings to pairs) for few matrices: a step is a chain of dependent products, LDS round trips and
-// barriers.  Column blocks of 32 and the 32 x 32 x 16 instruction read half as much LDS but keep half as many waves busy: 64 x 64 26 us, 128 x 128 63 us
-// for five float32 steps; blocks of 16: see k_ns_small.
+// barriers.  Five float32 steps of a 64 x 64 matrix take 22 us, of a 128 x 128 one 55 us; column blocks of 32 and the 32 x 32 x 16 instruction read half
+// as much LDS but keep half as many waves busy (26 and 63 us).
 template <int PB>
 struct NsRows {
   static constexpr int P = 32 * PB, RB = 2 * PB;              // rows, row blocks
@@ -828,9 +828,11 @@ struct NsSlabs {
   int count;
   double eps;
   NsScales* scales;
-  float *x, *a;          // a matrix's X; its slabs' shares of A (32 PB x 32 PB floats each, in register order)
+  float* x;              // a matrix's X
+  const float* a;        // its slabs' shares of A (32 PB x 32 PB floats each, in register order)
+  float* next_a;         // .. of the next A: in another place, for a workgroup may be done before another one has begun
   size_t x_batch, a_batch;  // floats from matrix to matrix
-  int slabs, shares;     // shares of A to add up
+  int shares;            // .. to add up
   int steps, t, end;     // the chain; first launch: t < 0
   void* out;
   int tall;
@@ -848,7 +850,6 @@ __global__ __launch_bounds__(512) void k_ns_slab(NsSlabs g, NsCoef cf) {
   const long j0 = (long)blockIdx.x * NS_SLAB;
   const int blocks = (int)((min((long)NS_SLAB, g.m.q - j0) + 31) / 32) * 2;
   float* xs = g.x + blockIdx.y * g.x_batch + ((size_t)blockIdx.x * 8 + w) * CB * FLOATS + l * 4;
-  float* as = g.a + blockIdx.y * g.a_batch;
   const T* from = (const T*)g.m.g + blockIdx.y * g.m.batch_stride;
   const bool fresh = FIRST || g.t == 0;  // X_0 comes from G
   const bool last = !FIRST && g.end + 1 == g.steps;
@@ -881,7 +882,7 @@ __global__ __launch_bounds__(512) void k_ns_slab(NsSlabs g, NsCoef cf) {
   } else {
     for (int i = threadIdx.x; i < (int)(sizeof(NsScales) / 4); i += 512) ((int*)&z)[i] = ((const int*)(g.scales + blockIdx.y))[i];
     if (w < S::RB) {
-      const float* at = as + w * FLOATS + l * 4;
+      const float* at = g.a + blockIdx.y * g.a_batch + w * FLOATS + l * 4;
 #pragma unroll
       for (int a = 0; a < S::RB; ++a)
 #pragma unroll
@@ -921,7 +922,7 @@ __global__ __launch_bounds__(512) void k_ns_slab(NsSlabs g, NsCoef cf) {
   __syncthreads();
   ns_gram<PB, CB>(lds, blocks, m);
   if (w < S::RB) {
-    float* at = as + (size_t)blockIdx.x * S::P * S::P + w * FLOATS + l * 4;
+    float* at = g.next_a + blockIdx.y * g.a_batch + (size_t)blockIdx.x * S::P * S::P + w * FLOATS + l * 4;
 #pragma unroll
     for (int a = 0; a < S::RB; ++a) *(f32x4*)(at + a * 256) = f32x4{m[a][0], m[a][1], m[a][2], m[a][3]};
   }

@@ -344,6 +344,14 @@ def test_orthogonalize_in_every_tile(batch, m, n, name):
         assert all(torch.equal(out[j], out[i]) for j in range(i, batch, 2))
 
 
+@pytest.mark.parametrize("m,n,name", [(100, 70001, "float32"), (80001, 128, "bfloat16"), (60, 150000, "float16")])
+def test_orthogonalize_with_more_slabs_than_the_card_holds(m, n, name):
+    """Workgroups that begin when others are done with the step read what those others read."""
+    rng = np.random.default_rng(n)
+    g = torch.tensor(rng.standard_normal((m, n)), dtype=torch.float32).to(DTYPES[name]).cuda()
+    newton_schulz_check(nls.orthogonalize(g), host(g), nls.NEWTON_SCHULZ, 5, 1e-7, name, 1)
+
+
 @pytest.mark.parametrize("m,n", [(40, 50), (100, 900), (150, 140)])
 def test_orthogonalize_as_many_steps_as_there_may_be(m, n):
     g = torch.tensor(gradient(np.random.default_rng(m), m, n), dtype=torch.float32).cuda()
