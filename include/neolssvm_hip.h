@@ -444,7 +444,7 @@ int nls_dual_predict(nls_ctx* ctx, const double* Xq, int64_t m, const double* Xt
  * arguments, which may be nothing; two calls that may run at the same
  * time - other streams, graphs that are replayed side by side - need two).  Calls can be captured into a graph.  The caller's current device is left
  * as it was.  Results do not depend on timing: the same call gives the same bits.  Sizes of zero rows, columns or matrices are fine (nothing is
- * written); sums over nothing (k = 0) are refused. */
+ * written); sums over nothing (k = 0) are refused.  A context has to exist before a capture begins. */
 #define NLS_TYPE_F32 0
 #define NLS_TYPE_F16 1
 #define NLS_TYPE_BF16 2
@@ -459,7 +459,7 @@ int nls_quantize_rows(nls_ctx* ctx, const void* x, int type, int64_t rows, int64
  * y: m x n without gaps, of `type`.  The sum is exact (32-bit integers, hence k <= NLS_INT8_MAX_K), the rest is float32, rounded once to `type`.
  * bias: n elements, float32 or of `type` (bias_type), or NULL.  Rows that start at multiples of 16 bytes are read in place; k need not be a multiple of
  * 16 if the flag says that the bytes up to the next one may be read in every row, the last included (what they hold does not matter).  Other rows are
- * copied to the workspace first. */
+ * copied to the workspace first, but for m <= 16, which reads from any address.  k <= lda, ldb <= 2^23 - 1 (matrices of one row included); m, n < 2^31 - 256. */
 #define NLS_INT8_MAX_K 131071
 #define NLS_INT8_A_PADDED 1
 #define NLS_INT8_B_PADDED 2
@@ -476,7 +476,8 @@ int nls_int8_linear(nls_ctx* ctx, const void* x, int type, int64_t row_stride, i
  * transposed).  coefficients: steps x 3 (a, b, c), host.  G: `batch` matrices m x n of `type`, element (l, i, j) at l batch_stride + i row_stride +
  * j col_stride; out: batch x m x n without gaps, of `type`, not overlapping G.  Each matrix has its own norm; one that holds a NaN or an infinity
  * comes out as NaN, one of zeros as zeros.  Products and sums carry 22 bits or more; for 16-bit results the early steps carry 11 (error of the result
- * against 64 bits below its own rounding).  The coefficients may not let a singular value of X pass 1e6. */
+ * against 64 bits below its own rounding).  Up to 128 rows on the shorter side, 16-bit results are worked out over several steps on the small matrix
+ * alone, with 22 bits.  The coefficients may not let a singular value of X pass 1e6.  1 .. 32 steps, at most 2^20 rows and columns and 65535 matrices. */
 int nls_orthogonalize_workspace(int64_t batch, int64_t m, int64_t n, int64_t row_stride, int64_t col_stride, size_t* bytes);
 int nls_orthogonalize(nls_ctx* ctx, const void* g, int type, int64_t batch, int64_t m, int64_t n, int64_t batch_stride, int64_t row_stride,
                       int64_t col_stride, const double* coefficients, int steps, double eps, void* out, void* workspace, size_t workspace_bytes,

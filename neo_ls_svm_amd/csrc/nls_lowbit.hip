@@ -213,12 +213,13 @@ int operands(nls_ctx* ctx, const Int8Rows& a, const Int8Rows& b, long k, char* w
 
 // ---- Newton-Schulz ----
 // Matrices of at most 128 rows (nls_ortho.h): NS_SMALL, one workgroup holds X in registers and in LDS; NS_SLABS, workgroups share its columns.  Both
-// read a matrix with 32-bit offsets.  NS_TILES: all others.
+// read a matrix with 32-bit offsets.  NS_TILES: all others.  (float32 of up to 32 rows, whose products are of float32 itself, takes slabs earlier:
+// 23 x 761 .. us against 53 in one workgroup.)
 enum NsPath { NS_SMALL, NS_SLABS, NS_TILES };
-NsPath ns_path(long p, long q, long row_stride, long col_stride) {
+NsPath ns_path(long p, long q, long row_stride, long col_stride, bool f32) {
   const long reach = 1l << 28;
   if (p > 128 || row_stride < 0 || col_stride < 0 || row_stride >= reach || col_stride >= reach || (p + 32) * row_stride + 16 * col_stride >= reach) return NS_TILES;
-  return (q <= 256 || (p <= 64 && q <= 512) || (p <= 32 && q <= 1024)) ? NS_SMALL : NS_SLABS;
+  return (q <= 256 || (p <= 64 && q <= 512) || (p <= 32 && q <= 1024 && !f32)) ? NS_SMALL : NS_SLABS;
 }
 // Workgroups that sum squares: four rows (of the direction that is dense in memory) each
 int ns_parts(const NsMatrix& w) { return (int)std::min<long>(NS_PARTS, ((w.col_stride <= w.row_stride ? w.p : w.q) + 3) / 4); }
@@ -240,11 +241,11 @@ NsPlan ns_slab_plan(long p, long q, long batch) {
   w.total = w.parts + w.scales + (size_t)batch * (w.x + 2 * w.a);
   return w;
 }
-NsPlan ns_plan(long m, long n, long batch, long row_stride, long col_stride) {
+NsPlan ns_plan(long m, long n, long batch, long row_stride, long col_stride, bool f32) {
   NsPlan w{};
   w.p = std::min(m, n);
   w.q = std::max(m, n);
-  const NsPath path = ns_path(w.p, w.q, m > n ? col_stride : row_stride, m > n ? row_stride : col_stride);
+  const NsPath path = ns_path(w.p, w.q, m > n ? col_stride : row_stride, m > n ? row_stride : col_stride, f32);
   if (path == NS_SLABS) w = ns_slab_plan(w.p, w.q, batch);
   w.path = path;
   if (path != NS_TILES) return w;
@@ -296,7 +297,7 @@ int ns_product(nls_ctx* ctx, const NsArgs& g, bool pairs, long batch, hipStream_
 
 template <class T, int PB, int CB>
 int ns_small(nls_ctx* ctx, const NsMatrix& w, bool tall, long batch, const NsCoef& cf, int steps, double eps, T* out, hipStream_t st) {
-  constexpr int lds = NsLds<PB, CB>::BYTES;
+  constexpr int lds = NsLds<PB, CB, ns_full<T, PB>()>::BYTES;
   NLSCHK((ask_lds<&k_ns_small<T, PB, CB>>(ctx, lds)));
   k_ns_small<T, PB, CB><<<dim3((unsigned)batch), 512, lds, st>>>(w, cf, steps, eps, out, tall);
   LAUNCHED(ctx, "orthogonalize");
@@ -328,7 +329,7 @@ int ns_small_any(nls_ctx* ctx, const NsMatrix& w, bool tall, long batch, const N
 // p <= 128, more columns than one workgroup holds.  Up to four slabs' shares of A are added up by every workgroup, more by a launch of their own.
 template <class T, int PB>
 int ns_slabs(nls_ctx* ctx, const NsMatrix& w, bool tall, long batch, const NsCoef& cf, int steps, double eps, T* out, char* ws, hipStream_t st) {
-  constexpr int P = 32 * PB, lds = NsLds<PB, NS_SLAB / 128>::BYTES;
+  constexpr int P = 32 * PB, lds = NsLds<PB, NS_SLAB / 128, ns_full<T, PB>()>::BYTES;
   NLSCHK((ask_lds<&k_ns_slab<T, PB, true>>(ctx, lds)));
   NLSCHK((ask_lds<&k_ns_slab<T, PB, false>>(ctx, lds)));
   NsSlabs g{};
@@ -562,7 +563,7 @@ extern "C" int nls_int8_linear(nls_ctx* ctx, const void* x, int type, int64_t ro
 
 extern "C" int nls_orthogonalize_workspace(int64_t batch, int64_t m, int64_t n, int64_t row_stride, int64_t col_stride, size_t* bytes) {
   if (!bytes || batch < 0 || m < 0 || n < 0) return NLS_ERR_ARG;
-  *bytes = ns_plan(m, n, batch, row_stride, col_stride).total;
+  *bytes = std::max(ns_plan(m, n, batch, row_stride, col_stride, false).total, ns_plan(m, n, batch, row_stride, col_stride, true).total);
   return NLS_OK;
 }
 
@@ -584,7 +585,7 @@ extern "C" int nls_orthogonalize(nls_ctx* ctx, const void* g, int type, int64_t 
   }
   if (m > (1 << 20) || n > (1 << 20) || batch > 65535) return fail(ctx, NLS_ERR_ARG, "orthogonalize: at most 2^20 rows and columns and 65535 matrices");
   if (batch == 0 || m == 0 || n == 0) return NLS_OK;
-  const NsPlan plan = ns_plan(m, n, batch, row_stride, col_stride);
+  const NsPlan plan = ns_plan(m, n, batch, row_stride, col_stride, type == NLS_TYPE_F32);
   if (!g || !out || (plan.total && !workspace)) return fail(ctx, NLS_ERR_ARG, "orthogonalize: null pointer");
   if (workspace_bytes < plan.total) return fail(ctx, NLS_ERR_ARG, "orthogonalize: workspace of %zu bytes, %zu needed", workspace_bytes, plan.total);
   if ((uintptr_t)workspace % 256) return fail(ctx, NLS_ERR_ARG, "orthogonalize: the workspace must be aligned to 256 bytes");

@@ -436,31 +436,37 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
 // Bound by latency and by vector instructions (roundings to pairs) for few matrices: a step is a chain of dependent products, LDS round trips and
 // barriers.  Five float32 steps of a 64 x 64 matrix take 22 us, of a 128 x 128 one 55 us; column blocks of 32 and the 32 x 32 x 16 instruction read half
 // as much LDS but keep half as many waves busy (26 and 63 us).
-template <int PB>
+template <int PB, bool F>
 struct NsRows {
   static constexpr int P = 32 * PB, RB = 2 * PB;              // rows, row blocks
-  static constexpr int PITCH = P * 2 + 16, IMAGE = 2 * P * PITCH;
+  // F: products of float32 itself, 16 x 16 x 4 a time, for float32 matrices of up to 32 rows: few rows are where 22 bits show beside plain float32 (4 x 304:
+  // 3.4e-6 against 0.8e-6, so 1.0e-6).  The price: 23 x 761 55 us against 37, 16 x 403 .. .
+  static constexpr int PITCH = P * (F ? 4 : 2) + 16, IMAGE = (F ? 1 : 2) * P * PITCH;
   static constexpr bool BOTH = PB > 2;                        // A's and Q's column blocks on the same waves, else A on the first four, Q on the others
   static constexpr int KS = 8 / RB;                           // most waves that share a column block of A
   static constexpr int PARTS = KS > 1 ? (KS - 1) * P * P * 4 : 0;
   // Adding shares up costs about as much as the K steps it saves for short rows.  blocks: column blocks of X
   __device__ static int shares(int blocks) { return KS == 1 ? 1 : min(KS, max(1, blocks / 8)); }
 };
-template <int PB, int CB>
+template <int PB, int CB, bool F>
 struct NsLds {  // X of 128 CB columns as rows (a constant pitch: their addresses are offsets of one another), or two images, or the shares
-  using S = NsRows<PB>;
-  static constexpr int PITCH = CB * 256 + 16, X = 2 * S::P * PITCH;
+  using S = NsRows<PB, F>;
+  static constexpr int PITCH = CB * (F ? 512 : 256) + 16, X = (F ? 1 : 2) * S::P * PITCH;
   static constexpr int IMAGES = X > 2 * S::IMAGE ? X : 2 * S::IMAGE;
   static constexpr int BYTES = IMAGES > S::PARTS ? IMAGES : S::PARTS;
 };
+template <class T, int PB>
+constexpr bool ns_full() {
+  return PB == 1 && sizeof(T) == 4;
+}
 template <int PB>
 using NsCols = float[2 * PB][4];  // a column block of a p-row matrix
 
-// y = S x for N column blocks, S an image: every wave reads all of S, so blocks done together share what bounds it, the reads of LDS.  One fragment of x
+// y = S x for N column blocks, S an image (rb: its row blocks of 16 that are not zeros): every wave reads all of S, so blocks done together share what bounds it, the reads of LDS.  One fragment of x
 // at a time is split and met by all row blocks.
-template <int PB, int N>
-__device__ __forceinline__ void ns_times(const char* image, const NsCols<PB>* const (&x)[N], NsCols<PB>* const (&y)[N]) {
-  using S = NsRows<PB>;
+template <int PB, bool F, int N>
+__device__ __forceinline__ void ns_times(const char* image, int rb, const NsCols<PB>* const (&x)[N], NsCols<PB>* const (&y)[N]) {
+  using S = NsRows<PB, F>;
   const int l = lane_id();
   const char* at = image + (l & 15) * S::PITCH + (l >> 4) * 16;
   constexpr int APART = N == 1 && PB <= 2 ? 2 : 1;  // few accumulators: the small products in ones of their own
@@ -471,8 +477,21 @@ __device__ __forceinline__ void ns_times(const char* image, const NsCols<PB>* co
     for (int o = 0; o < APART; ++o)
 #pragma unroll
       for (int a = 0; a < S::RB; ++a) acc[n][o][a] = f32x4{};
+  if constexpr (F) {  // register r of row block k is the rows 16 k + 4 (l / 16) + r: an operand as it is
 #pragma unroll
-  for (int k = 0; k < PB; ++k) {
+    for (int k = 0; k < S::RB; ++k)
+#pragma unroll
+      for (int a = 0; a < S::RB; ++a) {
+        if (k >= rb || a >= rb) continue;
+        const f32x4 b = *(const f32x4*)(at + a * 16 * S::PITCH + k * 64);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int n = 0; n < N; ++n) acc[n][r % APART][a] = __builtin_amdgcn_mfma_f32_16x16x4f32(b[r], (*x[n])[k][r], acc[n][r % APART][a], 0, 0, 0);
+      }
+  }
+#pragma unroll
+  for (int k = 0; k < (F ? 0 : PB); ++k) {
     f16x8 xh[N], xl[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
@@ -508,11 +527,11 @@ __device__ __forceinline__ void ns_times(const char* image, const NsCols<PB>* co
 #pragma unroll
       for (int r = 0; r < 4; ++r) (*y[n])[a][r] = APART == 1 ? acc[n][0][a][r] : acc[n][0][a][r] + acc[n][APART - 1][a][r];
 }
-template <int PB>
-__device__ __forceinline__ void ns_times(const char* image, const NsCols<PB>& x, NsCols<PB>& y) {
+template <int PB, bool F>
+__device__ __forceinline__ void ns_times(const char* image, int rb, const NsCols<PB>& x, NsCols<PB>& y) {
   const NsCols<PB>* const from[1] = {&x};
   NsCols<PB>* const to[1] = {&y};
-  ns_times<PB, 1>(image, from, to);
+  ns_times<PB, F, 1>(image, rb, from, to);
 }
 // A column block to rows of LDS (hi plane, lo plane `plane` bytes on): the lane's column is at byte `at`, rows are `pitch` apart.  Neighbouring lanes swap
 // halves of two rows, so that each writes two neighbours of one.
@@ -536,26 +555,42 @@ __device__ __forceinline__ void ns_scatter(char* lds, int pitch, int plane, int 
       *(unsigned*)(to + plane) = __builtin_amdgcn_perm(nl, ml, pick);
     }
 }
+// .. to rows of float32, from column c on
+template <int PB>
+__device__ __forceinline__ void ns_lay(char* lds, int pitch, int c, const NsCols<PB>& x) {
+  const int l = lane_id();
+  char* base = lds + 4 * (l >> 4) * pitch + (c + (l & 15)) * 4;
+#pragma unroll
+  for (int a = 0; a < 2 * PB; ++a)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) *(float*)(base + (16 * a + r) * pitch) = x[a][r];
+}
 // Column block b of a p x p matrix into an image.  (Row i of the image is row i: the matrices of a chain are symmetric but for their roundings, and an
 // image of the transpose would make those grow - the products of a chain commute only as long as all are polynomials of the SAME A.)
-template <int PB>
+template <int PB, bool F>
 __device__ __forceinline__ void ns_put(char* image, int b, const NsCols<PB>& x) {
-  using S = NsRows<PB>;
+  using S = NsRows<PB, F>;
   const int c = lane_id() & 15;
-  ns_scatter<PB>(image, S::PITCH, S::P * S::PITCH, 64 * (b >> 1) + 16 * (c >> 2) + 8 * (b & 1) + 2 * (c & 3), x);
+  if constexpr (F)
+    ns_lay<PB>(image, S::PITCH, 16 * b, x);
+  else
+    ns_scatter<PB>(image, S::PITCH, S::P * S::PITCH, 64 * (b >> 1) + 16 * (c >> 2) + 8 * (b & 1) + 2 * (c & 3), x);
 }
 // Column block number c of X to rows
-template <int PB, int CB>
+template <int PB, int CB, bool F>
 __device__ __forceinline__ void ns_rows(char* lds, int c, const NsCols<PB>& x) {
-  using L = NsLds<PB, CB>;
-  ns_scatter<PB>(lds, L::PITCH, NsRows<PB>::P * L::PITCH, 32 * c + 2 * (lane_id() & 15), x);
+  using L = NsLds<PB, CB, F>;
+  if constexpr (F)
+    ns_lay<PB>(lds, L::PITCH, 16 * c, x);
+  else
+    ns_scatter<PB>(lds, L::PITCH, NsRows<PB, F>::P * L::PITCH, 32 * c + 2 * (lane_id() & 15), x);
 }
 // Column block w % RB of X X^T from the rows in LDS, wave w's share w / RB of the K range, then the shares added up: waves 0 .. RB - 1 have the result.
 // blocks: an even number of column blocks of X.  All rows have been read when this returns (a barrier).
-template <int PB, int CB>
-__device__ __forceinline__ void ns_gram(char* lds, int blocks, NsCols<PB>& m) {
-  using S = NsRows<PB>;
-  constexpr int pitch = NsLds<PB, CB>::PITCH;
+template <int PB, int CB, bool F>
+__device__ __forceinline__ void ns_gram(char* lds, int rb, int blocks, NsCols<PB>& m) {
+  using S = NsRows<PB, F>;
+  constexpr int pitch = NsLds<PB, CB, F>::PITCH;
   const int w = wave_id(), l = lane_id(), shares = S::shares(blocks);
   constexpr int APART = PB <= 2 ? 2 : 1;
   f32x4 acc[APART][S::RB];
@@ -563,10 +598,24 @@ __device__ __forceinline__ void ns_gram(char* lds, int blocks, NsCols<PB>& m) {
   for (int o = 0; o < APART; ++o)
 #pragma unroll
     for (int a = 0; a < S::RB; ++a) acc[o][a] = f32x4{};
-  if (w < S::RB * shares) {
+  if (w < S::RB * shares && w % S::RB < rb) {
     const char* at = lds + (l & 15) * pitch + (l >> 4) * 16;
     const int j = w % S::RB * 16;
-    for (int k = w / S::RB; 2 * k < blocks; k += shares) {
+    if constexpr (F) {
+      for (int k = w / S::RB; 2 * k < blocks; k += shares)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const f32x4 jv = *(const f32x4*)(at + j * pitch + k * 128 + h * 64);
+#pragma unroll
+          for (int a = 0; a < S::RB; ++a) {
+            if (a >= rb) continue;
+            const f32x4 iv = *(const f32x4*)(at + 16 * a * pitch + k * 128 + h * 64);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[r % APART][a] = __builtin_amdgcn_mfma_f32_16x16x4f32(iv[r], jv[r], acc[r % APART][a], 0, 0, 0);
+          }
+        }
+    }
+    for (int k = w / S::RB; !F && 2 * k < blocks; k += shares) {
       const f16x8 jh = *(const f16x8*)(at + j * pitch + k * 64), jl = *(const f16x8*)(at + (j + S::P) * pitch + k * 64);
 #pragma unroll
       for (int a = 0; a < S::RB; ++a) {
@@ -621,9 +670,9 @@ __device__ __forceinline__ void ns_scale(float v, NsCols<PB>& m) {
 }
 // From A (waves 0 .. RB - 1: its column blocks, as summed) the image that X is multiplied with: B of a single step, or Q of the chain t .. end.
 // Images at lds and lds + IMAGE; returns the one that holds it; a barrier has passed.
-template <int PB>
-__device__ __forceinline__ char* ns_chain(char* lds, NsCols<PB>& m, const NsScales& z, int t, int end) {
-  using S = NsRows<PB>;
+template <int PB, bool F>
+__device__ __forceinline__ char* ns_chain(char* lds, int rb, NsCols<PB>& m, const NsScales& z, int t, int end) {
+  using S = NsRows<PB, F>;
   const int w = wave_id(), first_q = S::BOTH ? 0 : 4;
   const bool a_wave = w < S::RB, q_wave = w >= first_q && w < first_q + S::RB;
   char *ia = lds, *ip = lds + S::IMAGE;
@@ -640,17 +689,17 @@ __device__ __forceinline__ char* ns_chain(char* lds, NsCols<PB>& m, const NsScal
   }
   for (;; ++t) {
     const NsFactors f = z.f[t];
-    if (a_wave) ns_put<PB>(ia, w, m);
+    if (a_wave) ns_put<PB, F>(ia, w, m);
     __syncthreads();
     if (a_wave) {
       NsCols<PB> p;
-      ns_times<PB>(ia, m, p);
+      ns_times<PB, F>(ia, rb, m, p);
 #pragma unroll
       for (int a = 0; a < S::RB; ++a)
 #pragma unroll
         for (int r = 0; r < 4; ++r) p[a][r] = f.lin * m[a][r] + f.quad * p[a][r];
       if (!alone) ns_diagonal<PB>(w, f.unit, p);
-      ns_put<PB>(ip, w, p);
+      ns_put<PB, F>(ip, w, p);
     }
     __syncthreads();
     if (alone) return ip;
@@ -659,19 +708,19 @@ __device__ __forceinline__ char* ns_chain(char* lds, NsCols<PB>& m, const NsScal
       NsCols<PB> r, y;
       const NsCols<PB>* const from[2] = {&m, &q};
       NsCols<PB>* const to[2] = {&r, &y};
-      ns_times<PB, 2>(ip, from, to);
+      ns_times<PB, F, 2>(ip, rb, from, to);
       ns_scale<PB>(f.half, r);
 #pragma unroll
       for (int a = 0; a < S::RB; ++a)
 #pragma unroll
         for (int e = 0; e < 4; ++e) q[a][e] = f.chain * y[a][e];
-      ns_times<PB>(ip, r, m);
+      ns_times<PB, F>(ip, rb, r, m);
       ns_scale<PB>(f.next, m);
       continue;
     }
     if (q_wave) {
       NsCols<PB> y;
-      ns_times<PB>(ip, q, y);
+      ns_times<PB, F>(ip, rb, q, y);
 #pragma unroll
       for (int a = 0; a < S::RB; ++a)
 #pragma unroll
@@ -680,13 +729,13 @@ __device__ __forceinline__ char* ns_chain(char* lds, NsCols<PB>& m, const NsScal
     if (t == end) break;
     if (!S::BOTH && a_wave) {
       NsCols<PB> r;
-      ns_times<PB>(ip, m, r);
+      ns_times<PB, F>(ip, rb, m, r);
       ns_scale<PB>(f.half, r);
-      ns_times<PB>(ip, r, m);
+      ns_times<PB, F>(ip, rb, r, m);
       ns_scale<PB>(f.next, m);
     }
   }
-  if (q_wave) ns_put<PB>(ia, w - first_q, q);
+  if (q_wave) ns_put<PB, F>(ia, w - first_q, q);
   __syncthreads();
   return ia;
 }
@@ -741,8 +790,8 @@ __device__ __forceinline__ void ns_first(double first, NsCols<PB>& x) {
     for (int r = 0; r < 4; ++r) x[a][r] = (float)((double)x[a][r] * first);
 }
 // X <- keep X + add S X for the wave's column blocks w, w + 8, .. below `blocks`, two at a time
-template <int PB, int CB>
-__device__ __forceinline__ void ns_advance(const char* image, float keep, float add, int blocks, NsCols<PB> (&x)[CB]) {
+template <int PB, int CB, bool F>
+__device__ __forceinline__ void ns_advance(const char* image, int rb, float keep, float add, int blocks, NsCols<PB> (&x)[CB]) {
   const int w = wave_id();
   constexpr int N = CB > 1 ? 2 : 1;
 #pragma unroll
@@ -756,7 +805,7 @@ __device__ __forceinline__ void ns_advance(const char* image, float keep, float 
         from[n] = &x[c + n];
         to[n] = &y[n];
       }
-      ns_times<PB, N>(image, from, to);
+      ns_times<PB, F, N>(image, rb, from, to);
 #pragma unroll
       for (int n = 0; n < N; ++n)
 #pragma unroll
@@ -775,7 +824,8 @@ __global__ __launch_bounds__(512) void k_ns_small(NsMatrix m, NsCoef cf, int ste
   __shared__ double part[8];
   const int l = lane_id(), w = wave_id();
   ns_fetch(cf, steps, &mine, z.f);
-  const int blocks = (int)((m.q + 31) / 32) * 2;
+  constexpr bool F = ns_full<T, PB>();
+  const int blocks = (int)((m.q + 31) / 32) * 2, rb = (int)(m.p + 15) / 16;
   const T* g = (const T*)m.g + blockIdx.x * m.batch_stride;
   NsCols<PB> x[CB];
   double sum = 0.0;
@@ -804,12 +854,12 @@ __global__ __launch_bounds__(512) void k_ns_small(NsMatrix m, NsCoef cf, int ste
     while (!(mine.ends >> end & 1)) ++end;
 #pragma unroll
     for (int c = 0; c < CB; ++c)
-      if (w + 8 * c < blocks) ns_rows<PB, CB>(lds, w + 8 * c, x[c]);
+      if (w + 8 * c < blocks) ns_rows<PB, CB, F>(lds, w + 8 * c, x[c]);
     __syncthreads();
     NsCols<PB> a;
-    ns_gram<PB, CB>(lds, blocks, a);
-    const char* image = ns_chain<PB>(lds, a, z, t, end);
-    ns_advance<PB, CB>(image, z.f[end].keep, z.f[end].add, blocks, x);
+    ns_gram<PB, CB, F>(lds, rb, blocks, a);
+    const char* image = ns_chain<PB, F>(lds, rb, a, z, t, end);
+    ns_advance<PB, CB, F>(image, rb, z.f[end].keep, z.f[end].add, blocks, x);
     t = end + 1;
     if (t < steps) __syncthreads();
   }
@@ -841,14 +891,15 @@ constexpr int NS_SLAB = 256;
 
 template <class T, int PB, bool FIRST>
 __global__ __launch_bounds__(512) void k_ns_slab(NsSlabs g, NsCoef cf) {
-  using S = NsRows<PB>;
+  constexpr bool F = ns_full<T, PB>();
+  using S = NsRows<PB, F>;
   constexpr int CB = NS_SLAB / 128, FLOATS = S::RB * 4 * 64;  // of a column block
   extern __shared__ char lds[];
   __shared__ NsScales z;
   __shared__ NsCoef mine;
   const int l = lane_id(), w = wave_id();
   const long j0 = (long)blockIdx.x * NS_SLAB;
-  const int blocks = (int)((min((long)NS_SLAB, g.m.q - j0) + 31) / 32) * 2;
+  const int blocks = (int)((min((long)NS_SLAB, g.m.q - j0) + 31) / 32) * 2, rb = (int)(g.m.p + 15) / 16;
   float* xs = g.x + blockIdx.y * g.x_batch + ((size_t)blockIdx.x * 8 + w) * CB * FLOATS + l * 4;
   const T* from = (const T*)g.m.g + blockIdx.y * g.m.batch_stride;
   const bool fresh = FIRST || g.t == 0;  // X_0 comes from G
@@ -902,8 +953,8 @@ __global__ __launch_bounds__(512) void k_ns_slab(NsSlabs g, NsCoef cf) {
     for (int c = 0; c < CB; ++c) ns_first<PB>(z.first, x[c]);
   }
   if constexpr (!FIRST) {
-    const char* image = ns_chain<PB>(lds, m, z, g.t, g.end);
-    ns_advance<PB, CB>(image, z.f[g.end].keep, z.f[g.end].add, blocks, x);
+    const char* image = ns_chain<PB, F>(lds, rb, m, z, g.t, g.end);
+    ns_advance<PB, CB, F>(image, rb, z.f[g.end].keep, z.f[g.end].add, blocks, x);
     if (last) {
       T* y = (T*)g.out + blockIdx.y * (size_t)(g.m.p * g.m.q);
 #pragma unroll
@@ -918,9 +969,9 @@ __global__ __launch_bounds__(512) void k_ns_slab(NsSlabs g, NsCoef cf) {
   }
 #pragma unroll
   for (int c = 0; c < CB; ++c)
-    if (w + 8 * c < blocks) ns_rows<PB, CB>(lds, w + 8 * c, x[c]);
+    if (w + 8 * c < blocks) ns_rows<PB, CB, F>(lds, w + 8 * c, x[c]);
   __syncthreads();
-  ns_gram<PB, CB>(lds, blocks, m);
+  ns_gram<PB, CB, F>(lds, rb, blocks, m);
   if (w < S::RB) {
     float* at = g.next_a + blockIdx.y * g.a_batch + (size_t)blockIdx.x * S::P * S::P + w * FLOATS + l * 4;
 #pragma unroll

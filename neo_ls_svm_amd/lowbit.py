@@ -4,7 +4,7 @@ They stand next to the 64-bit matrix calls of ``hotpath`` (``gram``, ``rotate``,
 matrices.  (The reference computes in 64 bits throughout: it has no counterpart.)  Three kinds of arrays go in, and the same kind comes out:
 
 * tensors of a tensor library that the caller has imported (torch on the GPU): the call is put on the tensor's device's current stream and does not
-  wait; it can be captured into a graph.  Nothing is imported here for it.  The operators are not differentiated: a tensor that asks for gradients is
+  wait; it can be captured into a graph, but for the first call on a device.  Nothing is imported here for it.  The operators are not differentiated: a tensor that asks for gradients is
   refused while gradients are recorded.
 * ``DeviceArray``: the context's own stream; the call returns when the result is there.
 * NumPy arrays: copied to the GPU and back.
@@ -356,8 +356,8 @@ def int8_matmul(a, a_scale, b, b_scale, bias=None, dtype="float32", ctx: Context
     """``y[..., j] = a_scale[...] * b_scale[j] * sum_k a[..., k] b[j, k] (+ bias[j])`` of ``dtype``.
 
     ``a`` (..., k) and ``b`` (n, k) int8, ``a_scale`` (...) and ``b_scale`` (n) float32, ``bias`` (n) float32 or of ``dtype``.  The sum is exact
-    (k <= 131071), the rest is float32, rounded once.  Rows that do not start at multiples of 16 bytes are copied first; ``quantize_rows`` lays them
-    out so that they do."""
+    (k <= 131071), the rest is float32, rounded once.  Rows that do not start at multiples of 16 bytes are copied first (but for up to 16 rows of
+    ``a``); ``quantize_rows`` lays them out so that they do."""
     sp = _space(a, ctx)
     kind = sp.named.get(dtype) if dtype.__hash__ is not None else None
     if kind is None:
@@ -420,7 +420,8 @@ def orthogonalize(g, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: float = 1e
     stay: with coefficients that lead to 1 the result is the orthogonal factor of the polar decomposition (what a QR of a Gaussian matrix gives
     ``orf_frequencies`` up to rotation of the draw), with the default ones the near-orthogonal update of a training step.
 
-    Products and sums carry 22 bits or more; for a 16-bit ``g`` the early steps carry 11, which stays below the rounding of the result."""
+    Products and sums carry 22 bits or more; for a 16-bit ``g`` the early steps carry 11, which stays below the rounding of the result.  At most 32
+    steps, 2^20 rows and columns, and 65535 matrices."""
     sp = _space(g, ctx)
     g = sp.take(g, "g")
     shape = tuple(g.shape)
