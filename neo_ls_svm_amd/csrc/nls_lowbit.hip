@@ -214,7 +214,7 @@ int operands(nls_ctx* ctx, const Int8Rows& a, const Int8Rows& b, long k, char* w
 // ---- Newton-Schulz ----
 // Matrices of at most 128 rows (nls_ortho.h): NS_SMALL, one workgroup holds X in registers and in LDS; NS_SLABS, workgroups share its columns.  Both
 // read a matrix with 32-bit offsets.  NS_TILES: all others.  (float32 of up to 32 rows, whose products are of float32 itself, takes slabs earlier:
-// 23 x 761 .. us against 53 in one workgroup.)
+// 23 x 761 42 us against 53 in one workgroup.)
 enum NsPath { NS_SMALL, NS_SLABS, NS_TILES };
 NsPath ns_path(long p, long q, long row_stride, long col_stride, bool f32) {
   const long reach = 1l << 28;

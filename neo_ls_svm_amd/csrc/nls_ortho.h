@@ -439,9 +439,11 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
 template <int PB, bool F>
 struct NsRows {
   static constexpr int P = 32 * PB, RB = 2 * PB;              // rows, row blocks
-  // F: products of float32 itself, 16 x 16 x 4 a time, for float32 matrices of up to 32 rows: few rows are where 22 bits show beside plain float32 (4 x 304:
-  // 3.4e-6 against 0.8e-6, so 1.0e-6).  The price: 23 x 761 55 us against 37, 16 x 403 .. .
-  static constexpr int PITCH = P * (F ? 4 : 2) + 16, IMAGE = (F ? 1 : 2) * P * PITCH;
+  // F: the result is float32.  Up to 32 rows its products are of float32 itself, 16 x 16 x 4 a time: few rows are where 22 bits show beside plain float32
+  // (4 x 304, six steps: error 3.4e-6 against 0.8e-6, so 0.9e-6).  The price: 23 x 761 42 us against 37.  More rows: pairs, with lo lo where a matrix of
+  // the chain is multiplied (58 x 2574: 2.2e-6, plain float32 1.4e-6; so 1.9e-6; 32 of 64 x 128 28 us against 27).
+  static constexpr bool FULL = F && PB == 1;
+  static constexpr int PITCH = P * (FULL ? 4 : 2) + 16, IMAGE = (FULL ? 1 : 2) * P * PITCH;
   static constexpr bool BOTH = PB > 2;                        // A's and Q's column blocks on the same waves, else A on the first four, Q on the others
   static constexpr int KS = 8 / RB;                           // most waves that share a column block of A
   static constexpr int PARTS = KS > 1 ? (KS - 1) * P * P * 4 : 0;
@@ -451,13 +453,13 @@ struct NsRows {
 template <int PB, int CB, bool F>
 struct NsLds {  // X of 128 CB columns as rows (a constant pitch: their addresses are offsets of one another), or two images, or the shares
   using S = NsRows<PB, F>;
-  static constexpr int PITCH = CB * (F ? 512 : 256) + 16, X = (F ? 1 : 2) * S::P * PITCH;
+  static constexpr int PITCH = CB * (S::FULL ? 512 : 256) + 16, X = (S::FULL ? 1 : 2) * S::P * PITCH;
   static constexpr int IMAGES = X > 2 * S::IMAGE ? X : 2 * S::IMAGE;
   static constexpr int BYTES = IMAGES > S::PARTS ? IMAGES : S::PARTS;
 };
 template <class T, int PB>
 constexpr bool ns_full() {
-  return PB == 1 && sizeof(T) == 4;
+  return sizeof(T) == 4;
 }
 template <int PB>
 using NsCols = float[2 * PB][4];  // a column block of a p-row matrix
@@ -477,7 +479,7 @@ __device__ __forceinline__ void ns_times(const char* image, int rb, const NsCols
     for (int o = 0; o < APART; ++o)
 #pragma unroll
       for (int a = 0; a < S::RB; ++a) acc[n][o][a] = f32x4{};
-  if constexpr (F) {  // register r of row block k is the rows 16 k + 4 (l / 16) + r: an operand as it is
+  if constexpr (S::FULL) {  // register r of row block k is the rows 16 k + 4 (l / 16) + r: an operand as it is
 #pragma unroll
     for (int k = 0; k < S::RB; ++k)
 #pragma unroll
@@ -491,7 +493,7 @@ __device__ __forceinline__ void ns_times(const char* image, int rb, const NsCols
       }
   }
 #pragma unroll
-  for (int k = 0; k < (F ? 0 : PB); ++k) {
+  for (int k = 0; k < (S::FULL ? 0 : PB); ++k) {
     f16x8 xh[N], xl[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
@@ -508,6 +510,9 @@ __device__ __forceinline__ void ns_times(const char* image, int rb, const NsCols
       for (int n = 0; n < N; ++n) acc[n][APART - 1][a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bl, xh[n], acc[n][APART - 1][a], 0, 0, 0);
 #pragma unroll
       for (int n = 0; n < N; ++n) acc[n][APART - 1][a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bh, xl[n], acc[n][APART - 1][a], 0, 0, 0);
+      if (F)
+#pragma unroll
+        for (int n = 0; n < N; ++n) acc[n][APART - 1][a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bl, xl[n], acc[n][APART - 1][a], 0, 0, 0);
       if (PB > 2 && a % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
     if (PB > 1) {  // one step's fragments at a time: all of them would not fit the registers
@@ -571,7 +576,7 @@ template <int PB, bool F>
 __device__ __forceinline__ void ns_put(char* image, int b, const NsCols<PB>& x) {
   using S = NsRows<PB, F>;
   const int c = lane_id() & 15;
-  if constexpr (F)
+  if constexpr (NsRows<PB, F>::FULL)
     ns_lay<PB>(image, S::PITCH, 16 * b, x);
   else
     ns_scatter<PB>(image, S::PITCH, S::P * S::PITCH, 64 * (b >> 1) + 16 * (c >> 2) + 8 * (b & 1) + 2 * (c & 3), x);
@@ -580,7 +585,7 @@ __device__ __forceinline__ void ns_put(char* image, int b, const NsCols<PB>& x) 
 template <int PB, int CB, bool F>
 __device__ __forceinline__ void ns_rows(char* lds, int c, const NsCols<PB>& x) {
   using L = NsLds<PB, CB, F>;
-  if constexpr (F)
+  if constexpr (NsRows<PB, F>::FULL)
     ns_lay<PB>(lds, L::PITCH, 16 * c, x);
   else
     ns_scatter<PB>(lds, L::PITCH, NsRows<PB, F>::P * L::PITCH, 32 * c + 2 * (lane_id() & 15), x);
@@ -601,7 +606,7 @@ __device__ __forceinline__ void ns_gram(char* lds, int rb, int blocks, NsCols<PB
   if (w < S::RB * shares && w % S::RB < rb) {
     const char* at = lds + (l & 15) * pitch + (l >> 4) * 16;
     const int j = w % S::RB * 16;
-    if constexpr (F) {
+    if constexpr (S::FULL) {
       for (int k = w / S::RB; 2 * k < blocks; k += shares)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -615,7 +620,7 @@ __device__ __forceinline__ void ns_gram(char* lds, int rb, int blocks, NsCols<PB
           }
         }
     }
-    for (int k = w / S::RB; !F && 2 * k < blocks; k += shares) {
+    for (int k = w / S::RB; !S::FULL && 2 * k < blocks; k += shares) {
       const f16x8 jh = *(const f16x8*)(at + j * pitch + k * 64), jl = *(const f16x8*)(at + (j + S::P) * pitch + k * 64);
 #pragma unroll
       for (int a = 0; a < S::RB; ++a) {
