@@ -11,11 +11,13 @@ using namespace lb;
 
 namespace {
 
-// The context's device for the length of a call; the caller's current device comes back afterwards.
+// The context's device for the length of a call; the caller's current device comes back afterwards.  An error that some call before left behind is not
+// this one's: it would be taken for a failed launch.
 struct DeviceGuard {
   int before = -1;
   hipError_t err = hipSuccess;
   explicit DeviceGuard(int device) {
+    (void)hipGetLastError();
     err = hipGetDevice(&before);
     if (err == hipSuccess && before != device)
       err = hipSetDevice(device);

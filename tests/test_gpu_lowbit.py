@@ -544,6 +544,16 @@ def test_arguments_the_c_calls_refuse():
     assert torch.equal(y, torch.full_like(y, 48.0))  # (47 products and a bias of one)
 
 
+def test_an_error_left_by_another_call_is_not_taken_for_a_failed_launch():
+    ctx = nls.default_context()
+    x = torch.ones(4, 32, device="cuda")
+    torch.cuda.synchronize()
+    page = np.zeros(4096)
+    assert ctx.lib.nls_host_unregister(ctx.handle, page.ctypes.data) != 0  # (never registered)
+    q, s = nls.quantize_rows(x)
+    assert torch.equal(nls.int8_linear(x, q, s), nls.int8_matmul(q, s, q, s)) and nls.orthogonalize(x).shape == (4, 32)
+
+
 def test_gradients_are_refused_not_lost():
     x = torch.ones(4, 32, device="cuda", requires_grad=True)
     q, s = nls.quantize_rows(x.detach())
