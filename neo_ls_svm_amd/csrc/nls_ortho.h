@@ -268,6 +268,7 @@ __global__ __launch_bounds__(256) void k_ns_pack(NsMatrix w, const double* parts
     split8(e + 8, &hi[1], &lo[1]);
     *(f16x8*)base = hi[0];
     *(f16x8*)(base + 16) = hi[1];
+    if (turn && !for_pairs) continue;  // single products read no lo halves, and nothing else reads the transpose
     *(f16x8*)(base + pair_lo(for_pairs)) = lo[0];
     *(f16x8*)(base + pair_lo(for_pairs) + 16) = lo[1];
   }
