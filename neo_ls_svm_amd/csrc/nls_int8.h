@@ -160,6 +160,82 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const T* x, long rows, lo
   }
 }
 
+// Rows whose neighbours are neighbours in memory (the rows of a transposed matrix): a workgroup takes 32 of them, 16 bytes of a column a thread - once for
+// the maxima, and once more, turned in LDS, for the numbers (which rows take it: see the host code).
+template <class T>
+struct Turned {
+  static constexpr int ROWS = 32, N = 16 / (int)sizeof(T), ACROSS = ROWS / N, COLS = 1024 / ACROSS;  // columns at a time
+  static constexpr int PITCH = ROWS * (int)sizeof(T) + 16, OUT = COLS + 16;
+};
+template <class T>
+__global__ __launch_bounds__(1024) void k_quantize_turned(const T* x, long rows, long k, long col_stride, signed char* q, long ldq, float* scale) {
+  using S = Turned<T>;
+  constexpr int N = S::N;
+  typedef T V __attribute__((ext_vector_type(N)));
+  typedef T Loose __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+  __shared__ __align__(16) char in[S::COLS * S::PITCH];
+  __shared__ __align__(16) signed char out[S::ROWS * S::OUT];
+  __shared__ unsigned most[S::ROWS];
+  const long r0 = group_id() * S::ROWS;
+  if (r0 >= rows) return;
+  const int a = threadIdx.x % S::ACROSS, c0 = threadIdx.x / S::ACROSS;
+  const int left = (int)min(rows - r0 - a * N, (long)N);
+  auto piece = [&](long c) {
+    V v = {};
+    if (c >= k) return v;
+    const T* from = x + c * col_stride + r0 + a * N;
+    if (left == N) {
+      v = *(const Loose*)from;
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (e < left) v[e] = from[e];
+    }
+    return v;
+  };
+  if (threadIdx.x < S::ROWS) most[threadIdx.x] = 0;
+  unsigned top[N] = {};
+#pragma unroll 4
+  for (long c = c0; c < k; c += S::COLS) {
+    const V v = piece(c);
+#pragma unroll
+    for (int e = 0; e < N; ++e) top[e] = max(top[e], __float_as_uint(to_f32(v[e])) & 0x7fffffffu);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+#pragma unroll
+    for (int o = S::ACROSS; o < 64; o *= 2) top[e] = max(top[e], (unsigned)__shfl_xor((int)top[e], o));
+    if ((threadIdx.x & 63) < S::ACROSS) atomicMax(&most[a * N + e], top[e]);
+  }
+  __syncthreads();
+  const int row = threadIdx.x % S::ROWS, group = threadIdx.x / S::ROWS;
+  const RowScale s = row_scale(most[row]);
+  if (group == 0 && r0 + row < rows) scale[r0 + row] = s.top / 127.0f;
+  V next = piece(c0);
+  for (long cb = 0; cb < ldq; cb += S::COLS) {
+    *(V*)(in + c0 * S::PITCH + a * 16) = next;
+    __syncthreads();
+    if (cb + S::COLS < ldq) next = piece(cb + S::COLS + c0);
+#pragma unroll
+    for (int g = 0; g < S::COLS; g += 128) {
+      const int c = g + 4 * group;
+      float f[4];
+      unsigned b[1];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] = to_f32(*(const T*)(in + (c + e) * S::PITCH + row * sizeof(T)));
+      quantise<4>(f, s, b);
+      *(unsigned*)(out + row * S::OUT + c) = b[0];
+    }
+    __syncthreads();
+    const int t = threadIdx.x;
+    if (t < S::ROWS * (S::COLS / 16)) {
+      const int orow = t / (S::COLS / 16), c = t % (S::COLS / 16) * 16;
+      if (r0 + orow < rows && cb + c < ldq) *(i32x4*)(q + (r0 + orow) * ldq + cb + c) = *(const i32x4*)(out + orow * S::OUT + c);
+    }
+  }
+}
+
 // n (up to 16) bytes from anywhere, the others zero
 typedef int i32x4_loose __attribute__((ext_vector_type(4), aligned(1)));
 __device__ __forceinline__ i32x4 loose_bytes(const signed char* p, int n) {

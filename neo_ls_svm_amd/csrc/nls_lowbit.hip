@@ -94,6 +94,13 @@ int quantize(nls_ctx* ctx, const T* x, long rows, long k, long rs, long cs, sign
 }
 template <class T>
 int quantize(nls_ctx* ctx, const T* x, long rows, long k, long rs, long cs, signed char* q, long ldq, float* scale, hipStream_t st) {
+  // Transposed: where 32 rows a workgroup are enough workgroups (8192 x 8192 bfloat16 109 us against 441, 4096 x 4096 45 / 76, 4096 x 128 float32 5.2 / 6.8;
+  // 1024 x 4096 42 / 28, 2048 x 64 6.2 / 4.3).
+  if (rs == 1 && cs != 1 && rows >= 2048 && k >= 128) {
+    k_quantize_turned<T><<<grid_of((rows + Turned<T>::ROWS - 1) / Turned<T>::ROWS), 1024, 0, st>>>(x, rows, k, cs, q, ldq, scale);
+    LAUNCHED(ctx, "quantize_rows");
+    return NLS_OK;
+  }
   return cs == 1 ? quantize<T, true>(ctx, x, rows, k, rs, cs, q, ldq, scale, st) : quantize<T, false>(ctx, x, rows, k, rs, cs, q, ldq, scale, st);
 }
 int quantize_any(nls_ctx* ctx, const void* x, int type, long rows, long k, long rs, long cs, signed char* q, long ldq, float* scale, hipStream_t st) {

@@ -125,6 +125,25 @@ def test_quantize_strides(name):
         assert np.array_equal(q.cpu().numpy(), wq) and np.array_equal(scale.cpu().numpy(), ws)
 
 
+@pytest.mark.parametrize("name", sorted(DTYPES))
+@pytest.mark.parametrize("rows,k,skip", [(2048, 128, 0), (2061, 130, 1), (4096, 257, 0), (2500, 1003, 3), (70000, 129, 0)])
+def test_quantize_the_rows_of_a_transposed_matrix(rows, k, skip, name):
+    rng = np.random.default_rng(rows + k)
+    base = torch.tensor(activations(rng, k, rows + skip), dtype=torch.float32).to(DTYPES[name]).cuda()
+    x = base[:, skip:].T
+    x[7] = 0
+    q, scale = nls.quantize_rows(x)
+    want_q, want_scale = quantize_oracle(host(x))
+    assert np.array_equal(q.cpu().numpy(), want_q) and np.array_equal(scale.cpu().numpy(), want_scale)
+    held = q.as_strided((rows, q.stride(0)), (q.stride(0), 1))
+    assert not held[:, k:].any()
+    x[11, k - 1], x[rows - 1, 0] = float("nan"), -float("inf")
+    q2, scale2 = nls.quantize_rows(x)
+    assert torch.isnan(scale2[11]) and torch.isinf(scale2[rows - 1]) and not q2[11].any() and not q2[rows - 1].any()
+    q2[11], q2[rows - 1], scale2[11], scale2[rows - 1] = q[11], q[rows - 1], scale[11], scale[rows - 1]
+    assert torch.equal(q2, q) and torch.equal(scale2, scale)
+
+
 def test_quantize_pads_its_rows_with_zeros():
     q, _ = nls.quantize_rows(torch.ones(3, 21, device="cuda"))
     assert q.stride() == (32, 1)
