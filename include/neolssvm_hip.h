@@ -467,7 +467,8 @@ int nls_int8_matmul_workspace(const int8_t* a, int64_t lda, const int8_t* b, int
 int nls_int8_matmul(nls_ctx* ctx, const int8_t* a, int64_t lda, const float* a_scale, const int8_t* b, int64_t ldb, const float* b_scale,
                     const void* bias, int bias_type, int64_t m, int64_t n, int64_t k, void* y, int type, int flags, void* workspace,
                     size_t workspace_bytes, void* stream);
-/* The two calls above in one: x (m x k, `type`, any strides) is quantised row by row and multiplied; y is of `type` too. */
+/* The two calls above in one: x (m x k, `type`, any strides) is quantised row by row and multiplied; y is of `type` too.  Where b is read in place the
+ * workspace is never more than m (k rounded up to 16) and 4 m bytes, each rounded up to 256. */
 int nls_int8_linear_workspace(const int8_t* b, int64_t ldb, int64_t m, int64_t n, int64_t k, int flags, size_t* bytes);
 int nls_int8_linear(nls_ctx* ctx, const void* x, int type, int64_t row_stride, int64_t col_stride, const int8_t* b, int64_t ldb, const float* b_scale,
                     const void* bias, int bias_type, int64_t m, int64_t n, int64_t k, void* y, int flags, void* workspace, size_t workspace_bytes,

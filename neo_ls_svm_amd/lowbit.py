@@ -330,7 +330,7 @@ def _bias(sp, bias, n, kind):
         return None, 0
     bias = sp.take(bias, "bias")
     code = _kind(sp, bias, "bias")
-    if tuple(bias.shape) != (n,) or code not in (0, kind):
+    if bias.shape != (n,) or code not in (0, kind):
         raise ValueError(f"bias must have shape ({n},) and be float32 or of the result's type, not {bias.dtype} of shape {tuple(bias.shape)}")
     return sp.dense(bias), code
 
@@ -402,12 +402,16 @@ def int8_linear(x, b, b_scale, bias=None, ctx: Context | None = None):
         lib = sp.ctx.lib
         pb = sp.ptr(b)
         flags = _B_PADDED if b_ready else 0
-        need = C.c_size_t()
-        lib.nls_int8_linear_workspace(pb, ldb, m, n, k, flags, need)
-        ws = sp.scratch(need.value) if need.value else None
+        if m > 4 and b_ready and not (pb | ldb) & 15:  # b is read where it is: room for the rows of x in 8 bits and their scales
+            nbytes = (m * _up16(k) + 255 & -256) + (4 * m + 255 & -256)
+        else:
+            need = C.c_size_t()
+            lib.nls_int8_linear_workspace(pb, ldb, m, n, k, flags, need)
+            nbytes = need.value
+        ws = sp.scratch(nbytes) if nbytes else None
         _call(
             sp.ctx, lib.nls_int8_linear, sp.ptr(x), kind, rs, cs, pb, ldb, sp.ptr(b_scale), None if bias is None else sp.ptr(bias), bias_kind, m, n, k,
-            sp.ptr(y), flags, None if ws is None else sp.ptr(ws), need.value, stream,
+            sp.ptr(y), flags, None if ws is None else sp.ptr(ws), nbytes, stream,
         )  # fmt: skip
     return sp.done(y)
 

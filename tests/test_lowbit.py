@@ -87,3 +87,15 @@ def test_arrays_of_the_other_byte_order_are_turned():
     other = X.dtype.newbyteorder()
     turned = lowbit._Arrays(X, None).take(X.astype(other), "x")
     assert turned.dtype == np.float32 and turned.dtype.isnative and np.array_equal(turned, X)
+
+
+@pytest.mark.parametrize("m", [5, 16, 17, 48, 49, 4096])
+@pytest.mark.parametrize("n,k,ld,flag", [(64, 64, 64, 0), (9000, 48, 64, 0), (300, 301, 304, 2), (8192, 33, 4096, 2)])
+def test_the_room_int8_linear_takes_without_asking_is_enough(m, n, k, ld, flag):
+    import ctypes as C
+
+    from neo_ls_svm_amd import _lib
+
+    need = C.c_size_t()
+    assert _lib.load_library().nls_int8_linear_workspace(4096, ld, m, n, k, flag, need) == 0
+    assert need.value <= (m * ((k + 15) & -16) + 255 & -256) + (4 * m + 255 & -256)
