@@ -58,7 +58,7 @@ int type_size(int t) { return t == NLS_TYPE_F32 ? 4 : (t == NLS_TYPE_F16 || t ==
 //   64 x 64, four waves side by side, three workgroups a unit: more of them than units, or few K steps: 1536^2 symmetric pairs 25 us against 34 (128 x 128)
 //     and 27 (K dealt out), int8 512 x 4096 x 4096 18.2 / 25 / 20; more than three steps held 0 .. 10 us slower (fewer workgroups a unit);
 //   64 x 64 with the K steps dealt out over the waves otherwise: X X^T of 512 x 2048 pairs 15.5 us against 22 (side by side) and 42 (128 x 128), int8
-//     256 x 4096 x 4096 11.6 / 14.5 / 24; at 16 steps (512^2 pairs, a whole call) 145 / 148, at 8 (single) 125 / 120.
+//     256 x 4096 x 4096 11.6 / 14.5 / 24; at 16 steps (512^2 pairs, a whole call) 145 / 148; at 8 steps (single halves) the order turned: 125 / 120.
 enum TileKind { TILE_256, TILE_128, TILE_128_DEEP, TILE_64, TILE_64_RING };
 template <class F>
 TileKind tile_kind(const nls_ctx* ctx, F tiles, int steps) {
@@ -236,7 +236,7 @@ int ns_parts(const NsMatrix& w) { return (int)std::min<long>(NS_PARTS, ((w.col_s
 struct NsPlan {
   NsPath path;
   long p, q;
-  size_t x, xt, a, parts, scales, batch_bytes, total;  // (NS_TILES: two X, two X^T, A and B a matrix)
+  size_t x, xt, a, parts, scales, batch_bytes, total;  // (NS_TILES: X, two X^T, A and B a matrix)
 };
 NsPlan ns_slab_plan(long p, long q, long batch) {
   NsPlan w{};
@@ -261,14 +261,14 @@ NsPlan ns_plan(long m, long n, long batch, long row_stride, long col_stride, boo
   w.x = (size_t)w.p * pair_ld(w.q);
   w.xt = (size_t)w.q * pair_ld(w.p);
   w.a = (size_t)w.p * pair_ld(w.p);
-  w.batch_bytes = 2 * w.x + 2 * w.xt + 2 * w.a;
+  w.batch_bytes = w.x + 2 * w.xt + 2 * w.a;
   w.parts = up256((size_t)batch * NS_PARTS * sizeof(double));
   w.scales = up256((size_t)batch * sizeof(NsScales));
   w.total = w.parts + w.scales + (size_t)batch * w.batch_bytes;
   return w;
 }
 
-template <int KIND, class T, class TL, int MODE, int B>
+template <int KIND, class T, class TL, int B>
 int ns_product_tile(nls_ctx* ctx, NsArgs g, long batch, hipStream_t st) {
   g.ti = (g.I + B - 1) / B;
   g.tj = (g.J + B - 1) / B;
@@ -276,32 +276,29 @@ int ns_product_tile(nls_ctx* ctx, NsArgs g, long batch, hipStream_t st) {
   constexpr bool SYM = KIND == NS_GRAM || KIND == NS_POLY;
   constexpr int LDS = tile_bytes<TL>();
   const long tiles = SYM ? (long)g.ti * (g.ti + 1) / 2 : (long)g.ti * g.tj;
-  NLSCHK((ask_lds<&k_ns_product<KIND, T, TL, MODE, B, B>>(ctx, LDS)));
-  k_ns_product<KIND, T, TL, MODE, B, B><<<dim3((unsigned)tiles, 1, (unsigned)batch), TL::THREADS, LDS, st>>>(g);
+  NLSCHK((ask_lds<&k_ns_product<KIND, T, TL, B, B>>(ctx, LDS)));
+  k_ns_product<KIND, T, TL, B, B><<<dim3((unsigned)tiles, 1, (unsigned)batch), TL::THREADS, LDS, st>>>(g);
   LAUNCHED(ctx, "orthogonalize");
   return NLS_OK;
 }
-template <int KIND, class T, int MODE>
+template <int KIND, class T>
 int ns_product(nls_ctx* ctx, const NsArgs& g, long batch, hipStream_t st) {
+  constexpr int MODE = MODE_F16PAIR;
   constexpr bool SYM = KIND == NS_GRAM || KIND == NS_POLY;
   auto tiles = [&](long b) {
     const long i = (g.I + b - 1) / b, j = (g.J + b - 1) / b;
     return (SYM ? i * (i + 1) / 2 : i * j) * batch;
   };
   // 192 x 192, four waves with a SIMD each, where they cover the card in one go and 128 x 128 in more than one: symmetric 4096^2 pairs 230 us against 280
-  // (128 x 128: 528 tiles for 512 places) and 287 (256 x 256: 136 tiles), single 95 against 117 and 114.
-  if (tiles(128) > 2 * ctx->cus && tiles(192) <= ctx->cus) return ns_product_tile<KIND, T, Tile<MODE, 192, 192, 2, 2, 3>, MODE, 192>(ctx, g, batch, st);
-  switch (tile_kind(ctx, tiles, (g.K + (MODE == MODE_F16 ? 63 : 31)) / (MODE == MODE_F16 ? 64 : 32))) {
-    case TILE_256: return ns_product_tile<KIND, T, Tile<MODE, 256, 256, 2, 4, 2>, MODE, 256>(ctx, g, batch, st);
-    case TILE_128: return ns_product_tile<KIND, T, Tile<MODE, 128, 128, 2, 2, 2>, MODE, 128>(ctx, g, batch, st);
-    case TILE_128_DEEP: return ns_product_tile<KIND, T, Tile<MODE, 128, 128, 4, 2, 3>, MODE, 128>(ctx, g, batch, st);
-    case TILE_64: return ns_product_tile<KIND, T, Tile<MODE, 64, 64, 2, 2, 3>, MODE, 64>(ctx, g, batch, st);
-    default: return ns_product_tile<KIND, T, Ring<MODE, 2>, MODE, 64>(ctx, g, batch, st);
+  // (128 x 128: 528 tiles for 512 places) and 287 (256 x 256: 136 tiles).
+  if (tiles(128) > 2 * ctx->cus && tiles(192) <= ctx->cus) return ns_product_tile<KIND, T, Tile<MODE, 192, 192, 2, 2, 3>, 192>(ctx, g, batch, st);
+  switch (tile_kind(ctx, tiles, (g.K + 31) / 32)) {
+    case TILE_256: return ns_product_tile<KIND, T, Tile<MODE, 256, 256, 2, 4, 2>, 256>(ctx, g, batch, st);
+    case TILE_128: return ns_product_tile<KIND, T, Tile<MODE, 128, 128, 2, 2, 2>, 128>(ctx, g, batch, st);
+    case TILE_128_DEEP: return ns_product_tile<KIND, T, Tile<MODE, 128, 128, 4, 2, 3>, 128>(ctx, g, batch, st);
+    case TILE_64: return ns_product_tile<KIND, T, Tile<MODE, 64, 64, 2, 2, 3>, 64>(ctx, g, batch, st);
+    default: return ns_product_tile<KIND, T, Ring<MODE, 2>, 64>(ctx, g, batch, st);
   }
-}
-template <int KIND, class T>
-int ns_product(nls_ctx* ctx, const NsArgs& g, bool pairs, long batch, hipStream_t st) {
-  return pairs ? ns_product<KIND, T, MODE_F16PAIR>(ctx, g, batch, st) : ns_product<KIND, T, MODE_F16>(ctx, g, batch, st);
 }
 
 template <class T, int PB, int CB>
@@ -395,9 +392,10 @@ void ns_chains(NsCoef& cf, int steps, double most) {
 }
 template <class T>
 int orthogonalize(nls_ctx* ctx, const NsMatrix& w, const NsPlan& plan, bool tall, long batch, NsCoef& cf, int steps, double eps, T* out, char* ws, hipStream_t st) {
-  // The first steps may work on the hi halves alone where the result has few bits: what a rounding to 11 bits does to an early iterate is carried
-  // along as a slightly different matrix would be, and the steps after it pull its singular values to the same curve.
-  const int exact = sizeof(T) == 4 ? steps : std::is_same<T, __bf16>::value ? 2 : 3;
+  // 16-bit matrices take pairs in every step as well.  Single products of the hi halves in the early ones would be a third of the work (4096^2 bfloat16, three
+  // of five steps: 2.6 ms against 4.0), but the roundings of A and B to 11 bits couple strong and weak singular directions and the steps after them spread that: the error
+  // against 64 bits was 0.75 (bfloat16) and 1.4 (float16) of the result's own rounding after five standard steps, 1.1 and 6.5 after six, 2.7 and 21 after
+  // twelve, where pairs stay at float32's error throughout.
   if (plan.path != NS_TILES) {
     ns_chains(cf, steps, sizeof(T) == 4 ? 0.0 : std::is_same<T, __bf16>::value ? 500.0 : 45.0);
     if (plan.path == NS_SMALL) return ns_small_any(ctx, w, tall, batch, cf, steps, eps, out, st);
@@ -410,44 +408,41 @@ int orthogonalize(nls_ctx* ctx, const NsMatrix& w, const NsPlan& plan, bool tall
   double* parts = (double*)ws;
   NsScales* scales = (NsScales*)(ws + plan.parts);
   char* base = ws + plan.parts + plan.scales;
-  char *X = base, *XV = X + plan.x, *XT = XV + plan.x, *XU = XT + plan.xt, *A = XU + plan.xt, *B = A + plan.a;
+  char *X = base, *XT = X + plan.x, *XU = XT + plan.xt, *A = XU + plan.xt, *B = A + plan.a;
   const int count = ns_parts(w);
   k_ns_norm<T><<<dim3(count, (unsigned)batch), 256, 0, st>>>(w, parts);
   k_ns_pack<T><<<dim3((unsigned)((w.q + 63) / 64), (unsigned)((w.p + 63) / 64), (unsigned)batch), 256, 0, st>>>(w, parts, count, eps, cf, steps, scales, X, XT,
-                                                                                                              plan.batch_bytes, steps <= exact);
+                                                                                                              plan.batch_bytes);
   LAUNCHED(ctx, "orthogonalize");
   NsArgs g{};
   g.scales = scales;
   g.batch_bytes = plan.batch_bytes;
   const int p = (int)w.p, q = (int)w.q;
   for (int t = 0; t < steps; ++t) {
-    const bool pairs = t >= steps - exact;
     g.t = t;
     g.P = g.Q = X;
     g.D = A;
     g.I = g.J = p;
     g.K = q;
-    NLSCHK((ns_product<NS_GRAM, float>(ctx, g, pairs, batch, st)));
+    NLSCHK((ns_product<NS_GRAM, float>(ctx, g, batch, st)));
     g.P = g.Q = g.E = A;
     g.D = B;
     g.K = p;
-    NLSCHK((ns_product<NS_POLY, float>(ctx, g, pairs, batch, st)));
+    NLSCHK((ns_product<NS_POLY, float>(ctx, g, batch, st)));
     g.P = XT;
     g.Q = B;
     g.E = X;
     g.I = q;
     if (t + 1 < steps) {
-      g.next_pairs = t + 1 >= steps - exact;
-      if (g.next_pairs != pairs) std::swap(X, XV);  // X stays where it is - a thread reads what it writes - but where its layout changes
-      g.D = X;
+      g.D = X;  // X stays where it is: a thread reads what it writes
       g.DT = XU;
-      NLSCHK((ns_product<NS_STEP, float>(ctx, g, pairs, batch, st)));
+      NLSCHK((ns_product<NS_STEP, float>(ctx, g, batch, st)));
       std::swap(XT, XU);
     } else {
       g.out = out;
       g.out_stride = (size_t)p * q;
       g.transposed = tall;
-      NLSCHK((ns_product<NS_LAST, T>(ctx, g, pairs, batch, st)));
+      NLSCHK((ns_product<NS_LAST, T>(ctx, g, batch, st)));
     }
   }
   return NLS_OK;

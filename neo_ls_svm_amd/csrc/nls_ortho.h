@@ -42,13 +42,10 @@ struct NsCoef {
   unsigned ends;              // bit t: a chain of steps ends with step t
 };
 
-// A matrix of fp16 pairs: rows padded with zeros to 64 elements, 4 bytes an element; hi and lo halves lie in blocks of 32 or 64 elements by the kind of
-// product that reads them (nls_tile.h).
+// A matrix of fp16 pairs: rows padded with zeros to 64 elements, 4 bytes an element; for every 32 elements the hi halves, then the lo halves.
 __host__ __device__ inline size_t pair_ld(long k) { return (size_t)((k + 63) / 64 * 64) * 4; }
-__device__ __forceinline__ size_t pair_at(size_t row, size_t k, size_t ld, bool for_pairs) {
-  return row * ld + (k >> 6) * 256 + (for_pairs ? (k >> 5 & 1) * 128 + (k & 31) * 2 : (k & 63) * 2);
-}
-__device__ __forceinline__ int pair_lo(bool for_pairs) { return for_pairs ? 64 : 128; }  // bytes from a hi half to its lo half
+__device__ __forceinline__ size_t pair_at(size_t row, size_t k, size_t ld) { return row * ld + (k >> 5) * 128 + (k & 31) * 2; }
+constexpr int PAIR_LO = 64;  // bytes from a hi half to its lo half
 
 struct NsMatrix {
   const void* g;
@@ -220,7 +217,7 @@ __device__ __forceinline__ void split8(const float* v, f16x8* hi, f16x8* lo) {
 // elements are on the way (a launch of its own for that took 4 us), the first of a matrix leaves the factors for the products.
 template <class T>
 __global__ __launch_bounds__(256) void k_ns_pack(NsMatrix w, const double* parts, int count, double eps, NsCoef cf, int steps, NsScales* scales, char* x,
-                                                 char* xt, size_t batch_bytes, int for_pairs) {
+                                                 char* xt, size_t batch_bytes) {
   __shared__ float tile[64][65];
   __shared__ NsCoef mine;
   __shared__ NsScales z;
@@ -258,7 +255,7 @@ __global__ __launch_bounds__(256) void k_ns_pack(NsMatrix w, const double* parts
   const size_t ldx = pair_ld(w.q), ldt = pair_ld(w.p);
   const int row = threadIdx.x >> 2, from = (threadIdx.x & 3) * 16;
   for (int turn = 0; turn < 2; ++turn) {
-    char* base = turn ? xt + pair_at(q0 + row, p0 + from, ldt, for_pairs) : x + pair_at(p0 + row, q0 + from, ldx, for_pairs);
+    char* base = turn ? xt + pair_at(q0 + row, p0 + from, ldt) : x + pair_at(p0 + row, q0 + from, ldx);
     if (turn ? q0 + row >= w.q : p0 + row >= w.p) continue;
     f16x8 hi[2], lo[2];
     float e[16];
@@ -268,18 +265,17 @@ __global__ __launch_bounds__(256) void k_ns_pack(NsMatrix w, const double* parts
     split8(e + 8, &hi[1], &lo[1]);
     *(f16x8*)base = hi[0];
     *(f16x8*)(base + 16) = hi[1];
-    if (turn && !for_pairs) continue;  // single products read no lo halves, and nothing else reads the transpose
-    *(f16x8*)(base + pair_lo(for_pairs)) = lo[0];
-    *(f16x8*)(base + pair_lo(for_pairs) + 16) = lo[1];
+    *(f16x8*)(base + PAIR_LO) = lo[0];
+    *(f16x8*)(base + PAIR_LO + 16) = lo[1];
   }
 }
 
 enum NsKind { NS_GRAM, NS_POLY, NS_STEP, NS_LAST };
 
 struct NsArgs {
-  const char *P, *Q;      // operands of the product (pairs)
+  const char *P, *Q;      // operands of the product
   const char* E;          // the matrix the epilogue adds, natural orientation (POLY: A, STEP / LAST: X)
-  char *D, *DT;           // result and its transpose (pairs); symmetric products write both halves of D
+  char *D, *DT;           // result and its transpose; symmetric products write both halves of D
   void* out;              // LAST: the caller's matrix
   const NsScales* scales;
   size_t batch_bytes;     // from a matrix of the batch to the next, workspace
@@ -288,17 +284,16 @@ struct NsArgs {
   int ti, tj, strip;
   int t;                  // step
   int transposed;         // LAST: out is stored q x p
-  int next_pairs;         // STEP: the next step's products are of pairs
 };
 
-__device__ __forceinline__ void store_pairs(char* at, const float (&v)[8], int lo) {  // eight neighbours of a row of pairs; lo: where their lo halves go, 0: nowhere
+__device__ __forceinline__ void store_pairs(char* at, const float (&v)[8]) {  // eight neighbours of a row of pairs
   f16x8 h, o;
   split8(v, &h, &o);
   *(f16x8*)at = h;
-  if (lo) *(f16x8*)(at + lo) = o;
+  *(f16x8*)(at + PAIR_LO) = o;
 }
 
-template <int KIND, class T, class TL, int MODE, int BI, int BJ>
+template <int KIND, class T, class TL, int BI, int BJ>
 __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
   extern __shared__ char lds[];
   constexpr bool SYM = KIND == NS_GRAM || KIND == NS_POLY;
@@ -319,7 +314,6 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
   const NsFactors f = z.f[g.t];
   const int last = z.last;
   const char* E = g.E + off;
-  constexpr bool PAIRS = MODE == MODE_F16PAIR;
   // A chunk's groups of eight elements, TURNS a thread: row r, words iw .. iw + 7
   constexpr int ACROSS = TL::W / 8, TURNS = TL::ROWS * ACROSS / TL::TEAM;
   static_assert(TURNS * TL::TEAM == TL::ROWS * ACROSS, "chunks must divide over the threads");
@@ -332,9 +326,9 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
   auto addend = [&](int i, int j, f16x8* h, f16x8* o) {  // eight elements of E; rows are padded: whole groups of eight, zeros behind the end
     *h = *o = f16x8{};
     if (j < g.J && (size_t)i * 4 < ldi) {
-      const char* at = E + pair_at(j, i, ldi, PAIRS);
+      const char* at = E + pair_at(j, i, ldi);
       *h = *(const f16x8*)at;
-      if (KIND != NS_POLY || PAIRS) *o = *(const f16x8*)(at + pair_lo(PAIRS));
+      *o = *(const f16x8*)(at + PAIR_LO);
     }
   };
   // What the epilogue adds is fetched in batches: for tiles of one chunk before the product, else before the chunk goes to LDS, four turns at a time.
@@ -353,14 +347,10 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
   };
   if constexpr (EARLY) batch(0, 0);
   TL t;
-  const int per = MODE == MODE_F16 ? 64 : 32;
-  t.run(Operand{g.P + off, (unsigned)ldk, g.I}, i0, Operand{g.Q + off, (unsigned)ldk, g.J}, j0, (g.K + per - 1) / per, 128, lds);
+  t.run(Operand{g.P + off, (unsigned)ldk, g.I}, i0, Operand{g.Q + off, (unsigned)ldk, g.J}, j0, (g.K + 31) / 32, 128, lds);
   char* D = g.D + off;
   char* DT = SYM ? D : g.DT + off;
   T* out = (T*)g.out + blockIdx.z * g.out_stride;
-  // Lo halves nobody reads are not written: of A and B where the step's products are single ones, of the transpose of X where the next step's are.
-  const bool to_pairs = SYM ? PAIRS : g.next_pairs != 0;  // the products that will read D and DT
-  const int lo_d = !SYM || PAIRS ? pair_lo(to_pairs) : 0, lo_t = to_pairs ? pair_lo(true) : 0;
   const bool natural = KIND != NS_LAST || !g.transposed, turned = KIND == NS_LAST ? g.transposed != 0 : SYM ? bi != bj : true;
   // Chunks of the tile through LDS: the result in the product's own orientation (rows j, eight neighbours i a thread), then, from the values left
   // there, its transpose (rows i, eight neighbours j).
@@ -395,7 +385,7 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
 #pragma unroll
         for (int e = 0; e < 8; e += 4) *(f32x4*)((float*)mine + r * TL::PITCH + iw + e) = f32x4{v[e], v[e + 1], v[e + 2], v[e + 3]};
       if (KIND != NS_LAST) {
-        if (j < g.J && (size_t)i * 4 < ldi) store_pairs(D + pair_at(j, i, ldi, to_pairs), v, lo_d);
+        if (j < g.J && (size_t)i * 4 < ldi) store_pairs(D + pair_at(j, i, ldi), v);
       } else if (natural && j < g.J && i < g.I) {
         store_some<T, 8>(out + (size_t)j * g.I + i, v, g.I - i);
       }
@@ -411,7 +401,7 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = ((const float*)mine)[(rv + e) * TL::PITCH + ii];
         if (KIND != NS_LAST) {
-          if ((size_t)j * 4 < ldj) store_pairs(DT + pair_at(irow, j, ldj, to_pairs), v, lo_t);
+          if ((size_t)j * 4 < ldj) store_pairs(DT + pair_at(irow, j, ldj), v);
         } else if (j < g.J) {
           store_some<T, 8>(out + (size_t)irow * g.J + j, v, g.J - j);
         }

@@ -1,9 +1,7 @@
 // Matrix-core tile engine of the few-bit operators (nls_lowbit.hip): D[i][j] = sum_k P[i][k] Q[j][k], both operands row-major with k running
-// along the row, in 8-bit integers, in fp16, or in fp16 pairs (hi + lo).
+// along the row, in 8-bit integers or in fp16 pairs (hi + lo).
 //
-// One K step is 128 bytes of every operand row, one whole line, whatever the type: 128 int8, 64 fp16 (hi halves alone), or 32 fp16 pairs.  Rows of pairs
-// are laid out for the products that read them: 64 bytes hi and 64 bytes lo for every 32 elements where those are of pairs, 128 and 128 bytes for every 64
-// where they are single.  (Each read from the other's layout costs a tenth to a third: half of every line fetched lies idle.)
+// One K step is 128 bytes of every operand row, one whole line, whatever the type: 128 int8, or 32 fp16 pairs (64 bytes hi, then 64 bytes lo).
 // The rows travel from memory to LDS without touching registers (16 bytes a lane, a wave moves 8 whole rows = eight full lines), into the next of STAGES
 // buffers while the matrix cores work on this one: the fewer workgroups share a compute unit, the more steps have to be under way to cover the way
 // to memory.
@@ -27,7 +25,7 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 
-enum Mode { MODE_I8 = 0, MODE_F16 = 1, MODE_F16PAIR = 2 };
+enum Mode { MODE_I8 = 0, MODE_F16PAIR = 1 };
 
 template <int MODE>
 struct AccOf {
@@ -38,11 +36,7 @@ struct AccOf<MODE_I8> {
   using type = i32x16;
 };
 
-// Where K step t of an operand row begins.
-template <int MODE>
-__device__ __forceinline__ size_t step_at(int t) {
-  return (size_t)t * (MODE == MODE_F16 ? 256 : 128);
-}
+__device__ __forceinline__ size_t step_at(int t) { return (size_t)t * 128; }  // where K step t of an operand row begins
 
 __device__ __forceinline__ i32x4 keep_bytes(i32x4 v, int n) {  // the first n of 16 bytes, the others zero
 #pragma unroll
@@ -139,7 +133,7 @@ struct Tile {
 #pragma unroll
       for (int b = 0; b < MJ; ++b) acc[a][b] = Acc{};
   }
-  // valid: bytes of the step that exist (>= 128: all); only 8-bit operands have ragged ends, fp16 operands are padded to whole steps
+  // valid: bytes of the step that exist (>= 128: all); only 8-bit operands have ragged ends, pairs are padded to whole steps
   __device__ __forceinline__ void fetch(const char* p, const char* q, char* buf, int valid) const {
     const int w = wave_id();
     const unsigned back = MODE == MODE_I8 && valid < 128 ? move_back(valid) : 0;
@@ -175,7 +169,7 @@ struct Tile {
     start(P, i0, Q, j0);
     const char* p = P.base + (size_t)i0 * P.ld;
     const char* q = Q.base + (size_t)j0 * Q.ld;
-    auto move = [&](int t, char* buf) { fetch(p + step_at<MODE>(t), q + step_at<MODE>(t), buf, t + 1 == steps ? last_valid : 128); };
+    auto move = [&](int t, char* buf) { fetch(p + step_at(t), q + step_at(t), buf, t + 1 == steps ? last_valid : 128); };
     constexpr int FIRST = AHEAD ? STAGES : STAGES - 1;
     for (int t = 0; t < min(FIRST, steps); ++t) move(t, lds + t * BUF);
     int now = 0;
@@ -292,7 +286,7 @@ struct Ring {
     lds += w * STAGES * BUF;
     const int mine = (steps - w + 3) / 4;  // steps w, w + 4, ..
     auto valid_of = [&](int t) { return 4 * t + w + 1 == steps ? last_valid : 128; };
-    for (int t = 0; t < min(STAGES, mine); ++t) fetch(p + step_at<MODE>(4 * t + w), q + step_at<MODE>(4 * t + w), lds + t * BUF, valid_of(t));
+    for (int t = 0; t < min(STAGES, mine); ++t) fetch(p + step_at(4 * t + w), q + step_at(4 * t + w), lds + t * BUF, valid_of(t));
     int now = 0;
     for (int t = 0; t < mine; ++t) {
       if (t + STAGES <= mine)
@@ -306,7 +300,7 @@ struct Ring {
         read<false>(f, lds + now, 128);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the step is in registers, its buffer free
       const int ahead = t + STAGES;
-      if (ahead < mine) fetch(p + step_at<MODE>(4 * ahead + w), q + step_at<MODE>(4 * ahead + w), lds + now, valid_of(ahead));
+      if (ahead < mine) fetch(p + step_at(4 * ahead + w), q + step_at(4 * ahead + w), lds + now, valid_of(ahead));
 #pragma unroll
       for (int s = 0; s < f.SUB; ++s) f.multiply(s, acc);
       now = now + BUF == STAGES * BUF ? 0 : now + BUF;

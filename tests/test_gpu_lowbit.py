@@ -627,3 +627,47 @@ def test_orthogonalize_float32_is_as_good_as_plain_float32(m, n):
         mine += np.linalg.norm(out[i] - want) ** 2
         plain += np.linalg.norm((x.T if m > n else x) - want) ** 2
     assert mine <= 4 * plain, (mine / plain) ** 0.5
+
+
+# ---- 16-bit results: float32's error, rounded once ------------------------------------------------------------------------------------------
+FINISH = (1.875, -1.25, 0.375)
+TABLES = {
+    "5": [nls.NEWTON_SCHULZ] * 5,
+    "6": [nls.NEWTON_SCHULZ] * 6,
+    "12": [nls.NEWTON_SCHULZ] * 12,
+    "5 + 3 finishing": [nls.NEWTON_SCHULZ] * 5 + [FINISH] * 3,
+    "5 + 3 of the identity": [nls.NEWTON_SCHULZ] * 5 + [(1.0, 0.0, 0.0)] * 3,
+    "16 cubic": [CUBIC] * 16,
+}
+
+
+def sixteen_bit_errors(rng, kind, m, n, table, name):
+    """(how far the result is from 64 bits, what its own rounding makes, the error of NumPy float32 products before any rounding, the norm), of one matrix."""
+    if kind == "gradient":
+        g = gradient(rng, m, n)
+    else:  # so many strong directions over a noise floor
+        rank, noise = kind
+        g = rng.standard_normal((m, rank)) @ rng.standard_normal((rank, n)) + noise * rng.standard_normal((m, n)) if rank else rng.standard_normal((m, n))
+    t = torch.tensor(1e-2 * g, dtype=torch.float32).to(DTYPES[name])
+    g = host(t)
+    want = newton_schulz_oracle(g, table, len(table), 1e-7)
+    x = (g.T if m > n else g) / (np.linalg.norm(g) + 1e-7)
+    x = x.astype(np.float32)
+    for a, b, c in np.asarray(table, dtype=np.float32):
+        s = x @ x.T
+        x = a * x + (b * s + c * (s @ s)) @ x
+    own = np.linalg.norm(host(torch.tensor(want).to(DTYPES[name])) - want)
+    got = host(nls.orthogonalize(t.cuda(), steps=len(table), coefficients=table))
+    return np.linalg.norm(got - want), own, np.linalg.norm((x.T if m > n else x) - want), np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("steps", sorted(TABLES))
+@pytest.mark.parametrize("name", ["float16", "bfloat16"])
+@pytest.mark.parametrize("m,n", [(130, 200), (300, 420), (400, 400), (700, 150)])
+def test_sixteen_bit_results_of_more_than_128_rows_are_float32s_rounded(m, n, name, steps):
+    """The error is that of the result's own rounding (norms of tens of thousands of roundings: alike within 5 %) and what the products do before it, which
+    is float32's: pairs round at 2^-23 where float32 does at 2^-24, hence twice, and twice that for how single cases fall."""
+    rng = np.random.default_rng(m + n)
+    for kind in ("gradient", (0, 1.0), (4, 1e-3), (1, 1e-2)):
+        off, own, plain, _ = sixteen_bit_errors(rng, kind, m, n, TABLES[steps], name)
+        assert off <= 1.05 * own + 4 * plain, (kind, off / own, plain / own)
