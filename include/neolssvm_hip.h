@@ -477,7 +477,8 @@ int nls_int8_linear(nls_ctx* ctx, const void* x, int type, int64_t row_stride, i
  * transposed).  coefficients: steps x 3 (a, b, c), host.  G: `batch` matrices m x n of `type`, element (l, i, j) at l batch_stride + i row_stride +
  * j col_stride; out: batch x m x n without gaps, of `type`, not overlapping G.  Each matrix has its own norm; one that holds a NaN or an infinity
  * comes out as NaN, one of zeros as zeros.  Products and sums carry 22 bits or more, whatever the type: what the products do to a result is what float32
- * products do to it.  Up to 128 rows on the shorter side, 16-bit results are worked out over several steps on the small matrix alone.  The coefficients may not let a singular value of X pass 1e6.  1 .. 32 steps, at most 2^20 rows and columns and 65535 matrices. */
+ * products do to it.  Up to 128 rows on the shorter side, 16-bit results are worked out over several steps on the small matrix alone
+ * (which adds less than a quarter of the result's own rounding).  The coefficients may not let a singular value of X pass 1e6.  1 .. 32 steps, at most 2^20 rows and columns and 65535 matrices. */
 int nls_orthogonalize_workspace(int64_t batch, int64_t m, int64_t n, int64_t row_stride, int64_t col_stride, size_t* bytes);
 int nls_orthogonalize(nls_ctx* ctx, const void* g, int type, int64_t batch, int64_t m, int64_t n, int64_t batch_stride, int64_t row_stride,
                       int64_t col_stride, const double* coefficients, int steps, double eps, void* out, void* workspace, size_t workspace_bytes,

@@ -397,7 +397,8 @@ int orthogonalize(nls_ctx* ctx, const NsMatrix& w, const NsPlan& plan, bool tall
   // against 64 bits was 0.75 (bfloat16) and 1.4 (float16) of the result's own rounding after five standard steps, 1.1 and 6.5 after six, 2.7 and 21 after
   // twelve, where pairs stay at float32's error throughout.
   if (plan.path != NS_TILES) {
-    ns_chains(cf, steps, sizeof(T) == 4 ? 0.0 : std::is_same<T, __bf16>::value ? 500.0 : 45.0);
+    const double half = std::is_same<T, __bf16>::value ? 0x1p-8 : 0x1p-11;  // half a step of the result, relative
+    ns_chains(cf, steps, sizeof(T) == 4 ? 0.0 : std::sqrt(0x1p23 * half / 16.0));
     if (plan.path == NS_SMALL) return ns_small_any(ctx, w, tall, batch, cf, steps, eps, out, st);
     if (w.p <= 32) return ns_slabs<T, 1>(ctx, w, tall, batch, cf, steps, eps, out, ws, st);
     if (w.p <= 64) return ns_slabs<T, 2>(ctx, w, tall, batch, cf, steps, eps, out, ws, st);

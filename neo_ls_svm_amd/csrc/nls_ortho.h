@@ -420,10 +420,11 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
 // Rows of LDS planes are 16 bytes longer than their numbers: eight neighbouring rows start in different banks.
 //
 // Chains: with P_t = a + b A_t + c A_t A_t the iterates are X_t+1 = P_t X_t and A_t+1 = P_t A_t P_t, so steps t .. t' can be done on p x p matrices
-// alone, Q <- P Q, and X is multiplied once, by Q.  What it costs is accuracy: A's roundings are relative to its LARGEST eigenvalue, and Q amplifies
-// what they do to small ones by the square of the polynomials' slope.  Measured against 64 bits (five standard steps, Gaussian, 1 / k and exponential
-// spectra, low rank + noise; 64 .. 512 rows): relative error of the result up to 4e-4 in one chain, 2e-5 in chains of 3 + 2, 9e-6 without (as
-// float32 products: 9e-6).  So bfloat16 results (rounding 1.7e-3) take chains of growth up to 500, float16 (2e-4) up to 45, float32 none.
+// alone, Q <- P Q, and X is multiplied once, by Q.  What it costs is accuracy: A's roundings, 2^-23 of its LARGEST eigenvalue, grow with the square of what a
+// chain lets small singular values grow by.  A chain may be so long that this stays below a sixteenth of half a step of the result: growth up to 45 for
+// bfloat16 (three standard steps), 16 for float16 (two), none for float32.  (Worst of one to four strong directions over noise of 1e-1 .. 3e-4, up to 16
+// standard and 32 cubic steps, 16 .. 128 rows, in units of the result's own rounding: growth 500 in bfloat16 3.8, 45 in float16 0.4; as
+// above 0.1 and 0.2.  64 x 512 bfloat16 34.5 us against 27.9 in one chain, 64 x 8192 47 / 35; float16 40 / 34 and 58 / 47 in 3 + 2; float32 52 and 80.)
 // Bound by latency and by vector instructions (roundings to pairs) for few matrices: a step is a chain of dependent products, LDS round trips and
 // barriers.  Five float32 steps of a 64 x 64 matrix take 22 us, of a 128 x 128 one 55 us; column blocks of 32 and the 32 x 32 x 16 instruction read half
 // as much LDS but keep half as many waves busy (26 and 63 us).

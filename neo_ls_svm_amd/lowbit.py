@@ -424,8 +424,8 @@ def orthogonalize(g, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: float = 1e
     stay: with coefficients that lead to 1 the result is the orthogonal factor of the polar decomposition (what a QR of a Gaussian matrix gives
     ``orf_frequencies`` up to rotation of the draw), with the default ones the near-orthogonal update of a training step.
 
-    Products and sums carry 22 bits or more, whatever the type of ``g``: the error before the result's own rounding is that of float32 products.  At most
-    32 steps, 2^20 rows and columns, and 65535 matrices."""
+    Products and sums carry 22 bits or more, whatever the type of ``g``: the error before the result's own rounding is that of float32 products
+    (16-bit matrices of up to 128 rows: and less than a quarter of that rounding).  At most 32 steps, 2^20 rows and columns, and 65535 matrices."""
     sp = _space(g, ctx)
     g = sp.take(g, "g")
     shape = tuple(g.shape)

@@ -671,3 +671,16 @@ def test_sixteen_bit_results_of_more_than_128_rows_are_float32s_rounded(m, n, na
     for kind in ("gradient", (0, 1.0), (4, 1e-3), (1, 1e-2)):
         off, own, plain, _ = sixteen_bit_errors(rng, kind, m, n, TABLES[steps], name)
         assert off <= 1.05 * own + 4 * plain, (kind, off / own, plain / own)
+
+
+@pytest.mark.parametrize("steps", [5, 10, 16])
+@pytest.mark.parametrize("name", ["float16", "bfloat16"])
+@pytest.mark.parametrize("m,n", [(16, 40), (32, 200), (32, 1000), (300, 20), (64, 512), (96, 200), (128, 700), (20, 3000)])
+def test_sixteen_bit_results_of_up_to_128_rows(m, n, name, steps):
+    """As above, and what the chains of steps on p x p matrices may do to weak directions beside strong ones: roundings of 2^-23 that grow by the square of a
+    chain's growth to a sixteenth of half a step of the result, and twice that for the steps behind the chain.  (Hundreds of roundings: alike within 10 %.)"""
+    rng = np.random.default_rng(m + n)
+    for kind in ((1, 3e-2), (1, 1e-2), (2, 3e-2), (4, 1e-1), (1, 3e-4)):
+        for one in (nls.NEWTON_SCHULZ, CUBIC):
+            off, own, plain, norm = sixteen_bit_errors(rng, kind, m, n, [one] * steps, name)
+            assert off <= 1.1 * own + 4 * plain + HALF[name] / 8 * norm, (kind, one, off / own, plain / own)
