@@ -100,6 +100,8 @@ def exact_complexity_matrix(Z) -> np.ndarray:
 
 def _f64(a, name, shape=None):
     if isinstance(a, DeviceArray):
+        if a.dtype != np.float64:  # (its memory would be read as twice as many bytes and more)
+            raise ValueError(f"{name} is a DeviceArray of {a.dtype}; the 64-bit calls take float64")
         if shape is not None and tuple(a.shape) != tuple(shape):
             raise ValueError(f"{name} has shape {a.shape}, expected {shape}")
         return a
@@ -133,6 +135,8 @@ def featuremap(X, shift, scale, B, ctx: Context | None = None, out: DeviceArray 
         phi = np.empty((n, D + 1), dtype=np.complex128)
         target = phi.ctypes.data
     else:
+        if out.dtype not in (np.float64, np.complex128) or out.nbytes < n * (D + 1) * 16:
+            raise ValueError(f"out must hold {n} x {D + 1} complex128 numbers, not {out.dtype} of shape {out.shape}")
         phi, target = out, out.ptr
     ctx._check(
         ctx.lib.nls_featuremap(ctx.handle, _lib._ptr(X), n, d, shift.ctypes.data, scale.ctypes.data, B.ctypes.data, D, target)

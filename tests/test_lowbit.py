@@ -99,3 +99,43 @@ def test_the_room_int8_linear_takes_without_asking_is_enough(m, n, k, ld, flag):
     need = C.c_size_t()
     assert _lib.load_library().nls_int8_linear_workspace(4096, ld, m, n, k, flag, need) == 0
     assert need.value <= (m * ((k + 15) & -16) + 255 & -256) + (4 * m + 255 & -256)
+
+
+def device_array(shape, dtype):
+    a = nls.DeviceArray.__new__(nls.DeviceArray)  # (no GPU is needed to be refused)
+    a.ctx, a.shape, a.dtype, a.ptr = None, shape, np.dtype(dtype), None
+    a.nbytes = int(np.prod(shape)) * a.dtype.itemsize
+    return a
+
+
+class NoContext:
+    def held(self, a):
+        return a
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "int8", "complex128"])
+def test_the_64_bit_calls_refuse_device_arrays_of_other_types(dtype):
+    """The few-bit operators hand out DeviceArrays of 32, 16 and 8 bits: read as float64 they would be read past their end."""
+    n, d, D = 6, 3, 4
+    ctx, x, y = NoContext(), device_array((n, d), dtype), np.ones(n)
+    good, shift, scale, B = device_array((n, d), "float64"), np.zeros(d), np.ones(d), np.ones((d, D))
+    for call in (
+        lambda: nls.featuremap(x, shift, scale, B, ctx=ctx),
+        lambda: nls.gram(x, y, y, shift, scale, B, ctx=ctx),
+        lambda: nls.gram(good, device_array((n,), dtype), y, shift, scale, B, ctx=ctx),
+        lambda: nls.gram(good, y, device_array((n,), dtype), shift, scale, B, ctx=ctx),
+        lambda: nls.rotate(x, shift, scale, B, np.eye(D + 1), np.ones(D + 1), ctx=ctx),
+        lambda: nls.primal_fit(x, y, y, shift, scale, B, False, ctx=ctx),
+        lambda: nls.primal_predict(x, shift, scale, B, beta=np.ones(D + 1), ctx=ctx),
+        lambda: nls.dual_fit(x, y, y, False, ctx=ctx),
+        lambda: nls.dual_predict(good, x, alpha=y, ctx=ctx),
+        lambda: nls.dual_predict(good, good, L=device_array((n, n), dtype), ctx=ctx),
+    ):
+        with pytest.raises(ValueError, match="64-bit calls take float64"):
+            call()
+
+
+@pytest.mark.parametrize("out", [((6, 10), "float32"), ((6, 5), "float64"), ((6, 4), "complex128"), ((6, 10), "int8")])
+def test_featuremap_refuses_to_write_past_the_end_of_out(out):
+    with pytest.raises(ValueError, match="out must hold"):
+        nls.featuremap(np.ones((6, 3)), np.zeros(3), np.ones(3), np.ones((3, 4)), ctx=NoContext(), out=device_array(*out))
