@@ -74,7 +74,7 @@ TileKind tile_kind(const nls_ctx* ctx, F tiles, int steps) {
 template <class T, bool VEC>
 int quantize(nls_ctx* ctx, const T* x, long rows, long k, long rs, long cs, signed char* q, long ldq, float* scale, hipStream_t st) {
   constexpr long N = Few<T, VEC>::N;
-  const dim3 waves = grid_of((rows + 3) / 4), groups = grid_of(rows);
+  const dim3 waves = grid_of<256>((rows + 3) / 4), groups = grid_of<256>(rows);
 #define QUANTIZE(G, HELD, GRID) k_quantize_rows<T, G, VEC, HELD><<<GRID, 256, 0, st>>>(x, rows, k, rs, cs, q, ldq, scale)
   if (k <= 64 * N)
     QUANTIZE(64, 1, waves);
@@ -97,7 +97,7 @@ int quantize(nls_ctx* ctx, const T* x, long rows, long k, long rs, long cs, sign
   // Transposed: where 32 rows a workgroup are enough workgroups (8192 x 8192 bfloat16 109 us against 441, 4096 x 4096 45 / 76, 4096 x 128 float32 5.2 / 6.8;
   // 1024 x 4096 42 / 28, 2048 x 64 6.2 / 4.3).
   if (rs == 1 && cs != 1 && rows >= 2048 && k >= 128) {
-    k_quantize_turned<T><<<grid_of((rows + Turned<T>::ROWS - 1) / Turned<T>::ROWS), 1024, 0, st>>>(x, rows, k, cs, q, ldq, scale);
+    k_quantize_turned<T><<<grid_of<1024>((rows + Turned<T>::ROWS - 1) / Turned<T>::ROWS), 1024, 0, st>>>(x, rows, k, cs, q, ldq, scale);
     LAUNCHED(ctx, "quantize_rows");
     return NLS_OK;
   }
@@ -136,7 +136,7 @@ template <class T, int MG, int NG, bool FUSED>
 int int8_few(nls_ctx* ctx, const Int8Args& g, const FewX& f, hipStream_t st) {
   const size_t rows = FUSED ? ((size_t)g.m * ((g.k + 63) / 64 * 64 + 16) + 64 + 512 + 255) / 256 * 256 : 0;
   const size_t lds = rows + (size_t)8 * MG * NG * 1024;
-  k_int8_few<T, MG, NG, FUSED><<<grid_of((g.n + 16l * NG - 1) / (16 * NG)), 512, lds, st>>>(g, f);
+  k_int8_few<T, MG, NG, FUSED><<<grid_of<512>((g.n + 16l * NG - 1) / (16 * NG)), 512, lds, st>>>(g, f);
   LAUNCHED(ctx, "int8_matmul");
   return NLS_OK;
 }

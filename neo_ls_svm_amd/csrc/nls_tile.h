@@ -346,9 +346,13 @@ __device__ __forceinline__ void chunk_sums(const char* mine, int r, int i, V (&v
   }
 }
 
-// Workgroups of a launch in two dimensions: threads of one dimension are counted in 32 bits.
-constexpr long GRID_X = 1l << 22;
-inline dim3 grid_of(long groups) { return dim3((unsigned)(groups < GRID_X ? groups : GRID_X), (unsigned)((groups + GRID_X - 1) / GRID_X)); }
+// Workgroups of THREADS threads in two dimensions: the threads of one dimension are counted in 32 bits.
+constexpr long GRID_X = 1l << 21;
+template <int THREADS>
+inline dim3 grid_of(long groups) {
+  static_assert(GRID_X * THREADS < 1l << 32, "more threads along x than a launch counts");
+  return dim3((unsigned)(groups < GRID_X ? groups : GRID_X), (unsigned)((groups + GRID_X - 1) / GRID_X));
+}
 __device__ __forceinline__ long group_id() { return blockIdx.y * GRID_X + blockIdx.x; }
 
 // Tiles in an order that keeps the ones a die works on together: workgroups are dealt to the 8 dies in turn, so die x takes the x-th eighth of the

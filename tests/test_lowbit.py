@@ -2,7 +2,10 @@
 
 from __future__ import annotations
 
+import shutil
+import subprocess
 from fractions import Fraction
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -139,3 +142,14 @@ def test_the_64_bit_calls_refuse_device_arrays_of_other_types(dtype):
 def test_featuremap_refuses_to_write_past_the_end_of_out(out):
     with pytest.raises(ValueError, match="out must hold"):
         nls.featuremap(np.ones((6, 3)), np.zeros(3), np.ones(3), np.ones((3, 4)), ctx=NoContext(), out=device_array(*out))
+
+
+def test_launches_of_many_workgroups(tmp_path):
+    """csrc/nls_tile.h compiled for the host: a kernel of 1024 threads used to get 2^32 threads along x from 2^22 workgroups on."""
+    hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
+    if not Path(hipcc).exists():
+        pytest.skip("hipcc not available")
+    root, exe = Path(__file__).resolve().parent.parent, tmp_path / "test_grid"
+    subprocess.run([hipcc, "-x", "hip", "--offload-host-only", "-O1", "-std=c++17", "-I", str(root / "neo_ls_svm_amd" / "csrc"), str(root / "tests" / "csrc" / "test_grid.cpp"), "-o", str(exe)], check=True)  # fmt: skip
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stdout + r.stderr
