@@ -4,8 +4,8 @@ They stand next to the 64-bit matrix calls of ``hotpath`` (``gram``, ``rotate``,
 matrices.  (The reference computes in 64 bits throughout: it has no counterpart.)  Three kinds of arrays go in, and the same kind comes out:
 
 * tensors of a tensor library that the caller has imported (torch on the GPU): the call is put on the tensor's device's current stream and does not
-  wait; it can be captured into a graph, but for the first call on a device.  Nothing is imported here for it.  The operators are not differentiated: a tensor that asks for gradients is
-  refused while gradients are recorded.
+  wait; it can be captured into a graph, but for the first call on a device.  Nothing is imported here for it.  The operators are not differentiated: a
+  tensor that asks for gradients is refused while gradients are recorded, one with a tangent of forward mode always.
 * ``DeviceArray``: the context's own stream; the call returns when the result is there.
 * NumPy arrays: copied to the GPU and back.
 
@@ -67,7 +67,7 @@ class _Tensors:
         self.ptr, self.strides, self.dense = lib.Tensor.data_ptr, lib.Tensor.stride, lib.Tensor.contiguous
         self.types = tuple(getattr(lib, name) for name in _NAMES)
         self.int8, self.float32, self.uint8, self.strided, self.Tensor = lib.int8, lib.float32, lib.uint8, lib.strided, lib.Tensor
-        self._empty = lib.empty
+        self._empty, self._forward = lib.empty, lib.autograd.forward_ad
         self._raw_stream = getattr(lib._C, "_cuda_getCurrentRawStream", None)
 
     def begin(self):
@@ -84,6 +84,8 @@ class _Tensors:
             raise ValueError(f"{what} must be a dense tensor")
         if x.requires_grad and self.lib.is_grad_enabled():
             raise ValueError(f"{what} asks for gradients, which this operator does not give: detach it, or call under no_grad")
+        if self._forward.unpack_dual(x).tangent is not None:
+            raise ValueError(f"{what} has a tangent, and this operator gives no gradients in forward mode either: hand over its primal")
         return x.resolve_neg() if x.is_neg() else x
 
     @staticmethod
@@ -98,9 +100,13 @@ class _Tensors:
         held = self._empty(*lead, ld, dtype=self.int8, device=self.device)
         return held, held if ld == k else held[..., :k]
 
+    def derived(self):
+        """Whether tensors may have tangents: a level of forward mode is open (or not to be seen from here)."""
+        return getattr(self._forward, "_current_level", 0) >= 0
+
     # The usual arguments - dense matrices - in the few checks they need; all others, wrong ones among them, the long way.
     def float_rows(self, x, what):
-        if isinstance(x, self.Tensor) and x.get_device() == self.index and x.layout is self.strided and x.is_contiguous() and not x.requires_grad and not x.is_neg():
+        if not self.derived() and isinstance(x, self.Tensor) and x.get_device() == self.index and x.layout is self.strided and x.is_contiguous() and not x.requires_grad and not x.is_neg():
             shape, kind = x.shape, self.kinds.get(x.dtype)
             if kind is not None and len(shape) == 2 and shape[1] > 0:
                 return x, shape[:1], shape[0], shape[1], shape[1], 1, kind
@@ -111,7 +117,7 @@ class _Tensors:
         if (
             isinstance(x, T) and isinstance(scale, T) and x.dtype is self.int8 and scale.dtype is self.float32
             and x.get_device() == self.index == scale.get_device() and x.layout is strided is scale.layout
-            and scale.is_contiguous() and not scale.requires_grad and not scale.is_neg()
+            and scale.is_contiguous() and not scale.requires_grad and not scale.is_neg() and not self.derived()
         ):  # fmt: skip
             shape = x.shape
             if len(shape) == 2 and scale.shape == shape[:1] and 0 < shape[1] <= MAX_K:

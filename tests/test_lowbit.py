@@ -153,3 +153,24 @@ def test_launches_of_many_workgroups(tmp_path):
     subprocess.run([hipcc, "-x", "hip", "--offload-host-only", "-O1", "-std=c++17", "-I", str(root / "neo_ls_svm_amd" / "csrc"), str(root / "tests" / "csrc" / "test_grid.cpp"), "-o", str(exe)], check=True)  # fmt: skip
     r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
     assert r.returncode == 0, r.stdout + r.stderr
+
+
+def test_forward_mode_derivatives_are_refused_not_lost():
+    """A dual tensor asks for no gradients, has memory like any other, and its result would have none."""
+    torch = pytest.importorskip("torch")
+    from neo_ls_svm_amd import lowbit
+
+    sp = lowbit._Tensors(torch, 0, None)
+    sp.index = -1  # (tensors of the host pass for the device's)
+    x, q, s = torch.ones(3, 32), torch.ones(3, 32, dtype=torch.int8), torch.ones(3)
+    assert sp.float_rows(x, "x")[0] is x
+    with torch.autograd.forward_ad.dual_level():
+        assert sp.float_rows(x, "x")[0] is x and sp.int8_rows(q, "b", s, "b_scale")[0] is q
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        scale = torch.autograd.forward_ad.make_dual(s, torch.ones_like(s))
+        for call in (lambda: sp.take(dual, "x"), lambda: sp.float_rows(dual, "x"), lambda: sp.float_rows(dual[:, ::2], "x"), lambda: sp.int8_rows(q, "b", scale, "b_scale"), lambda: lowbit._bias(sp, scale, 3, 0)):  # fmt: skip
+            with pytest.raises(ValueError, match="tangent"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="tangent"):
+                call()
+    assert sp.float_rows(x, "x")[0] is x
