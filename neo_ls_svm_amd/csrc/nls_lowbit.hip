@@ -11,13 +11,11 @@ using namespace lb;
 
 namespace {
 
-// The context's device for the length of a call; the caller's current device comes back afterwards.  An error that some call before left behind is not
-// this one's: it would be taken for a failed launch.
+// The context's device for the length of a call; the caller's current device comes back afterwards.
 struct DeviceGuard {
   int before = -1;
   hipError_t err = hipSuccess;
   explicit DeviceGuard(int device) {
-    (void)hipGetLastError();
     err = hipGetDevice(&before);
     if (err == hipSuccess && before != device)
       err = hipSetDevice(device);
@@ -29,11 +27,19 @@ struct DeviceGuard {
   }
 };
 
-#define LAUNCHED(ctx, what)                                                                             \
-  do {                                                                                                  \
-    const hipError_t e__ = hipGetLastError();                                                           \
-    if (e__ != hipSuccess) return fail(ctx, NLS_ERR_HIP, "%s: launch failed: %s", what, hipGetErrorString(e__)); \
-  } while (0)
+// A launch that says itself whether it failed: the thread's last error may be that of some call before, which is neither this one's nor this one's to clear.
+template <class P>
+struct Given {
+  using type = P;
+};
+template <class... P>
+int launch(nls_ctx* ctx, const char* what, void (*kernel)(P...), dim3 grid, int threads, size_t lds, hipStream_t st, typename Given<P>::type... args) {
+  void* at[] = {&args...};
+  const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, dim3((unsigned)threads), at, lds, st);
+  if (e == hipSuccess) return NLS_OK;
+  (void)hipGetLastError();  // (reported here)
+  return fail(ctx, NLS_ERR_HIP, "%s: launch failed: %s", what, hipGetErrorString(e));
+}
 
 // Dynamic LDS beyond 64 KB has to be asked for, once per kernel and device.
 template <auto F>
@@ -75,32 +81,21 @@ template <class T, bool VEC>
 int quantize(nls_ctx* ctx, const T* x, long rows, long k, long rs, long cs, signed char* q, long ldq, float* scale, hipStream_t st) {
   constexpr long N = Few<T, VEC>::N;
   const dim3 waves = grid_of<256>((rows + 3) / 4), groups = grid_of<256>(rows);
-#define QUANTIZE(G, HELD, GRID) k_quantize_rows<T, G, VEC, HELD><<<GRID, 256, 0, st>>>(x, rows, k, rs, cs, q, ldq, scale)
-  if (k <= 64 * N)
-    QUANTIZE(64, 1, waves);
-  else if (k <= 128 * N)
-    QUANTIZE(64, 2, waves);
-  else if (k <= 512 * N)
-    QUANTIZE(256, 2, groups);
-  else if (k <= 1024 * N)
-    QUANTIZE(256, 4, groups);
-  else if (k <= 2048 * N)
-    QUANTIZE(256, 8, groups);
-  else
-    QUANTIZE(256, 0, groups);
+#define QUANTIZE(G, HELD, GRID) return launch(ctx, "quantize_rows", k_quantize_rows<T, G, VEC, HELD>, GRID, 256, 0, st, x, rows, k, rs, cs, q, ldq, scale)
+  if (k <= 64 * N) QUANTIZE(64, 1, waves);
+  if (k <= 128 * N) QUANTIZE(64, 2, waves);
+  if (k <= 512 * N) QUANTIZE(256, 2, groups);
+  if (k <= 1024 * N) QUANTIZE(256, 4, groups);
+  if (k <= 2048 * N) QUANTIZE(256, 8, groups);
+  QUANTIZE(256, 0, groups);
 #undef QUANTIZE
-  LAUNCHED(ctx, "quantize_rows");
-  return NLS_OK;
 }
 template <class T>
 int quantize(nls_ctx* ctx, const T* x, long rows, long k, long rs, long cs, signed char* q, long ldq, float* scale, hipStream_t st) {
   // Transposed: where 32 rows a workgroup are enough workgroups (8192 x 8192 bfloat16 109 us against 441, 4096 x 4096 45 / 76, 4096 x 128 float32 5.2 / 6.8;
   // 1024 x 4096 42 / 28, 2048 x 64 6.2 / 4.3).
-  if (rs == 1 && cs != 1 && rows >= 2048 && k >= 128) {
-    k_quantize_turned<T><<<grid_of<1024>((rows + Turned<T>::ROWS - 1) / Turned<T>::ROWS), 1024, 0, st>>>(x, rows, k, cs, q, ldq, scale);
-    LAUNCHED(ctx, "quantize_rows");
-    return NLS_OK;
-  }
+  if (rs == 1 && cs != 1 && rows >= 2048 && k >= 128)
+    return launch(ctx, "quantize_rows", k_quantize_turned<T>, grid_of<1024>((rows + Turned<T>::ROWS - 1) / Turned<T>::ROWS), 1024, 0, st, x, rows, k, cs, q, ldq, scale);
   return cs == 1 ? quantize<T, true>(ctx, x, rows, k, rs, cs, q, ldq, scale, st) : quantize<T, false>(ctx, x, rows, k, rs, cs, q, ldq, scale, st);
 }
 int quantize_any(nls_ctx* ctx, const void* x, int type, long rows, long k, long rs, long cs, signed char* q, long ldq, float* scale, hipStream_t st) {
@@ -117,9 +112,7 @@ int int8_tile(nls_ctx* ctx, const Int8Args& g, hipStream_t st) {
   const int ti = (g.n + BI - 1) / BI, tj = (g.m + BJ - 1) / BJ;
   constexpr int LDS = tile_bytes<TL>() + BJ * 4;
   NLSCHK((ask_lds<&k_int8_tile<T, TL, BI, BJ>>(ctx, LDS)));
-  k_int8_tile<T, TL, BI, BJ><<<dim3((unsigned)((long)ti * tj)), TL::THREADS, LDS, st>>>(g, ti, tj, 8);
-  LAUNCHED(ctx, "int8_matmul");
-  return NLS_OK;
+  return launch(ctx, "int8_matmul", k_int8_tile<T, TL, BI, BJ>, dim3((unsigned)((long)ti * tj)), TL::THREADS, LDS, st, g, ti, tj, 8);
 }
 template <class T>
 int int8_tile(nls_ctx* ctx, const Int8Args& g, hipStream_t st) {
@@ -136,9 +129,7 @@ template <class T, int MG, int NG, bool FUSED>
 int int8_few(nls_ctx* ctx, const Int8Args& g, const FewX& f, hipStream_t st) {
   const size_t rows = FUSED ? ((size_t)g.m * ((g.k + 63) / 64 * 64 + 16) + 64 + 512 + 255) / 256 * 256 : 0;
   const size_t lds = rows + (size_t)8 * MG * NG * 1024;
-  k_int8_few<T, MG, NG, FUSED><<<grid_of<512>((g.n + 16l * NG - 1) / (16 * NG)), 512, lds, st>>>(g, f);
-  LAUNCHED(ctx, "int8_matmul");
-  return NLS_OK;
+  return launch(ctx, "int8_matmul", k_int8_few<T, MG, NG, FUSED>, grid_of<512>((g.n + 16l * NG - 1) / (16 * NG)), 512, lds, st, g, f);
 }
 // Two row groups of b a workgroup halve what is read of a; taken where that leaves a workgroup for every compute unit.
 template <class T, int MG>
@@ -215,9 +206,7 @@ int operands(nls_ctx* ctx, const Int8Rows& a, const Int8Rows& b, long k, char* w
     most = std::max(most, r.rows * (ldy / 16));
   }
   if (!count) return NLS_OK;
-  k_align_rows<<<dim3((unsigned)std::min<long>((most + 255) / 256, 32768), (unsigned)count), 256, 0, st>>>(todo[0], todo[1], k, ldy);
-  LAUNCHED(ctx, "int8_matmul (alignment)");
-  return NLS_OK;
+  return launch(ctx, "int8_matmul (alignment)", k_align_rows, dim3((unsigned)std::min<long>((most + 255) / 256, 32768), (unsigned)count), 256, 0, st, todo[0], todo[1], k, ldy);
 }
 
 // ---- Newton-Schulz ----
@@ -277,9 +266,7 @@ int ns_product_tile(nls_ctx* ctx, NsArgs g, long batch, hipStream_t st) {
   constexpr int LDS = tile_bytes<TL>();
   const long tiles = SYM ? (long)g.ti * (g.ti + 1) / 2 : (long)g.ti * g.tj;
   NLSCHK((ask_lds<&k_ns_product<KIND, T, TL, B, B>>(ctx, LDS)));
-  k_ns_product<KIND, T, TL, B, B><<<dim3((unsigned)tiles, 1, (unsigned)batch), TL::THREADS, LDS, st>>>(g);
-  LAUNCHED(ctx, "orthogonalize");
-  return NLS_OK;
+  return launch(ctx, "orthogonalize", k_ns_product<KIND, T, TL, B, B>, dim3((unsigned)tiles, 1, (unsigned)batch), TL::THREADS, LDS, st, g);
 }
 template <int KIND, class T>
 int ns_product(nls_ctx* ctx, const NsArgs& g, long batch, hipStream_t st) {
@@ -305,9 +292,7 @@ template <class T, int PB, int CB>
 int ns_small(nls_ctx* ctx, const NsMatrix& w, bool tall, long batch, const NsCoef& cf, int steps, double eps, T* out, hipStream_t st) {
   constexpr int lds = NsLds<PB, CB, ns_full<T, PB>()>::BYTES;
   NLSCHK((ask_lds<&k_ns_small<T, PB, CB>>(ctx, lds)));
-  k_ns_small<T, PB, CB><<<dim3((unsigned)batch), 512, lds, st>>>(w, cf, steps, eps, out, tall);
-  LAUNCHED(ctx, "orthogonalize");
-  return NLS_OK;
+  return launch(ctx, "orthogonalize", k_ns_small<T, PB, CB>, dim3((unsigned)batch), 512, lds, st, w, cf, steps, eps, out, tall);
 }
 template <class T>
 int ns_small_any(nls_ctx* ctx, const NsMatrix& w, bool tall, long batch, const NsCoef& cf, int steps, double eps, T* out, hipStream_t st) {
@@ -356,20 +341,19 @@ int ns_slabs(nls_ctx* ctx, const NsMatrix& w, bool tall, long batch, const NsCoe
   g.x_batch = plan.x / 4;
   g.a_batch = plan.a / 4;
   const dim3 grid((unsigned)slabs, (unsigned)batch);
-  k_ns_norm<T><<<dim3(g.count, (unsigned)batch), 256, 0, st>>>(w, (double*)ws);
-  k_ns_slab<T, PB, true><<<grid, 512, lds, st>>>(g, cf);
+  NLSCHK(launch(ctx, "orthogonalize", k_ns_norm<T>, dim3(g.count, (unsigned)batch), 256, 0, st, w, (double*)ws));
+  NLSCHK((launch(ctx, "orthogonalize", k_ns_slab<T, PB, true>, grid, 512, lds, st, g, cf)));
   const bool sum = slabs > 4;
   g.shares = sum ? 1 : slabs;
   for (g.t = 0; g.t < steps; g.t = g.end + 1) {
     g.end = g.t;
     while (!(cf.ends >> g.end & 1)) ++g.end;
-    if (sum) k_ns_sum<<<dim3(P * P / 256, (unsigned)batch), 64, 0, st>>>(a, g.a_batch, P * P, slabs);
+    if (sum) NLSCHK(launch(ctx, "orthogonalize", k_ns_sum, dim3(P * P / 256, (unsigned)batch), 64, 0, st, a, g.a_batch, P * P, slabs));
     g.a = a;
     g.next_a = next_a;
-    k_ns_slab<T, PB, false><<<grid, 512, lds, st>>>(g, cf);
+    NLSCHK((launch(ctx, "orthogonalize", k_ns_slab<T, PB, false>, grid, 512, lds, st, g, cf)));
     std::swap(a, next_a);
   }
-  LAUNCHED(ctx, "orthogonalize");
   return NLS_OK;
 }
 
@@ -411,10 +395,9 @@ int orthogonalize(nls_ctx* ctx, const NsMatrix& w, const NsPlan& plan, bool tall
   char* base = ws + plan.parts + plan.scales;
   char *X = base, *XT = X + plan.x, *XU = XT + plan.xt, *A = XU + plan.xt, *B = A + plan.a;
   const int count = ns_parts(w);
-  k_ns_norm<T><<<dim3(count, (unsigned)batch), 256, 0, st>>>(w, parts);
-  k_ns_pack<T><<<dim3((unsigned)((w.q + 63) / 64), (unsigned)((w.p + 63) / 64), (unsigned)batch), 256, 0, st>>>(w, parts, count, eps, cf, steps, scales, X, XT,
-                                                                                                              plan.batch_bytes);
-  LAUNCHED(ctx, "orthogonalize");
+  NLSCHK(launch(ctx, "orthogonalize", k_ns_norm<T>, dim3(count, (unsigned)batch), 256, 0, st, w, parts));
+  NLSCHK(launch(ctx, "orthogonalize", k_ns_pack<T>, dim3((unsigned)((w.q + 63) / 64), (unsigned)((w.p + 63) / 64), (unsigned)batch), 256, 0, st, w, parts, count, eps, cf,
+                steps, scales, X, XT, plan.batch_bytes));
   NsArgs g{};
   g.scales = scales;
   g.batch_bytes = plan.batch_bytes;

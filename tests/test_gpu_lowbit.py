@@ -684,3 +684,17 @@ def test_sixteen_bit_results_of_up_to_128_rows(m, n, name, steps):
         for one in (nls.NEWTON_SCHULZ, CUBIC):
             off, own, plain, norm = sixteen_bit_errors(rng, kind, m, n, [one] * steps, name)
             assert off <= 1.1 * own + 4 * plain + HALF[name] / 8 * norm, (kind, one, off / own, plain / own)
+
+
+def test_an_error_that_the_caller_has_yet_to_ask_for_is_still_there():
+    ctx = nls.default_context()
+    x = torch.ones(200, 320, device="cuda")
+    q, s = nls.quantize_rows(x)
+    want = nls.int8_linear(x, q, s), nls.orthogonalize(x), nls.orthogonalize(x[:20])
+    torch.cuda.synchronize()
+    assert ctx.lib.hipSetDevice(1 << 20) != 0  # (no such device)
+    left = ctx.lib.hipPeekAtLastError()
+    nls.quantize_rows(x)
+    got = nls.int8_linear(x, q, s), nls.orthogonalize(x), nls.orthogonalize(x[:20])
+    assert left != 0 and ctx.lib.hipGetLastError() == left and ctx.lib.hipPeekAtLastError() == 0
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
