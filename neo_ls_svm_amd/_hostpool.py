@@ -7,18 +7,18 @@ last array (or view) on it is garbage collected the mapping goes back to the poo
 Smaller outputs are plain ``np.zeros``.
 
 Only the triangle the library defines is meaningful in such an array (scipy's ``cho_factor`` contract: the other triangle "contains random
-data"); a recycled buffer holds a previous factor's entries there, a fresh one zeros.  ``release()`` unmaps what the pool holds
+data"); a recycled or page-locked buffer holds whatever was there, a fresh mapping zeros.  ``release()`` unmaps what the pool holds
 (``Context.release_workspace`` calls it).
 
 The arrays start 64 bytes into their mapping on purpose: into a PAGE-ALIGNED pageable destination the HIP runtime locks the user pages in place
 for every copy (measured: 12 ms per 268 MB when the pages are resident, 38 ms when they are fresh), into an unaligned one it stages the copy
 (0.4 ms visible once the pages are resident) - numpy's own arrays are never page-aligned either.
 
-A mapping can additionally be page-locked ONCE (``nls_host_register``; 16-40 ms per 268 MB, 110-140 ms per 800 MB): the library then sends the
-finished block columns with asynchronous copies.  With the unaligned start this buys nothing measurable any more (0.36 against 0.43 ms of visible
-download at D = 4096), so the default policy is ``False``; ``pin_large_outputs("reuse")`` page-locks a mapping when it is handed out for the
-second time, ``pin_large_outputs(True)`` at creation, and ``reserve(shape, dtype, ctx)`` puts page-locked mappings into the pool ahead of a loop
-(``bench.py``).  A failed registration (locked-memory limit) simply leaves the buffer pageable.
+A buffer can also be page-locked memory (``nls_host_alloc``, once a buffer; memory that exists already cannot be page-locked on every system): the
+library then sends the finished block columns with asynchronous copies.  With the unaligned start this buys nothing measurable any more (0.36 against
+0.43 ms of visible download at D = 4096), so the default policy is ``False``; ``pin_large_outputs("reuse")`` puts a page-locked buffer in the place of a
+pageable one when that would be handed out for the second time, ``pin_large_outputs(True)`` hands out page-locked ones only, and ``reserve(shape, dtype,
+ctx)`` puts page-locked ones into the pool ahead of a loop (``bench.py``).  Where the allocation fails (locked-memory limit) the buffer is pageable.
 """
 
 from __future__ import annotations
@@ -38,28 +38,57 @@ MAX_POOLED_BYTES = 4 << 30
 # arrays do.
 OFFSET = 64
 PIN_OUTPUTS = False  # False | "reuse" | True, see the module docstring
-LAST_REGISTER_RC = None  # return code of the most recent nls_host_register (diagnostic)
+LAST_REGISTER_RC = None  # return code of the most recent nls_host_alloc (diagnostic)
 
 _lock = threading.RLock()  # re-entrant: a cyclic-GC pass triggered by an allocation inside a locked region may finalise another lease on this thread
-_free: dict[int, list[mmap.mmap]] = {}
+_free: dict[int, list] = {}  # bytes -> mappings (mmap.mmap or _Locked)
 _registered: dict[int, object] = {}  # id(mapping) -> the ctypes library that page-locked it
 
 
-def _address(mm: mmap.mmap) -> int:
-    view = ctypes.c_char.from_buffer(mm)
+class _Locked:
+    """A page-locked buffer in the place of an anonymous mapping."""
+
+    def __init__(self, lib, address: int, size: int):
+        self.lib, self.size = lib, size
+        self.memory = (ctypes.c_char * size).from_address(address)
+
+    def __len__(self):
+        return self.size
+
+    def close(self):
+        lib, self.lib = self.lib, None
+        if lib is not None:
+            lib.nls_host_free(None, ctypes.c_void_p(ctypes.addressof(self.memory)))
+
+
+def _lock_pages(ctx, nbytes: int):
+    """A page-locked buffer for an output of that size; None where there is none to be had."""
+    global LAST_REGISTER_RC
+    if ctx is None or not getattr(ctx, "handle", None):
+        return None
+    p = ctypes.c_void_p()
     try:
-        return ctypes.addressof(view) + OFFSET
-    finally:
-        del view
+        LAST_REGISTER_RC = ctx.lib.nls_host_alloc(ctx.handle, ctypes.c_size_t(nbytes + 4096), ctypes.byref(p))
+    except Exception as exc:  # pragma: no cover
+        LAST_REGISTER_RC = repr(exc)
+    if LAST_REGISTER_RC != 0 or not p.value:
+        return None
+    mm = _Locked(ctx.lib, p.value, nbytes + 4096)
+    _registered[id(mm)] = ctx.lib
+    return mm
 
 
-def _close(mm: mmap.mmap) -> None:
-    lib = _registered.pop(id(mm), None)
-    if lib is not None:
-        try:
-            lib.nls_host_unregister(None, ctypes.c_void_p(_address(mm)))
-        except Exception:
-            pass
+def _map(nbytes: int) -> mmap.mmap:
+    mm = mmap.mmap(-1, nbytes + 4096)  # anonymous, zero-filled on first touch (+ a page: the array starts OFFSET bytes in)
+    try:  # transparent huge pages where the system allows them on request (what numpy asks for its own large arrays): 512 x fewer faults / TLB entries
+        mm.madvise(mmap.MADV_HUGEPAGE)
+    except (AttributeError, OSError, ValueError):
+        pass
+    return mm
+
+
+def _close(mm) -> None:
+    _registered.pop(id(mm), None)
     mm.close()
 
 
@@ -72,9 +101,9 @@ class _Lease:
 
     __slots__ = ("_mm", "_view", "__array_interface__")
 
-    def __init__(self, mm: mmap.mmap, shape, dtype):
+    def __init__(self, mm, shape, dtype):
         self._mm = mm
-        self._view = ctypes.c_char.from_buffer(mm)  # (pins the mapping: it cannot be resized or closed under the arrays)
+        self._view = mm.memory if isinstance(mm, _Locked) else ctypes.c_char.from_buffer(mm)  # (pins a mapping: it cannot be resized or closed under the arrays)
         self.__array_interface__ = {"data": (ctypes.addressof(self._view) + OFFSET, False), "shape": tuple(shape), "typestr": np.dtype(dtype).str, "version": 3}
 
     def __del__(self):
@@ -109,27 +138,18 @@ def factor_output(shape, dtype, ctx=None) -> np.ndarray:
     with _lock:
         lst = _free.get(nbytes)
         mm = lst.pop() if lst else None
-    recycled = mm is not None
-    if mm is None:
-        mm = mmap.mmap(-1, nbytes + 4096)  # anonymous, zero-filled on first touch (+ a page: the array starts OFFSET bytes in)
-        try:  # transparent huge pages where the system allows them on request (what numpy asks for its own large arrays): 512 x fewer faults / TLB entries
-            mm.madvise(mmap.MADV_HUGEPAGE)
-        except (AttributeError, OSError, ValueError):
-            pass
-    if (PIN_OUTPUTS is True or (PIN_OUTPUTS == "reuse" and recycled)) and ctx is not None and id(mm) not in _registered and getattr(ctx, "handle", None):
-        global LAST_REGISTER_RC
-        try:
-            LAST_REGISTER_RC = ctx.lib.nls_host_register(ctx.handle, ctypes.c_void_p(_address(mm)), ctypes.c_size_t(nbytes))
-            if LAST_REGISTER_RC == 0:
-                _registered[id(mm)] = ctx.lib
-        except Exception as exc:  # pragma: no cover
-            LAST_REGISTER_RC = repr(exc)
-    return np.asarray(_Lease(mm, shape, dtype))
+    if (PIN_OUTPUTS is True or (PIN_OUTPUTS == "reuse" and mm is not None)) and not isinstance(mm, _Locked):
+        locked = _lock_pages(ctx, nbytes)
+        if locked is not None:
+            if mm is not None:
+                _close(mm)
+            mm = locked
+    return np.asarray(_Lease(_map(nbytes) if mm is None else mm, shape, dtype))
 
 
 def reserve(shape, dtype, ctx=None, count: int = 2) -> int:
     """Put ``count`` mappings for outputs of this shape into the pool ahead of time - page-locked when a context is given - so that a loop of
-    fits starts in its steady state (what a C caller does when it allocates and registers its output buffer once).  Returns how many were added."""
+    fits starts in its steady state (what a C caller does when it allocates its output buffer once).  Returns how many were added."""
     nbytes = int(np.prod(shape)) * np.dtype(dtype).itemsize
     if nbytes < MIN_BYTES or os.environ.get("NLS_HOST_POOL", "1") == "0":
         return 0
@@ -138,17 +158,7 @@ def reserve(shape, dtype, ctx=None, count: int = 2) -> int:
         with _lock:
             if len(_free.get(nbytes, [])) >= MAX_POOLED_PER_SIZE or _pooled_bytes() + nbytes > MAX_POOLED_BYTES:
                 break
-        mm = mmap.mmap(-1, nbytes + 4096)
-        try:
-            mm.madvise(mmap.MADV_HUGEPAGE)
-        except (AttributeError, OSError, ValueError):
-            pass
-        if ctx is not None and getattr(ctx, "handle", None):
-            try:
-                if ctx.lib.nls_host_register(ctx.handle, ctypes.c_void_p(_address(mm)), ctypes.c_size_t(nbytes)) == 0:
-                    _registered[id(mm)] = ctx.lib
-            except Exception:
-                pass
+        mm = _lock_pages(ctx, nbytes) or _map(nbytes)
         with _lock:
             _free.setdefault(nbytes, []).append(mm)
         added += 1

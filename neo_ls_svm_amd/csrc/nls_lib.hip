@@ -297,6 +297,24 @@ extern "C" int nls_host_unregister(nls_ctx* ctx, void* ptr) {  // (ctx may be NU
   (void)hipGetLastError();
   return fail(ctx, NLS_ERR_HIP, "hipHostUnregister: %s", hipGetErrorString(e));
 }
+extern "C" int nls_host_alloc(nls_ctx* ctx, size_t bytes, void** ptr) {
+  if (!ctx) return NLS_ERR_ARG;
+  if (!ptr || bytes == 0) return fail(ctx, NLS_ERR_ARG, "nls_host_alloc: null pointer or zero size");
+  *ptr = nullptr;
+  HIPCHK(ctx, hipSetDevice(ctx->device));
+  const hipError_t e = hipHostMalloc(ptr, bytes, hipHostMallocPortable);
+  if (e == hipSuccess) return NLS_OK;
+  (void)hipGetLastError();
+  return fail(ctx, NLS_ERR_HIP, "hipHostMalloc of %zu bytes: %s", bytes, hipGetErrorString(e));
+}
+extern "C" int nls_host_free(nls_ctx* ctx, void* ptr) {  // (ctx may be NULL, as above)
+  if (!ptr) return NLS_OK;
+  if (ctx) HIPCHK(ctx, hipSetDevice(ctx->device));
+  const hipError_t e = hipHostFree(ptr);
+  if (e == hipSuccess) return NLS_OK;
+  (void)hipGetLastError();
+  return fail(ctx, NLS_ERR_HIP, "hipHostFree: %s", hipGetErrorString(e));
+}
 
 extern "C" int nls_ws_release(nls_ctx* ctx, size_t min_bytes, size_t* still_held) {
   if (!ctx) return NLS_ERR_ARG;
