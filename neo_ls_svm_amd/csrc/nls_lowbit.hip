@@ -64,7 +64,8 @@ int type_size(int t) { return t == NLS_TYPE_F32 ? 4 : (t == NLS_TYPE_F16 || t ==
 //   64 x 64, four waves side by side, three workgroups a unit: more of them than units, or few K steps: 1536^2 symmetric pairs 25 us against 34 (128 x 128)
 //     and 27 (K dealt out), int8 512 x 4096 x 4096 18.2 / 25 / 20; more than three steps held 0 .. 10 us slower (fewer workgroups a unit);
 //   64 x 64 with the K steps dealt out over the waves otherwise: X X^T of 512 x 2048 pairs 15.5 us against 22 (side by side) and 42 (128 x 128), int8
-//     256 x 4096 x 4096 11.6 / 14.5 / 24; at 16 steps (512^2 pairs, a whole call) 145 / 148; at 8 steps (single halves) the order turned: 125 / 120.
+//     256 x 4096 x 4096 11.6 / 14.5 / 24; at 16 steps (five Newton-Schulz steps of 512^2) 145 / 147, at 13 (400^2) 135 / 128, at 5 .. 7 (130 x 200) 98 / 86,
+//     int8 at 8 .. 12 steps equal within 4 %.
 enum TileKind { TILE_256, TILE_128, TILE_128_DEEP, TILE_64, TILE_64_RING };
 template <class F>
 TileKind tile_kind(const nls_ctx* ctx, F tiles, int steps) {
@@ -137,8 +138,10 @@ int int8_few(nls_ctx* ctx, const Int8Args& g, const FewX& f, hipStream_t st) {
   if (MG > 1 && (g.n + 31) / 32 >= ctx->cus) return int8_few<T, MG, 2, false>(ctx, g, f, st);
   return int8_few<T, MG, 1, false>(ctx, g, f, st);
 }
-// Few rows of a: fragments straight from memory, or tiles.  Measured: 16 x 4096 x 4096 8.4 us against 11.4 with tiles, 48 x 4096 x 4096 12.6 / 12.9,
-// 64 x 4096 x 4096 14.8 / 13.5; 16 x 8192 x 8192 22.1 / 22.4, 32 x 8192 x 8192 25.5 / 23.9, 48 x 8192 x 8192 29 / 25 (128 tiles keep enough of the card busy).
+// Few rows of a: fragments straight from memory, or tiles.  Measured, m x n x k, the kernel alone with b from memory (the last of it still in the
+// caches: 1 .. 6 us less): 16 x 4096 x 4096 8.3 us against 11.0 with tiles, 16 x 2048 x 2048 5.2 / 7.6, 16 x 1024 x 8192 10.8 / 16.8, 48 x 4096 x 4096 12.4 / 12.2,
+// 48 x 2048 x 2048 7.3 / 8.4; from 8192 channels on there are tiles enough: 32 x 8192 x 8192 24.3 / 20.7, 48 x 8192 x 8192 28.4 / 22.4.  Up to 16 rows stay
+// with the fragments there, which take b from any address: 16 x 8192 x 8192 20.2 / 19.3 (in the caches 18.9 / 14.5), 16 x 14336 x 4096 20.9 / 14.8.
 bool int8_is_few(long m, long n) { return m <= 16 || (m <= 48 && n < 8192); }
 template <class T>
 int int8_product(nls_ctx* ctx, const Int8Args& g, const FewX& f, hipStream_t st) {
@@ -276,8 +279,9 @@ int ns_product(nls_ctx* ctx, const NsArgs& g, long batch, hipStream_t st) {
     const long i = (g.I + b - 1) / b, j = (g.J + b - 1) / b;
     return (SYM ? i * (i + 1) / 2 : i * j) * batch;
   };
-  // 192 x 192, four waves with a SIMD each, where they cover the card in one go and 128 x 128 in more than one: symmetric 4096^2 pairs 230 us against 280
-  // (128 x 128: 528 tiles for 512 places) and 287 (256 x 256: 136 tiles).
+  // 192 x 192, four waves with a SIMD each, where they cover the card in one go and 128 x 128 in more than one: five steps of a call against the rule below
+  // alone, 2850 x 2950 2.02 ms / 2.26, 4000^2 3.90 / 4.51, 4096^2 4.12 / 4.61, 4200^2 5.46 / 6.11, 2048 x 4200 1.31 / 1.43, three of 2300^2 2.48 / 2.72, five of
+  // 1700^2 1.95 / 2.18 (its symmetric or its last product, or both, have such sizes).
   if (tiles(128) > 2 * ctx->cus && tiles(192) <= ctx->cus) return ns_product_tile<KIND, T, Tile<MODE, 192, 192, 2, 2, 3>, 192>(ctx, g, batch, st);
   switch (tile_kind(ctx, tiles, (g.K + 31) / 32)) {
     case TILE_256: return ns_product_tile<KIND, T, Tile<MODE, 256, 256, 2, 4, 2>, 256>(ctx, g, batch, st);

@@ -159,10 +159,10 @@ struct Tile {
   __device__ __forceinline__ static void arrive() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
   }
-  // Waves with many blocks have the first fragments of a step in registers when the last products of the step before begin: the reads behind the
-  // barrier are then off the matrix cores' path.  (256 x 256, int8 8192^3: 499 us against 520 .. 541, 8192 x 8192 x 2048 176 / 183, K = 512 92 / 90; fp16
-  // symmetric 4096^2 114 / 145.  128 x 128 with eight waves, two workgroups' worth of waves to fill the gaps: pairs 2048^2 52 against 47.5.)
-  static constexpr bool AHEAD = MI * MJ >= 8;
+  // 8-bit waves with many blocks have the first fragments of a step in registers when the last products of the step before begin: the reads behind the
+  // barrier are then off the matrix cores' path.  (256 x 256, int8 8192^3: 464 us against 497, 8192 x 8192 x 2048 149 / 153, K = 512 69 / 66.)  A step of
+  // pairs has three products a fragment to cover them: five steps of 4096^2 4.12 ms against 4.06 without, of 8192^2 34.5 / 34.0.
+  static constexpr bool AHEAD = MODE == MODE_I8 && MI * MJ >= 8;
   // steps >= 1 K steps; last_valid: valid bytes of the last one (128: whole).
   // STAGES - 1 steps are under way at any time; one barrier a step: behind it the next step is there and a buffer that all have read is free.
   __device__ __forceinline__ void run(const Operand& P, int i0, const Operand& Q, int j0, int steps, int last_valid, char* lds) {
