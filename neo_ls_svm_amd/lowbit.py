@@ -457,6 +457,8 @@ def orthogonalize(g, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: float = 1e
     table = (C.c_double * (3 * steps))(*flat)
     m, n = shape[-2:]
     batch = math.prod(shape[:-2])
+    if max(m, n) > 1 << 20 or batch > 65535:  # (before room is made for the result and its workspace)
+        raise ValueError(f"g of shape {shape}: at most 2^20 rows and columns and 65535 matrices")
     if isinstance(g, DeviceArray):
         st = (m * n, n, 1)
     elif len(shape) == 2:

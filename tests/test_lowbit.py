@@ -174,3 +174,9 @@ def test_forward_mode_derivatives_are_refused_not_lost():
             with torch.no_grad(), pytest.raises(ValueError, match="tangent"):
                 call()
     assert sp.float_rows(x, "x")[0] is x
+
+
+@pytest.mark.parametrize("shape", [(2**20 + 1, 1), (1, 2**20 + 1), (65536, 1, 1), (256, 256, 1, 1), (2, 2**20 + 1, 0)])
+def test_orthogonalize_refuses_sizes_before_it_makes_room_for_them(shape):
+    with pytest.raises(ValueError, match="65535 matrices"):
+        nls.orthogonalize(np.zeros(shape, dtype=np.float32))
