@@ -426,8 +426,9 @@ __global__ __launch_bounds__(TL::THREADS) void k_ns_product(NsArgs g) {
 // standard and 32 cubic steps, 16 .. 128 rows, in units of the result's own rounding: growth 500 in bfloat16 3.8, 45 in float16 0.4; as
 // above 0.1 and 0.2.  64 x 512 bfloat16 34.5 us against 27.9 in one chain, 64 x 8192 47 / 35; float16 40 / 34 and 58 / 47 in 3 + 2; float32 52 and 80.)
 // Bound by latency and by vector instructions (roundings to pairs) for few matrices: a step is a chain of dependent products, LDS round trips and
-// barriers.  Five float32 steps of a 64 x 64 matrix take 22 us, of a 128 x 128 one 55 us; column blocks of 32 and the 32 x 32 x 16 instruction read half
-// as much LDS but keep half as many waves busy (26 and 63 us).
+// barriers.  Five float32 steps of a 64 x 64 matrix take 20 us, of a 128 x 128 one 54 us; column blocks of 32 and the 32 x 32 x 16 instruction read half
+// as much LDS but keep half as many waves busy (26 and 63 us).  Two column blocks at a time beside all of X are more than 256 registers for 64 x 512 (66
+// of them spill, 54 us in float32), 128 x 256 (42, 84 us) and 64 x 256 (32).
 template <int PB, bool F>
 struct NsRows {
   static constexpr int P = 32 * PB, RB = 2 * PB;              // rows, row blocks

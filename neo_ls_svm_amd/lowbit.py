@@ -24,7 +24,7 @@ from ._lib import Context, DeviceArray, _default_ctx, default_context
 
 __all__ = ["NEWTON_SCHULZ", "quantize_rows", "int8_matmul", "int8_linear", "orthogonalize"]
 
-#: (a, b, c) of X <- a X + (b A + c A A) X: odd polynomial of degree five that takes singular values in (0, 1] to about 0.7 .. 1.2 in five steps
+#: (a, b, c) of X <- a X + (b A + c A A) X, as published by K. Jordan et al. (2024): odd polynomial of degree five that takes singular values in (0, 1] to about 0.7 .. 1.2 in five steps
 #: (slope 3.44 at zero).  A step with (1.5, -0.5, 0) or (1.875, -1.25, 0.375) afterwards takes them on towards 1.
 NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
 
@@ -345,8 +345,9 @@ def quantize_rows(x, ctx: Context | None = None):
     """(q, scale): the rows of ``x`` (its last axis) as 8-bit integers with one scale a row, ``x ~ scale[..., None] * q``.
 
     ``scale = max|x| / 127`` and ``q = 127 x / max|x|`` to the nearest integer, ties to even, decided as in exact arithmetic.  A row of zeros has
-    scale 0; a row with a NaN or an infinity has that for its scale and zeros in ``q``.  The rows of a ``q`` on the GPU start at multiples of 16
-    bytes (its last axis is dense, its rows may have gaps): that is how ``int8_matmul`` and ``int8_linear`` read them without a copy."""
+    scale 0; a row with a NaN or an infinity has that for its scale and zeros in ``q``.  The rows of a ``q`` that is a tensor start at
+    multiples of 16 bytes (its last axis is dense, its rows may have gaps): that is how ``int8_matmul`` and ``int8_linear`` read them without a copy.  A
+    ``DeviceArray`` has no gaps: where k is not a multiple of 16 its rows are put together by way of the host, and laid out again by each product."""
     sp = _space(x, ctx)
     x, lead, rows, k, rs, cs, kind = sp.float_rows(x, "x")
     stream = sp.begin()
