@@ -381,9 +381,9 @@ void ns_chains(NsCoef& cf, int steps, double most) {
 template <class T>
 int orthogonalize(nls_ctx* ctx, const NsMatrix& w, const NsPlan& plan, bool tall, long batch, NsCoef& cf, int steps, double eps, T* out, char* ws, hipStream_t st) {
   // 16-bit matrices take pairs in every step as well.  Single products of the hi halves in the early ones would be a third of the work (4096^2 bfloat16, three
-  // of five steps: 2.6 ms against 3.9), but the roundings of A and B to 11 bits couple strong and weak singular directions and the steps after them spread that: the error
-  // against 64 bits was 0.75 (bfloat16) and 1.4 (float16) of the result's own rounding after five standard steps, 1.1 and 6.5 after six, 2.7 and 21 after
-  // twelve, where pairs stay at float32's error throughout.
+  // of five steps: 2.6 ms against 3.9), but the roundings of A and B to 11 bits couple strong and weak singular directions and the steps after them spread
+  // that: the error against 64 bits was 0.75 (bfloat16) and 1.4 (float16) of the result's own rounding after five standard steps, 1.1 and 6.5 after six, 2.7
+  // and 21 after twelve, where pairs stay at float32's error throughout.
   if (plan.path != NS_TILES) {
     const double half = std::is_same<T, __bf16>::value ? 0x1p-8 : 0x1p-11;  // half a step of the result, relative
     ns_chains(cf, steps, sizeof(T) == 4 ? 0.0 : std::sqrt(0x1p23 * half / 16.0));
